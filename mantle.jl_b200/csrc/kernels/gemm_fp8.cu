@@ -1,0 +1,561 @@
+// Matrix products of 8-bit floating point with one scale per block of 128 values
+// along K, on the 5th-generation tensor cores:
+//
+//   C[m, n] = sum_kb sA[kb, m] * sB[kb, n] * ( sum_{k in block kb} A[m, k] * B[n, k] )
+//
+// A: M rows of K codes, B: N rows of K codes (both e4m3 or e5m2, rows K rounded up
+// to 16 bytes apart, as quantize_fp8 writes them), sA: (K blocks, M), sB: one scale
+// per 128 x 128 block (N blocks, K blocks) or per row (K blocks, N); C fp32 or bf16.
+// The same kernel runs a batch of products and products grouped by expert
+// (gemm_grouped_fp8: rows offsets[e] .. offsets[e + 1] of A times B[e]).
+//
+// The scales are arbitrary fp32 values, so a block's products cannot simply
+// accumulate in tensor memory: each K block of 128 is one chain of four
+// tcgen05.mma (kind::f8f6f4, K = 32) into its own accumulator, and eight warps
+// read it back (tcgen05.ld), multiply by the scales and add to fp32 sums in
+// registers, rounding to nearest, while the tensor core runs the next K block
+// into another accumulator. A K block of a 128 x 256 tile is 512 cycles of MMAs;
+// its read-back and packed FMAs take about as many issue slots of the two warps
+// per scheduler.
+//
+// One persistent CTA per SM, three warpgroups; the first gives registers up
+// (setmaxnreg) so that the sums of the other two stay in theirs:
+//   warp 0      TMA producer: per K block 128 rows of A and BN rows of B, 128 bytes
+//               each (128-byte swizzle), into a ring of stages;
+//   warp 1      owns the tensor memory, one thread issues the MMAs;
+//   warps 4-11  the scaled sums: warp w reads lanes 32 (w % 4) .., half of BN columns.
+// Rows of a partial tile are loaded in boxes of 32, so that a group of a few rows
+// reads few; what the skipped rows hold only reaches rows that are not stored.
+//
+// Waits are bounded; one that runs out makes the CTA wind down, wait for its own
+// loads and MMAs in flight, free its tensor memory and return.
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "../mtl_internal.hpp"
+#include "tc_groups.cuh"
+
+namespace mtl {
+
+constexpr int kF8Threads = 384, kF8M = 128, kF8K = 128;
+constexpr int kF8FewRegs = 56, kF8ManyRegs = 224;  // registers a thread of the first / the other warpgroups
+constexpr int kF8GroupM = 16;  // row tiles per raster group of a dense product
+
+template <int BN>
+struct F8Cfg {
+  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int kAcc = BN == 256 ? 2 : 4;  // accumulators of BN columns
+  static constexpr uint32_t kTmemCols = kAcc * BN;
+  static constexpr uint32_t kAStage = kF8M * kF8K, kStageBytes = kAStage + BN * kF8K;
+};
+struct F8Shared {
+  uint64_t full[8], empty[8], tfull[4], tempty[4], drain;
+  uint32_t tmem;
+  int abort;
+  float scale_b[8][2][128];  // per warp: a K block's row scales of B, double buffered
+  GroupTable groups;
+};
+template <int BN>
+constexpr int f8_smem() {
+  return F8Cfg<BN>::kStages * (int)F8Cfg<BN>::kStageBytes + (int)sizeof(F8Shared) + 1024;
+}
+
+struct F8Args {
+  void* C;
+  const float *sA, *sB;
+  const int* offsets;  // grouped: groups + 1 row offsets
+  int M, N, K;         // M: rows of A in all (grouped) or per product
+  int batch;           // products or groups
+  int kblocks, nblocks;
+  uint32_t idesc;
+  int a_box;  // rows per TMA box of A
+  int vec;    // rows of C start on 16 bytes
+};
+
+__device__ int g_fp8_timeouts;
+
+__device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// A tile's place: rows row0 .. of operand A in slice a_b, columns n0 .. of operand
+// B in slice b_b, C's first row, the first element of A's scales, valid rows.
+struct F8Tile {
+  int a_row, a_b, b_b, n0, rows;
+  int64_t crow, sa;
+};
+
+template <bool GROUPED>
+struct F8Walk {
+  GroupWalk g;
+  __device__ __forceinline__ F8Tile find(const F8Args& p, const GroupTable* groups, int64_t t, int tiles_m, int tiles_n,
+                                         int bn) {
+    F8Tile c;
+    if (GROUPED) {
+      g.find(groups, (int)t, tiles_n, kF8M, bn, &c.a_row, &c.rows, &c.n0);
+      c.a_b = 0;
+      c.b_b = g.e;
+      c.crow = c.sa = c.a_row;
+    } else {
+      const int64_t per = (int64_t)tiles_m * tiles_n;
+      c.a_b = c.b_b = (int)(t / per);
+      const int r = (int)(t % per), group = r / (kF8GroupM * tiles_n), first = group * kF8GroupM;
+      const int size = min(kF8GroupM, tiles_m - first), in = r - group * kF8GroupM * tiles_n;
+      c.a_row = (first + in % size) * kF8M;
+      c.n0 = in / size * bn;
+      c.rows = p.M - c.a_row;
+      c.crow = (int64_t)c.a_b * p.M + c.a_row;
+      c.sa = (int64_t)c.a_b * p.kblocks * p.M + c.a_row;
+    }
+    c.rows = min(c.rows, kF8M);
+    return c;
+  }
+};
+
+// One row's `n` neighbouring sums to C, from column `col` on.
+template <typename OUT, int COLS>
+__device__ __forceinline__ void store_row(const F8Args& p, int64_t row, int col, const unsigned long long (&acc)[COLS / 2]) {
+  OUT* c = static_cast<OUT*>(p.C) + row * p.N + col;
+  if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+    for (int i = 0; i < COLS; i += 4) {
+      float v[4];
+      unpack2(acc[i / 2], v[0], v[1]);
+      unpack2(acc[i / 2 + 1], v[2], v[3]);
+      if (p.vec && col + i + 4 <= p.N) {
+        *reinterpret_cast<float4*>(c + i) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + i + j < p.N) c[i + j] = v[j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < COLS; i += 8) {
+      __nv_bfloat162 b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        unpack2(acc[i / 2 + j], lo, hi);
+        b[j] = __floats2bfloat162_rn(lo, hi);
+      }
+      if (p.vec && col + i + 8 <= p.N) {
+        *reinterpret_cast<uint4*>(c + i) = *reinterpret_cast<uint4*>(b);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col + i + j < p.N) c[i + j] = j & 1 ? b[j / 2].y : b[j / 2].x;
+      }
+    }
+  }
+}
+
+// BN columns a tile; GROUPED: rows by offsets; ROWB: B's scales per row (else
+// 128 x 128); OUT: float or bf16.
+template <int BN, bool GROUPED, bool ROWB, typename OUT>
+__global__ void __launch_bounds__(kF8Threads, 1)
+    gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const F8Args p) {
+  using Cfg = F8Cfg<BN>;
+  constexpr int kStages = Cfg::kStages, kAcc = Cfg::kAcc, kCols = BN / 2;
+  extern __shared__ unsigned char f8_raw[];
+  unsigned char* ring =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
+  F8Shared* sh = reinterpret_cast<F8Shared*>(ring + kStages * Cfg::kStageBytes);
+  volatile int* abort = &sh->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sh->full[s]), 1);
+      mbar_init(smem_u32(&sh->empty[s]), 1);
+    }
+    for (int a = 0; a < kAcc; ++a) {
+      mbar_init(smem_u32(&sh->tfull[a]), 1);
+      mbar_init(smem_u32(&sh->tempty[a]), 8);
+    }
+    mbar_init(smem_u32(&sh->drain), 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)),
+                 "r"(Cfg::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (GROUPED) build_groups(&sh->groups, p.offsets, p.batch, p.M, kF8M);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+
+  const int tiles_m = (p.M + kF8M - 1) / kF8M, tiles_n = (p.N + BN - 1) / BN;
+  const int64_t ntiles = GROUPED ? (int64_t)sh->groups.cum[p.batch] * tiles_n : (int64_t)tiles_m * tiles_n * p.batch;
+  F8Walk<GROUPED> walk;
+
+  // 384 threads start with 168 registers each: 128 x 56 + 256 x 224 = 384 x 168
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8FewRegs));
+  if (warp == 0) {
+    // ── TMA producer ──
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      int64_t issued = 0;
+      for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
+        const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
+        const int boxes = (c.rows + p.a_box - 1) / p.a_box;
+        const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!wait_phase(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts)) goto producer_done;
+          const uint32_t fb = smem_u32(&sh->full[s]);
+          mbar_expect_tx(fb, bytes);
+          const uint32_t dst = smem_u32(ring + s * Cfg::kStageBytes);
+          for (int r = 0; r < boxes; ++r)
+            tma_load_3d(dst + r * p.a_box * kF8K, &tmA, kb * kF8K, c.a_row + r * p.a_box, c.a_b, fb);
+          tma_load_3d(dst + Cfg::kAStage, &tmB, kb * kF8K, c.n0, c.b_b, fb);
+          ++issued;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    producer_done:
+      if (*abort)  // the loads in flight land before the CTA leaves
+        for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+    }
+  } else if (warp == 1) {
+    // ── MMA issuer ──
+    if (lane == 0) {
+      int s = 0, a = 0;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true;
+      for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          ok = wait_phase(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts) &&
+               wait_phase(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(a * BN);
+          const uint32_t a_addr = smem_u32(ring + s * Cfg::kStageBytes), b_addr = a_addr + Cfg::kAStage;
+          // both operands K-major: rows of 128 bytes, 8-row groups 1024 bytes apart; a
+          // K = 32 slice is 32 bytes further along the swizzled row
+#pragma unroll
+          for (int kk = 0; kk < kF8K / 32; ++kk)
+            tc_mma_f8(d, smem_desc(a_addr + kk * 32, 16, 1024), smem_desc(b_addr + kk * 32, 16, 1024), p.idesc, kk != 0);
+          tc_commit(smem_u32(&sh->empty[s]));
+          tc_commit(smem_u32(&sh->tfull[a]));
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++a == kAcc) {
+            a = 0;
+            aph ^= 1;
+          }
+        }
+      }
+      if (!ok) {  // the MMAs in flight finish before the tensor memory is freed
+        tc_commit(smem_u32(&sh->drain));
+        drain_phase(smem_u32(&sh->drain), 0);
+      }
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8ManyRegs));
+    // ── scaled sums: warp reads TMEM lanes 32 q .. +32, columns half * kCols .. ──
+    const int q = warp & 3, half = (warp - 4) / 4;
+    float(*sb_sh)[128] = sh->scale_b[warp - 4];
+    int a = 0;
+    uint32_t aph = 0;
+    bool ok = true;
+    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
+      const int row = q * 32 + lane, col = c.n0 + half * kCols;
+      const bool busy = q * 32 < c.rows, valid = row < c.rows;
+      const float* sa = p.sA + c.sa + (valid ? row : 0);
+      // square blocks: one scale for the warp's columns; row blocks: four columns a lane
+      const float* sb = ROWB ? p.sB + (int64_t)c.b_b * p.kblocks * p.N
+                             : p.sB + ((int64_t)c.b_b * p.nblocks + min(col / 128, p.nblocks - 1)) * p.kblocks;
+      unsigned long long acc[kCols / 2];
+#pragma unroll
+      for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
+      // A's scales (times B's, square blocks) four K blocks ahead
+      float cur[4], na[4], nb[4];
+      float rb[ROWB ? 4 : 1];
+      auto fetch = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = kb + j < p.kblocks && busy;
+          na[j] = in ? __ldg(sa + (int64_t)(kb + j) * p.M) : 0.0f;
+          if (!ROWB) nb[j] = in ? __ldg(sb + kb + j) : 0.0f;
+        }
+      };
+      auto fetch_rows = [&](int kb) {
+        if constexpr (ROWB) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int n = col + j * 32 + lane;
+            rb[j] = j * 32 < kCols && kb < p.kblocks && busy && n < p.N ? __ldg(sb + (int64_t)kb * p.N + n) : 0.0f;
+          }
+        }
+      };
+      fetch(0);
+      fetch_rows(0);
+      for (int kb0 = 0; ok && kb0 < p.kblocks; kb0 += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cur[j] = ROWB ? na[j] : na[j] * nb[j];
+        fetch(kb0 + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int kb = kb0 + j;
+          if (kb >= p.kblocks || !ok) break;
+          if constexpr (ROWB) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sb_sh[kb & 1][i * 32 + lane] = rb[i];
+            __syncwarp();
+            fetch_rows(kb + 1);
+          }
+          ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->tfull[a]), aph, abort, &g_fp8_timeouts));
+          if (!ok) break;
+          tc_fence_after();
+          if (busy) {
+            const unsigned long long s2 = pack2(cur[j], cur[j]);
+            const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half * kCols);
+#pragma unroll
+            for (int ch = 0; ch < kCols / 32; ++ch) {
+              uint32_t r[32];
+              tmem_ld32(base + ch * 32, r);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                unsigned long long s = s2;
+                if constexpr (ROWB) {
+                  const float2 b = *reinterpret_cast<const float2*>(&sb_sh[kb & 1][ch * 32 + 2 * i]);
+                  s = mul2(s2, pack2(b.x, b.y));
+                }
+                acc[ch * 16 + i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s, acc[ch * 16 + i]);
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+          if (++a == kAcc) {
+            a = 0;
+            aph ^= 1;
+          }
+        }
+      }
+      if (ok && valid && col < p.N) store_row<OUT, kCols>(p, c.crow + row, col, acc);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
+}
+
+// ── host side ───────────────────────────────────────────────────────────────
+static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Codes as bytes: {K, rows, slices}, rows K rounded up to 16 bytes apart, a box of
+// 128 bytes x box_rows, 128-byte swizzle, zeros outside.
+static mtl_status make_code_map(CUtensorMap* map, const void* base, int64_t K, int64_t rows, int64_t slices, int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return fail(MTL_ERR_CUDA, "gemm_fp8: cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)slices};
+  cuuint64_t strides[2] = {(cuuint64_t)up16(K), (cuuint64_t)(up16(K) * rows)};
+  cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MTL_ERR_ARGUMENT, "gemm_fp8: tensor map rejected (CUresult %d)", (int)r);
+  return MTL_OK;
+}
+
+cudaError_t fp8_set_wait_limit(unsigned long long ns) { return set_wait_limit_this_file(ns); }
+int fp8_timeouts(bool reset) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_fp8_timeouts, sizeof v) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (reset && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_fp8_timeouts, &zero, sizeof zero);
+  }
+  return v;
+}
+
+template <int BN, bool GROUPED, bool ROWB, typename OUT>
+static cudaError_t fp8_launch(const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p, int64_t tiles, int sms,
+                              int device, cudaStream_t s) {
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(gemm_fp8_kernel<BN, GROUPED, ROWB, OUT>, f8_smem<BN>(), device, &done);
+  if (e != cudaSuccess) return e;
+  // the register split draws on what the block starts with: with less it would wait for good
+  static const int regs = [] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, gemm_fp8_kernel<BN, GROUPED, ROWB, OUT>) == cudaSuccess ? at.numRegs : 0;
+  }();
+  if (regs * kF8Threads < 128 * kF8FewRegs + 256 * kF8ManyRegs) return cudaErrorLaunchOutOfResources;
+  const int grid = (int)std::min<int64_t>(tiles, sms);
+  gemm_fp8_kernel<BN, GROUPED, ROWB, OUT><<<grid, kF8Threads, f8_smem<BN>(), s>>>(ta, tb, p);
+  return cudaGetLastError();
+}
+template <int BN, bool GROUPED>
+static cudaError_t fp8_launch_by(bool rowb, bool bf16, const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p,
+                                 int64_t tiles, int sms, int device, cudaStream_t s) {
+  if constexpr (!GROUPED) {
+    if (rowb)
+      return bf16 ? fp8_launch<BN, GROUPED, true, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
+                  : fp8_launch<BN, GROUPED, true, float>(ta, tb, p, tiles, sms, device, s);
+  }
+  return bf16 ? fp8_launch<BN, GROUPED, false, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
+              : fp8_launch<BN, GROUPED, false, float>(ta, tb, p, tiles, sms, device, s);
+}
+
+// What gemm_fp8 and gemm_grouped_fp8 check alike. `rows`: rows of A and C over the
+// whole launch; `slices`: products or experts.
+static mtl_status fp8_check_common(const char* who, const LaunchArgs& la, const uint64_t* bytes, int64_t batch, int64_t M,
+                                   int64_t N, int64_t K, int64_t rows, int bblock, int fa, int fb, int out) {
+  if (la.ndim != 1) return fail(MTL_ERR_ARGUMENT, "%s: ndrange must be one-dimensional", who);
+  if (M < 0 || N < 0 || K < 0) return fail(MTL_ERR_ARGUMENT, "%s: negative dimension", who);
+  if (bblock != 1 && bblock != 128)
+    return fail(MTL_ERR_ARGUMENT, "%s: B's scales cover 1 or 128 rows each, got %d", who, bblock);
+  if ((fa | fb | out) & ~1)
+    return fail(MTL_ERR_ARGUMENT, "%s: formats are 0 (e4m3) or 1 (e5m2), the output 0 (fp32) or 1 (bf16), got %d, %d, %d", who, fa, fb, out);
+  const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
+  const uint64_t need[5] = {(uint64_t)(rows * N * (out ? 2 : 4)), (uint64_t)(rows * up16(K)), (uint64_t)(kb * rows * 4),
+                            (uint64_t)(batch * N * up16(K)), (uint64_t)(batch * kb * (bblock == 1 ? N : nb) * 4)};
+  const char* what[5] = {"C", "A", "A's scales", "B", "B's scales"};
+  const unsigned align[5] = {out ? 1u : 3u, 15, 3, 15, 3};
+  for (int i = 0; i < 5; ++i) {
+    if (bytes[i] && bytes[i] < need[i])
+      return fail(MTL_ERR_ARGUMENT, "%s: %s has %llu bytes, the launch touches %llu", who, what[i], (unsigned long long)bytes[i],
+                  (unsigned long long)need[i]);
+    if (la.a[i].ptr & align[i]) return fail(MTL_ERR_ARGUMENT, "%s: %s must be %u-byte aligned", who, what[i], align[i] + 1);
+  }
+  if (((M + 127) / 128 + kMaxGroups) * ((N + 63) / 64) > INT_MAX)
+    return fail(MTL_ERR_UNSUPPORTED, "%s: more than 2^31 tiles a product", who);
+  return MTL_OK;
+}
+
+// Arguments: C (B), A (B), sA (B), B (B), sB (B), M, N, K, rows per scale of B, format
+// of A, format of B, output type (i); ndrange = batch.
+mtl_status gemm_fp8_check(const LaunchArgs& la, const uint64_t* bytes) {
+  const int64_t batch = la.nd[0], M = la.a[5].i32;
+  if (batch > 65535) return fail(MTL_ERR_UNSUPPORTED, "gemm_fp8: batch above 65535");
+  return fp8_check_common("gemm_fp8", la, bytes, batch, M, la.a[6].i32, la.a[7].i32, batch * M, la.a[8].i32, la.a[9].i32,
+                          la.a[10].i32, la.a[11].i32);
+}
+
+// Arguments: Y (B), X (B), sX (B), W (B), sW (B), offsets (B, i32, groups + 1), T, N, K,
+// format of X, format of W, output type (i); ndrange = groups.
+mtl_status gemm_grouped_fp8_check(const LaunchArgs& la, const uint64_t* bytes) {
+  const int64_t groups = la.nd[0], T = la.a[6].i32;
+  if (groups > kMaxGroups) return fail(MTL_ERR_UNSUPPORTED, "gemm_grouped_fp8: more than %d groups", kMaxGroups);
+  if (mtl_status st = fp8_check_common("gemm_grouped_fp8", la, bytes, groups, T, la.a[7].i32, la.a[8].i32, T, 128, la.a[9].i32,
+                                       la.a[10].i32, la.a[11].i32))
+    return st;
+  if (la.a[8].i32 == 0) return fail(MTL_ERR_ARGUMENT, "gemm_grouped_fp8: K must be positive");
+  if ((bytes[5] && bytes[5] < (uint64_t)(groups + 1) * 4) || la.a[5].ptr % 4)
+    return fail(MTL_ERR_ARGUMENT, "gemm_grouped_fp8: the offsets are %lld 4-byte aligned Int32 values", (long long)groups + 1);
+  return MTL_OK;
+}
+
+// The widest tile whose tiles reach every SM; with fewer tiles than that, the
+// narrowest: tiles half as wide load A twice as often, but idle SMs cost more.
+static int fp8_tile_n(int64_t row_tiles, int64_t N, int sms) {
+  for (int bn : {256, 128})
+    if (row_tiles * ((N + bn - 1) / bn) >= sms) return bn;
+  return 64;
+}
+
+template <bool GROUPED>
+static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, int K, int batch, int bblock, int fa, int fb,
+                          int out, cudaStream_t s) {
+  F8Args p = {};
+  p.C = reinterpret_cast<void*>(la.a[0].ptr);
+  const void* A = reinterpret_cast<const void*>(la.a[1].ptr);
+  p.sA = reinterpret_cast<const float*>(la.a[2].ptr);
+  const void* B = reinterpret_cast<const void*>(la.a[3].ptr);
+  p.sB = reinterpret_cast<const float*>(la.a[4].ptr);
+  if (GROUPED) p.offsets = reinterpret_cast<const int*>(la.a[5].ptr);
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.batch = batch;
+  p.kblocks = (K + 127) / 128;
+  p.nblocks = (N + 127) / 128;
+  p.vec = la.a[0].ptr % 16 == 0 && (int64_t)N * (out ? 2 : 4) % 16 == 0;
+  // rows a product (dense) or a group on average decide how A is loaded and how
+  // many tiles there are; the groups' real sizes are on the device
+  const int64_t row_tiles = GROUPED ? std::max<int64_t>(batch, (M + kF8M - 1) / kF8M) : (int64_t)((M + kF8M - 1) / kF8M) * batch;
+  const int bn = fp8_tile_n(row_tiles, N, la.sm_count);
+  p.a_box = (GROUPED ? M / batch : M) >= kF8M ? kF8M : 32;
+  // kind::f8f6f4: fp32 accumulator (bit 4), formats at bits 7 and 10, N >> 3 at bit 17, M >> 4 at bit 24
+  p.idesc = (1u << 4) | ((uint32_t)fa << 7) | ((uint32_t)fb << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kF8M >> 4) << 24);
+  CUtensorMap ta, tb;
+  if (mtl_status st = make_code_map(&ta, A, K, M, GROUPED ? 1 : batch, p.a_box)) return st;
+  if (mtl_status st = make_code_map(&tb, B, K, N, batch, bn)) return st;
+  const int64_t tiles = (GROUPED ? (int64_t)batch + M / kF8M : row_tiles) * ((N + bn - 1) / bn);
+  const bool rowb = bblock == 1;
+  cudaError_t e = bn == 256   ? fp8_launch_by<256, GROUPED>(rowb, out, ta, tb, p, tiles, la.sm_count, la.device, s)
+                  : bn == 128 ? fp8_launch_by<128, GROUPED>(rowb, out, ta, tb, p, tiles, la.sm_count, la.device, s)
+                              : fp8_launch_by<64, GROUPED>(rowb, out, ta, tb, p, tiles, la.sm_count, la.device, s);
+  return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+mtl_status gemm_fp8_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
+  const int M = la.a[5].i32, N = la.a[6].i32, K = la.a[7].i32, out = la.a[11].i32;
+  const int64_t batch = la.nd[0];
+  cudaStream_t s = (cudaStream_t)stream;
+  if (batch == 0 || M == 0 || N == 0) return MTL_OK;
+  if (K == 0) {  // the empty sum
+    cudaError_t e = cudaMemsetAsync(reinterpret_cast<void*>(la.a[0].ptr), 0, (size_t)batch * M * N * (out ? 2 : 4), s);
+    return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "gemm_fp8: %s", cudaGetErrorString(e));
+  }
+  return fp8_run<false>("gemm_fp8", la, M, N, K, (int)batch, la.a[8].i32, la.a[9].i32, la.a[10].i32, out, s);
+}
+
+mtl_status gemm_grouped_fp8_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
+  const int T = la.a[6].i32, N = la.a[7].i32, K = la.a[8].i32;
+  const int64_t groups = la.nd[0];
+  if (groups == 0 || T == 0 || N == 0) return MTL_OK;
+  return fp8_run<true>("gemm_grouped_fp8", la, T, N, K, (int)groups, 128, la.a[9].i32, la.a[10].i32, la.a[11].i32,
+                       (cudaStream_t)stream);
+}
+
+}  // namespace mtl

@@ -1,0 +1,447 @@
+// Matrix products grouped by expert, bf16 in, fp32 sums, and their gradients. The
+// rows of a T-row matrix lie in groups, rows offsets[e] .. offsets[e + 1] going
+// with expert e's weights W[e] (K x N):
+//
+//   forward          Y[r]  = X[r] W[e]            (T x N)    gemm_grouped_bf16
+//   input gradient   dX[r] = dY[r] W[e]^T         (T x K)    gemm_grouped_dx_bf16
+//   weight gradient  dW[e] = X_e^T dY_e           (K x N)    gemm_grouped_dw_bf16
+//
+// Rows of no group keep what the output held; an empty group's dW is zeros.
+//
+// One persistent CTA per SM over tiles of RUNS x 128 rows by BN columns, the roles
+// and the ring of gemm_bf16: a TMA producer, a tcgen05.mma issuer, four epilogue
+// warps. No operand is transposed in memory: the forward product reads W N-major
+// (as it lies) and the input gradient reads the same memory K-major; the weight
+// gradient reads both X and dY "MN-major", a token a row of 128 bytes. The groups
+// start at any row, which TMA allows (only the inner coordinate is aligned).
+//
+// The weight gradient's last K block holds rows of the next group (or past T): the
+// issuer's warp zeroes them in shared memory in both operands, up to the next
+// multiple of 16, and issues only the MMAs (K = 16) that hold rows of the group. So
+// what other groups' rows hold, infinities or NaN, cannot reach the sums.
+//
+// Rows of a partial tile are loaded in boxes of 32 where groups are small, so that a
+// group of two rows costs 4 KiB of A a K block and the weights are what is read.
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "../mtl_internal.hpp"
+#include "tc_groups.cuh"
+
+namespace mtl {
+
+enum { kFwd = 0, kDx = 1, kDw = 2 };
+constexpr int kGrThreads = 192, kGrM = 128, kGrK = 64;
+
+template <int RUNS, int BN>
+struct GrCfg {
+  static constexpr uint32_t kAStage = kGrM * kGrK * 2, kBStage = kGrK * BN * 2;
+  static constexpr uint32_t kStageBytes = RUNS * kAStage + kBStage;
+  static constexpr int kStages = (int)(196608 / kStageBytes);
+  static constexpr int kAcc = RUNS * BN >= 512 ? 1 : 2;  // accumulator sets
+  static constexpr uint32_t kTmemCols = kAcc * RUNS * BN;
+  static constexpr int kTileM = RUNS * kGrM;
+};
+struct GrShared {
+  uint64_t full[8], empty[8], tfull[2], tempty[2], drain;
+  uint32_t tmem;
+  int abort;
+  GroupTable groups;
+};
+template <int RUNS, int BN>
+constexpr int gr_smem() {
+  return GrCfg<RUNS, BN>::kStages * (int)GrCfg<RUNS, BN>::kStageBytes + (int)sizeof(GrShared) + 1024;
+}
+
+struct GrArgs {
+  void* out;
+  const int* offsets;
+  int T, cols, depth;  // rows of the row matrices; columns of the output; contraction (forward, dX)
+  int out_rows;        // rows of dW[e]
+  int groups;
+  int a_box;  // rows per TMA box of A (forward, dX)
+  int vec;    // rows of the output start on 16 bytes
+};
+
+__device__ int g_grouped_timeouts;
+
+struct GrTile {
+  int e, m0, n0, rows;  // rows: valid output rows from m0 on
+  int row0, depth;      // forward, dX: first row of A; dW: the group's first row and its row count
+  int64_t crow;
+};
+template <int FORM, int RUNS, int BN>
+struct GrWalk {
+  GroupWalk g;
+  __device__ __forceinline__ GrTile find(const GrArgs& p, const GroupTable* groups, int64_t t, int tiles_m, int tiles_n) {
+    constexpr int tm = RUNS * kGrM;
+    GrTile c;
+    if (FORM == kDw) {
+      const int per = tiles_m * tiles_n, in = (int)(t % per);
+      c.e = (int)(t / per);
+      c.m0 = in % tiles_m * tm;
+      c.n0 = in / tiles_m * BN;
+      c.rows = p.out_rows - c.m0;
+      c.row0 = groups->lo[c.e];
+      c.depth = groups->hi[c.e] - c.row0;
+      c.crow = (int64_t)c.e * p.out_rows + c.m0;
+    } else {
+      g.find(groups, (int)t, tiles_n, tm, BN, &c.row0, &c.rows, &c.n0);
+      c.e = g.e;
+      c.m0 = 0;
+      c.depth = p.depth;
+      c.crow = c.row0;
+    }
+    c.rows = min(c.rows, tm);
+    return c;
+  }
+};
+
+// 32 neighbouring sums of one row.
+template <typename OUT>
+__device__ __forceinline__ void store32(const GrArgs& p, OUT* crow, int col, const uint32_t (&r)[32]) {
+  OUT* c = crow + col;
+  if constexpr (sizeof(OUT) == 4) {
+    if (p.vec && col + 32 <= p.cols) {
+#pragma unroll
+      for (int v = 0; v < 8; ++v)
+        reinterpret_cast<float4*>(c)[v] = make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
+                                                      __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3]));
+    } else {
+#pragma unroll
+      for (int v = 0; v < 32; ++v)
+        if (col + v < p.cols) c[v] = __uint_as_float(r[v]);
+    }
+  } else {
+    __nv_bfloat162 b[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) b[v] = __floats2bfloat162_rn(__uint_as_float(r[2 * v]), __uint_as_float(r[2 * v + 1]));
+    if (p.vec && col + 32 <= p.cols) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(c)[v] = reinterpret_cast<const uint4*>(b)[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < 32; ++v)
+        if (col + v < p.cols) c[v] = v & 1 ? b[v / 2].y : b[v / 2].x;
+    }
+  }
+}
+
+template <int FORM, int RUNS, int BN, typename OUT>
+__global__ void __launch_bounds__(kGrThreads, 1)
+    gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
+  using Cfg = GrCfg<RUNS, BN>;
+  constexpr int kStages = Cfg::kStages, kAcc = Cfg::kAcc;
+  constexpr uint32_t kIdesc = idesc_bf16_f32(kGrM, BN, FORM == kDw, FORM != kDx);
+  extern __shared__ unsigned char gr_raw[];
+  unsigned char* ring =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gr_raw) + 1023) & ~uintptr_t(1023));
+  GrShared* sh = reinterpret_cast<GrShared*>(ring + kStages * Cfg::kStageBytes);
+  volatile int* abort = &sh->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sh->full[s]), 1);
+      mbar_init(smem_u32(&sh->empty[s]), 1);
+    }
+    for (int a = 0; a < kAcc; ++a) {
+      mbar_init(smem_u32(&sh->tfull[a]), 1);
+      mbar_init(smem_u32(&sh->tempty[a]), 4);
+    }
+    mbar_init(smem_u32(&sh->drain), 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)),
+                 "r"(Cfg::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  build_groups(&sh->groups, p.offsets, p.groups, p.T, Cfg::kTileM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+
+  const int tiles_m = FORM == kDw ? (p.out_rows + Cfg::kTileM - 1) / Cfg::kTileM : 0, tiles_n = (p.cols + BN - 1) / BN;
+  const int64_t ntiles =
+      FORM == kDw ? (int64_t)tiles_m * tiles_n * p.groups : (int64_t)sh->groups.cum[p.groups] * tiles_n;
+  GrWalk<FORM, RUNS, BN> walk;
+
+  if (warp == 0) {
+    // ── TMA producer ──
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      int64_t issued = 0;
+      for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
+        const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+        // boxes that would lie wholly past the output's rows or columns are not loaded:
+        // what stale shared memory they leave feeds outputs that are not stored
+        const int a_boxes = FORM == kDw ? (c.rows + 63) / 64 : (c.rows + p.a_box - 1) / p.a_box;
+        const int b_boxes = FORM == kDx ? 1 : min(BN / 64, (p.cols - c.n0 + 63) / 64);
+        const uint32_t bytes = (uint32_t)(a_boxes * (FORM == kDw ? kGrK * 128 : p.a_box * 128)) +
+                               (FORM == kDx ? Cfg::kBStage : (uint32_t)(b_boxes * kGrK * 128));
+        const int kblocks = (c.depth + kGrK - 1) / kGrK;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!wait_phase(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts)) goto producer_done;
+          const uint32_t fb = smem_u32(&sh->full[s]);
+          mbar_expect_tx(fb, bytes);
+          const uint32_t a_dst = smem_u32(ring + s * Cfg::kStageBytes), b_dst = a_dst + RUNS * Cfg::kAStage;
+          if (FORM == kDw) {
+            for (int b = 0; b < a_boxes; ++b)
+              tma_load_3d(a_dst + b * (kGrK * 128), &tmA, c.m0 + b * 64, c.row0 + kb * kGrK, 0, fb);
+            for (int b = 0; b < b_boxes; ++b)
+              tma_load_3d(b_dst + b * (kGrK * 128), &tmB, c.n0 + b * 64, c.row0 + kb * kGrK, 0, fb);
+          } else {
+            for (int b = 0; b < a_boxes; ++b)
+              tma_load_3d(a_dst + b * p.a_box * 128, &tmA, kb * kGrK, c.row0 + b * p.a_box, 0, fb);
+            if (FORM == kDx) {
+              tma_load_3d(b_dst, &tmB, kb * kGrK, c.n0, c.e, fb);
+            } else {
+              for (int b = 0; b < b_boxes; ++b)
+                tma_load_3d(b_dst + b * (kGrK * 128), &tmB, c.n0 + b * 64, kb * kGrK, c.e, fb);
+            }
+          }
+          ++issued;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    producer_done:
+      if (*abort)  // the loads in flight land before the CTA leaves
+        for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+    }
+  } else if (warp == 1) {
+    // ── MMA issuer (the whole warp waits; one lane issues) ──
+    int s = 0, i = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      const int kblocks = (c.depth + kGrK - 1) / kGrK;
+      if (kblocks == 0) continue;
+      const int a = i % kAcc, runs = RUNS == 1 ? 1 : (c.rows + kGrM - 1) / kGrM;
+      ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->tempty[a]), ((i / kAcc) & 1) ^ 1, abort, &g_grouped_timeouts));
+      ++i;
+      const uint32_t d = tmem + (uint32_t)(a * RUNS * BN);
+      for (int kb = 0; ok && kb < kblocks; ++kb) {
+        ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts));
+        if (!ok) break;
+        const uint32_t a_addr = smem_u32(ring + s * Cfg::kStageBytes), b_addr = a_addr + RUNS * Cfg::kAStage;
+        int steps = kGrK / 16;
+        if (FORM == kDw && c.depth - kb * kGrK < kGrK) {
+          const int live = c.depth - kb * kGrK, end = (live + 15) / 16 * 16;
+          steps = end / 16;
+          const int chunks = (RUNS * kGrM + BN) / 64, words = (end - live) * 8;  // 16-byte words a chunk
+          unsigned char* stage = ring + s * Cfg::kStageBytes;
+          for (int w = lane; w < chunks * words; w += 32)
+            *reinterpret_cast<uint4*>(stage + (w / words) * (kGrK * 128) + live * 128 + (w % words) * 16) =
+                make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          for (int kk = 0; kk < steps; ++kk) {
+            // MN-major: 64-value chunks kGrK * 128 bytes apart, a K = 16 slice is 16 rows
+            // of 128 bytes; K-major: a slice is 32 bytes further along the swizzled row
+            const uint64_t bd = FORM == kDx ? smem_desc(b_addr + kk * 32, 16, 1024)
+                                            : smem_desc(b_addr + kk * 2048, kGrK * 128, 1024);
+#pragma unroll
+            for (int r = 0; r < RUNS; ++r) {
+              if (r >= runs) break;
+              const uint32_t ar = a_addr + r * Cfg::kAStage;
+              const uint64_t ad = FORM == kDw ? smem_desc(ar + kk * 2048, kGrK * 128, 1024) : smem_desc(ar + kk * 32, 16, 1024);
+              tc_mma(d + (uint32_t)(r * BN), ad, bd, kIdesc, (kb | kk) != 0);
+            }
+          }
+          tc_commit(smem_u32(&sh->empty[s]));
+          if (kb + 1 == kblocks) tc_commit(smem_u32(&sh->tfull[a]));
+        }
+        __syncwarp();
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
+      tc_commit(smem_u32(&sh->drain));
+      drain_phase(smem_u32(&sh->drain), 0);
+    }
+  } else {
+    // ── epilogue: warps 2..5 read TMEM lanes 32 (warp % 4) .. +32 ──
+    const int q = warp & 3;
+    int i = 0;
+    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
+      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      const bool empty = c.depth == 0;
+      const int a = i % kAcc;
+      if (!empty) {
+        if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh->tfull[a]), (i / kAcc) & 1, abort, &g_grouped_timeouts))) break;
+        tc_fence_after();
+        ++i;
+      }
+#pragma unroll 1
+      for (int run = 0; run < RUNS; ++run) {
+        const int row = run * kGrM + q * 32 + lane;
+        if (run * kGrM + q * 32 >= c.rows) break;  // uniform in the warp
+        OUT* crow = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+        const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * RUNS + run) * BN);
+#pragma unroll 1
+        for (int ch = 0; ch < BN / 32; ++ch) {
+          const int col = c.n0 + ch * 32;
+          if (col >= p.cols) break;
+          uint32_t r[32];
+          if (empty) {
+#pragma unroll
+            for (int v = 0; v < 32; ++v) r[v] = 0;
+          } else {
+            tmem_ld32(tbase + ch * 32, r);
+          }
+          if (row < c.rows) store32<OUT>(p, crow, col, r);
+        }
+      }
+      if (!empty) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
+}
+
+// ── host side ───────────────────────────────────────────────────────────────
+cudaError_t grouped_set_wait_limit(unsigned long long ns) { return set_wait_limit_this_file(ns); }
+int grouped_timeouts(bool reset) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_grouped_timeouts, sizeof v) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (reset && v) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_grouped_timeouts, &zero, sizeof zero);
+  }
+  return v;
+}
+
+static const char* const kGrName[3] = {"gemm_grouped_bf16", "gemm_grouped_dx_bf16", "gemm_grouped_dw_bf16"};
+
+// Arguments: out (B), two operands (B): X, W / dY, W / X, dY, offsets (B, i32, groups +
+// 1), T, N, K, output type (i); ndrange = groups.
+template <int FORM>
+static mtl_status gr_check(const LaunchArgs& la, const uint64_t* bytes) {
+  const char* who = kGrName[FORM];
+  if (la.ndim != 1) return fail(MTL_ERR_ARGUMENT, "%s: ndrange must be one-dimensional (the group count)", who);
+  const int64_t E = la.nd[0], T = la.a[4].i32, N = la.a[5].i32, K = la.a[6].i32;
+  const int out = la.a[7].i32;
+  if (T < 0 || N < 0 || K < 0) return fail(MTL_ERR_ARGUMENT, "%s: negative dimension", who);
+  if (N % 8 || K % 8)
+    return fail(MTL_ERR_UNSUPPORTED, "%s: N and K must be multiples of 8 (16-byte rows), got N=%lld K=%lld", who, (long long)N,
+                (long long)K);
+  if (FORM != kDw && (FORM == kFwd ? K : N) == 0) return fail(MTL_ERR_ARGUMENT, "%s: the contraction must be positive", who);
+  if (out != 0 && out != 1) return fail(MTL_ERR_ARGUMENT, "%s: the output type is 0 (fp32) or 1 (bf16), got %d", who, out);
+  if (E > kMaxGroups) return fail(MTL_ERR_UNSUPPORTED, "%s: more than %d groups", who, kMaxGroups);
+  const int64_t w = E * K * N, x = T * K, y = T * N, wide = out ? 2 : 4;
+  const uint64_t need[4] = {(uint64_t)((FORM == kFwd ? y : FORM == kDx ? x : w) * wide),
+                            (uint64_t)((FORM == kDx ? y : x) * 2), (uint64_t)((FORM == kDw ? y : w) * 2),
+                            (uint64_t)(E + 1) * 4};
+  const char* what[3][4] = {{"Y", "X", "W", "the offsets"}, {"dX", "dY", "W", "the offsets"}, {"dW", "X", "dY", "the offsets"}};
+  const unsigned align[4] = {out ? 1u : 3u, 15, 15, 3};
+  for (int i = 0; i < 4; ++i) {
+    if (bytes[i] && bytes[i] < need[i])
+      return fail(MTL_ERR_ARGUMENT, "%s: %s: %llu bytes, the launch touches %llu", who, what[FORM][i], (unsigned long long)bytes[i],
+                  (unsigned long long)need[i]);
+    if (la.a[i].ptr & align[i])
+      return fail(MTL_ERR_ARGUMENT, "%s: %s must be %u-byte aligned", who, what[FORM][i], align[i] + 1);
+  }
+  const int64_t rows = FORM == kDw ? (K + 127) / 128 * E : (T + 127) / 128 + E, cols = FORM == kDx ? K : N;
+  if (rows * ((cols + 127) / 128) > INT_MAX) return fail(MTL_ERR_UNSUPPORTED, "%s: more than 2^31 tiles", who);
+  return MTL_OK;
+}
+mtl_status gemm_grouped_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kFwd>(la, bytes); }
+mtl_status gemm_grouped_dx_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kDx>(la, bytes); }
+mtl_status gemm_grouped_dw_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kDw>(la, bytes); }
+
+template <int FORM, int RUNS, int BN, typename OUT>
+static cudaError_t gr_launch(const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
+                             const LaunchArgs& la, cudaStream_t s) {
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(gemm_grouped_kernel<FORM, RUNS, BN, OUT>, gr_smem<RUNS, BN>(), la.device, &done);
+  if (e != cudaSuccess) return e;
+  const int grid = (int)std::min<int64_t>(tiles, la.sm_count);
+  gemm_grouped_kernel<FORM, RUNS, BN, OUT><<<grid, kGrThreads, gr_smem<RUNS, BN>(), s>>>(ta, tb, p);
+  return cudaGetLastError();
+}
+
+template <int FORM>
+static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
+  const char* who = kGrName[FORM];
+  const int T = la.a[4].i32, N = la.a[5].i32, K = la.a[6].i32, out = la.a[7].i32;
+  const int E = (int)la.nd[0];
+  const int cols = FORM == kDx ? K : N;
+  if (E == 0 || cols == 0 || (FORM == kDw ? K : T) == 0) return MTL_OK;
+  if (FORM == kDw && T == 0) {  // every group is empty
+    cudaError_t e = cudaMemsetAsync(reinterpret_cast<void*>(la.a[0].ptr), 0, (size_t)E * K * N * (out ? 2 : 4), s);
+    return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  }
+  GrArgs p = {};
+  p.out = reinterpret_cast<void*>(la.a[0].ptr);
+  p.offsets = reinterpret_cast<const int*>(la.a[3].ptr);
+  p.T = T;
+  p.cols = cols;
+  p.depth = FORM == kFwd ? K : N;
+  p.out_rows = K;
+  p.groups = E;
+  p.vec = la.a[0].ptr % 16 == 0;  // N and K are multiples of 8
+  const bool wide = FORM == kDw ? false : T / E > kGrM;  // two runs of 128 rows a tile
+  p.a_box = T / E >= kGrM ? kGrM : 32;
+  const void *A = reinterpret_cast<const void*>(la.a[1].ptr), *B = reinterpret_cast<const void*>(la.a[2].ptr);
+  const int64_t row_tiles = FORM == kDw ? (int64_t)E * ((K + 127) / 128) : std::max<int64_t>(E, (T + 127) / 128);
+  const bool narrow = !wide && row_tiles * ((cols + 255) / 256) < la.sm_count;
+  const int bn = narrow ? 128 : 256;
+  CUtensorMap ta, tb;
+  if (mtl_status st = make_bf16_map(&ta, A, FORM == kDx ? N : K, T, 1, FORM == kDw ? kGrK : p.a_box)) return st;
+  if (FORM == kDw) {
+    if (mtl_status st = make_bf16_map(&tb, B, N, T, 1, kGrK)) return st;
+  } else {
+    if (mtl_status st = make_bf16_map(&tb, B, N, K, E, FORM == kDx ? bn : kGrK)) return st;
+  }
+  const int64_t tile_m = wide ? 256 : 128;
+  const int64_t tiles = (FORM == kDw ? (int64_t)E * ((K + tile_m - 1) / tile_m) : T / tile_m + E) * ((cols + bn - 1) / bn);
+  cudaError_t e;
+  if (wide) {
+    if constexpr (FORM != kDw)
+      e = out ? gr_launch<FORM, 2, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 2, 256, float>(ta, tb, p, tiles, la, s);
+    else
+      e = cudaErrorInvalidValue;
+  } else if (narrow) {
+    e = out ? gr_launch<FORM, 1, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 1, 128, float>(ta, tb, p, tiles, la, s);
+  } else {
+    e = out ? gr_launch<FORM, 1, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 1, 256, float>(ta, tb, p, tiles, la, s);
+  }
+  return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+mtl_status gemm_grouped_run(const LaunchArgs& la, void*, uint64_t, void* stream) { return gr_run<kFwd>(la, (cudaStream_t)stream); }
+mtl_status gemm_grouped_dx_run(const LaunchArgs& la, void*, uint64_t, void* stream) { return gr_run<kDx>(la, (cudaStream_t)stream); }
+mtl_status gemm_grouped_dw_run(const LaunchArgs& la, void*, uint64_t, void* stream) { return gr_run<kDw>(la, (cudaStream_t)stream); }
+
+}  // namespace mtl

@@ -1,0 +1,373 @@
+// Values to 8-bit floating point in blocks of 128 with one scale a block, the
+// operands of gemm_fp8 and gemm_grouped_fp8.
+//
+// With a the largest magnitude in the block, but at least 2^-96, and L the
+// format's largest value (448 for e4m3, 57344 for e5m2):
+//
+//   scale = fl32(a / L)    r = fl32(L / a)    code = round8(fl32(x * r))
+//
+// rounded to the nearest, ties to even; |x * r| exceeds L by one unit of fp32 at
+// most, which rounds back to L. With pow2 the scale is the smallest power of two
+// s with a <= L * s and r = 1 / s, so both products are exact. The floor keeps
+// r finite and gives a block of zeros a scale that can be divided by. A NaN in
+// a block makes its scale and all its codes NaN (the largest magnitude is found
+// on the bits, where NaN is above infinity); an infinity makes the scale
+// infinite, itself NaN and the finite values 0.
+//
+// A block is 1 x 128 along a row or a 128 x 128 square. The transposed outputs
+// are what the input's transpose would give: for a row block, columns in runs of
+// 128 rows. Rows of codes start every 16 bytes rounded up (TMA's row stride) and
+// the bytes between are zeros.
+//
+// Both kernels are bound by HBM: a value is read once, kept in registers, and
+// written once per output. See the figures at each kernel.
+
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "../mtl_internal.hpp"
+
+namespace mtl {
+
+struct QuantArgs {
+  uint8_t* q;         // R rows of Cp codes, or null
+  float* s;
+  uint8_t* qt;        // C rows of Rp codes, or null
+  float* st;
+  const void* x;
+  const int* rows_of;  // source row of each row, or null
+  int64_t R, C, Cp, Rp;
+  int64_t rb, cb;      // blocks of 128 rows / columns
+  int xrows;           // rows of x that rows_of may name
+  int e5m2, pow2, vec;  // vec: every row of x starts on 16 bytes
+};
+
+// ── values ──────────────────────────────────────────────────────────────────
+struct Row8 {
+  float v[8];
+};
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
+
+// Eight neighbouring values as loaded, zeros from column C on.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<uint16_t> {
+  uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const uint16_t* row, int64_t c, int64_t C, int vec) {
+    if (vec && c + 8 <= C) {
+      u = __ldg(reinterpret_cast<const uint4*>(row + c));
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = c + i < C ? row[c + i] : 0;
+      u = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+  }
+  __device__ __forceinline__ Row8 get() const {
+    return Row8{{bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y), bf16_lo(u.z), bf16_hi(u.z), bf16_lo(u.w),
+                 bf16_hi(u.w)}};
+  }
+};
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void zero() { a = b = make_float4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const float* row, int64_t c, int64_t C, int vec) {
+    if (vec && c + 8 <= C) {
+      a = __ldg(reinterpret_cast<const float4*>(row + c));
+      b = __ldg(reinterpret_cast<const float4*>(row + c + 4));
+    } else {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = c + i < C ? row[c + i] : 0.0f;
+      a = make_float4(w[0], w[1], w[2], w[3]);
+      b = make_float4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  __device__ __forceinline__ Row8 get() const { return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
+};
+
+// The input row behind output row r: null where it is past the end or rows_of
+// names none (its values are then zeros).
+template <typename T>
+__device__ __forceinline__ const T* source_row(const QuantArgs& a, int64_t batch, int64_t r) {
+  if (r >= a.R) return nullptr;
+  const T* x = static_cast<const T*>(a.x);
+  if (a.rows_of) {
+    const int from = a.rows_of[r];
+    return from >= 0 && from < a.xrows ? x + (int64_t)from * a.C : nullptr;
+  }
+  return x + (batch * a.R + r) * a.C;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct Scale {
+  float s, r;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t bits, int e5m2, int pow2) {
+  bits = max(bits, (uint32_t)(127 - 96) << 23);
+  const float a = __uint_as_float(bits), top = e5m2 ? 57344.0f : 448.0f;
+  if (pow2 && bits < 0x7f800000u) {
+    // a = m 2^e, m in [1, 2), and L = 1.75 2^8 or 1.75 2^15
+    const int j = (int)(bits >> 23) - 127 - (e5m2 ? 15 : 8) + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return Scale{__uint_as_float((uint32_t)(127 + j) << 23), __uint_as_float((uint32_t)(127 - j) << 23)};
+  }
+  return Scale{__fdiv_rn(a, top), __fdiv_rn(top, a)};
+}
+
+__device__ __forceinline__ uint32_t codes2(float lo, float hi, int e5m2) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+}
+__device__ __forceinline__ uint2 codes8(const Row8& v, const float (&r)[8], int e5m2) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c[i] = codes2(__fmul_rn(v.v[2 * i], r[2 * i]), __fmul_rn(v.v[2 * i + 1], r[2 * i + 1]), e5m2);
+  return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+}
+__device__ __forceinline__ uint2 codes8(const Row8& v, float r, int e5m2) {
+  const float rs[8] = {r, r, r, r, r, r, r, r};
+  return codes8(v, rs, e5m2);
+}
+
+// ── row blocks, no transpose ────────────────────────────────────────────────
+// Sixteen lanes a block of 128 (eight values each), a CTA sixteen rows of U
+// neighbouring blocks: the U loads of a thread are in flight together, and the
+// scales of sixteen rows leave as one 64-byte run.
+constexpr int kQuantThreads = 256;
+template <typename T, int U>
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs a, int64_t row_tiles, int64_t col_tiles) {
+  const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4;
+  const int64_t t = blockIdx.x;
+  const int64_t batch = t / (row_tiles * col_tiles), in = t % (row_tiles * col_tiles);
+  const int64_t r = in / col_tiles * 16 + sub, kb0 = in % col_tiles * U;
+  const T* row = source_row<T>(a, batch, r);
+  Raw8<T> raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    raw[u].zero();
+    if (row) raw[u].load(row, (kb0 + u) * 128 + lane16 * 8, a.C, a.vec);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Row8 v = raw[u].get();
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, magnitude(v.v[i]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const Scale sc = scale_of(m, a.e5m2, a.pow2);
+    const int64_t kb = kb0 + u, c = kb * 128 + lane16 * 8;
+    if (r < a.R && c < a.Cp)
+      *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8(v, sc.r, a.e5m2);
+    if (r < a.R && kb < a.cb && lane16 == 0) a.s[(batch * a.cb + kb) * a.R + r] = sc.s;
+  }
+}
+
+// ── 128 x 128 tiles: square blocks, transposed outputs ──────────────────────
+// A thread holds an 8 x 8 patch (eight rows of eight columns), so it can pack
+// eight codes along a row and eight down a column. Row maxima meet over the
+// sixteen lanes of a row, column maxima over the CTA through shared memory. The
+// transposed codes go through a 16 KiB tile whose 8-byte chunks are placed by
+// chunk ^ (column / 8): the sixteen lanes that write one instruction's columns
+// hit all 32 banks, and so do the sixteen that read a transposed row.
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) quantize_tile_kernel(QuantArgs a, int square) {
+  __shared__ uint32_t colmax[8][128];
+  __shared__ uint2 turned[128 * 16];
+  __shared__ float inv[128];
+  __shared__ uint32_t tilemax[8];
+  const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4, warp = threadIdx.x >> 5;
+  const int64_t t = blockIdx.x;
+  const int64_t batch = t / (a.rb * a.cb), in = t % (a.rb * a.cb);
+  const int64_t rblk = in / a.cb, kb = in % a.cb;
+  const int64_t r0 = rblk * 128 + sub * 8, c = kb * 128 + lane16 * 8;
+  Raw8<T> raw[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const T* row = source_row<T>(a, batch, r0 + p);
+    raw[p].zero();
+    if (row) raw[p].load(row, c, a.C, a.vec);
+  }
+  uint32_t cm[8] = {0, 0, 0, 0, 0, 0, 0, 0}, rm[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const Row8 v = raw[p].get();
+    rm[p] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t m = magnitude(v.v[i]);
+      rm[p] = max(rm[p], m);
+      cm[i] = max(cm[i], m);
+    }
+  }
+  if (square) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) m = max(m, rm[p]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if ((threadIdx.x & 31) == 0) tilemax[warp] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, tilemax[w]);
+    const Scale sc = scale_of(m, a.e5m2, a.pow2);
+    if (threadIdx.x == 0) {
+      if (a.s) a.s[(batch * a.rb + rblk) * a.cb + kb] = sc.s;
+      if (a.st) a.st[(batch * a.cb + kb) * a.rb + rblk] = sc.s;
+    }
+    if (a.q) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        if (r0 + p < a.R && c < a.Cp)
+          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8(raw[p].get(), sc.r, a.e5m2);
+    }
+    if (!a.qt) return;
+    if (threadIdx.x < 128) inv[threadIdx.x] = sc.r;
+  } else {
+    if (a.q) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        uint32_t m = rm[p];
+#pragma unroll
+        for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const Scale sc = scale_of(m, a.e5m2, a.pow2);
+        const int64_t r = r0 + p;
+        if (r < a.R && c < a.Cp)
+          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8(raw[p].get(), sc.r, a.e5m2);
+        if (r < a.R && lane16 == 0) a.s[(batch * a.cb + kb) * a.R + r] = sc.s;
+      }
+    }
+    if (!a.qt) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t m = max(cm[i], __shfl_xor_sync(0xffffffffu, cm[i], 16));
+      if ((threadIdx.x & 31) < 16) colmax[warp][lane16 * 8 + i] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = max(m, colmax[w][threadIdx.x]);
+      const Scale sc = scale_of(m, a.e5m2, a.pow2);
+      inv[threadIdx.x] = sc.r;
+      const int64_t col = kb * 128 + threadIdx.x;
+      if (col < a.C) a.st[(batch * a.rb + rblk) * a.C + col] = sc.s;
+    }
+  }
+  __syncthreads();
+  // columns as rows: eight codes down each of the thread's eight columns
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    Row8 down;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) down.v[p] = raw[p].get().v[i];
+    turned[(lane16 * 8 + i) * 16 + (sub ^ lane16)] = codes8(down, inv[lane16 * 8 + i], a.e5m2);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int col = sub * 8 + i;  // sixteen lanes write one transposed row's 128 bytes
+    const int64_t at = rblk * 128 + lane16 * 8;
+    if (kb * 128 + col < a.C && at < a.Rp)
+      *reinterpret_cast<uint2*>(a.qt + (batch * a.C + kb * 128 + col) * a.Rp + at) = turned[col * 16 + (lane16 ^ sub)];
+  }
+}
+
+// ── host side ───────────────────────────────────────────────────────────────
+// Arguments: q (b), s (b), qt (b), st (b), x (B), rows_of (b, i32), R, C, xrows,
+// block, type (0 f32, 1 bf16), format (0 e4m3, 1 e5m2), pow2 (i); ndrange = batch.
+static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
+  if (la.ndim != 1) return fail(MTL_ERR_ARGUMENT, "quantize_fp8: ndrange must be one-dimensional (the batch count)");
+  const int64_t R = la.a[6].i32, C = la.a[7].i32, xrows = la.a[8].i32, batch = la.nd[0];
+  const int block = la.a[9].i32;
+  if (R < 0 || C < 0 || xrows < 0) return fail(MTL_ERR_ARGUMENT, "quantize_fp8: negative dimension");
+  if (block != 1 && block != 128)
+    return fail(MTL_ERR_ARGUMENT, "quantize_fp8: block must be 1 (1 x 128) or 128 (128 x 128), got %d", block);
+  for (int i = 10; i < 13; ++i)
+    if (la.a[i].i32 != 0 && la.a[i].i32 != 1)
+      return fail(MTL_ERR_ARGUMENT, "quantize_fp8: argument %d must be 0 or 1, got %d", i + 1, la.a[i].i32);
+  const bool gather = la.a[5].kind == MTL_ARG_PTR && la.a[5].ptr;
+  if (gather && batch > 1) return fail(MTL_ERR_UNSUPPORTED, "quantize_fp8: rows_of goes with a batch of one, got %lld", (long long)batch);
+  if (!gather && xrows != R)
+    return fail(MTL_ERR_ARGUMENT, "quantize_fp8: without rows_of the input has as many rows as the output: %lld, got %lld", (long long)R,
+                (long long)xrows);
+  const bool q = la.a[0].ptr, s = la.a[1].ptr, qt = la.a[2].ptr, st = la.a[3].ptr;
+  if (q != s || qt != st || (!q && !qt))
+    return fail(MTL_ERR_ARGUMENT, "quantize_fp8: give the codes and the scales of the row form, of the transposed form, or of both");
+  const int64_t rb = (R + 127) / 128, cb = (C + 127) / 128, per = la.a[10].i32 ? 2 : 4;
+  const int64_t scales = block == 128 ? rb * cb : 0;
+  const uint64_t need[6] = {(uint64_t)(batch * R * up(C, 16)), (uint64_t)(batch * 4 * (scales ? scales : cb * R)),
+                            (uint64_t)(batch * C * up(R, 16)), (uint64_t)(batch * 4 * (scales ? scales : rb * C)),
+                            (uint64_t)((gather ? 1 : batch) * xrows * C * per), (uint64_t)(R * 4)};
+  const char* what[6] = {"the codes", "the scales", "the transposed codes", "the transposed scales", "the input", "rows_of"};
+  const unsigned align[6] = {15, 3, 15, 3, la.a[10].i32 ? 1u : 3u, 3};
+  for (int i = 0; i < 6; ++i) {
+    if (!la.a[i].ptr) continue;
+    if (bytes[i] && bytes[i] < need[i])
+      return fail(MTL_ERR_ARGUMENT, "quantize_fp8: %s: %llu bytes, the launch touches %llu", what[i], (unsigned long long)bytes[i],
+                  (unsigned long long)need[i]);
+    if (la.a[i].ptr & align[i])
+      return fail(MTL_ERR_ARGUMENT, "quantize_fp8: %s must be %u-byte aligned", what[i], align[i] + 1);
+  }
+  if (batch * std::max<int64_t>(1, (R + 15) / 16) * std::max<int64_t>(1, cb) > INT_MAX)
+    return fail(MTL_ERR_UNSUPPORTED, "quantize_fp8: more than 2^31 tiles");
+  return MTL_OK;
+}
+
+mtl_status quantize_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
+  QuantArgs a = {};
+  a.q = reinterpret_cast<uint8_t*>(la.a[0].ptr);
+  a.s = reinterpret_cast<float*>(la.a[1].ptr);
+  a.qt = reinterpret_cast<uint8_t*>(la.a[2].ptr);
+  a.st = reinterpret_cast<float*>(la.a[3].ptr);
+  a.x = reinterpret_cast<const void*>(la.a[4].ptr);
+  a.rows_of = reinterpret_cast<const int*>(la.a[5].ptr);
+  a.R = la.a[6].i32;
+  a.C = la.a[7].i32;
+  a.xrows = la.a[8].i32;
+  a.Cp = up(a.C, 16);
+  a.Rp = up(a.R, 16);
+  a.rb = (a.R + 127) / 128;
+  a.cb = (a.C + 127) / 128;
+  const int block = la.a[9].i32, bf16 = la.a[10].i32;
+  a.e5m2 = la.a[11].i32;
+  a.pow2 = la.a[12].i32;
+  a.vec = la.a[4].ptr % 16 == 0 && a.C % (bf16 ? 8 : 4) == 0;
+  const int64_t batch = la.nd[0];
+  cudaStream_t st = (cudaStream_t)stream;
+  if (batch == 0 || a.R == 0 || a.C == 0) return MTL_OK;
+  if (block == 1 && !a.qt) {
+    const int64_t row_tiles = (a.R + 15) / 16;
+    const bool four = batch * row_tiles * a.cb >= 8 * (int64_t)la.sm_count;
+    const int64_t col_tiles = four ? (a.cb + 3) / 4 : a.cb;
+    const unsigned grid = (unsigned)(batch * row_tiles * col_tiles);
+    if (bf16)
+      four ? quantize_rows_kernel<uint16_t, 4><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles)
+           : quantize_rows_kernel<uint16_t, 1><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles);
+    else
+      four ? quantize_rows_kernel<float, 4><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles)
+           : quantize_rows_kernel<float, 1><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles);
+  } else {
+    const unsigned grid = (unsigned)(batch * a.rb * a.cb);
+    if (bf16)
+      quantize_tile_kernel<uint16_t><<<grid, kQuantThreads, 0, st>>>(a, block == 128);
+    else
+      quantize_tile_kernel<float><<<grid, kQuantThreads, 0, st>>>(a, block == 128);
+  }
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "quantize_fp8: %s", cudaGetErrorString(e));
+}
+
+}  // namespace mtl

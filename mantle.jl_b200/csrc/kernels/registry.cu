@@ -19,6 +19,16 @@ mtl_status fft_check(const LaunchArgs& la, const uint64_t* bytes);
 mtl_status fft_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream);
 mtl_status gemm_check(const LaunchArgs& la, const uint64_t* bytes);
 mtl_status gemm_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream);
+#define LM_DECL(k)                                               \
+  mtl_status k##_check(const LaunchArgs& la, const uint64_t* bytes); \
+  mtl_status k##_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream);
+LM_DECL(quantize)
+LM_DECL(gemm_fp8)
+LM_DECL(gemm_grouped_fp8)
+LM_DECL(gemm_grouped)
+LM_DECL(gemm_grouped_dx)
+LM_DECL(gemm_grouped_dw)
+#undef LM_DECL
 mtl_status conv_check(const LaunchArgs& la, const uint64_t* bytes);
 mtl_status conv_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream);
 mtl_status nchwconv_check(const LaunchArgs& la, const uint64_t* bytes);
@@ -63,8 +73,12 @@ mtl_status raster_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* s
 int gemm_timeouts(bool reset);
 int conv_timeouts(bool reset);
 int fft_timeouts(bool reset);
+int fp8_timeouts(bool reset);
+int grouped_timeouts(bool reset);
 cudaError_t gemm_set_wait_limit(unsigned long long ns);
 cudaError_t conv_set_wait_limit(unsigned long long ns);
+cudaError_t fp8_set_wait_limit(unsigned long long ns);
+cudaError_t grouped_set_wait_limit(unsigned long long ns);
 void gemm_inject_stall(int launches);
 
 // ── checks ──────────────────────────────────────────────────────────────────
@@ -278,6 +292,24 @@ static KernelDesc g_kernels[] = {
     {"fft_c2c", "BBii", false, 0b10, 0b01, fft_check, nullptr, fft_run, nullptr},
     // batched bf16 GEMM, fp32 accumulate and output: C, A, B, M, N, K; ndrange = batch
     {"gemm_bf16", "BBBiii", false, 0b110, 0b001, gemm_check, nullptr, gemm_run, nullptr},
+    // values to 8-bit floating point, one scale per block of 128: q, s, transposed
+    // q, transposed s, x, rows_of, R, C, rows of x, block (1 or 128), type of x (0
+    // f32, 1 bf16), format (0 e4m3, 1 e5m2), power-of-two scales; ndrange = batch
+    {"quantize_fp8", "bbbbBbiiiiiii", false, 0b110000, 0b001111, quantize_check, nullptr, quantize_run, nullptr},
+    // C = A B^T of such values: C, A, A's scales, B, B's scales, M, N, K, rows per
+    // scale of B (1 or 128), formats of A and B, output (0 f32, 1 bf16); ndrange = batch
+    {"gemm_fp8", "BBBBBiiiiiii", false, 0b11110, 0b1, gemm_fp8_check, nullptr, gemm_fp8_run, nullptr},
+    // the same by expert: Y, X, X's scales, W, W's scales, offsets, T, N, K, formats
+    // of X and W, output; ndrange = groups
+    {"gemm_grouped_fp8", "BBBBBBiiiiii", false, 0b111110, 0b1, gemm_grouped_fp8_check, nullptr, gemm_grouped_fp8_run,
+     nullptr},
+    // bf16 products by expert and their gradients: Y, X, W / dX, dY, W / dW, X, dY;
+    // offsets, T, N, K, output; ndrange = groups
+    {"gemm_grouped_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_check, nullptr, gemm_grouped_run, nullptr},
+    {"gemm_grouped_dx_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_dx_check, nullptr, gemm_grouped_dx_run,
+     nullptr},
+    {"gemm_grouped_dw_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_dw_check, nullptr, gemm_grouped_dw_run,
+     nullptr},
     // NHWC bf16 convolution (implicit GEMM): out, in, w (HWIO), H, W, Cin, Cout,
     // k, stride, pad, relu, in_wpad, out_wpad; ndrange = images
     {"conv2d_bf16", "BBBiiiiiiiiii", false, 0b110, 0b001, conv_check, conv_workspace, conv_run, nullptr},
@@ -383,7 +415,8 @@ int32_t mtl_kernel_count(void) { return mtl::kernel_count(); }
 mtl_status mtl_kernel_timeouts(int32_t reset, int64_t* count) {
   if (!count) return mtl::fail(MTL_ERR_ARGUMENT, "mtl_kernel_timeouts: NULL argument");
   int64_t total = 0;
-  for (int v : {mtl::gemm_timeouts(reset != 0), mtl::conv_timeouts(reset != 0), mtl::fft_timeouts(reset != 0)}) {
+  for (int v : {mtl::gemm_timeouts(reset != 0), mtl::conv_timeouts(reset != 0), mtl::fft_timeouts(reset != 0),
+                mtl::fp8_timeouts(reset != 0), mtl::grouped_timeouts(reset != 0)}) {
     if (v < 0) return mtl::fail(MTL_ERR_CUDA, "mtl_kernel_timeouts: cannot read the device counters");
     total += v;
   }
@@ -394,7 +427,8 @@ mtl_status mtl_kernel_timeouts(int32_t reset, int64_t* count) {
 mtl_status mtl_set_wait_limit(uint64_t ns) {
   const uint64_t v = ns ? ns : 2000000000ull;
   if (v < 1000000ull) return mtl::fail(MTL_ERR_ARGUMENT, "mtl_set_wait_limit: %llu ns is below 1 ms", (unsigned long long)v);
-  for (cudaError_t e : {mtl::gemm_set_wait_limit(v), mtl::conv_set_wait_limit(v)})
+  for (cudaError_t e : {mtl::gemm_set_wait_limit(v), mtl::conv_set_wait_limit(v), mtl::fp8_set_wait_limit(v),
+                        mtl::grouped_set_wait_limit(v)})
     if (e != cudaSuccess) return mtl::fail(MTL_ERR_CUDA, "mtl_set_wait_limit: %s", cudaGetErrorString(e));
   return MTL_OK;
 }

@@ -1,0 +1,75 @@
+// What the expert-grouped products share: the table of a launch's groups in
+// shared memory and the walk of a persistent CTA over their tiles.
+//
+// Group e holds rows offsets[e] .. offsets[e + 1] of the row matrix. The
+// offsets live on the device, so the host cannot check them: each is clamped to
+// [the previous group's start, rows], and a group that ends before it starts is
+// empty. Whatever they hold, no access leaves the buffers.
+#pragma once
+
+#include "tc_common.cuh"
+
+namespace mtl {
+
+constexpr int kMaxGroups = 1024;
+
+struct GroupTable {
+  int lo[kMaxGroups];       // first row
+  int hi[kMaxGroups];       // one past the last
+  int cum[kMaxGroups + 1];  // row tiles of the groups before
+};
+
+// Every thread of the CTA calls this; `tile_m` rows a tile.
+__device__ __forceinline__ void build_groups(GroupTable* g, const int* __restrict__ offsets, int groups, int rows,
+                                             int tile_m) {
+  for (int e = threadIdx.x; e < groups; e += blockDim.x) {
+    const int lo = min(max(offsets[e], 0), rows), hi = min(max(offsets[e + 1], lo), rows);
+    g->lo[e] = lo;
+    g->hi[e] = hi;
+    g->cum[e + 1] = (hi - lo + tile_m - 1) / tile_m;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int carry = 0;
+    for (int base = 0; base < groups; base += 32) {
+      const int e = base + (int)threadIdx.x;
+      int v = e < groups ? g->cum[e + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, d);
+        if ((int)threadIdx.x >= d) v += u;
+      }
+      if (e < groups) g->cum[e + 1] = carry + v;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (threadIdx.x == 0) g->cum[0] = 0;
+  }
+  __syncthreads();
+}
+
+// Tile t of a grouped launch, tiles in the order (group, column tile, row tile):
+// neighbouring CTAs take the row tiles of one column panel of a group's weights.
+// A walk asks for growing t, so the group is found by moving forward.
+struct GroupWalk {
+  int e = 0;
+  __device__ __forceinline__ void find(const GroupTable* g, int t, int tiles_n, int tile_m, int tile_n, int* row0,
+                                       int* rows, int* n0) {
+    while (t >= g->cum[e + 1] * tiles_n) ++e;
+    const int first = g->cum[e], mt = g->cum[e + 1] - first, in = t - first * tiles_n;
+    const int m0 = in % mt * tile_m;
+    *row0 = g->lo[e] + m0;
+    *rows = g->hi[e] - *row0;
+    *n0 = in / mt * tile_n;
+  }
+};
+
+// A kernel's dynamic shared memory above 48 KiB, allowed once per device.
+template <typename F>
+static cudaError_t allow_smem(F* kernel, int bytes, int device, unsigned long long* done) {
+  if (device >= 0 && device < 64 && (__atomic_load_n(done, __ATOMIC_RELAXED) >> device & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device >= 0 && device < 64) __atomic_fetch_or(done, 1ull << device, __ATOMIC_RELAXED);
+  return e;
+}
+
+}  // namespace mtl

@@ -589,11 +589,60 @@ def _nd(ndrange) -> tuple[int, ...]:
     return tuple(int(v) for v in ndrange) if isinstance(ndrange, (tuple, list)) else (int(ndrange),)
 
 
+# Bytes per element of the operands of the 8-bit and expert-grouped kernels, by
+# argument (a tuple indexed by the kernel's type argument where it decides), and
+# that argument's index. The library sees addresses and byte counts only, so what a
+# tensor or buffer says of itself is checked here.
+_OUT = (4, 2)
+_OPERANDS = {
+    "quantize_fp8": ((1, 4, 1, 4, _OUT, 4), 10),
+    "gemm_fp8": ((_OUT, 1, 4, 1, 4), 11),
+    "gemm_grouped_fp8": ((_OUT, 1, 4, 1, 4, 4), 11),
+    "gemm_grouped_bf16": ((_OUT, 2, 2, 4), 7),
+    "gemm_grouped_dx_bf16": ((_OUT, 2, 2, 4), 7),
+    "gemm_grouped_dw_bf16": ((_OUT, 2, 2, 4), 7),
+}
+
+
+def _check_operands(k: Kernel, args: Sequence) -> None:
+    """Element sizes, and for torch tensors contiguity and one CUDA device, which
+    has to be the current one."""
+    sizes, flag = _OPERANDS[k.name]
+    device = None
+    for i, (x, size) in enumerate(zip(args, sizes)):
+        if isinstance(size, tuple):
+            kind = args[flag]
+            if kind not in (0, 1):
+                continue  # the library refuses it
+            size = size[kind]
+        if isinstance(x, UseHandle):
+            x = x.resource
+        if hasattr(x, "data_ptr"):
+            got = x.element_size()
+            if not x.is_cuda or not x.is_contiguous():
+                raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} must be a contiguous CUDA tensor")
+            if device is None:
+                import torch
+                device = x.device
+                if device.index != torch.cuda.current_device():
+                    raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: the tensors are on {device}, which is not the current device")
+            elif x.device != device:
+                raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} is on {x.device}, others on {device}")
+        elif hasattr(x, "dtype"):
+            got = x.dtype.itemsize
+        else:
+            continue  # null, or an address with a byte count
+        if got != size:
+            raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} has elements of {got} bytes, expected {size}")
+
+
 def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None:
     """dispatch!(p, kernel, args, ndrange; group), ext/MantleLavaExt.jl:751-752."""
     k = _kernel(kernel)
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"dispatch!: {k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
+    if k.name in _OPERANDS:
+        _check_operands(k, args)
     arr = (L.Arg * max(len(args), 1))(*[_arg(p.graph, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))
@@ -609,6 +658,10 @@ def launch(kernel, args: Sequence, ndrange, stream: int = 0, workspace=None) -> 
     """Launch a built-in kernel outside any graph on `stream` (pointer args:
     Buffers, torch tensors or DevicePtr)."""
     k = _kernel(kernel)
+    if k.name in _OPERANDS:
+        if len(args) != len(k.signature):
+            raise ArgumentError(L.ERR_ARGUMENT, f"launch: {k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
+        _check_operands(k, args)
     arr = (L.Arg * max(len(args), 1))(*[_arg(None, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))

@@ -1,0 +1,184 @@
+"""The bf16 products grouped by expert and their gradients against 64-bit arithmetic.
+
+Tolerance: the products of bf16 values are exact in fp32; an MMA adds 16 of them to
+the running sum, each addition off by at most one unit of fp32 (2^-23) of a partial
+sum that S = sum |a b| bounds: |out - exact| <= (D + 16) * 2^-23 * S over D terms, and
+a bf16 output adds half a step, 2^-8 of the value. fp32 outputs are also held to a
+relative Frobenius error of 1e-5, the bound of the dense GEMM's tests.
+"""
+import pytest
+import torch
+
+import mantle_cuda as M
+
+ptr = lambda n, at=1 << 20: M.DevicePtr(at, n)  # noqa: E731
+
+
+def args(way, e, t, n, k, out=0, **change):
+    w, x, y = e * k * n, t * k, t * n
+    c, a, b = {"fwd": (y, x, w), "dx": (x, y, w), "dw": (w, x, y)}[way]
+    z = dict(c=c * (2 if out == 1 else 4), a=a * 2, b=b * 2, off=4 * (e + 1)) | change
+    return [ptr(z["c"]), ptr(z["a"]), ptr(z["b"]), ptr(z["off"]), t, n, k, out]
+
+
+KERNEL = {"fwd": "gemm_grouped_bf16", "dx": "gemm_grouped_dx_bf16", "dw": "gemm_grouped_dw_bf16"}
+WAYS = list(KERNEL)
+
+
+@pytest.mark.parametrize("way", WAYS)
+def test_refusals(way):
+    k = getattr(M.kernels, KERNEL[way])
+    for a, e, match in [
+        (args(way, 3, 10, 40, 24, out=2), 3, "output type"),
+        (args(way, 3, 10, 44, 24), 3, "multiples of 8"),
+        (args(way, 3, 10, 40, 20), 3, "multiples of 8"),
+        (args(way, 3, -1, 40, 24), 3, "negative"),
+        (args(way, 3, 10, 40, 24, off=12), 3, "offsets"),
+        (args(way, 1100, 10, 40, 24), 1100, "more than 1024 groups"),
+    ]:
+        with pytest.raises(M.MantleError, match=match):
+            M.launch(k, a, e)
+    for i, which in enumerate("cab"):
+        full = args(way, 3, 10, 40, 24)[i].nbytes
+        with pytest.raises(M.MantleError, match="the launch touches"):
+            M.launch(k, args(way, 3, 10, 40, 24, **{which: full - 1}), 3)
+    bad = args(way, 3, 10, 40, 24)
+    bad[1] = M.DevicePtr((1 << 20) + 2, 1 << 20)
+    with pytest.raises(M.MantleError, match="16-byte aligned"):
+        M.launch(k, bad, 3)
+    with pytest.raises(M.ArgumentError, match="contiguous CUDA tensor"):
+        M.launch(k, [torch.zeros(400)] + args(way, 3, 10, 40, 24)[1:], 3)
+    if way != "dw":
+        zero = args(way, 3, 10, 40, 0) if way == "fwd" else args(way, 3, 10, 0, 24)
+        with pytest.raises(M.MantleError, match="contraction"):
+            M.launch(k, zero, 3)
+
+
+# ── on the GPU ───────────────────────────────────────────────────────────────
+def normal(shape, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(torch.bfloat16)
+
+
+def launch(way, out, a, b, offsets, t, n, k, e, kind):
+    M.launch(getattr(M.kernels, KERNEL[way]), (out, a, b, torch.tensor(offsets, dtype=torch.int32, device="cuda"), t, n, k, kind), e,
+             stream=torch.cuda.current_stream().cuda_stream)
+
+
+def check(got, a, b, kind):
+    """got against a @ b (float64 operands)."""
+    want, total = a @ b, a.abs() @ b.abs()
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    tol = (a.shape[1] + 16) * 2.0 ** -23 * total + (2.0 ** -8 * want.abs() if kind else 0.0)
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() - tol).max())
+    if not kind and want.numel():
+        assert (got - want).norm() <= 1e-5 * want.norm()
+
+
+SIZES = [
+    ([1], 0, 1, 8, 8),
+    ([3, 0, 1, 16], 0, 20, 72, 200),
+    ([5, 130, 0, 64, 1, 17], 3, 230, 264, 136),     # rows before the first and behind the last group
+    ([128, 256, 127, 129], 0, 640, 512, 264),
+    ([700, 20, 600], 0, 1320, 520, 1000),
+    ([2] * 40, 0, 80, 640, 512),
+    ([0, 0, 0], 0, 5, 64, 64),
+    ([1000, 1100], 0, 2100, 2056, 1032),
+    ([300] * 6 + [0, 31], 0, 1831, 1024, 648),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("sizes,first,t,n,k", SIZES)
+def test_forward_and_gradients(dev, sizes, first, t, n, k, kind):
+    e = len(sizes)
+    o = [first + sum(sizes[:i]) for i in range(e + 1)]
+    x, dy, w = normal((t, k), t + k), normal((t, n), t + n), normal((e, k, n), n + k)
+    dt = torch.bfloat16 if kind else torch.float32
+    xg, dyg, wg = x.cuda(), dy.cuda(), w.cuda()
+    y = torch.full((t, n), 3.0, dtype=dt, device="cuda")
+    dx = torch.full((t, k), 3.0, dtype=dt, device="cuda")
+    dw = torch.full((e, k, n), float("nan"), dtype=dt, device="cuda")
+    launch("fwd", y, xg, wg, o, t, n, k, e, kind)
+    launch("dx", dx, dyg, wg, o, t, n, k, e, kind)
+    launch("dw", dw, xg, dyg, o, t, n, k, e, kind)
+    torch.cuda.synchronize()
+    x, dy, w = x.double(), dy.double(), w.double()
+    for i in range(e):
+        r = slice(o[i], o[i + 1])
+        check(y[r], x[r], w[i], kind)
+        check(dx[r], dy[r], w[i].t(), kind)
+        check(dw[i], x[r].t(), dy[r], kind)
+    for v in (y, dx):
+        assert (v[:o[0]] == 3.0).all() and (v[o[-1]:] == 3.0).all()
+    assert M.kernel_timeouts() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", WAYS)
+def test_other_groups_rows_do_not_reach_a_group(dev, way):
+    # groups 0 and 2 and the rows of no group hold NaN and infinities; group 1's results stay exact
+    sizes, t, n, k = [37, 45, 50], 140, 136, 200
+    o = [4, 41, 86, 136]
+    x, dy, w = normal((t, k), 1), normal((t, n), 2), normal((3, k, n), 3)
+    for v in (x, dy):
+        v[:41] = float("nan")
+        v[86:] = float("inf")
+    w[0], w[2] = float("nan"), float("nan")
+    out = torch.zeros({"fwd": (t, n), "dx": (t, k), "dw": (3, k, n)}[way], device="cuda")
+    a, b = {"fwd": (x, w), "dx": (dy, w), "dw": (x, dy)}[way]
+    launch(way, out, a.cuda(), b.cuda(), o, t, n, k, 3, 0)
+    torch.cuda.synchronize()
+    r = slice(41, 86)
+    x, dy, w = x.double(), dy.double(), w.double()
+    if way == "dw":
+        check(out[1], x[r].t(), dy[r], 0)
+    else:
+        check(out[r], *((x[r], w[1]) if way == "fwd" else (dy[r], w[1].t())), 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", WAYS)
+def test_bad_offsets_stay_in_bounds(dev, way):
+    t, n, k = 100, 136, 72
+    x, dy, w = normal((t, k), 1).cuda(), normal((t, n), 2).cuda(), normal((4, k, n), 3).cuda()
+    off = [-5, 40, 20, 90, 1 << 30]  # clamped: 0..40, none, 20..90, 90..100
+    rows = {"fwd": (t, n), "dx": (t, k), "dw": (4 * k, n)}[way]
+    guard = torch.full((rows[0] + 64, rows[1]), 3.0, device="cuda")
+    a, b = {"fwd": (x, w), "dx": (dy, w), "dw": (x, dy)}[way]
+    launch(way, guard[:rows[0]], a, b, off, t, n, k, 4, 0)
+    torch.cuda.synchronize()
+    assert (guard[rows[0]:] == 3.0).all() and torch.isfinite(guard).all()
+    x, dy, w, got = x.double().cpu(), dy.double().cpu(), w.double().cpu(), guard.double().cpu()
+    for e, lo, hi in ((0, 0, 20), (3, 90, 100)):
+        if way == "dw":
+            if e == 3:
+                check(got[3 * k:4 * k], x[90:100].t(), dy[90:100], 0)
+        else:
+            check(got[lo:hi], *((x[lo:hi], w[e]) if way == "fwd" else (dy[lo:hi], w[e].t())), 0)
+
+
+@pytest.mark.gpu
+def test_the_gradients_are_the_products_derivatives(dev):
+    # the directional derivative of L = sum(Y * dY) by central differences: L is linear in X and in W, so a step
+    # of h along a direction D changes L by h <grad, D> exactly, up to the sums' rounding (fp32, S as above) and
+    # the rounding of X + h D to bf16, which is avoided by taking steps that bf16 holds exactly
+    sizes, t, n, k, h = [33, 0, 70], 103, 64, 72, 1.0
+    o = [0, 33, 33, 103]
+    g = torch.Generator().manual_seed(4)
+    whole = lambda *s: torch.randint(-4, 5, s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
+    x, w, dy, dirx, dirw = whole(t, k), whole(3, k, n), whole(t, n), whole(t, k), whole(3, k, n)
+
+    def loss(xv, wv):
+        y = torch.zeros((t, n), device="cuda")
+        launch("fwd", y, xv, wv, o, t, n, k, 3, 0)
+        return (y.double() * dy.double()).sum()
+
+    dx, dw = torch.zeros((t, k), device="cuda"), torch.zeros((3, k, n), device="cuda")
+    launch("dx", dx, dy, w, o, t, n, k, 3, 0)
+    launch("dw", dw, x, dy, o, t, n, k, 3, 0)
+    # whole numbers below 2^24 throughout: every product and sum is exact
+    assert float((loss(x + h * dirx, w) - loss(x - h * dirx, w)) / (2 * h)) == float((dx.double() * dirx.double()).sum())
+    assert float((loss(x, w + h * dirw) - loss(x, w - h * dirw)) / (2 * h)) == float((dw.double() * dirw.double()).sum())
