@@ -23,6 +23,7 @@
 //   warp 0      TMA producer: per K block 128 rows of A and BN rows of B, 128 bytes
 //               each (128-byte swizzle), into a ring of stages;
 //   warp 1      owns the tensor memory, one thread issues the MMAs;
+//   warp 2      brings the scales of each K block to shared memory (cp.async), ahead;
 //   warps 4-11  the scaled sums: warp w reads lanes 32 (w % 4) .., half of BN columns.
 // Rows of a partial tile are loaded in boxes of 32, so that a group of a few rows
 // reads few; what the skipped rows hold only reaches rows that are not stored.
@@ -53,11 +54,13 @@ struct F8Cfg {
   static constexpr uint32_t kTmemCols = kAcc * BN;
   static constexpr uint32_t kAStage = kF8M * kF8K, kStageBytes = kAStage + BN * kF8K;
 };
+constexpr int kF8Scales = 8;  // K blocks of scales on their way or in use
 struct F8Shared {
-  uint64_t full[8], empty[8], tfull[4], tempty[4], drain;
+  uint64_t full[8], empty[8], tfull[4], tempty[4], sfull[kF8Scales], sempty[kF8Scales], drain;
   uint32_t tmem;
   int abort;
-  float scale_b[8][2][128];  // per warp: a K block's row scales of B, double buffered
+  float sa[kF8Scales][kF8M];  // a K block's scales of the tile's rows of A
+  float sb[kF8Scales][256];   // and of its rows of B, or of its 128-row blocks
   GroupTable groups;
 };
 template <int BN>
@@ -85,23 +88,13 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, ui
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
+// Four bytes to shared memory without a register; they land before the barrier's
+// phase completes (cp_async_arrive, one arrival per lane).
+__device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // A tile's place: rows row0 .. of operand A in slice a_b, columns n0 .. of operand
@@ -138,22 +131,19 @@ struct F8Walk {
   }
 };
 
-// One row's `n` neighbouring sums to C, from column `col` on.
+// One row's neighbouring sums to C, from column `col` on.
 template <typename OUT, int COLS>
-__device__ __forceinline__ void store_row(const F8Args& p, int64_t row, int col, const unsigned long long (&acc)[COLS / 2]) {
+__device__ __forceinline__ void store_row(const F8Args& p, int64_t row, int col, const float (&v)[COLS]) {
   OUT* c = static_cast<OUT*>(p.C) + row * p.N + col;
   if constexpr (sizeof(OUT) == 4) {
 #pragma unroll
     for (int i = 0; i < COLS; i += 4) {
-      float v[4];
-      unpack2(acc[i / 2], v[0], v[1]);
-      unpack2(acc[i / 2 + 1], v[2], v[3]);
       if (p.vec && col + i + 4 <= p.N) {
-        *reinterpret_cast<float4*>(c + i) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (col + i + j < p.N) c[i + j] = v[j];
+          if (col + i + j < p.N) c[i + j] = v[i + j];
       }
     }
   } else {
@@ -161,11 +151,7 @@ __device__ __forceinline__ void store_row(const F8Args& p, int64_t row, int col,
     for (int i = 0; i < COLS; i += 8) {
       __nv_bfloat162 b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float lo, hi;
-        unpack2(acc[i / 2 + j], lo, hi);
-        b[j] = __floats2bfloat162_rn(lo, hi);
-      }
+      for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
       if (p.vec && col + i + 8 <= p.N) {
         *reinterpret_cast<uint4*>(c + i) = *reinterpret_cast<uint4*>(b);
       } else {
@@ -199,6 +185,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     for (int a = 0; a < kAcc; ++a) {
       mbar_init(smem_u32(&sh->tfull[a]), 1);
       mbar_init(smem_u32(&sh->tempty[a]), 8);
+    }
+    for (int a = 0; a < kF8Scales; ++a) {
+      mbar_init(smem_u32(&sh->sfull[a]), 32);
+      mbar_init(smem_u32(&sh->sempty[a]), 8);
     }
     mbar_init(smem_u32(&sh->drain), 1);
     *abort = 0;
@@ -290,93 +280,89 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         drain_phase(smem_u32(&sh->drain), 0);
       }
     }
+  } else if (warp == 2) {
+    // ── scales: a K block's 128 + BN (or its 128-row blocks') into a ring of their own ──
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
+      const float* sa = p.sA + c.sa;
+      const float* sb = ROWB ? p.sB + (int64_t)c.b_b * p.kblocks * p.N + c.n0
+                             : p.sB + ((int64_t)c.b_b * p.nblocks + c.n0 / 128) * p.kblocks;
+      const int cols = min(BN, p.N - c.n0);
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->sempty[s]), ph ^ 1, abort, &g_fp8_timeouts));
+        if (!ok) break;
+        const uint32_t da = smem_u32(sh->sa[s]), db = smem_u32(sh->sb[s]);
+#pragma unroll
+        for (int i = 0; i < kF8M / 32; ++i)
+          if (i * 32 + lane < c.rows) cp_async4(da + (i * 32 + lane) * 4, sa + (int64_t)kb * p.M + i * 32 + lane);
+        if (ROWB) {
+#pragma unroll
+          for (int i = 0; i < BN / 32; ++i)
+            if (i * 32 + lane < cols) cp_async4(db + (i * 32 + lane) * 4, sb + (int64_t)kb * p.N + i * 32 + lane);
+        } else if (lane * 128 < cols) {
+          cp_async4(db + lane * 4, sb + (int64_t)lane * p.kblocks + kb);
+        }
+        cp_async_arrive(smem_u32(&sh->sfull[s]));
+        if (++s == kF8Scales) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8ManyRegs));
     // ── scaled sums: warp reads TMEM lanes 32 q .. +32, columns half * kCols .. ──
     const int q = warp & 3, half = (warp - 4) / 4;
-    float(*sb_sh)[128] = sh->scale_b[warp - 4];
-    int a = 0;
-    uint32_t aph = 0;
+    int a = 0, s = 0;
+    uint32_t aph = 0, sph = 0;
     bool ok = true;
     for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
       const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
       const int row = q * 32 + lane, col = c.n0 + half * kCols;
-      const bool busy = q * 32 < c.rows, valid = row < c.rows;
-      const float* sa = p.sA + c.sa + (valid ? row : 0);
-      // square blocks: one scale for the warp's columns; row blocks: four columns a lane
-      const float* sb = ROWB ? p.sB + (int64_t)c.b_b * p.kblocks * p.N
-                             : p.sB + ((int64_t)c.b_b * p.nblocks + min(col / 128, p.nblocks - 1)) * p.kblocks;
-      unsigned long long acc[kCols / 2];
+      const bool busy = q * 32 < c.rows;  // uniform in the warp
+      float acc[kCols];
 #pragma unroll
-      for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
-      // A's scales (times B's, square blocks) four K blocks ahead
-      float cur[4], na[4], nb[4];
-      float rb[ROWB ? 4 : 1];
-      auto fetch = [&](int kb) {
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+#pragma unroll 1
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->sfull[s]), sph, abort, &g_fp8_timeouts) &&
+                                         wait_phase(smem_u32(&sh->tfull[a]), aph, abort, &g_fp8_timeouts));
+        if (!ok) break;
+        tc_fence_after();
+        if (busy) {
+          const float sr = ROWB ? sh->sa[s][row] : sh->sa[s][row] * sh->sb[s][BN == 256 ? half : 0];
+          const float* sb = sh->sb[s] + half * kCols;
+          const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half * kCols);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool in = kb + j < p.kblocks && busy;
-          na[j] = in ? __ldg(sa + (int64_t)(kb + j) * p.M) : 0.0f;
-          if (!ROWB) nb[j] = in ? __ldg(sb + kb + j) : 0.0f;
-        }
-      };
-      auto fetch_rows = [&](int kb) {
-        if constexpr (ROWB) {
+          for (int ch = 0; ch < kCols / 32; ++ch) {
+            uint32_t r[32];
+            tmem_ld32(base + ch * 32, r);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int n = col + j * 32 + lane;
-            rb[j] = j * 32 < kCols && kb < p.kblocks && busy && n < p.N ? __ldg(sb + (int64_t)kb * p.N + n) : 0.0f;
+            for (int i = 0; i < 32; ++i)
+              acc[ch * 32 + i] = fmaf(__uint_as_float(r[i]), ROWB ? sr * sb[ch * 32 + i] : sr, acc[ch * 32 + i]);
           }
         }
-      };
-      fetch(0);
-      fetch_rows(0);
-      for (int kb0 = 0; ok && kb0 < p.kblocks; kb0 += 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) cur[j] = ROWB ? na[j] : na[j] * nb[j];
-        fetch(kb0 + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int kb = kb0 + j;
-          if (kb >= p.kblocks || !ok) break;
-          if constexpr (ROWB) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sb_sh[kb & 1][i * 32 + lane] = rb[i];
-            __syncwarp();
-            fetch_rows(kb + 1);
-          }
-          ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->tfull[a]), aph, abort, &g_fp8_timeouts));
-          if (!ok) break;
-          tc_fence_after();
-          if (busy) {
-            const unsigned long long s2 = pack2(cur[j], cur[j]);
-            const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half * kCols);
-#pragma unroll
-            for (int ch = 0; ch < kCols / 32; ++ch) {
-              uint32_t r[32];
-              tmem_ld32(base + ch * 32, r);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                unsigned long long s = s2;
-                if constexpr (ROWB) {
-                  const float2 b = *reinterpret_cast<const float2*>(&sb_sh[kb & 1][ch * 32 + 2 * i]);
-                  s = mul2(s2, pack2(b.x, b.y));
-                }
-                acc[ch * 16 + i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s, acc[ch * 16 + i]);
-              }
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
-          if (++a == kAcc) {
-            a = 0;
-            aph ^= 1;
-          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&sh->tempty[a]));
+          mbar_arrive(smem_u32(&sh->sempty[s]));
+        }
+        if (++a == kAcc) {
+          a = 0;
+          aph ^= 1;
+        }
+        if (++s == kF8Scales) {
+          s = 0;
+          sph ^= 1;
         }
       }
-      if (ok && valid && col < p.N) store_row<OUT, kCols>(p, c.crow + row, col, acc);
+      if (ok && row < c.rows && col < p.N) store_row<OUT, kCols>(p, c.crow + row, col, acc);
     }
   }
   tc_fence_before();
