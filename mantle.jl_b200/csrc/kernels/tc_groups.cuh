@@ -63,6 +63,22 @@ struct GroupWalk {
   }
 };
 
+// wait_phase by a whole converged warp: the answer is the same in every lane.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort, int* timeouts) {
+  bool ok = __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
+  if (!ok) ok = __all_sync(0xffffffffu, wait_phase(bar, parity, abort, timeouts));
+  return ok;
+}
+
+// One lane of a converged warp, the choice known to the compiler to be uniform: the
+// instructions behind it take their descriptors from uniform registers. Behind
+// `lane == 0` four MMAs and two commits took 470 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+  return p != 0;
+}
+
 // A kernel's dynamic shared memory above 48 KiB, allowed once per device.
 template <typename F>
 static cudaError_t allow_smem(F* kernel, int bytes, int device, unsigned long long* done) {
