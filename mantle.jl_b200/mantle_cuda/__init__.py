@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 import threading
 from collections import deque
 from dataclasses import dataclass
@@ -604,36 +605,68 @@ _OPERANDS = {
 }
 
 
-def _check_operands(k: Kernel, args: Sequence) -> None:
-    """Element sizes, and for torch tensors contiguity and one CUDA device, which
-    has to be the current one."""
+def _operands(k: Kernel, args: Sequence) -> list:
+    """(kind, rid, address, bytes) of each buffer argument of a kernel in _OPERANDS, in
+    one flat list, checked: element sizes, and for torch tensors contiguity and the
+    current CUDA device. A graph resource's address is its plan's and stays 0."""
     sizes, flag = _OPERANDS[k.name]
-    device = None
-    for i, (x, size) in enumerate(zip(args, sizes)):
-        if isinstance(size, tuple):
+    if len(args) != len(k.signature):
+        raise ArgumentError(L.ERR_ARGUMENT, f"{k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
+    flat, device = [], None
+    for i, size in enumerate(sizes):
+        x = args[i]
+        if x is None:
+            flat += (L.ARG_NULL, 0, 0, 0)
+            continue
+        if size is _OUT:
             kind = args[flag]
-            if kind not in (0, 1):
-                continue  # the library refuses it
-            size = size[kind]
-        if isinstance(x, UseHandle):
-            x = x.resource
+            size = _OUT[kind] if kind in (0, 1) else 0  # the library refuses another type
         if hasattr(x, "data_ptr"):
-            got = x.element_size()
-            if not x.is_cuda or not x.is_contiguous():
-                raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} must be a contiguous CUDA tensor")
             if device is None:
                 import torch
-                device = x.device
-                if device.index != torch.cuda.current_device():
-                    raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: the tensors are on {device}, which is not the current device")
-            elif x.device != device:
-                raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} is on {x.device}, others on {device}")
-        elif hasattr(x, "dtype"):
-            got = x.dtype.itemsize
+                device = torch.cuda.current_device() if torch.cuda.is_initialized() else 0
+            if x.get_device() != device or not x.is_contiguous():
+                raise ArgumentError(L.ERR_ARGUMENT,
+                                    f"{k.name}: argument {i + 1} must be a contiguous CUDA tensor on the current device ({device})")
+            got = x.element_size()
+            flat += (L.ARG_PTR, 0, x.data_ptr(), x.numel() * got)
+        elif isinstance(x, DevicePtr):
+            flat += (L.ARG_PTR, 0, x.ptr, x.nbytes & 0xFFFFFFFFFFFFFFFF)
+            continue
         else:
-            continue  # null, or an address with a byte count
-        if got != size:
+            x = x.resource if isinstance(x, UseHandle) else x
+            if not hasattr(x, "dtype"):
+                raise ArgumentError(L.ERR_ARGUMENT, f"cannot pass {x!r} where the kernel takes a buffer")
+            got = x.dtype.itemsize
+            flat += (L.ARG_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
+        if got != size and size:
             raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} has elements of {got} bytes, expected {size}")
+    return flat
+
+
+_packed = {}  # per kernel: the layout of its argument array, and the entry point taking it as bytes
+
+
+def _launch_packed(k: Kernel, args: Sequence, nd: tuple, stream: int) -> None:
+    """launch() of a kernel in _OPERANDS: the argument array is packed in one call (a
+    call costs the host 5 us instead of 25, and a decode step's kernel runs for 2 to 15)."""
+    flat = _operands(k, args)
+    if k.name not in _packed:
+        # every argument is {int32 kind, int32 rid, 8-byte value, uint64 bytes}
+        f = lib()["mtl_launch"]
+        f.restype = C.c_int32
+        f.argtypes = [C.c_int32, C.c_char_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
+        _packed[k.name] = (struct.Struct("<" + "".join("iiQQ" if s in "Bb" else "iii4xQ" for s in k.signature)), f)
+    layout, f = _packed[k.name]
+    for x in args[len(flat) // 4:]:
+        flat += (L.ARG_I32, 0, x, 0)
+    try:
+        packed = layout.pack(*flat)
+    except struct.error as e:
+        raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: a scalar argument is no Int32 ({e})") from None
+    status = f(k.id, packed, len(k.signature), struct.pack("<3q", *nd, *([1] * (3 - len(nd)))), len(nd), None, 0, stream)
+    if status:
+        check(status)
 
 
 def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None:
@@ -642,7 +675,7 @@ def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"dispatch!: {k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
     if k.name in _OPERANDS:
-        _check_operands(k, args)
+        _operands(k, args)
     arr = (L.Arg * max(len(args), 1))(*[_arg(p.graph, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))
@@ -659,9 +692,7 @@ def launch(kernel, args: Sequence, ndrange, stream: int = 0, workspace=None) -> 
     Buffers, torch tensors or DevicePtr)."""
     k = _kernel(kernel)
     if k.name in _OPERANDS:
-        if len(args) != len(k.signature):
-            raise ArgumentError(L.ERR_ARGUMENT, f"launch: {k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
-        _check_operands(k, args)
+        return _launch_packed(k, args, _nd(ndrange), stream)
     arr = (L.Arg * max(len(args), 1))(*[_arg(None, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))
