@@ -48,6 +48,7 @@ struct GrCfg {
   static constexpr int kTileM = RUNS * kGrM;
 };
 struct GrShared {
+  uint4 stage[4][32 * 8];  // per epilogue warp: 128 bytes of 32 output rows
   uint64_t full[8], empty[8], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
@@ -102,34 +103,56 @@ struct GrWalk {
   }
 };
 
-// 32 neighbouring sums of one row.
-template <typename OUT>
-__device__ __forceinline__ void store32(const GrArgs& p, OUT* crow, int col, const uint32_t (&r)[32]) {
-  OUT* c = crow + col;
-  if constexpr (sizeof(OUT) == 4) {
-    if (p.vec && col + 32 <= p.cols) {
+__device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
+__device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[64]) {
+  uint32_t(&lo)[32] = reinterpret_cast<uint32_t(&)[32]>(r[0]);
+  uint32_t(&hi)[32] = reinterpret_cast<uint32_t(&)[32]>(r[32]);
+  tmem_ld32_nowait(addr, lo);
+  tmem_ld32(addr + 32, hi);
+  tmem_wait_ld(lo);
+}
+
+// 128 bytes of 32 output rows (a lane holds its row's sums in r), `rows` of them
+// valid, through shared memory, so that an instruction writes whole 128-byte pieces
+// of four rows instead of 16 bytes of 32 (the weight gradient of the 16-expert case
+// took 253 us that way). 16-byte words are placed by word ^ (row % 8): no bank is hit
+// twice on either side.
+template <typename OUT, int COLS>
+__device__ __forceinline__ void store_rows(const GrArgs& p, uint4* stage, int lane, int rows, OUT* out, int col,
+                                           const uint32_t (&r)[COLS]) {
+  constexpr int kPer = 16 / sizeof(OUT);  // values a word
 #pragma unroll
-      for (int v = 0; v < 8; ++v)
-        reinterpret_cast<float4*>(c)[v] = make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
-                                                      __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3]));
+  for (int w = 0; w < 8; ++w) {
+    uint4 v;
+    if constexpr (sizeof(OUT) == 4) {
+      v = make_uint4(r[4 * w], r[4 * w + 1], r[4 * w + 2], r[4 * w + 3]);
     } else {
+      __nv_bfloat162 b[4];
 #pragma unroll
-      for (int v = 0; v < 32; ++v)
-        if (col + v < p.cols) c[v] = __uint_as_float(r[v]);
+      for (int i = 0; i < 4; ++i)
+        b[i] = __floats2bfloat162_rn(__uint_as_float(r[8 * w + 2 * i]), __uint_as_float(r[8 * w + 2 * i + 1]));
+      v = *reinterpret_cast<uint4*>(b);
     }
-  } else {
-    __nv_bfloat162 b[16];
+    stage[lane * 8 + (w ^ (lane & 7))] = v;
+  }
+  __syncwarp();
+  const int w = lane & 7, c = col + w * kPer;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) b[v] = __floats2bfloat162_rn(__uint_as_float(r[2 * v]), __uint_as_float(r[2 * v + 1]));
-    if (p.vec && col + 32 <= p.cols) {
+  for (int i = 0; i < 8; ++i) {
+    const int row = i * 4 + lane / 8;
+    const uint4 v = stage[row * 8 + (w ^ (row & 7))];
+    if (row < rows && c < p.cols) {  // columns come in eights: a word is inside or outside
+      OUT* dst = out + (int64_t)row * p.cols + c;
+      if (p.vec) {
+        *reinterpret_cast<uint4*>(dst) = v;
+      } else {
+        const OUT* e = reinterpret_cast<const OUT*>(&v);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(c)[v] = reinterpret_cast<const uint4*>(b)[v];
-    } else {
-#pragma unroll
-      for (int v = 0; v < 32; ++v)
-        if (col + v < p.cols) c[v] = v & 1 ? b[v / 2].y : b[v / 2].x;
+        for (int k = 0; k < kPer; ++k) dst[k] = e[k];
+      }
     }
   }
+  __syncwarp();
 }
 
 template <int FORM, int RUNS, int BN, typename OUT>
@@ -228,18 +251,22 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     int s = 0, i = 0;
     uint32_t ph = 0;
     bool ok = true;
+    // MN-major: 64-value chunks kGrK * 128 bytes apart, a K = 16 slice is 16 rows of 128
+    // bytes; K-major: rows of 128 bytes, a slice is 32 bytes further along the swizzled row
+    constexpr uint32_t kAStep = (FORM == kDw ? 2048 : 32) >> 4, kBStep = (FORM == kDx ? 32 : 2048) >> 4;
+    const uint64_t a0 = smem_desc(smem_u32(ring), FORM == kDw ? kGrK * 128 : 16, 1024);
+    const uint64_t b0 = smem_desc(smem_u32(ring) + RUNS * Cfg::kAStage, FORM == kDx ? 16 : kGrK * 128, 1024);
     for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const int kblocks = (c.depth + kGrK - 1) / kGrK;
       if (kblocks == 0) continue;
       const int a = i % kAcc, runs = RUNS == 1 ? 1 : (c.rows + kGrM - 1) / kGrM;
-      ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->tempty[a]), ((i / kAcc) & 1) ^ 1, abort, &g_grouped_timeouts));
+      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i / kAcc) & 1) ^ 1, abort, &g_grouped_timeouts);
       ++i;
       const uint32_t d = tmem + (uint32_t)(a * RUNS * BN);
       for (int kb = 0; ok && kb < kblocks; ++kb) {
-        ok = __all_sync(0xffffffffu, wait_phase(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts));
+        ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
         if (!ok) break;
-        const uint32_t a_addr = smem_u32(ring + s * Cfg::kStageBytes), b_addr = a_addr + RUNS * Cfg::kAStage;
         int steps = kGrK / 16;
         if (FORM == kDw && c.depth - kb * kGrK < kGrK) {
           const int live = c.depth - kb * kGrK, end = (live + 15) / 16 * 16;
@@ -253,19 +280,20 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           __syncwarp();
         }
         tc_fence_after();
-        if (lane == 0) {
-          for (int kk = 0; kk < steps; ++kk) {
-            // MN-major: 64-value chunks kGrK * 128 bytes apart, a K = 16 slice is 16 rows
-            // of 128 bytes; K-major: a slice is 32 bytes further along the swizzled row
-            const uint64_t bd = FORM == kDx ? smem_desc(b_addr + kk * 32, 16, 1024)
-                                            : smem_desc(b_addr + kk * 2048, kGrK * 128, 1024);
+        if (elect_one()) {
+          const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
+          auto mmas = [&](int kk) {
 #pragma unroll
-            for (int r = 0; r < RUNS; ++r) {
-              if (r >= runs) break;
-              const uint32_t ar = a_addr + r * Cfg::kAStage;
-              const uint64_t ad = FORM == kDw ? smem_desc(ar + kk * 2048, kGrK * 128, 1024) : smem_desc(ar + kk * 32, 16, 1024);
-              tc_mma(d + (uint32_t)(r * BN), ad, bd, kIdesc, (kb | kk) != 0);
-            }
+            for (int r = 0; r < RUNS; ++r)
+              if (r < runs)
+                tc_mma(d + (uint32_t)(r * BN), a0 + off + (uint64_t)(r * (Cfg::kAStage >> 4) + kk * kAStep), b0 + off + kk * kBStep,
+                       kIdesc, (kb | kk) != 0);
+          };
+          if (steps == kGrK / 16) {
+#pragma unroll
+            for (int kk = 0; kk < kGrK / 16; ++kk) mmas(kk);
+          } else {
+            for (int kk = 0; kk < steps; ++kk) mmas(kk);
           }
           tc_commit(smem_u32(&sh->empty[s]));
           if (kb + 1 == kblocks) tc_commit(smem_u32(&sh->tfull[a]));
@@ -290,28 +318,29 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       const bool empty = c.depth == 0;
       const int a = i % kAcc;
       if (!empty) {
-        if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh->tfull[a]), (i / kAcc) & 1, abort, &g_grouped_timeouts))) break;
+        if (!wait_warp(smem_u32(&sh->tfull[a]), (i / kAcc) & 1, abort, &g_grouped_timeouts)) break;
         tc_fence_after();
         ++i;
       }
 #pragma unroll 1
       for (int run = 0; run < RUNS; ++run) {
-        const int row = run * kGrM + q * 32 + lane;
-        if (run * kGrM + q * 32 >= c.rows) break;  // uniform in the warp
-        OUT* crow = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+        const int row = run * kGrM + q * 32;
+        if (row >= c.rows) break;  // uniform in the warp
+        OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
         const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * RUNS + run) * BN);
+        constexpr int kW = 128 / sizeof(OUT);  // columns a chunk
 #pragma unroll 1
-        for (int ch = 0; ch < BN / 32; ++ch) {
-          const int col = c.n0 + ch * 32;
+        for (int ch = 0; ch < BN / kW; ++ch) {
+          const int col = c.n0 + ch * kW;
           if (col >= p.cols) break;
-          uint32_t r[32];
+          uint32_t r[kW];
           if (empty) {
 #pragma unroll
-            for (int v = 0; v < 32; ++v) r[v] = 0;
+            for (int v = 0; v < kW; ++v) r[v] = 0;
           } else {
-            tmem_ld32(tbase + ch * 32, r);
+            tmem_ld_row(tbase + ch * kW, r);
           }
-          if (row < c.rows) store32<OUT>(p, crow, col, r);
+          store_rows<OUT, kW>(p, sh->stage[warp - 2], lane, c.rows - row, out, col, r);
         }
       }
       if (!empty) {
