@@ -36,7 +36,7 @@
 namespace mtl {
 
 enum { kFwd = 0, kDx = 1, kDw = 2 };
-constexpr int kGrThreads = 192, kGrM = 128, kGrK = 64;
+constexpr int kGrThreads = 320, kGrM = 128, kGrK = 64;
 
 template <int RUNS, int BN>
 struct GrCfg {
@@ -48,7 +48,7 @@ struct GrCfg {
   static constexpr int kTileM = RUNS * kGrM;
 };
 struct GrShared {
-  uint4 stage[4][32 * 8];  // per epilogue warp: 128 bytes of 32 output rows
+  uint4 stage[8][32 * 4];  // per epilogue warp: 64 bytes of 32 output rows
   uint64_t full[8], empty[8], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
@@ -67,6 +67,7 @@ struct GrArgs {
   int groups;
   int a_box;  // rows per TMA box of A (forward, dX)
   int vec;    // rows of the output start on 16 bytes
+  int chunked_a, chunked_b;  // MN-major operands loaded one box a K block
 };
 
 __device__ int g_grouped_timeouts;
@@ -79,12 +80,12 @@ struct GrTile {
 template <int FORM, int RUNS, int BN>
 struct GrWalk {
   GroupWalk g;
-  __device__ __forceinline__ GrTile find(const GrArgs& p, const GroupTable* groups, int64_t t, int tiles_m, int tiles_n) {
+  __device__ __forceinline__ GrTile find(const GrArgs& p, const GroupTable* groups, int t, int tiles_m, int tiles_n) {
     constexpr int tm = RUNS * kGrM;
     GrTile c;
     if (FORM == kDw) {
-      const int per = tiles_m * tiles_n, in = (int)(t % per);
-      c.e = (int)(t / per);
+      const int per = tiles_m * tiles_n, in = t % per;
+      c.e = t / per;
       c.m0 = in % tiles_m * tm;
       c.n0 = in / tiles_m * BN;
       c.rows = p.out_rows - c.m0;
@@ -92,7 +93,7 @@ struct GrWalk {
       c.depth = groups->hi[c.e] - c.row0;
       c.crow = (int64_t)c.e * p.out_rows + c.m0;
     } else {
-      g.find(groups, (int)t, tiles_n, tm, BN, &c.row0, &c.rows, &c.n0);
+      g.find(groups, t, tiles_n, tm, BN, &c.row0, &c.rows, &c.n0);
       c.e = g.e;
       c.m0 = 0;
       c.depth = p.depth;
@@ -104,25 +105,19 @@ struct GrWalk {
 };
 
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
-__device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[64]) {
-  uint32_t(&lo)[32] = reinterpret_cast<uint32_t(&)[32]>(r[0]);
-  uint32_t(&hi)[32] = reinterpret_cast<uint32_t(&)[32]>(r[32]);
-  tmem_ld32_nowait(addr, lo);
-  tmem_ld32(addr + 32, hi);
-  tmem_wait_ld(lo);
-}
+__device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16(addr, r); }
 
-// 128 bytes of 32 output rows (a lane holds its row's sums in r), `rows` of them
-// valid, through shared memory, so that an instruction writes whole 128-byte pieces
-// of four rows instead of 16 bytes of 32 (the weight gradient of the 16-expert case
-// took 253 us that way). 16-byte words are placed by word ^ (row % 8): no bank is hit
-// twice on either side.
+// 64 bytes of 32 output rows (a lane holds its row's sums in r), `rows` of them valid,
+// through shared memory, so that an instruction writes whole 64-byte pieces of eight
+// rows instead of 16 bytes of 32 (the weight gradient of the 16-expert case took 253
+// us that way, 186 with these). 16-byte words are placed by word ^ (row / 2 % 4): no
+// bank is hit twice on either side.
 template <typename OUT, int COLS>
 __device__ __forceinline__ void store_rows(const GrArgs& p, uint4* stage, int lane, int rows, OUT* out, int col,
                                            const uint32_t (&r)[COLS]) {
   constexpr int kPer = 16 / sizeof(OUT);  // values a word
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < 4; ++w) {
     uint4 v;
     if constexpr (sizeof(OUT) == 4) {
       v = make_uint4(r[4 * w], r[4 * w + 1], r[4 * w + 2], r[4 * w + 3]);
@@ -133,14 +128,14 @@ __device__ __forceinline__ void store_rows(const GrArgs& p, uint4* stage, int la
         b[i] = __floats2bfloat162_rn(__uint_as_float(r[8 * w + 2 * i]), __uint_as_float(r[8 * w + 2 * i + 1]));
       v = *reinterpret_cast<uint4*>(b);
     }
-    stage[lane * 8 + (w ^ (lane & 7))] = v;
+    stage[lane * 4 + (w ^ (lane >> 1 & 3))] = v;
   }
   __syncwarp();
-  const int w = lane & 7, c = col + w * kPer;
+  const int w = lane & 3, c = col + w * kPer;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = i * 4 + lane / 8;
-    const uint4 v = stage[row * 8 + (w ^ (row & 7))];
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + lane / 4;
+    const uint4 v = stage[row * 4 + (w ^ (row >> 1 & 3))];
     if (row < rows && c < p.cols) {  // columns come in eights: a word is inside or outside
       OUT* dst = out + (int64_t)row * p.cols + c;
       if (p.vec) {
@@ -175,7 +170,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     }
     for (int a = 0; a < kAcc; ++a) {
       mbar_init(smem_u32(&sh->tfull[a]), 1);
-      mbar_init(smem_u32(&sh->tempty[a]), 4);
+      mbar_init(smem_u32(&sh->tempty[a]), 8);
     }
     mbar_init(smem_u32(&sh->drain), 1);
     *abort = 0;
@@ -195,8 +190,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   const uint32_t tmem = sh->tmem;
 
   const int tiles_m = FORM == kDw ? (p.out_rows + Cfg::kTileM - 1) / Cfg::kTileM : 0, tiles_n = (p.cols + BN - 1) / BN;
-  const int64_t ntiles =
-      FORM == kDw ? (int64_t)tiles_m * tiles_n * p.groups : (int64_t)sh->groups.cum[p.groups] * tiles_n;
+  const int ntiles = FORM == kDw ? tiles_m * tiles_n * p.groups : sh->groups.cum[p.groups] * tiles_n;  // checked by the host
   GrWalk<FORM, RUNS, BN> walk;
 
   if (warp == 0) {
@@ -205,12 +199,13 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       int s = 0;
       uint32_t ph = 0;
       int64_t issued = 0;
-      for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
+      for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
         const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
-        // boxes that would lie wholly past the output's rows or columns are not loaded:
+        // a chunked operand comes in one box, zeros past its edges; other boxes that would
+        // lie wholly past the output's rows or columns are not loaded:
         // what stale shared memory they leave feeds outputs that are not stored
-        const int a_boxes = FORM == kDw ? (c.rows + 63) / 64 : (c.rows + p.a_box - 1) / p.a_box;
-        const int b_boxes = FORM == kDx ? 1 : min(BN / 64, (p.cols - c.n0 + 63) / 64);
+        const int a_boxes = FORM == kDw ? (p.chunked_a ? RUNS * kGrM / 64 : (c.rows + 63) / 64) : (c.rows + p.a_box - 1) / p.a_box;
+        const int b_boxes = FORM == kDx ? 1 : p.chunked_b ? BN / 64 : min(BN / 64, (p.cols - c.n0 + 63) / 64);
         const uint32_t bytes = (uint32_t)(a_boxes * (FORM == kDw ? kGrK * 128 : p.a_box * 128)) +
                                (FORM == kDx ? Cfg::kBStage : (uint32_t)(b_boxes * kGrK * 128));
         const int kblocks = (c.depth + kGrK - 1) / kGrK;
@@ -220,15 +215,23 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           mbar_expect_tx(fb, bytes);
           const uint32_t a_dst = smem_u32(ring + s * Cfg::kStageBytes), b_dst = a_dst + RUNS * Cfg::kAStage;
           if (FORM == kDw) {
-            for (int b = 0; b < a_boxes; ++b)
-              tma_load_3d(a_dst + b * (kGrK * 128), &tmA, c.m0 + b * 64, c.row0 + kb * kGrK, 0, fb);
-            for (int b = 0; b < b_boxes; ++b)
-              tma_load_3d(b_dst + b * (kGrK * 128), &tmB, c.n0 + b * 64, c.row0 + kb * kGrK, 0, fb);
+            if (p.chunked_a)
+              tma_load_4d(a_dst, &tmA, 0, c.row0 + kb * kGrK, c.m0 / 64, 0, fb);
+            else
+              for (int b = 0; b < a_boxes; ++b)
+                tma_load_3d(a_dst + b * (kGrK * 128), &tmA, c.m0 + b * 64, c.row0 + kb * kGrK, 0, fb);
+            if (p.chunked_b)
+              tma_load_4d(b_dst, &tmB, 0, c.row0 + kb * kGrK, c.n0 / 64, 0, fb);
+            else
+              for (int b = 0; b < b_boxes; ++b)
+                tma_load_3d(b_dst + b * (kGrK * 128), &tmB, c.n0 + b * 64, c.row0 + kb * kGrK, 0, fb);
           } else {
             for (int b = 0; b < a_boxes; ++b)
               tma_load_3d(a_dst + b * p.a_box * 128, &tmA, kb * kGrK, c.row0 + b * p.a_box, 0, fb);
             if (FORM == kDx) {
               tma_load_3d(b_dst, &tmB, kb * kGrK, c.n0, c.e, fb);
+            } else if (p.chunked_b) {
+              tma_load_4d(b_dst, &tmB, 0, kb * kGrK, c.n0 / 64, c.e, fb);
             } else {
               for (int b = 0; b < b_boxes; ++b)
                 tma_load_3d(b_dst + b * (kGrK * 128), &tmB, c.n0 + b * 64, kb * kGrK, c.e, fb);
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     constexpr uint32_t kAStep = (FORM == kDw ? 2048 : 32) >> 4, kBStep = (FORM == kDx ? 32 : 2048) >> 4;
     const uint64_t a0 = smem_desc(smem_u32(ring), FORM == kDw ? kGrK * 128 : 16, 1024);
     const uint64_t b0 = smem_desc(smem_u32(ring) + RUNS * Cfg::kAStage, FORM == kDx ? 16 : kGrK * 128, 1024);
-    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const int kblocks = (c.depth + kGrK - 1) / kGrK;
       if (kblocks == 0) continue;
@@ -310,10 +313,10 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       drain_phase(smem_u32(&sh->drain), 0);
     }
   } else {
-    // ── epilogue: warps 2..5 read TMEM lanes 32 (warp % 4) .. +32 ──
-    const int q = warp & 3;
+    // ── epilogue: warps 2..9 read TMEM lanes 32 (warp % 4) .. +32, half of the columns each ──
+    const int q = warp & 3, half = (warp - 2) / 4;
     int i = 0;
-    for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
+    for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const bool empty = c.depth == 0;
       const int a = i % kAcc;
@@ -328,9 +331,9 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         if (row >= c.rows) break;  // uniform in the warp
         OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
         const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * RUNS + run) * BN);
-        constexpr int kW = 128 / sizeof(OUT);  // columns a chunk
+        constexpr int kW = 64 / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
 #pragma unroll 1
-        for (int ch = 0; ch < BN / kW; ++ch) {
+        for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
           const int col = c.n0 + ch * kW;
           if (col >= p.cols) break;
           uint32_t r[kW];
@@ -370,6 +373,24 @@ int grouped_timeouts(bool reset) {
     cudaMemcpyToSymbol(g_grouped_timeouts, &zero, sizeof zero);
   }
   return v;
+}
+
+// A row-major bf16 matrix of `cols` columns, a multiple of 64, as chunks of 64 columns:
+// {64, rows, chunks, slices}. One box of box_rows x box_chunks chunks lies in shared
+// memory as the MMA's MN-major operand does, so a K block is one TMA instruction
+// instead of two to four (16-expert case: forward 138 -> 124 us with one run).
+static mtl_status make_chunk_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t slices,
+                                 uint32_t box_rows, uint32_t box_chunks) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return fail(MTL_ERR_CUDA, "gemm_grouped: cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[4] = {64, rows, cols / 64, slices};
+  cuuint64_t strides[3] = {cols * 2, 128, rows * cols * 2};
+  cuuint32_t box[4] = {64, box_rows, box_chunks, 1}, estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MTL_ERR_ARGUMENT, "gemm_grouped: tensor map rejected (CUresult %d)", (int)r);
+  return MTL_OK;
 }
 
 static const char* const kGrName[3] = {"gemm_grouped_bf16", "gemm_grouped_dx_bf16", "gemm_grouped_dw_bf16"};
@@ -441,27 +462,27 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   p.out_rows = K;
   p.groups = E;
   p.vec = la.a[0].ptr % 16 == 0;  // N and K are multiples of 8
-  const bool wide = FORM == kDw ? false : T / E > kGrM;  // two runs of 128 rows a tile
+  const bool wide = false;
   p.a_box = T / E >= kGrM ? kGrM : 32;
   const void *A = reinterpret_cast<const void*>(la.a[1].ptr), *B = reinterpret_cast<const void*>(la.a[2].ptr);
   const int64_t row_tiles = FORM == kDw ? (int64_t)E * ((K + 127) / 128) : std::max<int64_t>(E, (T + 127) / 128);
   const bool narrow = !wide && row_tiles * ((cols + 255) / 256) < la.sm_count;
   const int bn = narrow ? 128 : 256;
+  p.chunked_a = FORM == kDw && K % 64 == 0;
+  p.chunked_b = FORM != kDx && N % 64 == 0;
   CUtensorMap ta, tb;
-  if (mtl_status st = make_bf16_map(&ta, A, FORM == kDx ? N : K, T, 1, FORM == kDw ? kGrK : p.a_box)) return st;
-  if (FORM == kDw) {
-    if (mtl_status st = make_bf16_map(&tb, B, N, T, 1, kGrK)) return st;
-  } else {
-    if (mtl_status st = make_bf16_map(&tb, B, N, K, E, FORM == kDx ? bn : kGrK)) return st;
-  }
+  mtl_status st = p.chunked_a ? make_chunk_map(&ta, A, K, T, 1, kGrK, (wide ? 2 : 1) * kGrM / 64)
+                              : make_bf16_map(&ta, A, FORM == kDx ? N : K, T, 1, FORM == kDw ? kGrK : p.a_box);
+  if (st) return st;
+  st = p.chunked_b ? make_chunk_map(&tb, B, N, FORM == kDw ? T : K, FORM == kDw ? 1 : E, kGrK, bn / 64)
+       : FORM == kDw ? make_bf16_map(&tb, B, N, T, 1, kGrK)
+                     : make_bf16_map(&tb, B, N, K, E, FORM == kDx ? bn : kGrK);
+  if (st) return st;
   const int64_t tile_m = wide ? 256 : 128;
   const int64_t tiles = (FORM == kDw ? (int64_t)E * ((K + tile_m - 1) / tile_m) : T / tile_m + E) * ((cols + bn - 1) / bn);
   cudaError_t e;
   if (wide) {
-    if constexpr (FORM != kDw)
-      e = out ? gr_launch<FORM, 2, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 2, 256, float>(ta, tb, p, tiles, la, s);
-    else
-      e = cudaErrorInvalidValue;
+    e = out ? gr_launch<FORM, 2, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 2, 256, float>(ta, tb, p, tiles, la, s);
   } else if (narrow) {
     e = out ? gr_launch<FORM, 1, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 1, 128, float>(ta, tb, p, tiles, la, s);
   } else {

@@ -43,7 +43,7 @@ struct QuantArgs {
   int64_t R, C, Cp, Rp;
   int64_t rb, cb;      // blocks of 128 rows / columns
   int xrows;           // rows of x that rows_of may name
-  int e5m2, pow2, vec;  // vec: every row of x starts on 16 bytes
+  int pow2, vec;  // vec: every row of x starts on 16 bytes
 };
 
 // ── values ──────────────────────────────────────────────────────────────────
@@ -112,30 +112,58 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(
 struct Scale {
   float s, r;
 };
-__device__ __forceinline__ Scale scale_of(uint32_t bits, int e5m2, int pow2) {
+template <bool E5M2>
+__device__ __forceinline__ Scale scale_of(uint32_t bits, int pow2) {
   bits = max(bits, (uint32_t)(127 - 96) << 23);
-  const float a = __uint_as_float(bits), top = e5m2 ? 57344.0f : 448.0f;
+  const float a = __uint_as_float(bits), top = E5M2 ? 57344.0f : 448.0f;
   if (pow2 && bits < 0x7f800000u) {
     // a = m 2^e, m in [1, 2), and L = 1.75 2^8 or 1.75 2^15
-    const int j = (int)(bits >> 23) - 127 - (e5m2 ? 15 : 8) + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const int j = (int)(bits >> 23) - 127 - (E5M2 ? 15 : 8) + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return Scale{__uint_as_float((uint32_t)(127 + j) << 23), __uint_as_float((uint32_t)(127 - j) << 23)};
   }
   return Scale{__fdiv_rn(a, top), __fdiv_rn(top, a)};
 }
 
-__device__ __forceinline__ uint32_t codes2(float lo, float hi, int e5m2) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+template <bool E5M2>
+__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
-__device__ __forceinline__ uint2 codes8(const Row8& v, const float (&r)[8], int e5m2) {
+template <bool E5M2>
+__device__ __forceinline__ uint2 codes8(const Row8& v, float r) {
   uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    c[i] = codes2(__fmul_rn(v.v[2 * i], r[2 * i]), __fmul_rn(v.v[2 * i + 1], r[2 * i + 1]), e5m2);
+  for (int i = 0; i < 4; ++i) c[i] = codes2<E5M2>(__fmul_rn(v.v[2 * i], r), __fmul_rn(v.v[2 * i + 1], r));
   return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
 }
-__device__ __forceinline__ uint2 codes8(const Row8& v, float r, int e5m2) {
-  const float rs[8] = {r, r, r, r, r, r, r, r};
-  return codes8(v, rs, e5m2);
+
+// The maxima of N values over 16 lanes at once: a step halves the values a lane
+// keeps, so N values take N + log2(16 / N) shuffles where N separate reductions take
+// 4 N, and each lane ends with one value's maximum: value held_by(lane). The two
+// divisions of a scale are then one lane's, and its inverse goes back by a shuffle.
+template <int N>
+__device__ __forceinline__ uint32_t maxima16(uint32_t (&v)[N], int lane16) {
+  int d = 8;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n /= 2, d /= 2) {
+    const bool up = lane16 & d;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const uint32_t mine = up ? v[i + n] : v[i], other = up ? v[i] : v[i + n];
+      v[i] = max(mine, __shfl_xor_sync(0xffffffffu, other, d));
+    }
+  }
+  uint32_t m = v[0];
+#pragma unroll
+  for (; d >= 1; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  return m;
+}
+template <int N>
+__device__ __forceinline__ int held_by(int lane16) {  // value lane16 holds
+  return lane16 / (16 / N);
+}
+template <int N>
+__device__ __forceinline__ int holder_of(int value) {  // the first lane that holds it
+  return value * (16 / N);
 }
 
 // ── row blocks, no transpose ────────────────────────────────────────────────
@@ -143,12 +171,11 @@ __device__ __forceinline__ uint2 codes8(const Row8& v, float r, int e5m2) {
 // neighbouring blocks: the U loads of a thread are in flight together, and the
 // scales of sixteen rows leave as one 64-byte run.
 constexpr int kQuantThreads = 256;
-template <typename T, int U>
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs a, int64_t row_tiles, int64_t col_tiles) {
+template <typename T, int U, bool E5M2>
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs a, unsigned row_tiles, unsigned col_tiles) {
   const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4;
-  const int64_t t = blockIdx.x;
-  const int64_t batch = t / (row_tiles * col_tiles), in = t % (row_tiles * col_tiles);
-  const int64_t r = in / col_tiles * 16 + sub, kb0 = in % col_tiles * U;
+  const unsigned b = blockIdx.x / (row_tiles * col_tiles), in = blockIdx.x % (row_tiles * col_tiles);
+  const int64_t batch = b, r = in / col_tiles * 16 + sub, kb0 = in % col_tiles * U;
   const T* row = source_row<T>(a, batch, r);
   Raw8<T> raw[U];
 #pragma unroll
@@ -156,19 +183,23 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
     raw[u].zero();
     if (row) raw[u].load(row, (kb0 + u) * 128 + lane16 * 8, a.C, a.vec);
   }
+  uint32_t m[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const Row8 v = raw[u].get();
-    uint32_t m = 0;
+    m[u] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, magnitude(v.v[i]));
+    for (int i = 0; i < 8; ++i) m[u] = max(m[u], magnitude(v.v[i]));
+  }
+  const Scale sc = scale_of<E5M2>(maxima16<U>(m, lane16), a.pow2);
+  const int64_t mine = kb0 + held_by<U>(lane16);
+  if (r < a.R && mine < a.cb && lane16 == holder_of<U>(held_by<U>(lane16))) a.s[(batch * a.cb + mine) * a.R + r] = sc.s;
 #pragma unroll
-    for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const Scale sc = scale_of(m, a.e5m2, a.pow2);
-    const int64_t kb = kb0 + u, c = kb * 128 + lane16 * 8;
+  for (int u = 0; u < U; ++u) {
+    const float inv = __shfl_sync(0xffffffffu, sc.r, holder_of<U>(u), 16);
+    const int64_t c = (kb0 + u) * 128 + lane16 * 8;
     if (r < a.R && c < a.Cp)
-      *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8(v, sc.r, a.e5m2);
-    if (r < a.R && kb < a.cb && lane16 == 0) a.s[(batch * a.cb + kb) * a.R + r] = sc.s;
+      *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8<E5M2>(raw[u].get(), inv);
   }
 }
 
@@ -179,16 +210,15 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
 // transposed codes go through a 16 KiB tile whose 8-byte chunks are placed by
 // chunk ^ (column / 8): the sixteen lanes that write one instruction's columns
 // hit all 32 banks, and so do the sixteen that read a transposed row.
-template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) quantize_tile_kernel(QuantArgs a, int square) {
+template <typename T, bool E5M2>
+__global__ void __launch_bounds__(kQuantThreads, 3) quantize_tile_kernel(QuantArgs a, int square) {
   __shared__ uint32_t colmax[8][128];
   __shared__ uint2 turned[128 * 16];
   __shared__ float inv[128];
   __shared__ uint32_t tilemax[8];
   const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  const int64_t batch = t / (a.rb * a.cb), in = t % (a.rb * a.cb);
-  const int64_t rblk = in / a.cb, kb = in % a.cb;
+  const unsigned cb = (unsigned)a.cb, tiles = (unsigned)a.rb * cb, b = blockIdx.x / tiles, in = blockIdx.x % tiles;
+  const int64_t batch = b, rblk = in / cb, kb = in % cb;
   const int64_t r0 = rblk * 128 + sub * 8, c = kb * 128 + lane16 * 8;
   Raw8<T> raw[8];
 #pragma unroll
@@ -220,7 +250,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_tile_kernel(QuantArgs 
     m = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = max(m, tilemax[w]);
-    const Scale sc = scale_of(m, a.e5m2, a.pow2);
+    const Scale sc = scale_of<E5M2>(m, a.pow2);
     if (threadIdx.x == 0) {
       if (a.s) a.s[(batch * a.rb + rblk) * a.cb + kb] = sc.s;
       if (a.st) a.st[(batch * a.cb + kb) * a.rb + rblk] = sc.s;
@@ -229,22 +259,20 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_tile_kernel(QuantArgs 
 #pragma unroll
       for (int p = 0; p < 8; ++p)
         if (r0 + p < a.R && c < a.Cp)
-          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8(raw[p].get(), sc.r, a.e5m2);
+          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p].get(), sc.r);
     }
     if (!a.qt) return;
     if (threadIdx.x < 128) inv[threadIdx.x] = sc.r;
   } else {
     if (a.q) {
+      const Scale sc = scale_of<E5M2>(maxima16<8>(rm, lane16), a.pow2);
+      const int64_t mine = r0 + held_by<8>(lane16);
+      if (mine < a.R && (lane16 & 1) == 0) a.s[(batch * a.cb + kb) * a.R + mine] = sc.s;
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
-        uint32_t m = rm[p];
-#pragma unroll
-        for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const Scale sc = scale_of(m, a.e5m2, a.pow2);
-        const int64_t r = r0 + p;
-        if (r < a.R && c < a.Cp)
-          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8(raw[p].get(), sc.r, a.e5m2);
-        if (r < a.R && lane16 == 0) a.s[(batch * a.cb + kb) * a.R + r] = sc.s;
+        const float rinv = __shfl_sync(0xffffffffu, sc.r, holder_of<8>(p), 16);
+        if (r0 + p < a.R && c < a.Cp)
+          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p].get(), rinv);
       }
     }
     if (!a.qt) return;
@@ -258,7 +286,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_tile_kernel(QuantArgs 
       uint32_t m = 0;
 #pragma unroll
       for (int w = 0; w < 8; ++w) m = max(m, colmax[w][threadIdx.x]);
-      const Scale sc = scale_of(m, a.e5m2, a.pow2);
+      const Scale sc = scale_of<E5M2>(m, a.pow2);
       inv[threadIdx.x] = sc.r;
       const int64_t col = kb * 128 + threadIdx.x;
       if (col < a.C) a.st[(batch * a.rb + rblk) * a.C + col] = sc.s;
@@ -271,7 +299,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_tile_kernel(QuantArgs 
     Row8 down;
 #pragma unroll
     for (int p = 0; p < 8; ++p) down.v[p] = raw[p].get().v[i];
-    turned[(lane16 * 8 + i) * 16 + (sub ^ lane16)] = codes8(down, inv[lane16 * 8 + i], a.e5m2);
+    turned[(lane16 * 8 + i) * 16 + (sub ^ lane16)] = codes8<E5M2>(down, inv[lane16 * 8 + i]);
   }
   __syncthreads();
 #pragma unroll
@@ -326,6 +354,22 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
   return MTL_OK;
 }
 
+template <typename T, bool E5M2>
+static void quantize_launch(const QuantArgs& a, int64_t batch, int block, int sms, cudaStream_t st) {
+  if (block == 1 && !a.qt) {
+    // four blocks of a row a thread group once that leaves every SM several CTAs
+    const unsigned row_tiles = (unsigned)((a.R + 15) / 16);
+    const bool four = batch * row_tiles * a.cb >= 8 * (int64_t)sms;
+    const unsigned col_tiles = (unsigned)(four ? (a.cb + 3) / 4 : a.cb), grid = (unsigned)batch * row_tiles * col_tiles;
+    if (four)
+      quantize_rows_kernel<T, 4, E5M2><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles);
+    else
+      quantize_rows_kernel<T, 1, E5M2><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles);
+  } else {
+    quantize_tile_kernel<T, E5M2><<<(unsigned)(batch * a.rb * a.cb), kQuantThreads, 0, st>>>(a, block == 128);
+  }
+}
+
 mtl_status quantize_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
   QuantArgs a = {};
   a.q = reinterpret_cast<uint8_t*>(la.a[0].ptr);
@@ -342,30 +386,16 @@ mtl_status quantize_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
   a.rb = (a.R + 127) / 128;
   a.cb = (a.C + 127) / 128;
   const int block = la.a[9].i32, bf16 = la.a[10].i32;
-  a.e5m2 = la.a[11].i32;
   a.pow2 = la.a[12].i32;
   a.vec = la.a[4].ptr % 16 == 0 && a.C % (bf16 ? 8 : 4) == 0;
   const int64_t batch = la.nd[0];
   cudaStream_t st = (cudaStream_t)stream;
   if (batch == 0 || a.R == 0 || a.C == 0) return MTL_OK;
-  if (block == 1 && !a.qt) {
-    const int64_t row_tiles = (a.R + 15) / 16;
-    const bool four = batch * row_tiles * a.cb >= 8 * (int64_t)la.sm_count;
-    const int64_t col_tiles = four ? (a.cb + 3) / 4 : a.cb;
-    const unsigned grid = (unsigned)(batch * row_tiles * col_tiles);
-    if (bf16)
-      four ? quantize_rows_kernel<uint16_t, 4><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles)
-           : quantize_rows_kernel<uint16_t, 1><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles);
-    else
-      four ? quantize_rows_kernel<float, 4><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles)
-           : quantize_rows_kernel<float, 1><<<grid, kQuantThreads, 0, st>>>(a, row_tiles, col_tiles);
-  } else {
-    const unsigned grid = (unsigned)(batch * a.rb * a.cb);
-    if (bf16)
-      quantize_tile_kernel<uint16_t><<<grid, kQuantThreads, 0, st>>>(a, block == 128);
-    else
-      quantize_tile_kernel<float><<<grid, kQuantThreads, 0, st>>>(a, block == 128);
-  }
+  const bool e5m2 = la.a[11].i32;
+  if (bf16)
+    e5m2 ? quantize_launch<uint16_t, true>(a, batch, block, la.sm_count, st) : quantize_launch<uint16_t, false>(a, batch, block, la.sm_count, st);
+  else
+    e5m2 ? quantize_launch<float, true>(a, batch, block, la.sm_count, st) : quantize_launch<float, false>(a, batch, block, la.sm_count, st);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "quantize_fp8: %s", cudaGetErrorString(e));
 }
