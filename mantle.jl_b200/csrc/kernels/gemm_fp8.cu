@@ -413,6 +413,132 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
 }
 
+// ── few rows of A: a decode step ────────────────────────────────────────────
+// With M <= 16 the product is a read of B. mma.sync takes its operands from
+// registers, so the codes go from global memory straight into them: a warp holds 16
+// rows of B as the MMA's A operand and the rows of A as its 8 columns. The K index is
+// permuted alike on both sides (a lane's 16-byte word feeds four K = 32 slices' worth
+// of fragments of its row), so every load is a 16-byte word and no shuffle or shared
+// memory is needed. The CTA's eight warps take the K blocks in turn, kAhead at a time
+// to keep loads in flight, and their sums meet in shared memory in warp order.
+// At one row, 8192 x 4096: 14.6 us with the tiles above.
+#ifndef MFEW
+#define MFEW 16
+#endif
+constexpr int kFewThreads = 256;
+
+template <bool A5, bool B5>  // A: the MMA's first operand (B's codes), e5m2 or e4m3
+__device__ __forceinline__ void mma_f8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+#define MTL_MMA_F8(ta, tb)                                                                                       \
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32." ta "." tb ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " \
+               "{%0,%1,%2,%3};"                                                                                  \
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                  \
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+  if constexpr (A5 && B5)
+    MTL_MMA_F8("e5m2", "e5m2");
+  else if constexpr (A5)
+    MTL_MMA_F8("e5m2", "e4m3");
+  else if constexpr (B5)
+    MTL_MMA_F8("e4m3", "e5m2");
+  else
+    MTL_MMA_F8("e4m3", "e4m3");
+#undef MTL_MMA_F8
+}
+
+// Sixteen codes of a row from column k on; those at or past K are zeros, whatever the
+// row's padding holds.
+__device__ __forceinline__ uint4 codes16(const uint8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int i = 0; i < 16; ++i)
+    if (k + i < K) w[i / 4] |= (uint32_t)row[k + i] << (i % 4 * 8);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int MT, bool ROWB, bool A5, bool B5, typename OUT>  // MT: groups of eight rows of A
+__global__ void __launch_bounds__(kFewThreads, 2)
+    gemm_fp8_few_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, const F8Args p) {
+  constexpr int kAhead = MT == 1 ? 2 : 1, kWarps = kFewThreads / 32;
+  __shared__ float sums[kWarps][MT][16][8];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int ntiles = (p.N + 15) / 16, b = blockIdx.x / ntiles, n0 = blockIdx.x % ntiles * 16;
+  const int64_t ld = (p.K + 15) / 16 * 16;
+  const uint8_t* rows_b[2];  // past N: the last row, its sums are not stored
+#pragma unroll
+  for (int h = 0; h < 2; ++h) rows_b[h] = B + ((int64_t)b * p.N + min(n0 + g + h * 8, p.N - 1)) * ld;
+  const float* sa = p.sA + (int64_t)b * p.kblocks * p.M;
+  const float* sb = ROWB ? p.sB + (int64_t)b * p.kblocks * p.N : p.sB + ((int64_t)b * p.nblocks + n0 / 128) * p.kblocks;
+  float acc[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
+
+  for (int kb0 = warp; kb0 < p.kblocks; kb0 += kWarps * kAhead) {
+    uint4 wb[kAhead][2][2], wa[kAhead][MT][2];
+    float fa[kAhead][MT][2], fb[kAhead][2];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int kb = kb0 + u * kWarps, k = kb * 128 + t * 16;
+      const bool in = kb < p.kblocks;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          wb[u][h][e] = in ? codes16(rows_b[h], k + e * 64, p.K) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int row = m * 8 + g;
+        const uint8_t* ra = A + ((int64_t)b * p.M + row) * ld;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          wa[u][m][e] = in && row < p.M ? codes16(ra, k + e * 64, p.K) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col = m * 8 + t * 2 + c;  // the row of A this lane's sums belong to
+          fa[u][m][c] = in && col < p.M ? __ldg(sa + (int64_t)kb * p.M + col) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        fb[u][h] = !in ? 0.0f : __ldg(ROWB ? sb + (int64_t)kb * p.N + min(n0 + g + h * 8, p.N - 1) : sb + kb);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float d[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 x = wb[u][0][e], y = wb[u][1][e], z = wa[u][m][e];
+          mma_f8<B5, A5>(d, x.x, y.x, x.y, y.y, z.x, z.y);
+          mma_f8<B5, A5>(d, x.z, y.z, x.w, y.w, z.z, z.w);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(d[i], fa[u][m][i & 1] * fb[u][i / 2], acc[m][i]);
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[warp][m][g + i / 2 * 8][t * 2 + (i & 1)] = acc[m][i];
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * 128; o += kFewThreads) {
+    const int n = o % 16, m = o / 16;  // sixteen neighbouring columns of a row of C
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v += sums[w][m / 8][n][m % 8];
+    if (m < p.M && n0 + n < p.N) {
+      OUT* c = static_cast<OUT*>(p.C) + ((int64_t)b * p.M + m) * p.N + n0 + n;
+      if constexpr (sizeof(OUT) == 4)
+        *c = v;
+      else
+        *c = __float2bfloat16_rn(v);
+    }
+  }
+}
+
 // ── host side ───────────────────────────────────────────────────────────────
 static int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -471,6 +597,23 @@ static cudaError_t fp8_launch_by(bool rowb, bool bf16, const CUtensorMap& ta, co
   }
   return bf16 ? fp8_launch<BN, GROUPED, false, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
               : fp8_launch<BN, GROUPED, false, float>(ta, tb, p, tiles, sms, device, s);
+}
+
+template <int MT, bool ROWB, bool A5, bool B5>
+static void fp8_few_by(bool bf16, const uint8_t* A, const uint8_t* B, const F8Args& p, unsigned grid, cudaStream_t s) {
+  if (bf16)
+    gemm_fp8_few_kernel<MT, ROWB, A5, B5, __nv_bfloat16><<<grid, kFewThreads, 0, s>>>(A, B, p);
+  else
+    gemm_fp8_few_kernel<MT, ROWB, A5, B5, float><<<grid, kFewThreads, 0, s>>>(A, B, p);
+}
+template <int MT, bool ROWB>
+static cudaError_t fp8_few(bool a5, bool b5, bool bf16, const uint8_t* A, const uint8_t* B, const F8Args& p, cudaStream_t s) {
+  const unsigned grid = (unsigned)((int64_t)p.batch * ((p.N + 15) / 16));
+  if (a5)
+    b5 ? fp8_few_by<MT, ROWB, true, true>(bf16, A, B, p, grid, s) : fp8_few_by<MT, ROWB, true, false>(bf16, A, B, p, grid, s);
+  else
+    b5 ? fp8_few_by<MT, ROWB, false, true>(bf16, A, B, p, grid, s) : fp8_few_by<MT, ROWB, false, false>(bf16, A, B, p, grid, s);
+  return cudaGetLastError();
 }
 
 // What gemm_fp8 and gemm_grouped_fp8 check alike. `rows`: rows of A and C over the
@@ -547,6 +690,15 @@ static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, i
   p.kblocks = (K + 127) / 128;
   p.nblocks = (N + 127) / 128;
   p.vec = la.a[0].ptr % 16 == 0 && (int64_t)N * (out ? 2 : 4) % 16 == 0;
+  const bool rowb = bblock == 1;
+  if constexpr (!GROUPED) {
+    if (M <= MFEW && (int64_t)batch * ((N + 15) / 16) <= INT_MAX) {
+      const uint8_t *a8 = static_cast<const uint8_t*>(A), *b8 = static_cast<const uint8_t*>(B);
+      const cudaError_t e = M <= 8 ? (rowb ? fp8_few<1, true>(fa, fb, out, a8, b8, p, s) : fp8_few<1, false>(fa, fb, out, a8, b8, p, s))
+                                   : (rowb ? fp8_few<2, true>(fa, fb, out, a8, b8, p, s) : fp8_few<2, false>(fa, fb, out, a8, b8, p, s));
+      return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    }
+  }
   // rows a product (dense) or a group on average decide how A is loaded and how
   // many tiles there are; the groups' real sizes are on the device
   const int64_t row_tiles = GROUPED ? std::max<int64_t>(batch, (M + kF8M - 1) / kF8M) : (int64_t)((M + kF8M - 1) / kF8M) * batch;
@@ -558,7 +710,6 @@ static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, i
   if (mtl_status st = make_code_map(&ta, A, K, M, GROUPED ? 1 : batch, p.a_box)) return st;
   if (mtl_status st = make_code_map(&tb, B, K, N, batch, bn)) return st;
   const int64_t tiles = (GROUPED ? (int64_t)batch + M / kF8M : row_tiles) * ((N + bn - 1) / bn);
-  const bool rowb = bblock == 1;
   cudaError_t e = bn == 256   ? fp8_launch_by<256, GROUPED>(rowb, out, ta, tb, p, tiles, la.sm_count, la.device, s)
                   : bn == 128 ? fp8_launch_by<128, GROUPED>(rowb, out, ta, tb, p, tiles, la.sm_count, la.device, s)
                               : fp8_launch_by<64, GROUPED>(rowb, out, ta, tb, p, tiles, la.sm_count, la.device, s);
