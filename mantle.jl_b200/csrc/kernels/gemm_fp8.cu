@@ -37,6 +37,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "../mtl_internal.hpp"
 #include "tc_groups.cuh"
@@ -54,18 +55,21 @@ struct F8Cfg {
   static constexpr uint32_t kTmemCols = kAcc * BN;
   static constexpr uint32_t kAStage = kF8M * kF8K, kStageBytes = kAStage + BN * kF8K;
 };
-constexpr int kF8Scales = 3;  // groups of four K blocks whose scales are on their way or in use
+constexpr int kF8Scales = 2;  // groups of four K blocks whose scales are on their way or in use
+struct F8None {};
+template <bool GROUPED, bool ROWB>
 struct F8Shared {
+  uint4 stage[8][kStageWords];  // per warp of sums: output rows on their way out
+  alignas(16) float sa[kF8Scales][4][kF8M];              // K blocks' scales of the tile's rows of A
+  alignas(16) float sb[kF8Scales][4][ROWB ? 256 : 4];    // and of its rows of B, or of its 128-row blocks
   uint64_t full[8], empty[8], tfull[4], tempty[4], sfull[kF8Scales], sempty[kF8Scales], drain;
   uint32_t tmem;
   int abort;
-  float sa[kF8Scales][4][kF8M];  // K blocks' scales of the tile's rows of A
-  float sb[kF8Scales][4][256];   // and of its rows of B, or of its 128-row blocks
-  GroupTable groups;
+  typename std::conditional<GROUPED, GroupTable, F8None>::type groups;
 };
-template <int BN>
+template <int BN, bool GROUPED, bool ROWB>
 constexpr int f8_smem() {
-  return F8Cfg<BN>::kStages * (int)F8Cfg<BN>::kStageBytes + (int)sizeof(F8Shared) + 1024;
+  return F8Cfg<BN>::kStages * (int)F8Cfg<BN>::kStageBytes + (int)sizeof(F8Shared<GROUPED, ROWB>) + 1024;
 }
 
 struct F8Args {
@@ -98,6 +102,12 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
 __device__ __forceinline__ void scaled_add(float& a, uint32_t p, float s) {
   asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(a) : "f"(__uint_as_float(p)), "f"(s));
 }
+// (x, y) times s as one packed operation.
+__device__ __forceinline__ void scale2(float& x, float& y, float s) {
+  asm("{ .reg .b64 a, b; mov.b64 a, {%0, %1}; mov.b64 b, {%2, %2}; mul.rn.f32x2 a, a, b; mov.b64 {%0, %1}, a; }"
+      : "+f"(x), "+f"(y)
+      : "f"(s));
+}
 __device__ __forceinline__ void tmem_ld_nowait(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32_nowait(addr, r); }
 __device__ __forceinline__ void tmem_ld_nowait(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16_nowait(addr, r); }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
@@ -114,10 +124,10 @@ struct F8Tile {
 template <bool GROUPED>
 struct F8Walk {
   GroupWalk g;
-  __device__ __forceinline__ F8Tile find(const F8Args& p, const GroupTable* groups, int64_t t, int tiles_m, int tiles_n,
-                                         int bn) {
+  template <typename G>  // the group table, grouped
+  __device__ __forceinline__ F8Tile find(const F8Args& p, const G* groups, int64_t t, int tiles_m, int tiles_n, int bn) {
     F8Tile c;
-    if (GROUPED) {
+    if constexpr (GROUPED) {
       g.find(groups, (int)t, tiles_n, kF8M, bn, &c.a_row, &c.rows, &c.n0);
       c.a_b = 0;
       c.b_b = g.e;
@@ -138,38 +148,6 @@ struct F8Walk {
   }
 };
 
-// One row's neighbouring sums to C, from column `col` on.
-template <typename OUT, int COLS>
-__device__ __forceinline__ void store_row(const F8Args& p, int64_t row, int col, const float (&v)[COLS]) {
-  OUT* c = static_cast<OUT*>(p.C) + row * p.N + col;
-  if constexpr (sizeof(OUT) == 4) {
-#pragma unroll
-    for (int i = 0; i < COLS; i += 4) {
-      if (p.vec && col + i + 4 <= p.N) {
-        *reinterpret_cast<float4*>(c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + i + j < p.N) c[i + j] = v[i + j];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < COLS; i += 8) {
-      __nv_bfloat162 b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-      if (p.vec && col + i + 8 <= p.N) {
-        *reinterpret_cast<uint4*>(c + i) = *reinterpret_cast<uint4*>(b);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + i + j < p.N) c[i + j] = j & 1 ? b[j / 2].y : b[j / 2].x;
-      }
-    }
-  }
-}
-
 // BN columns a tile; GROUPED: rows by offsets; ROWB: B's scales per row (else
 // 128 x 128); OUT: float or bf16.
 template <int BN, bool GROUPED, bool ROWB, typename OUT>
@@ -180,7 +158,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
   extern __shared__ unsigned char f8_raw[];
   unsigned char* ring =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
-  F8Shared* sh = reinterpret_cast<F8Shared*>(ring + kStages * Cfg::kStageBytes);
+  auto* sh = reinterpret_cast<F8Shared<GROUPED, ROWB>*>(ring + kStages * Cfg::kStageBytes);
   volatile int* abort = &sh->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -208,14 +186,15 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (GROUPED) build_groups(&sh->groups, p.offsets, p.batch, p.M, kF8M);
+  if constexpr (GROUPED) build_groups(&sh->groups, p.offsets, p.batch, p.M, kF8M);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
 
   const int tiles_m = (p.M + kF8M - 1) / kF8M, tiles_n = (p.N + BN - 1) / BN;
-  const int64_t ntiles = GROUPED ? (int64_t)sh->groups.cum[p.batch] * tiles_n : (int64_t)tiles_m * tiles_n * p.batch;
+  int64_t ntiles = (int64_t)tiles_m * tiles_n * p.batch;
+  if constexpr (GROUPED) ntiles = (int64_t)sh->groups.cum[p.batch] * tiles_n;
   F8Walk<GROUPED> walk;
 
   // 384 threads start with 168 registers each: 128 x 56 + 256 x 224 = 384 x 168
@@ -399,11 +378,30 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             next_acc();
           }
 #pragma unroll
-          for (int i = 0; i < kW; ++i) scaled_add(acc[ch * kW + i], r[ch & 1][i], ROWB ? sr * sb[ch * kW + i] : sr);
+          for (int i = 0; i < kW; i += 4) {
+            float4 f = make_float4(sr, sr, sr, sr);
+            if (ROWB) {  // the same word in every lane; two products an instruction
+              const float4 b = *reinterpret_cast<const float4*>(sb + ch * kW + i);
+              f = b;
+              scale2(f.x, f.y, sr);
+              scale2(f.z, f.w, sr);
+            }
+            scaled_add(acc[ch * kW + i], r[ch & 1][i], f.x);
+            scaled_add(acc[ch * kW + i + 1], r[ch & 1][i + 1], f.y);
+            scaled_add(acc[ch * kW + i + 2], r[ch & 1][i + 2], f.z);
+            scaled_add(acc[ch * kW + i + 3], r[ch & 1][i + 3], f.w);
+          }
         }
         next_scales(kb);
       }
-      if (ok && row < c.rows && col < p.N) store_row<OUT, kCols>(p, c.crow + row, col, acc);
+      if (!ok) break;
+      constexpr int kOut = 64 / sizeof(OUT);  // columns a piece
+      OUT* out = static_cast<OUT*>(p.C) + (c.crow + q * 32) * p.N;
+#pragma unroll
+      for (int i = 0; i < kCols; i += kOut)
+        if (col + i < p.N)
+          store_rows(sh->stage[warp - 4], lane, c.rows - q * 32, out, p.N, col + i, p.vec,
+                     reinterpret_cast<const float(&)[kOut]>(acc[i]));
     }
   }
   tc_fence_before();
@@ -422,10 +420,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 // memory is needed. The CTA's eight warps take the K blocks in turn, kAhead at a time
 // to keep loads in flight, and their sums meet in shared memory in warp order.
 // At one row, 8192 x 4096: 14.6 us with the tiles above.
-#ifndef MFEW
-#define MFEW 16
-#endif
-constexpr int kFewThreads = 256;
+constexpr int kFewThreads = 256, kFewRows = 16;
 
 template <bool A5, bool B5>  // A: the MMA's first operand (B's codes), e5m2 or e4m3
 __device__ __forceinline__ void mma_f8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -575,7 +570,7 @@ template <int BN, bool GROUPED, bool ROWB, typename OUT>
 static cudaError_t fp8_launch(const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p, int64_t tiles, int sms,
                               int device, cudaStream_t s) {
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(gemm_fp8_kernel<BN, GROUPED, ROWB, OUT>, f8_smem<BN>(), device, &done);
+  cudaError_t e = allow_smem(gemm_fp8_kernel<BN, GROUPED, ROWB, OUT>, f8_smem<BN, GROUPED, ROWB>(), device, &done);
   if (e != cudaSuccess) return e;
   // the register split draws on what the block starts with: with less it would wait for good
   static const int regs = [] {
@@ -584,7 +579,7 @@ static cudaError_t fp8_launch(const CUtensorMap& ta, const CUtensorMap& tb, cons
   }();
   if (regs * kF8Threads < 128 * kF8FewRegs + 256 * kF8ManyRegs) return cudaErrorLaunchOutOfResources;
   const int grid = (int)std::min<int64_t>(tiles, sms);
-  gemm_fp8_kernel<BN, GROUPED, ROWB, OUT><<<grid, kF8Threads, f8_smem<BN>(), s>>>(ta, tb, p);
+  gemm_fp8_kernel<BN, GROUPED, ROWB, OUT><<<grid, kF8Threads, f8_smem<BN, GROUPED, ROWB>(), s>>>(ta, tb, p);
   return cudaGetLastError();
 }
 template <int BN, bool GROUPED>
@@ -692,7 +687,7 @@ static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, i
   p.vec = la.a[0].ptr % 16 == 0 && (int64_t)N * (out ? 2 : 4) % 16 == 0;
   const bool rowb = bblock == 1;
   if constexpr (!GROUPED) {
-    if (M <= MFEW && (int64_t)batch * ((N + 15) / 16) <= INT_MAX) {
+    if (M <= kFewRows && (int64_t)batch * ((N + 15) / 16) <= INT_MAX) {
       const uint8_t *a8 = static_cast<const uint8_t*>(A), *b8 = static_cast<const uint8_t*>(B);
       const cudaError_t e = M <= 8 ? (rowb ? fp8_few<1, true>(fa, fb, out, a8, b8, p, s) : fp8_few<1, false>(fa, fb, out, a8, b8, p, s))
                                    : (rowb ? fp8_few<2, true>(fa, fb, out, a8, b8, p, s) : fp8_few<2, false>(fa, fb, out, a8, b8, p, s));

@@ -107,49 +107,6 @@ struct GrWalk {
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16(addr, r); }
 
-// 64 bytes of 32 output rows (a lane holds its row's sums in r), `rows` of them valid,
-// through shared memory, so that an instruction writes whole 64-byte pieces of eight
-// rows instead of 16 bytes of 32 (the weight gradient of the 16-expert case took 253
-// us that way, 186 with these). 16-byte words are placed by word ^ (row / 2 % 4): no
-// bank is hit twice on either side.
-template <typename OUT, int COLS>
-__device__ __forceinline__ void store_rows(const GrArgs& p, uint4* stage, int lane, int rows, OUT* out, int col,
-                                           const uint32_t (&r)[COLS]) {
-  constexpr int kPer = 16 / sizeof(OUT);  // values a word
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    uint4 v;
-    if constexpr (sizeof(OUT) == 4) {
-      v = make_uint4(r[4 * w], r[4 * w + 1], r[4 * w + 2], r[4 * w + 3]);
-    } else {
-      __nv_bfloat162 b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        b[i] = __floats2bfloat162_rn(__uint_as_float(r[8 * w + 2 * i]), __uint_as_float(r[8 * w + 2 * i + 1]));
-      v = *reinterpret_cast<uint4*>(b);
-    }
-    stage[lane * 4 + (w ^ (lane >> 1 & 3))] = v;
-  }
-  __syncwarp();
-  const int w = lane & 3, c = col + w * kPer;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = i * 8 + lane / 4;
-    const uint4 v = stage[row * 4 + (w ^ (row >> 1 & 3))];
-    if (row < rows && c < p.cols) {  // columns come in eights: a word is inside or outside
-      OUT* dst = out + (int64_t)row * p.cols + c;
-      if (p.vec) {
-        *reinterpret_cast<uint4*>(dst) = v;
-      } else {
-        const OUT* e = reinterpret_cast<const OUT*>(&v);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) dst[k] = e[k];
-      }
-    }
-  }
-  __syncwarp();
-}
-
 template <int FORM, int RUNS, int BN, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
@@ -343,7 +300,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           } else {
             tmem_ld_row(tbase + ch * kW, r);
           }
-          store_rows<OUT, kW>(p, sh->stage[warp - 2], lane, c.rows - row, out, col, r);
+          store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
         }
       }
       if (!empty) {
