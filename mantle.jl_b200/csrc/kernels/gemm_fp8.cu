@@ -28,6 +28,10 @@
 // Rows of a partial tile are loaded in boxes of 32, so that a group of a few rows
 // reads few; what the skipped rows hold only reaches rows that are not stored.
 //
+// A dense product of fewer tiles than SMs is split along K over a cluster of CTAs, one
+// tile a cluster: each leaves its sums in its shared memory, and the cluster's warps
+// add them in rank order (distributed shared memory) and store them.
+//
 // Waits are bounded; one that runs out makes the CTA wind down, wait for its own
 // loads and MMAs in flight, free its tensor memory and return.
 
@@ -82,6 +86,7 @@ struct F8Args {
   uint32_t idesc;
   int a_box;  // rows per TMA box of A
   int vec;    // rows of C start on 16 bytes
+  int splits;  // CTAs a tile (a cluster), SPLIT kernels
 };
 
 __device__ int g_fp8_timeouts;
@@ -148,9 +153,22 @@ struct F8Walk {
   }
 };
 
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %4, %5; ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a]; }"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr), "r"(rank));
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // BN columns a tile; GROUPED: rows by offsets; ROWB: B's scales per row (else
-// 128 x 128); OUT: float or bf16.
-template <int BN, bool GROUPED, bool ROWB, typename OUT>
+// 128 x 128); SPLIT: a cluster a tile, the K blocks split over its CTAs; OUT: float
+// or bf16.
+template <int BN, bool GROUPED, bool ROWB, bool SPLIT, typename OUT>
 __global__ void __launch_bounds__(kF8Threads, 1)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const F8Args p) {
   using Cfg = F8Cfg<BN>;
@@ -196,6 +214,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
   int64_t ntiles = (int64_t)tiles_m * tiles_n * p.batch;
   if constexpr (GROUPED) ntiles = (int64_t)sh->groups.cum[p.batch] * tiles_n;
   F8Walk<GROUPED> walk;
+  // this CTA's tiles and K blocks
+  const int rank = SPLIT ? (int)blockIdx.x % p.splits : 0;
+  const int64_t t0 = SPLIT ? blockIdx.x / p.splits : blockIdx.x, tstep = SPLIT ? ntiles : gridDim.x;
+  const int kbeg = SPLIT ? (int)((int64_t)p.kblocks * rank / p.splits) : 0;
+  const int kend = SPLIT ? (int)((int64_t)p.kblocks * (rank + 1) / p.splits) : p.kblocks;
 
   // 384 threads start with 168 registers each: 128 x 56 + 256 x 224 = 384 x 168
   if (warp < 4) {
@@ -206,11 +229,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       int s = 0;
       uint32_t ph = 0;
       int64_t issued = 0;
-      for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
+      for (int64_t t = t0; t < ntiles; t += tstep) {
         const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
         const int boxes = (c.rows + p.a_box - 1) / p.a_box;
         const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+        for (int kb = kbeg; kb < kend; ++kb) {
           if (!wait_phase(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts)) goto producer_done;
           const uint32_t fb = smem_u32(&sh->full[s]);
           mbar_expect_tx(fb, bytes);
@@ -238,8 +261,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     // both operands K-major: rows of 128 bytes, 8-row groups 1024 bytes apart; a K = 32
     // slice is 32 bytes further along the swizzled row
     const uint64_t a0 = smem_desc(smem_u32(ring), 16, 1024), b0 = smem_desc(smem_u32(ring) + Cfg::kAStage, 16, 1024);
-    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
-      for (int kb = 0; kb < p.kblocks; ++kb) {
+    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
+      for (int kb = kbeg; kb < kend; ++kb) {
         ok = wait_warp(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts) &&
              wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts);
         if (!ok) break;
@@ -272,16 +295,16 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
       const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
       const float* sa = p.sA + c.sa;
       const float* sb = ROWB ? p.sB + (int64_t)c.b_b * p.kblocks * p.N + c.n0
                              : p.sB + ((int64_t)c.b_b * p.nblocks + c.n0 / 128) * p.kblocks;
       const int cols = min(BN, p.N - c.n0);
-      for (int kb0 = 0; kb0 < p.kblocks; kb0 += 4) {
+      for (int kb0 = kbeg; kb0 < kend; kb0 += 4) {
         ok = wait_warp(smem_u32(&sh->sempty[s]), ph ^ 1, abort, &g_fp8_timeouts);
         if (!ok) break;
-        for (int j = 0; j < min(4, p.kblocks - kb0); ++j) {
+        for (int j = 0; j < min(4, kend - kb0); ++j) {
           const uint32_t da = smem_u32(sh->sa[s][j]), db = smem_u32(sh->sb[s][j]);
           const int64_t kb = kb0 + j;
 #pragma unroll
@@ -304,6 +327,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  if constexpr (SPLIT) {  // the two meetings of the cluster, see the other warps
+    cluster_sync();
+    cluster_sync();
+  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8ManyRegs));
     // ── scaled sums: warp reads TMEM lanes 32 q .. +32, columns half * kCols .. ──
@@ -311,7 +338,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     int a = 0, s = 0;
     uint32_t aph = 0, sph = 0;
     bool ok = true;
-    for (int64_t t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
       const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
       const int row = q * 32 + lane, col = c.n0 + half * kCols;
       const bool busy = q * 32 < c.rows;  // uniform in the warp
@@ -320,7 +347,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
       // K block kb's accumulator is there, and every fourth time the next four blocks' scales
       auto arrived = [&](int kb) {
-        bool here = (kb & 3) != 0 || wait_warp(smem_u32(&sh->sfull[s]), sph, abort, &g_fp8_timeouts);
+        bool here = ((kb - kbeg) & 3) != 0 || wait_warp(smem_u32(&sh->sfull[s]), sph, abort, &g_fp8_timeouts);
         here = here && wait_warp(smem_u32(&sh->tfull[a]), aph, abort, &g_fp8_timeouts);
         tc_fence_after();
         return here;
@@ -336,7 +363,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
       };
       auto next_scales = [&](int kb) {  // after K block kb
-        if ((kb & 3) == 3 || kb + 1 == p.kblocks) {
+        if (((kb - kbeg) & 3) == 3 || kb + 1 == kend) {
           give_back(&sh->sempty[s]);
           if (++s == kF8Scales) {
             s = 0;
@@ -345,7 +372,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
       };
       if (!busy) {
-        for (int kb = 0; ok && kb < p.kblocks; ++kb) {
+        for (int kb = kbeg; ok && kb < kend; ++kb) {
           ok = arrived(kb);
           if (!ok) break;
           give_back(&sh->tempty[a]);
@@ -360,13 +387,13 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       uint32_t r[2][kW];
       const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kCols);
 #pragma unroll 1
-      for (int kb = 0; kb < p.kblocks; ++kb) {
+      for (int kb = kbeg; kb < kend; ++kb) {
         ok = arrived(kb);
         if (!ok) break;
         const uint32_t from = lanes + (uint32_t)(a * BN);
         tmem_ld_nowait(from, r[0]);
-        const float sr = ROWB ? sh->sa[s][kb & 3][row] : sh->sa[s][kb & 3][row] * sh->sb[s][kb & 3][BN == 256 ? half : 0];
-        const float* sb = sh->sb[s][kb & 3] + half * kCols;
+        const float sr = ROWB ? sh->sa[s][(kb - kbeg) & 3][row] : sh->sa[s][(kb - kbeg) & 3][row] * sh->sb[s][(kb - kbeg) & 3][BN == 256 ? half : 0];
+        const float* sb = sh->sb[s][(kb - kbeg) & 3] + half * kCols;
 #pragma unroll
         for (int ch = 0; ch < kChunks; ++ch) {
           tmem_wait_ld(r[ch & 1]);
@@ -395,6 +422,13 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         next_scales(kb);
       }
       if (!ok) break;
+      if constexpr (SPLIT) {  // the ring is free: every load landed and every MMA is done
+        // four columns of a row a word, the rows of a word's columns next to one another
+        float4* part = reinterpret_cast<float4*>(ring) + (half * kCols / 4) * kF8M + row;
+#pragma unroll
+        for (int i = 0; i < kCols; i += 4) part[i / 4 * kF8M] = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        break;
+      }
       constexpr int kOut = 64 / sizeof(OUT);  // columns a piece
       OUT* out = static_cast<OUT*>(p.C) + (c.crow + q * 32) * p.N;
 #pragma unroll
@@ -402,6 +436,34 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         if (col + i < p.N)
           store_rows(sh->stage[warp - 4], lane, c.rows - q * 32, out, p.N, col + i, p.vec,
                      reinterpret_cast<const float(&)[kOut]>(acc[i]));
+    }
+    if constexpr (SPLIT) {
+      cluster_sync();  // every CTA of the tile has its sums in shared memory, column by column
+      const F8Tile c = walk.find(p, &sh->groups, t0, tiles_m, tiles_n, BN);
+      constexpr int kOut = 64 / sizeof(OUT);
+      const int quarters = (c.rows + 31) / 32, pieces = (min(BN, p.N - c.n0) + kOut - 1) / kOut;
+      for (int i = rank * 8 + warp - 4; i < quarters * pieces; i += p.splits * 8) {
+        const int rq = i % quarters, col = i / quarters * kOut;
+        const uint32_t at = smem_u32(ring) + (uint32_t)((col / 4 * kF8M + rq * 32 + lane) * 16);
+        float v[kOut];
+#pragma unroll
+        for (int k = 0; k < kOut; ++k) v[k] = 0.0f;
+        for (int r = 0; r < p.splits; ++r) {
+          float4 u[kOut / 4];
+#pragma unroll
+          for (int k = 0; k < kOut / 4; ++k) u[k] = ld_cluster(at + (uint32_t)(k * kF8M * 16), (uint32_t)r);
+#pragma unroll
+          for (int k = 0; k < kOut / 4; ++k) {
+            v[4 * k] += u[k].x;
+            v[4 * k + 1] += u[k].y;
+            v[4 * k + 2] += u[k].z;
+            v[4 * k + 3] += u[k].w;
+          }
+        }
+        store_rows(sh->stage[warp - 4], lane, c.rows - rq * 32, static_cast<OUT*>(p.C) + (c.crow + rq * 32) * p.N, p.N,
+                   c.n0 + col, p.vec, v);
+      }
+      cluster_sync();  // no CTA leaves while others read its sums
     }
   }
   tc_fence_before();
@@ -566,32 +628,55 @@ int fp8_timeouts(bool reset) {
   return v;
 }
 
-template <int BN, bool GROUPED, bool ROWB, typename OUT>
+template <int BN, bool GROUPED, bool ROWB, bool SPLIT, typename OUT>
 static cudaError_t fp8_launch(const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p, int64_t tiles, int sms,
                               int device, cudaStream_t s) {
+  auto kernel = gemm_fp8_kernel<BN, GROUPED, ROWB, SPLIT, OUT>;
+  constexpr int smem = f8_smem<BN, GROUPED, ROWB>();
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(gemm_fp8_kernel<BN, GROUPED, ROWB, OUT>, f8_smem<BN, GROUPED, ROWB>(), device, &done);
+  cudaError_t e = allow_smem(kernel, smem, device, &done);
   if (e != cudaSuccess) return e;
   // the register split draws on what the block starts with: with less it would wait for good
-  static const int regs = [] {
+  static const int regs = [&] {
     cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, gemm_fp8_kernel<BN, GROUPED, ROWB, OUT>) == cudaSuccess ? at.numRegs : 0;
+    return cudaFuncGetAttributes(&at, kernel) == cudaSuccess ? at.numRegs : 0;
   }();
   if (regs * kF8Threads < 128 * kF8FewRegs + 256 * kF8ManyRegs) return cudaErrorLaunchOutOfResources;
-  const int grid = (int)std::min<int64_t>(tiles, sms);
-  gemm_fp8_kernel<BN, GROUPED, ROWB, OUT><<<grid, kF8Threads, f8_smem<BN, GROUPED, ROWB>(), s>>>(ta, tb, p);
-  return cudaGetLastError();
+  if constexpr (SPLIT) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * p.splits));
+    cfg.blockDim = dim3(kF8Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  } else {
+    kernel<<<(int)std::min<int64_t>(tiles, sms), kF8Threads, smem, s>>>(ta, tb, p);
+    return cudaGetLastError();
+  }
+}
+template <int BN, bool GROUPED, bool ROWB, typename OUT>
+static cudaError_t fp8_launch_split(const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p, int64_t tiles, int sms,
+                                    int device, cudaStream_t s) {
+  if constexpr (!GROUPED)
+    if (p.splits > 1) return fp8_launch<BN, GROUPED, ROWB, true, OUT>(ta, tb, p, tiles, sms, device, s);
+  return fp8_launch<BN, GROUPED, ROWB, false, OUT>(ta, tb, p, tiles, sms, device, s);
 }
 template <int BN, bool GROUPED>
 static cudaError_t fp8_launch_by(bool rowb, bool bf16, const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p,
                                  int64_t tiles, int sms, int device, cudaStream_t s) {
   if constexpr (!GROUPED) {
     if (rowb)
-      return bf16 ? fp8_launch<BN, GROUPED, true, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
-                  : fp8_launch<BN, GROUPED, true, float>(ta, tb, p, tiles, sms, device, s);
+      return bf16 ? fp8_launch_split<BN, GROUPED, true, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
+                  : fp8_launch_split<BN, GROUPED, true, float>(ta, tb, p, tiles, sms, device, s);
   }
-  return bf16 ? fp8_launch<BN, GROUPED, false, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
-              : fp8_launch<BN, GROUPED, false, float>(ta, tb, p, tiles, sms, device, s);
+  return bf16 ? fp8_launch_split<BN, GROUPED, false, __nv_bfloat16>(ta, tb, p, tiles, sms, device, s)
+              : fp8_launch_split<BN, GROUPED, false, float>(ta, tb, p, tiles, sms, device, s);
 }
 
 template <int MT, bool ROWB, bool A5, bool B5>
@@ -660,12 +745,36 @@ mtl_status gemm_grouped_fp8_check(const LaunchArgs& la, const uint64_t* bytes) {
   return MTL_OK;
 }
 
-// The widest tile whose tiles reach every SM; with fewer tiles than that, the
-// narrowest: tiles half as wide load A twice as often, but idle SMs cost more.
-static int fp8_tile_n(int64_t row_tiles, int64_t N, int sms) {
-  for (int bn : {256, 128})
-    if (row_tiles * ((N + bn - 1) / bn) >= sms) return bn;
-  return 64;
+// Tile width and K parts of a launch, by a model of what was measured: the rounds of
+// K blocks, a block's time (a chain of hand-offs between loads, MMAs and sums) 550,
+// 420 and 350 ns for 256, 128 and 64 columns; a split costs 3 us and a quarter of a
+// microsecond per 32 x 64 sums it adds. It is right to some percent where it was
+// checked (us): 32 x 4096 x 4096 one part 14.2 (64 columns), two 11.2, four 10.6 (128
+// columns); 64 x 1024 x 8192 27.7, 17.7, 12.5; 512 x 1024 x 8192 25.3, 17.8, 16.6;
+// 256 x 4096 x 4096 15.6 whole, 15.4 and 17.2 split. Clusters of four leave SMs of a
+// GPC unused (seven eighths of them are counted on); clusters of eight fit worse still
+// (20 us where four took 12.5).
+struct F8Shape {
+  int bn, splits;
+};
+static F8Shape fp8_shape(int64_t row_tiles, int rows, int64_t N, int kblocks, int sms, bool may_split) {
+  F8Shape best = {256, 1};
+  double least = 1e30;
+  const int block_ns[3] = {550, 420, 350}, quarters = (std::min(rows, kF8M) + 31) / 32;
+  for (int i = 0; i < 3; ++i) {
+    const int bn = 256 >> i;
+    const int64_t tiles = row_tiles * ((N + bn - 1) / bn);
+    for (int splits = 1; splits <= (may_split ? 4 : 1); splits *= 2) {
+      if (splits > 1 && (tiles * splits > (splits == 2 ? sms : sms * 7 / 8) || splits * 2 > kblocks)) break;
+      const double t = (double)((tiles * splits + sms - 1) / sms) * ((kblocks + splits - 1) / splits) * block_ns[i] +
+                       (splits > 1 ? 3000 + 250 * quarters * (bn / 64) : 0);
+      if (t < least) {
+        least = t;
+        best = {bn, splits};
+      }
+    }
+  }
+  return best;
 }
 
 template <bool GROUPED>
@@ -697,7 +806,9 @@ static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, i
   // rows a product (dense) or a group on average decide how A is loaded and how
   // many tiles there are; the groups' real sizes are on the device
   const int64_t row_tiles = GROUPED ? std::max<int64_t>(batch, (M + kF8M - 1) / kF8M) : (int64_t)((M + kF8M - 1) / kF8M) * batch;
-  const int bn = fp8_tile_n(row_tiles, N, la.sm_count);
+  const F8Shape shape = fp8_shape(row_tiles, GROUPED ? M / batch : M, N, p.kblocks, la.sm_count, !GROUPED);
+  const int bn = shape.bn;
+  p.splits = shape.splits;
   p.a_box = (GROUPED ? M / batch : M) >= kF8M ? kF8M : 32;
   // kind::f8f6f4: fp32 accumulator (bit 4), formats at bits 7 and 10, N >> 3 at bit 17, M >> 4 at bit 24
   p.idesc = (1u << 4) | ((uint32_t)fa << 7) | ((uint32_t)fb << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kF8M >> 4) << 24);

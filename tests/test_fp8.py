@@ -226,7 +226,10 @@ def operands(bt, m, n, k, bblock, fa, fb, seed):
     (1, 1, 1, 1, 0, 0, 0), (1, 1, 256, 128, 0, 0, 1), (1, 3, 1000, 520, 1, 0, 0), (2, 16, 384, 1024, 0, 1, 1),
     (1, 17, 129, 257, 0, 0, 0), (3, 200, 264, 72, 0, 0, 0), (1, 128, 256, 640, 1, 1, 1), (1, 300, 515, 1000, 0, 0, 1),
     (2, 1000, 1000, 1000, 0, 0, 0), (1, 129, 4099, 130, 0, 0, 1), (1, 2500, 4200, 384, 0, 0, 0), (1, 5, 4096, 2048, 0, 0, 1),
-    (1, 40, 8200, 2056, 0, 0, 0)])
+    (1, 40, 8200, 2056, 0, 0, 0),
+    # fewer tiles than SMs: the K blocks split over two to eight CTAs, uneven parts, partial row quarters
+    (1, 20, 1000, 4100, 0, 0, 1), (1, 129, 640, 8190, 0, 0, 0), (2, 33, 264, 1100, 1, 0, 1), (1, 256, 8200, 700, 0, 0, 0),
+    (1, 65, 77, 2100, 0, 0, 0), (1, 512, 1024, 3000, 0, 0, 1)])
 def test_gemm_fp8(dev, bblock, bt, m, n, k, fa, fb, out):
     qa, sa, qb, sb, va, vb = operands(bt, m, n, k, bblock, fa, fb, m + n + k)
     c = torch.full((bt, m, n), float("nan"), dtype=torch.bfloat16 if out else torch.float32, device="cuda")
@@ -234,6 +237,18 @@ def test_gemm_fp8(dev, bblock, bt, m, n, k, fa, fb, out):
     torch.cuda.synchronize()
     check_product(c, va @ vb.transpose(1, 2), va.abs() @ vb.abs().transpose(1, 2), -(-k // 128), out)
     assert M.kernel_timeouts() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(3, 600, 3000), (70, 600, 3000), (700, 1500, 900)])
+def test_gemm_fp8_gives_the_same_bits_again(dev, m, n, k):
+    # split or not, the order of the sums is fixed
+    qa, sa, qb, sb, _, _ = operands(1, m, n, k, 128, 0, 0, 5)
+    c = torch.full((3, m, n), float("nan"), device="cuda")
+    for i in range(3):
+        M.launch(M.kernels.gemm_fp8, (c[i], qa, sa, qb, sb, m, n, k, 128, 0, 0, 0), 1, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(c[0], c[1]) and torch.equal(c[0], c[2])
 
 
 @pytest.mark.gpu
