@@ -160,11 +160,6 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
                : "r"(addr), "r"(rank));
   return v;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 // BN columns a tile; GROUPED: rows by offsets; ROWB: B's scales per row (else
 // 128 x 128); SPLIT: a cluster a tile, the K blocks split over its CTAs; OUT: float
 // or bf16.
@@ -224,35 +219,36 @@ __global__ void __launch_bounds__(kF8Threads, 1)
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8FewRegs));
   if (warp == 0) {
-    // ── TMA producer ──
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      int64_t issued = 0;
-      for (int64_t t = t0; t < ntiles; t += tstep) {
-        const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
-        const int boxes = (c.rows + p.a_box - 1) / p.a_box;
-        const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
-        for (int kb = kbeg; kb < kend; ++kb) {
-          if (!wait_phase(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts)) goto producer_done;
-          const uint32_t fb = smem_u32(&sh->full[s]);
+    // ── TMA producer (the whole warp waits, one lane issues) ──
+    int s = 0;
+    uint32_t ph = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
+      const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
+      const int boxes = (c.rows + p.a_box - 1) / p.a_box;
+      const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
+      for (int kb = kbeg; kb < kend; ++kb) {
+        ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t fb = smem_u32(&sh->full[s]), dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes);
           mbar_expect_tx(fb, bytes);
-          const uint32_t dst = smem_u32(ring + s * Cfg::kStageBytes);
+          tma_load_3d(dst + Cfg::kAStage, &tmB, kb * kF8K, c.n0, c.b_b, fb);
           for (int r = 0; r < boxes; ++r)
             tma_load_3d(dst + r * p.a_box * kF8K, &tmA, kb * kF8K, c.a_row + r * p.a_box, c.a_b, fb);
-          tma_load_3d(dst + Cfg::kAStage, &tmB, kb * kF8K, c.n0, c.b_b, fb);
-          ++issued;
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1;
-          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
         }
       }
-    producer_done:
-      if (*abort)  // the loads in flight land before the CTA leaves
-        for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-          drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
     }
+    if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
+      for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+        drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
   } else if (warp == 1) {
     // ── MMA issuer (the whole warp waits, one lane issues) ──
     int s = 0, a = 0;

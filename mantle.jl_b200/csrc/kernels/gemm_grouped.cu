@@ -151,12 +151,13 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   GrWalk<FORM, RUNS, BN> walk;
 
   if (warp == 0) {
-    // ── TMA producer ──
-    if (lane == 0) {
+    // ── TMA producer (the whole warp waits, one lane issues) ──
+    {
+      bool ok = true;
       int s = 0;
       uint32_t ph = 0;
       int64_t issued = 0;
-      for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
+      for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
         const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
         // a chunked operand comes in one box, zeros past its edges; other boxes that would
         // lie wholly past the output's rows or columns are not loaded:
@@ -167,10 +168,12 @@ __global__ void __launch_bounds__(kGrThreads, 1)
                                (FORM == kDx ? Cfg::kBStage : (uint32_t)(b_boxes * kGrK * 128));
         const int kblocks = (c.depth + kGrK - 1) / kGrK;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!wait_phase(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts)) goto producer_done;
+          ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts);
+          if (!ok) break;
+          if (elect_one()) {
           const uint32_t fb = smem_u32(&sh->full[s]);
           mbar_expect_tx(fb, bytes);
-          const uint32_t a_dst = smem_u32(ring + s * Cfg::kStageBytes), b_dst = a_dst + RUNS * Cfg::kAStage;
+          const uint32_t a_dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes), b_dst = a_dst + RUNS * Cfg::kAStage;
           if (FORM == kDw) {
             if (p.chunked_a)
               tma_load_4d(a_dst, &tmA, 0, c.row0 + kb * kGrK, c.m0 / 64, 0, fb);
@@ -194,6 +197,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
                 tma_load_3d(b_dst + b * (kGrK * 128), &tmB, c.n0 + b * 64, kb * kGrK, c.e, fb);
             }
           }
+          }
+          __syncwarp();
           ++issued;
           if (++s == kStages) {
             s = 0;
@@ -201,8 +206,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           }
         }
       }
-    producer_done:
-      if (*abort)  // the loads in flight land before the CTA leaves
+      if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
         for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
           drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
     }
