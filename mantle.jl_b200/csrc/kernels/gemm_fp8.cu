@@ -717,8 +717,8 @@ static mtl_status fp8_check_common(const char* who, const LaunchArgs& la, const 
   if ((fa | fb | out) & ~1)
     return fail(MTL_ERR_ARGUMENT, "%s: formats are 0 (e4m3) or 1 (e5m2), the output 0 (fp32) or 1 (bf16), got %d, %d, %d", who, fa, fb, out);
   const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
-  const uint64_t need[5] = {(uint64_t)(rows * N * (out ? 2 : 4)), (uint64_t)(rows * up16(K)), (uint64_t)(kb * rows * 4),
-                            (uint64_t)(batch * N * up16(K)), (uint64_t)(batch * kb * (bblock == 1 ? N : nb) * 4)};
+  const uint64_t need[5] = {bytes_of({rows, N, out ? 2 : 4}), bytes_of({rows, up16(K)}), bytes_of({kb, rows, 4}),
+                            bytes_of({batch, N, up16(K)}), bytes_of({batch, kb, bblock == 1 ? N : nb, 4})};
   const char* what[5] = {"C", "A", "A's scales", "B", "B's scales"};
   const unsigned align[5] = {out ? 1u : 3u, 15, 3, 15, 3};
   for (int i = 0; i < 5; ++i) {

@@ -371,10 +371,12 @@ static mtl_status gr_check(const LaunchArgs& la, const uint64_t* bytes) {
   if (FORM != kDw && (FORM == kFwd ? K : N) == 0) return fail(MTL_ERR_ARGUMENT, "%s: the contraction must be positive", who);
   if (out != 0 && out != 1) return fail(MTL_ERR_ARGUMENT, "%s: the output type is 0 (fp32) or 1 (bf16), got %d", who, out);
   if (E > kMaxGroups) return fail(MTL_ERR_UNSUPPORTED, "%s: more than %d groups", who, kMaxGroups);
-  const int64_t w = E * K * N, x = T * K, y = T * N, wide = out ? 2 : 4;
-  const uint64_t need[4] = {(uint64_t)((FORM == kFwd ? y : FORM == kDx ? x : w) * wide),
-                            (uint64_t)((FORM == kDx ? y : x) * 2), (uint64_t)((FORM == kDw ? y : w) * 2),
-                            (uint64_t)(E + 1) * 4};
+  const int wide = out ? 2 : 4;
+  auto w = [&](int size) { return bytes_of({E, K, N, size}); };
+  auto x = [&](int size) { return bytes_of({T, K, size}); };
+  auto y = [&](int size) { return bytes_of({T, N, size}); };
+  const uint64_t need[4] = {FORM == kFwd ? y(wide) : FORM == kDx ? x(wide) : w(wide), FORM == kDx ? y(2) : x(2),
+                            FORM == kDw ? y(2) : w(2), bytes_of({E + 1, 4})};
   const char* what[3][4] = {{"Y", "X", "W", "the offsets"}, {"dX", "dY", "W", "the offsets"}, {"dW", "X", "dY", "the offsets"}};
   const unsigned align[4] = {out ? 1u : 3u, 15, 15, 3};
   for (int i = 0; i < 4; ++i) {

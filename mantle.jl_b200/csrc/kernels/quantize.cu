@@ -22,7 +22,6 @@
 // Both kernels are bound by HBM: a value is read once, kept in registers, and
 // written once per output. See the figures at each kernel.
 
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -70,6 +69,13 @@ struct Raw8<uint16_t> {
       u = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
   }
+  // magnitudes, two to a word: m[i] = max(m[i], |values 2 i and 2 i + 1|)
+  static constexpr int kWords = 4;
+  __device__ __forceinline__ uint32_t mag(int i) const { return (i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w) & 0x7fff7fffu; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  // the fp32 bits of column c's magnitude, and of the largest in a word
+  static __device__ __forceinline__ uint32_t column(const uint32_t (&m)[4], int c) { return c & 1 ? m[c / 2] & 0xffff0000u : m[c / 2] << 16; }
+  static __device__ __forceinline__ uint32_t whole(uint32_t m) { return max(m & 0xffff0000u, m << 16); }
   __device__ __forceinline__ Row8 get() const {
     return Row8{{bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y), bf16_lo(u.z), bf16_hi(u.z), bf16_lo(u.w),
                  bf16_hi(u.w)}};
@@ -91,6 +97,11 @@ struct Raw8<float> {
       b = make_float4(w[4], w[5], w[6], w[7]);
     }
   }
+  static constexpr int kWords = 8;
+  __device__ __forceinline__ uint32_t mag(int i) const { return __float_as_uint(get().v[i]) & 0x7fffffffu; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ uint32_t column(const uint32_t (&m)[8], int c) { return m[c]; }
+  static __device__ __forceinline__ uint32_t whole(uint32_t m) { return m; }
   __device__ __forceinline__ Row8 get() const { return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
 };
 
@@ -107,8 +118,6 @@ __device__ __forceinline__ const T* source_row(const QuantArgs& a, int64_t batch
   return x + (batch * a.R + r) * a.C;
 }
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 struct Scale {
   float s, r;
 };
@@ -124,16 +133,26 @@ __device__ __forceinline__ Scale scale_of(uint32_t bits, int pow2) {
   return Scale{__fdiv_rn(a, top), __fdiv_rn(top, a)};
 }
 
+// Four codes, the first in the low byte.
 template <bool E5M2>
-__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  uint32_t u;
+  if constexpr (E5M2)
+    asm("{ .reg .b16 l, h; cvt.rn.satfinite.e5m2x2.f32 l, %2, %1; cvt.rn.satfinite.e5m2x2.f32 h, %4, %3; mov.b32 %0, {l, h}; }"
+        : "=r"(u)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+  else
+    asm("{ .reg .b16 l, h; cvt.rn.satfinite.e4m3x2.f32 l, %2, %1; cvt.rn.satfinite.e4m3x2.f32 h, %4, %3; mov.b32 %0, {l, h}; }"
+        : "=r"(u)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+  return u;
 }
 template <bool E5M2>
 __device__ __forceinline__ uint2 codes8(const Row8& v, float r) {
-  uint32_t c[4];
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = codes2<E5M2>(__fmul_rn(v.v[2 * i], r), __fmul_rn(v.v[2 * i + 1], r));
-  return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(v.v[i], r);
+  return make_uint2(codes4<E5M2>(x[0], x[1], x[2], x[3]), codes4<E5M2>(x[4], x[5], x[6], x[7]));
 }
 
 // The maxima of N values over 16 lanes at once: a step halves the values a lane
@@ -186,10 +205,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
   uint32_t m[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const Row8 v = raw[u].get();
-    m[u] = 0;
+    uint32_t w = raw[u].mag(0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[u] = max(m[u], magnitude(v.v[i]));
+    for (int i = 1; i < Raw8<T>::kWords; ++i) w = Raw8<T>::larger(w, raw[u].mag(i));
+    m[u] = Raw8<T>::whole(w);
   }
   const Scale sc = scale_of<E5M2>(maxima16<U>(m, lane16), a.pow2);
   const int64_t mine = kb0 + held_by<U>(lane16);
@@ -211,8 +230,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
 // chunk ^ (column / 8): the sixteen lanes that write one instruction's columns
 // hit all 32 banks, and so do the sixteen that read a transposed row.
 template <typename T, bool E5M2>
-__global__ void __launch_bounds__(kQuantThreads, 3) quantize_tile_kernel(QuantArgs a, int square) {
-  __shared__ uint32_t colmax[8][128];
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantize_tile_kernel(QuantArgs a, int square) {
+  __shared__ alignas(16) uint32_t colmax[8][128];
   __shared__ uint2 turned[128 * 16];
   __shared__ float inv[128];
   __shared__ uint32_t tilemax[8];
@@ -227,17 +246,20 @@ __global__ void __launch_bounds__(kQuantThreads, 3) quantize_tile_kernel(QuantAr
     raw[p].zero();
     if (row) raw[p].load(row, c, a.C, a.vec);
   }
-  uint32_t cm[8] = {0, 0, 0, 0, 0, 0, 0, 0}, rm[8];
+  using Raw = Raw8<T>;
+  uint32_t cm[Raw::kWords], rm[8];
+#pragma unroll
+  for (int i = 0; i < Raw::kWords; ++i) cm[i] = 0;
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
-    const Row8 v = raw[p].get();
-    rm[p] = 0;
+    uint32_t row = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t m = magnitude(v.v[i]);
-      rm[p] = max(rm[p], m);
-      cm[i] = max(cm[i], m);
+    for (int i = 0; i < Raw::kWords; ++i) {
+      const uint32_t m = raw[p].mag(i);
+      row = Raw::larger(row, m);
+      cm[i] = Raw::larger(cm[i], m);
     }
+    rm[p] = Raw::whole(row);
   }
   if (square) {
     uint32_t m = 0;
@@ -277,9 +299,12 @@ __global__ void __launch_bounds__(kQuantThreads, 3) quantize_tile_kernel(QuantAr
     }
     if (!a.qt) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t m = max(cm[i], __shfl_xor_sync(0xffffffffu, cm[i], 16));
-      if ((threadIdx.x & 31) < 16) colmax[warp][lane16 * 8 + i] = m;
+    for (int i = 0; i < Raw::kWords; ++i) cm[i] = Raw::larger(cm[i], __shfl_xor_sync(0xffffffffu, cm[i], 16));
+    if ((threadIdx.x & 31) < 16) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4)
+        *reinterpret_cast<uint4*>(&colmax[warp][lane16 * 8 + i]) =
+            make_uint4(Raw::column(cm, i), Raw::column(cm, i + 1), Raw::column(cm, i + 2), Raw::column(cm, i + 3));
     }
     __syncthreads();
     if (threadIdx.x < 128) {
@@ -335,10 +360,9 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
   if (q != s || qt != st || (!q && !qt))
     return fail(MTL_ERR_ARGUMENT, "quantize_fp8: give the codes and the scales of the row form, of the transposed form, or of both");
   const int64_t rb = (R + 127) / 128, cb = (C + 127) / 128, per = la.a[10].i32 ? 2 : 4;
-  const int64_t scales = block == 128 ? rb * cb : 0;
-  const uint64_t need[6] = {(uint64_t)(batch * R * up(C, 16)), (uint64_t)(batch * 4 * (scales ? scales : cb * R)),
-                            (uint64_t)(batch * C * up(R, 16)), (uint64_t)(batch * 4 * (scales ? scales : rb * C)),
-                            (uint64_t)((gather ? 1 : batch) * xrows * C * per), (uint64_t)(R * 4)};
+  const bool square = block == 128;
+  const uint64_t need[6] = {bytes_of({batch, R, up(C, 16)}), bytes_of({batch, cb, square ? rb : R, 4}), bytes_of({batch, C, up(R, 16)}),
+                            bytes_of({batch, rb, square ? cb : C, 4}), bytes_of({gather ? 1 : batch, xrows, C, per}), bytes_of({R, 4})};
   const char* what[6] = {"the codes", "the scales", "the transposed codes", "the transposed scales", "the input", "rows_of"};
   const unsigned align[6] = {15, 3, 15, 3, la.a[10].i32 ? 1u : 3u, 3};
   for (int i = 0; i < 6; ++i) {
@@ -349,7 +373,7 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
     if (la.a[i].ptr & align[i])
       return fail(MTL_ERR_ARGUMENT, "quantize_fp8: %s must be %u-byte aligned", what[i], align[i] + 1);
   }
-  if (batch * std::max<int64_t>(1, (R + 15) / 16) * std::max<int64_t>(1, cb) > INT_MAX)
+  if (bytes_of({batch, std::max<int64_t>(1, (R + 15) / 16), std::max<int64_t>(1, cb)}) > INT_MAX)
     return fail(MTL_ERR_UNSUPPORTED, "quantize_fp8: more than 2^31 tiles");
   return MTL_OK;
 }

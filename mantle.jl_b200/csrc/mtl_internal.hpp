@@ -4,6 +4,7 @@
 
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <set>
@@ -173,6 +174,15 @@ mtl_status ew_compile(const EwProgram& p, void** kernel);
 mtl_status ew_launch_compiled(void* kernel, const EwProgram& p, void* stream);
 // Validates and launches any built-in kernel (elementwise or not).
 mtl_status launch_kernel(int kernel, const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream);
+
+// A product of sizes in bytes, all ones where it passes 64 bits (so that no buffer is
+// large enough for it).
+inline uint64_t bytes_of(std::initializer_list<int64_t> sizes) {
+  uint64_t v = 1;
+  for (int64_t n : sizes)
+    if (__builtin_mul_overflow(v, (uint64_t)n, &v)) return ~uint64_t(0);
+  return v;
+}
 
 // ── graph model ─────────────────────────────────────────────────────────────
 enum ResKind { RES_PERSISTENT = 0, RES_TRANSIENT = 1, RES_VIEW = 2 };

@@ -18,7 +18,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-from . import Buffer, Graph, Plan, Transient, Update, compute, dispatch, kernels, use
+from . import Buffer, Graph, Plan, Transient, Update, compute, dispatch, kernels, launch, use
 
 
 def shard_range(total: int, rank: int, world: int) -> tuple[int, int]:
@@ -307,6 +307,93 @@ def build_gemm(dev, batch: int = 8, M: int = 8192, N: int = 8192, K: int = 8192,
         use(p, C, write=True), use(p, A, read=True), use(p, B, read=True), M, N, K), batch))
     plan = Plan(g, **plan_kw)
     return GemmWorkload(batch, M, N, K, A, B, C, g, plan, {"A": A_t, "B": B_t})
+
+
+# ── experts: products grouped by expert, weights and rows in 8 bits ─────────
+def rows_of_codes(n: int) -> int:
+    """Bytes from one row of `n` 8-bit codes to the next: n rounded up to 16."""
+    return -(-n // 16) * 16
+
+
+@dataclass
+class ExpertsWorkload:
+    tokens: int
+    experts: int
+    top: int
+    width: int
+    hidden: int
+    x: Buffer
+    y: Buffer
+    rows_of: np.ndarray   # (tokens * top,) the token of each row, rows in expert order
+    offsets: np.ndarray   # (experts + 1,) the rows of each expert
+    weights: dict         # name -> (codes, scales) Buffers
+    graph: Graph
+    plan: Plan
+    tensors: dict
+
+    @property
+    def flops_step(self) -> int:
+        return 4 * self.tokens * self.top * self.width * self.hidden
+
+
+def route_to_experts(tokens: int, experts: int, top: int, seed: int):
+    """`top` distinct experts for every token, seeded, as (rows_of, offsets): the
+    token of each row with the rows in expert order, and where each expert's
+    rows start."""
+    rng = np.random.Generator(np.random.PCG64([seed, 7]))
+    chosen = np.argsort(rng.random((tokens, experts)), axis=1)[:, :top]
+    order = np.argsort(chosen.reshape(-1), kind="stable")
+    counts = np.bincount(chosen.reshape(-1), minlength=experts)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    return (order // top).astype(np.int32), offsets
+
+
+def build_experts(dev, tokens: int = 4096, experts: int = 16, top: int = 2, width: int = 2048, hidden: int = 4096,
+                  seed: int = 12, **plan_kw) -> ExpertsWorkload:
+    """Two layers of experts in 8 bits as one graph: the tokens' rows gathered into
+    expert order and brought to 8 bits, times each expert's first weights
+    (width -> hidden, bf16 out), brought to 8 bits again, times its second
+    (hidden -> width). The weights are quantized once, in 128 x 128 blocks; the
+    codes, scales and hidden rows are transients. y holds the rows in expert
+    order. Inputs are drawn on the device by torch's generator (seed)."""
+    import torch
+    device = f"cuda:{dev.ordinal}"
+    gen = torch.Generator(device=device)
+    gen.manual_seed(seed)
+    rows_of, offsets = route_to_experts(tokens, experts, top, seed)
+    T = tokens * top
+    x_t = torch.randn((tokens, width), generator=gen, device=device).to(torch.bfloat16)
+    tensors, weights = {"x": x_t}, {}
+    for name, n, k in (("up", hidden, width), ("down", width, hidden)):
+        w = torch.randn((experts, n, k), generator=gen, device=device) / float(np.sqrt(k))
+        src = Buffer.wrap(dev, w, dtype=np.float32)
+        codes = Buffer(dev, np.uint8, experts * n * rows_of_codes(k))
+        scales = Buffer(dev, np.float32, experts * -(-n // 128) * -(-k // 128))
+        launch(kernels.quantize_fp8, (codes, scales, None, None, src, None, n, k, n, 128, 0, 0, 0), experts, stream=dev.stream)
+        dev.synchronize()
+        weights[name], tensors[name] = (codes, scales), w
+    x = Buffer.wrap(dev, x_t, dtype=np.uint16)
+    rows, off = Buffer(dev, rows_of), Buffer(dev, offsets)
+    y = Buffer(dev, np.uint16, T * width)
+    g = Graph(dev)
+    R = lambda p, b: use(p, b, read=True)  # noqa: E731
+    W = lambda p, b: use(p, b, write=True)  # noqa: E731
+    codes_of = lambda n: (Transient.Buffer(g, np.uint8, T * rows_of_codes(n)), Transient.Buffer(g, np.float32, T * -(-n // 128)))  # noqa: E731
+    q1, s1 = codes_of(width)
+    h = Transient.Buffer(g, np.uint16, T * hidden)
+    q2, s2 = codes_of(hidden)
+    compute(g, "quantize x", lambda p: dispatch(p, kernels.quantize_fp8, (
+        W(p, q1), W(p, s1), None, None, R(p, x), R(p, rows), T, width, tokens, 1, 1, 0, 0), 1))
+    compute(g, "up", lambda p: dispatch(p, kernels.gemm_grouped_fp8, (
+        W(p, h), R(p, q1), R(p, s1), R(p, weights["up"][0]), R(p, weights["up"][1]), R(p, off), T, hidden, width, 0, 0, 1),
+        experts))
+    compute(g, "quantize h", lambda p: dispatch(p, kernels.quantize_fp8, (
+        W(p, q2), W(p, s2), None, None, R(p, h), None, T, hidden, T, 1, 1, 0, 0), 1))
+    compute(g, "down", lambda p: dispatch(p, kernels.gemm_grouped_fp8, (
+        W(p, y), R(p, q2), R(p, s2), R(p, weights["down"][0]), R(p, weights["down"][1]), R(p, off), T, width, hidden, 0, 0, 1),
+        experts))
+    plan = Plan(g, **plan_kw)
+    return ExpertsWorkload(tokens, experts, top, width, hidden, x, y, rows_of, offsets, weights, g, plan, tensors)
 
 
 # ── CNN inference ───────────────────────────────────────────────────────────

@@ -1,0 +1,229 @@
+"""The 8-bit and the expert-grouped kernels as they are used together: a graph of two
+layers of experts, a linear layer's forward and backward products in 8 bits, graphs,
+streams and large buffers."""
+import numpy as np
+import pytest
+import torch
+
+import mantle_cuda as M
+from fp8_reference import CODE, quantize, up16, values
+from mantle_cuda.workloads import build_experts, route_to_experts, rows_of_codes
+
+U8 = torch.uint8
+
+
+def test_routes_are_complete_and_in_expert_order():
+    rows_of, offsets = route_to_experts(50, 7, 3, 4)
+    assert offsets[0] == 0 and offsets[-1] == 150 and (np.diff(offsets) >= 0).all()
+    assert sorted(rows_of.tolist()) == sorted(list(range(50)) * 3)
+    for e in range(7):  # a token is with an expert once at most
+        part = rows_of[offsets[e]:offsets[e + 1]]
+        assert len(set(part.tolist())) == len(part)
+    assert rows_of_codes(1) == 16 and rows_of_codes(32) == 32
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def codes(rows, cols, block, bt=1):
+    rb, cb = -(-rows // 128), -(-cols // 128)
+    return (torch.empty((bt, rows, up16(cols)), dtype=U8, device="cuda"),
+            torch.empty((bt, cb, rows) if block == 1 else (bt, rb, cb), device="cuda"))
+
+
+def quantized(x, block, both=False, rows_of=None, fmt=0):
+    bt, xr, c = x.shape
+    r = xr if rows_of is None else rows_of.numel()
+    q, s = codes(r, c, block, bt)
+    qt, st = codes(c, r, block, bt) if both else (None, None)
+    M.launch(M.kernels.quantize_fp8, (q, s, qt, st, x, rows_of, r, c, xr, block, int(x.dtype == torch.bfloat16), fmt, 0), bt,
+             stream=stream())
+    return (q, s, qt, st) if both else (q, s)
+
+
+def bound(a, b, out):
+    """|error| of a @ b summed in K blocks of 128 (see test_fp8.py)."""
+    t = (128 * 2.0 ** -23 + (-(-a.shape[1] // 128) + 2) * 2.0 ** -24) * (a.abs() @ b.abs())
+    return t + (2.0 ** -8 * (a @ b).abs() if out else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,top,width,hidden", [(1, 8, 2, 256, 384), (37, 6, 2, 200, 328), (300, 4, 2, 256, 512)])
+def test_two_layers_of_experts(dev, tokens, experts, top, width, hidden):
+    w = build_experts(dev, tokens, experts, top, width, hidden, seed=3)
+    M.run(w.plan)
+    first = w.y.array().copy()
+    M.run(w.plan)
+    assert np.array_equal(w.y.array(), first)
+    # the same launches outside the graph, each stage against 64 bits on what it read
+    T, E = tokens * top, experts
+    off = torch.from_numpy(w.offsets).cuda()
+    wq = {k: quantized(w.tensors[k], 128) for k in ("up", "down")}
+    h = torch.zeros((T, hidden), dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros((T, width), dtype=torch.bfloat16, device="cuda")
+    q1, s1 = quantized(w.tensors["x"][None], 1, rows_of=torch.from_numpy(w.rows_of).cuda())
+    M.launch(M.kernels.gemm_grouped_fp8, (h, q1, s1, *wq["up"], off, T, hidden, width, 0, 0, 1), E, stream=stream())
+    q2, s2 = quantized(h[None], 1)
+    M.launch(M.kernels.gemm_grouped_fp8, (y, q2, s2, *wq["down"], off, T, width, hidden, 0, 0, 1), E, stream=stream())
+    torch.cuda.synchronize()
+    assert np.array_equal(y.view(torch.int16).cpu().numpy().reshape(-1), first.view(np.int16))
+    for q, s, name, out, k in ((q1, s1, "up", h, width), (q2, s2, "down", y, hidden)):
+        a = values(q[0].view(CODE[0]), s[0], 1, k)
+        for e in range(E):
+            r = slice(int(w.offsets[e]), int(w.offsets[e + 1]))
+            b = values(wq[name][0][e].view(CODE[0]), wq[name][1][e], 128, k).t()
+            assert ((out[r].double().cpu() - a[r] @ b).abs() <= bound(a[r], b, True)).all()
+    want, _ = quantize(w.tensors["x"].cpu()[torch.from_numpy(w.rows_of).long()], 1, 0, 0)
+    assert torch.equal(q1[0].view(CODE[0]).double().cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,fmt", [(1, 128, 256, 0), (70, 200, 328, 0), (300, 520, 260, 1)])
+def test_a_linear_layer_forward_and_backward(dev, m, n, k, fmt):
+    g = torch.Generator().manual_seed(m)
+    x, wt, dy = (torch.randn(s, generator=g) for s in ((m, k), (n, k), (m, n)))
+    xq, xs, xqt, xst = quantized(x[None].cuda(), 1, both=True)
+    wq, ws, wqt, wst = quantized(wt[None].cuda(), 128, both=True)
+    dq, ds, dqt, dst = quantized(dy[None].cuda().to(torch.bfloat16), 1, both=True, fmt=fmt)
+    y, dx, dw = (torch.empty(s, device="cuda") for s in ((m, n), (m, k), (n, k)))
+    go = lambda out, a, sa, b, sb, r, c, d, bblock, fa: M.launch(  # noqa: E731
+        M.kernels.gemm_fp8, (out, a, sa, b, sb, r, c, d, bblock, fa, 0, 0), 1, stream=stream())
+    go(y, xq, xs, wq, ws, m, n, k, 128, 0)
+    go(dx, dq, ds, wqt, wst, m, k, n, 128, fmt)
+    go(dw, dqt, dst, xqt, xst, n, k, m, 1, fmt)
+    torch.cuda.synchronize()
+    v = lambda q, s, block, c, f=0: values(q[0].view(CODE[f]), s[0], block, c)  # noqa: E731
+    for got, a, b in ((y, v(xq, xs, 1, k), v(wq, ws, 128, k).t()), (dx, v(dq, ds, 1, n, fmt), v(wqt, wst, 128, n).t()),
+                      (dw, v(dqt, dst, 1, m, fmt), v(xqt, xst, 1, m).t())):
+        assert ((got.double().cpu() - a @ b).abs() <= bound(a, b, False)).all()
+    # a square block's transpose is the same values
+    assert torch.equal(v(wq, ws, 128, k), v(wqt, wst, 128, n).t())
+    # against the gradients of the unquantized layer: a code is off by half a step of its value (2^-4 in e4m3, 2^-3
+    # in e5m2) or, below the normal range, of its block's scale (2^-10, 2^-17), so a product of two is off by
+    # (1 + r)(1 + q) - 1 of |a| |b| and, for the small ones, less than a further thousandth of the largest products'
+    x, wt, dy = x.double(), wt.double(), dy.to(torch.bfloat16).double()
+    r = (2.0 ** -4, 2.0 ** -3)[fmt]
+    for got, a, b in ((dx, dy, wt), (dw, dy.t(), x)):
+        tol = ((1 + r) * (1 + 2.0 ** -4) - 1) * (a.abs() @ b.abs()) + 1e-3 * a.shape[1] * a.abs().max() * b.abs().max()
+        assert ((got.double().cpu() - a @ b).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_a_training_step_of_experts_in_a_graph(dev):
+    # forward and both gradients as passes of one plan, replayed, against the same launches outside it
+    t, e, k, n = 300, 5, 136, 264
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x, dy, w = (torch.randn(s, generator=g, device="cuda").to(torch.bfloat16) for s in ((t, k), (t, n), (e, k, n)))
+    off = np.array([0, 60, 60, 200, 299, 300], np.int32)
+    X, DY, W = (M.Buffer.wrap(dev, v, dtype=np.uint16) for v in (x, dy, w))
+    O = M.Buffer(dev, off)
+    Y, DX, DW = M.Buffer(dev, np.float32, t * n), M.Buffer(dev, np.float32, t * k), M.Buffer(dev, np.uint16, e * k * n)
+    graph = M.Graph(dev)
+    R, Wr = (lambda p, b: M.use(p, b, read=True)), (lambda p, b: M.use(p, b, write=True))
+    M.compute(graph, "forward", lambda p: M.dispatch(p, M.kernels.gemm_grouped_bf16, (Wr(p, Y), R(p, X), R(p, W), R(p, O), t, n, k, 0), e))
+    M.compute(graph, "dx", lambda p: M.dispatch(p, M.kernels.gemm_grouped_dx_bf16, (Wr(p, DX), R(p, DY), R(p, W), R(p, O), t, n, k, 0), e))
+    M.compute(graph, "dw", lambda p: M.dispatch(p, M.kernels.gemm_grouped_dw_bf16, (Wr(p, DW), R(p, X), R(p, DY), R(p, O), t, n, k, 1), e))
+    plan = M.Plan(graph)
+    for _ in range(2):
+        M.run(plan)
+    dev.synchronize()
+    o = torch.from_numpy(off).cuda()
+    y, dx, dw = torch.empty((t, n), device="cuda"), torch.empty((t, k), device="cuda"), torch.empty((e, k, n), dtype=torch.bfloat16, device="cuda")
+    for name, args in (("gemm_grouped_bf16", (y, x, w, o, t, n, k, 0)), ("gemm_grouped_dx_bf16", (dx, dy, w, o, t, n, k, 0)),
+                       ("gemm_grouped_dw_bf16", (dw, x, dy, o, t, n, k, 1))):
+        M.launch(getattr(M.kernels, name), args, e, stream=stream())
+    torch.cuda.synchronize()
+    assert np.array_equal(Y.array(), y.cpu().numpy().reshape(-1)) and np.array_equal(DX.array(), dx.cpu().numpy().reshape(-1))
+    assert np.array_equal(DW.array().view(np.int16), dw.view(torch.int16).cpu().numpy().reshape(-1))
+    with pytest.raises(M.ArgumentError, match="elements of 4 bytes"):
+        M.compute(graph, "bad", lambda p: M.dispatch(p, M.kernels.gemm_grouped_bf16, (
+            Wr(p, Y), R(p, Y), R(p, W), R(p, O), t, n, k, 0), e))
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed_on_new_inputs(dev):
+    m, n, k = 70, 520, 1300
+    xs = [torch.randn((1, m, k), device="cuda") for _ in range(2)]
+    wq, ws = quantized(torch.randn((1, n, k), device="cuda"), 128)
+    x, c = xs[0].clone(), torch.empty((1, m, n), device="cuda")
+
+    def step(out):
+        q, s = codes(m, k, 1)
+        M.launch(M.kernels.quantize_fp8, (q, s, None, None, x, None, m, k, m, 1, 0, 0, 0), 1, stream=stream())
+        M.launch(M.kernels.gemm_fp8, (out, q, s, wq, ws, m, n, k, 128, 0, 0, 0), 1, stream=stream())
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step(c)
+    got = []
+    for v in xs:
+        x.copy_(v)
+        graph.replay()
+        got.append(c.clone())
+    for v, want in zip(xs, got):
+        x.copy_(v)
+        again = torch.empty_like(c)
+        step(again)
+        torch.cuda.synchronize()
+        assert torch.equal(again, want)
+    assert not torch.equal(*got)
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(dev):
+    t, e, k, n = 600, 8, 512, 768
+    x, w = torch.randn((1, t, k), device="cuda"), torch.randn((e, n, k), device="cuda")
+    qx, sx = quantized(x, 1)
+    qw, sw = quantized(w, 128)
+    off = torch.linspace(0, t, e + 1).int().cuda()
+    args = lambda out: (out, qx, sx, qw, sw, off, t, n, k, 0, 0, 0)  # noqa: E731
+    alone = torch.empty((t, n), device="cuda")
+    M.launch(M.kernels.gemm_grouped_fp8, args(alone), e, stream=stream())
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [torch.zeros((t, n), device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        M.launch(M.kernels.gemm_grouped_fp8, args(out), e, stream=streams[i % 2].cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, alone) for out in outs)
+
+
+@pytest.mark.gpu
+def test_buffers_past_two_to_the_31(dev):
+    # 2.2e9 elements: offsets need 64 bits. The last rows and columns against the definition.
+    r, c = 540_000, 4096
+    x = torch.zeros((1, r, c), dtype=torch.bfloat16, device="cuda")
+    x[0, -300:] = torch.randn((300, c), device="cuda").to(torch.bfloat16)
+    for block in (1, 128):
+        q, s = quantized(x, block)
+        torch.cuda.synchronize()
+        cut = r - 256 - r % 128  # a multiple of 128
+        wq, ws = quantize(x[0, cut:].cpu(), block, 0, 0)
+        assert torch.equal(q[0, cut:].view(CODE[0]).double().cpu(), wq)
+        assert torch.equal((s[0][:, cut:] if block == 1 else s[0][cut // 128:]).double().cpu(), ws)
+        del wq
+    # q, s: 128 x 128 blocks. As B of a product: few rows of A, and a tile of them
+    for m in (2, 130):
+        a = torch.randn((1, m, c), device="cuda")
+        qa, sa = quantized(a, 1)
+        out = torch.empty((1, m, r), dtype=torch.bfloat16, device="cuda")
+        M.launch(M.kernels.gemm_fp8, (out, qa, sa, q, s, m, r, c, 128, 0, 0, 1), 1, stream=stream())
+        torch.cuda.synchronize()
+        va, vb = values(qa[0].view(CODE[0]), sa[0], 1, c), values(q[0, cut:].view(CODE[0]), s[0][cut // 128:], 128, c).t()
+        assert ((out[0, :, cut:].double().cpu() - va @ vb).abs() <= bound(va, vb, True)).all()
+        assert float(out[0, :, :cut - 128].abs().max()) == 0.0
+        del out
+    # as the rows of a grouped product whose last group lies at the end
+    w, t = torch.randn((2, 136, c), device="cuda"), r
+    del q, s
+    qx, sx = quantized(x, 1)
+    qw, sw = quantized(w, 128)
+    y = torch.full((t, 136), 3.0, device="cuda")
+    M.launch(M.kernels.gemm_grouped_fp8, (y, qx, sx, qw, sw, torch.tensor([0, 5, t - 7], dtype=torch.int32, device="cuda"), t, 136, c, 0, 0, 0),
+             2, stream=stream())
+    torch.cuda.synchronize()
+    vx, vw = values(qx[0, t - 200:].view(CODE[0]), sx[0][:, t - 200:], 1, c), values(qw[1].view(CODE[0]), sw[1], 128, c).t()
+    assert ((y[t - 200:t - 7].double().cpu() - (vx @ vw)[:193]).abs() <= bound(vx, vw, False)[:193]).all()
+    assert (y[t - 7:] == 3.0).all()
