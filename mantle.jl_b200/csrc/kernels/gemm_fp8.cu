@@ -469,6 +469,247 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
 }
 
+// ── groups of a few rows of A ───────────────────────────────────────────────
+// As the tiles above, with the roles of the operands changed: 256 rows of B (two runs of
+// 128) are the MMA's M operand and NT rows of a group its N operand, so a K block takes a
+// quarter of the MMAs or less, and its sums, transposed in tensor memory (a lane has one
+// column of C), are NT multiplications and additions a lane instead of 128 of which few
+// are stored. Four K blocks' sums fit in tensor memory at once.
+constexpr int kSlim = 32;  // rows of a group a tile
+template <int NT>
+struct SlimF8 {
+  static constexpr uint32_t kBStage = 256 * kF8K, kXStage = NT * kF8K, kStageBytes = kBStage + kXStage;
+  static constexpr int kStages = 196608 / (int)kStageBytes, kAcc = 4;
+  static constexpr uint32_t kTmemCols = kAcc * 2 * NT;
+};
+template <int NT>
+struct SlimF8Shared {
+  alignas(16) float sa[2][4][NT];  // two groups of four K blocks: the rows' scales
+  alignas(16) float sb[2][4][4];   // and the two runs'
+  uint64_t full[8], empty[8], tfull[4], tempty[4], sfull[2], sempty[2], drain;
+  uint32_t tmem;
+  int abort;
+  GroupTable groups;
+};
+template <int NT>
+constexpr int slim_f8_smem() {
+  return SlimF8<NT>::kStages * (int)SlimF8<NT>::kStageBytes + (int)sizeof(SlimF8Shared<NT>) + 1024;
+}
+
+template <int NT, typename OUT>
+__global__ void __launch_bounds__(kF8Threads, 1)
+    gemm_fp8_slim_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const F8Args p) {
+  using Cfg = SlimF8<NT>;
+  constexpr int kStages = Cfg::kStages, kAcc = Cfg::kAcc, BN = 256;
+  extern __shared__ unsigned char f8_raw[];
+  unsigned char* ring =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
+  auto* sh = reinterpret_cast<SlimF8Shared<NT>*>(ring + kStages * Cfg::kStageBytes);
+  volatile int* abort = &sh->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sh->full[s]), 1);
+      mbar_init(smem_u32(&sh->empty[s]), 1);
+    }
+    for (int a = 0; a < kAcc; ++a) {
+      mbar_init(smem_u32(&sh->tfull[a]), 1);
+      mbar_init(smem_u32(&sh->tempty[a]), 8);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&sh->sfull[a]), 32);
+      mbar_init(smem_u32(&sh->sempty[a]), 8);
+    }
+    mbar_init(smem_u32(&sh->drain), 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)),
+                 "r"(Cfg::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  build_groups(&sh->groups, p.offsets, p.batch, p.M, NT);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+  const int tiles_n = (p.N + BN - 1) / BN, ntiles = sh->groups.cum[p.batch] * tiles_n;
+  GroupWalk walk;
+  int row0, rows, n0;
+
+  if (warp == 0) {
+    // ── TMA producer ──
+    int s = 0;
+    uint32_t ph = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t fb = smem_u32(&sh->full[s]), dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes);
+          mbar_expect_tx(fb, Cfg::kStageBytes);
+          tma_load_3d(dst, &tmB, kb * kF8K, n0, walk.e, fb);
+          // rows behind the group's feed sums that are not stored
+          tma_load_3d(dst + Cfg::kBStage, &tmA, kb * kF8K, row0, 0, fb);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
+      for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+        drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+  } else if (warp == 1) {
+    // ── MMA issuer ──
+    int s = 0, a = 0;
+    uint32_t ph = 0, aph = 0;
+    bool ok = true;
+    const uint64_t b0 = smem_desc(smem_u32(ring), 16, 1024), x0 = smem_desc(smem_u32(ring) + Cfg::kBStage, 16, 1024);
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        ok = wait_warp(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts) &&
+             wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t d = tmem + (uint32_t)(a * 2 * NT);
+          const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
+#pragma unroll
+          for (int kk = 0; kk < kF8K / 32; ++kk)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              tc_mma_f8(d + (uint32_t)(r * NT), b0 + off + r * (Cfg::kBStage / 2 >> 4) + kk * 2, x0 + off + kk * 2, p.idesc, kk != 0);
+          tc_commit(smem_u32(&sh->empty[s]));
+          tc_commit(smem_u32(&sh->tfull[a]));
+        }
+        __syncwarp();
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+        if (++a == kAcc) {
+          a = 0;
+          aph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
+      tc_commit(smem_u32(&sh->drain));
+      drain_phase(smem_u32(&sh->drain), 0);
+    }
+  } else if (warp == 2) {
+    // ── scales, four K blocks at a time ──
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
+      const float* sb = p.sB + ((int64_t)walk.e * p.nblocks + n0 / 128) * p.kblocks;
+      for (int kb0 = 0; kb0 < p.kblocks; kb0 += 4) {
+        ok = wait_warp(smem_u32(&sh->sempty[s]), ph ^ 1, abort, &g_fp8_timeouts);
+        if (!ok) break;
+        for (int j = 0; j < min(4, p.kblocks - kb0); ++j) {
+          const int64_t kb = kb0 + j;
+#pragma unroll
+          for (int i = 0; i < NT / 32; ++i)
+            if (i * 32 + lane < rows) cp_async4(smem_u32(&sh->sa[s][j][i * 32 + lane]), p.sA + kb * p.M + row0 + i * 32 + lane);
+          if (lane < 2 && n0 + lane * 128 < p.N) cp_async4(smem_u32(&sh->sb[s][j][lane]), sb + (int64_t)lane * p.kblocks + kb);
+        }
+        cp_async_arrive(smem_u32(&sh->sfull[s]));
+        if (++s == 2) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= 4) {
+    // ── scaled sums: a warp has 32 columns of C, run (warp - 4) / 4 ──
+    const int q = warp & 3, run = (warp - 4) / 4;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(run * NT);
+    int a = 0, s = 0;
+    uint32_t aph = 0, sph = 0;
+    bool ok = true;
+    auto give_back = [&](uint64_t* bar) {
+      __syncwarp();
+      if (elect_one()) mbar_arrive(smem_u32(bar));
+    };
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
+      const int col = n0 + run * 128 + q * 32 + lane;
+      float acc[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i] = 0.0f;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        ok = ((kb & 3) != 0 || wait_warp(smem_u32(&sh->sfull[s]), sph, abort, &g_fp8_timeouts)) &&
+             wait_warp(smem_u32(&sh->tfull[a]), aph, abort, &g_fp8_timeouts);
+        if (!ok) break;
+        tc_fence_after();
+        const float sb = sh->sb[s][kb & 3][run];
+        const float4* sa = reinterpret_cast<const float4*>(sh->sa[s][kb & 3]);
+#pragma unroll
+        for (int c = 0; c < NT; c += 16) {
+          if (c >= rows) break;  // uniform in the CTA
+          uint32_t r[16];
+          tmem_ld16_nowait(lanes + (uint32_t)(a * 2 * NT + c), r);
+          float4 f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = sa[c / 4 + i];
+          tmem_wait_ld(r);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[c + 4 * i] = fmaf(__uint_as_float(r[4 * i]), f[i].x * sb, acc[c + 4 * i]);
+            acc[c + 4 * i + 1] = fmaf(__uint_as_float(r[4 * i + 1]), f[i].y * sb, acc[c + 4 * i + 1]);
+            acc[c + 4 * i + 2] = fmaf(__uint_as_float(r[4 * i + 2]), f[i].z * sb, acc[c + 4 * i + 2]);
+            acc[c + 4 * i + 3] = fmaf(__uint_as_float(r[4 * i + 3]), f[i].w * sb, acc[c + 4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+        give_back(&sh->tempty[a]);
+        if (++a == kAcc) {
+          a = 0;
+          aph ^= 1;
+        }
+        if ((kb & 3) == 3 || kb + 1 == p.kblocks) {
+          give_back(&sh->sempty[s]);
+          if (++s == 2) {
+            s = 0;
+            sph ^= 1;
+          }
+        }
+      }
+      if (!ok) break;
+      if (col < p.N) {
+        OUT* out = static_cast<OUT*>(p.C) + (int64_t)row0 * p.N + col;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (i < rows) {
+            if constexpr (sizeof(OUT) == 4)
+              out[(int64_t)i * p.N] = acc[i];
+            else
+              out[(int64_t)i * p.N] = __float2bfloat16_rn(acc[i]);
+          }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
+}
+
 // ── few rows of A: a decode step ────────────────────────────────────────────
 // With M <= 16 the product is a read of B. mma.sync takes its operands from
 // registers, so the codes go from global memory straight into them: a warp holds 16
@@ -706,6 +947,16 @@ static cudaError_t fp8_few(bool a5, bool b5, bool bf16, const uint8_t* A, const 
   return cudaGetLastError();
 }
 
+template <int NT, typename OUT>
+static cudaError_t fp8_launch_slim(const CUtensorMap& ta, const CUtensorMap& tb, const F8Args& p, int64_t tiles, int sms,
+                                   int device, cudaStream_t s) {
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(gemm_fp8_slim_kernel<NT, OUT>, slim_f8_smem<NT>(), device, &done);
+  if (e != cudaSuccess) return e;
+  gemm_fp8_slim_kernel<NT, OUT><<<(int)std::min<int64_t>(tiles, sms), kF8Threads, slim_f8_smem<NT>(), s>>>(ta, tb, p);
+  return cudaGetLastError();
+}
+
 // What gemm_fp8 and gemm_grouped_fp8 check alike. `rows`: rows of A and C over the
 // whole launch; `slices`: products or experts.
 static mtl_status fp8_check_common(const char* who, const LaunchArgs& la, const uint64_t* bytes, int64_t batch, int64_t M,
@@ -727,7 +978,7 @@ static mtl_status fp8_check_common(const char* who, const LaunchArgs& la, const 
                   (unsigned long long)need[i]);
     if (la.a[i].ptr & align[i]) return fail(MTL_ERR_ARGUMENT, "%s: %s must be %u-byte aligned", who, what[i], align[i] + 1);
   }
-  if (((M + 127) / 128 + kMaxGroups) * ((N + 63) / 64) > INT_MAX)
+  if (((M + 31) / 32 + kMaxGroups) * ((N + 63) / 64) > INT_MAX)
     return fail(MTL_ERR_UNSUPPORTED, "%s: more than 2^31 tiles a product", who);
   return MTL_OK;
 }
@@ -810,6 +1061,24 @@ static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, i
       const uint8_t *a8 = static_cast<const uint8_t*>(A), *b8 = static_cast<const uint8_t*>(B);
       const cudaError_t e = M <= 8 ? (rowb ? fp8_few<1, true>(fa, fb, out, a8, b8, p, s) : fp8_few<1, false>(fa, fb, out, a8, b8, p, s))
                                    : (rowb ? fp8_few<2, true>(fa, fb, out, a8, b8, p, s) : fp8_few<2, false>(fa, fb, out, a8, b8, p, s));
+      return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    }
+  }
+  if constexpr (GROUPED) {
+    // Rows of a group in the MMA's N operand, 32 of them, while a group has up to 16 on
+    // average and there are tiles for most SMs. Sustained, us, against tiles of 128 rows:
+    // 2 rows a group (64 groups, 4096 x 2048) 89.0 and 109.4, 16 rows (2048 x 2048) 50.6
+    // and 61.9, 32 rows (16 groups) 22.5 and 18.4, with 64 in the operand 18.5.
+    const int64_t tiles_n = (N + 255) / 256;
+    if (batch * tiles_n * 4 >= la.sm_count * 3 && M <= 16 * (int64_t)batch) {
+      // 128 rows of B, kSlim rows of A; formats in that order
+      p.idesc = (1u << 4) | ((uint32_t)fb << 7) | ((uint32_t)fa << 10) | ((uint32_t)(kSlim >> 3) << 17) | (8u << 24);
+      CUtensorMap ta, tb;
+      if (mtl_status st = make_code_map(&ta, A, K, M, 1, kSlim)) return st;
+      if (mtl_status st = make_code_map(&tb, B, K, N, batch, 256)) return st;
+      const int64_t tiles = ((int64_t)M / kSlim + batch) * tiles_n;
+      const cudaError_t e = out ? fp8_launch_slim<kSlim, __nv_bfloat16>(ta, tb, p, tiles, la.sm_count, la.device, s)
+                                : fp8_launch_slim<kSlim, float>(ta, tb, p, tiles, la.sm_count, la.device, s);
       return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     }
   }

@@ -321,6 +321,178 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
 }
 
+// ── groups of a few rows: a decode step ─────────────────────────────────────
+// A tile above costs 128 rows of MMAs however few its group has; with two rows an
+// expert the weights' read time hides them, but not their power. Here the weights are
+// the MMA's M operand (256 columns of the output as two runs of 128) and NT rows of the
+// group its N operand, so a K block costs a quarter of the MMAs or less and the sums lie
+// transposed: a lane of tensor memory holds one column of the output, and a row's 32
+// columns leave a warp as one run.
+template <int NT>
+struct SlimCfg {
+  static constexpr uint32_t kWStage = 256 * kGrK * 2, kXStage = NT * kGrK * 2, kStageBytes = kWStage + kXStage;
+  static constexpr int kStages = 196608 / (int)kStageBytes;  // 5
+  static constexpr uint32_t kTmemCols = 4 * NT < 32 ? 32 : 4 * NT;  // two accumulators of two runs
+};
+template <int NT>
+constexpr int slim_smem() {
+  return SlimCfg<NT>::kStages * (int)SlimCfg<NT>::kStageBytes + (int)sizeof(GrShared) + 1024;
+}
+
+template <int FORM, int NT, typename OUT>
+__global__ void __launch_bounds__(kGrThreads, 1)
+    gemm_grouped_slim_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const GrArgs p) {
+  using Cfg = SlimCfg<NT>;
+  constexpr int kStages = Cfg::kStages, BN = 256;
+  constexpr uint32_t kIdesc = idesc_bf16_f32(128, NT, FORM != kDx, false);
+  extern __shared__ unsigned char gr_raw[];
+  unsigned char* ring =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gr_raw) + 1023) & ~uintptr_t(1023));
+  GrShared* sh = reinterpret_cast<GrShared*>(ring + kStages * Cfg::kStageBytes);
+  volatile int* abort = &sh->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sh->full[s]), 1);
+      mbar_init(smem_u32(&sh->empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&sh->tfull[a]), 1);
+      mbar_init(smem_u32(&sh->tempty[a]), 8);
+    }
+    mbar_init(smem_u32(&sh->drain), 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)),
+                 "r"(Cfg::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  build_groups(&sh->groups, p.offsets, p.groups, p.T, NT);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+
+  const int tiles_n = (p.cols + BN - 1) / BN, ntiles = sh->groups.cum[p.groups] * tiles_n;
+  const int kblocks = (p.depth + kGrK - 1) / kGrK;
+  GroupWalk walk;
+  int row0, rows, n0;
+
+  if (warp == 0) {
+    // ── TMA producer (the whole warp waits, one lane issues) ──
+    int s = 0;
+    uint32_t ph = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
+      const int w_boxes = FORM == kDx ? 1 : p.chunked_b ? 4 : min(4, (p.cols - n0 + 63) / 64);
+      const uint32_t bytes = Cfg::kXStage + (FORM == kDx ? Cfg::kWStage : (uint32_t)(w_boxes * kGrK * 128));
+      for (int kb = 0; kb < kblocks; ++kb) {
+        ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t fb = smem_u32(&sh->full[s]), w_dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes);
+          mbar_expect_tx(fb, bytes);
+          if (FORM == kDx) {
+            tma_load_3d(w_dst, &tmW, kb * kGrK, n0, walk.e, fb);
+          } else if (p.chunked_b) {
+            tma_load_4d(w_dst, &tmW, 0, kb * kGrK, n0 / 64, walk.e, fb);
+          } else {
+            for (int b = 0; b < w_boxes; ++b) tma_load_3d(w_dst + b * (kGrK * 128), &tmW, n0 + b * 64, kb * kGrK, walk.e, fb);
+          }
+          // rows behind the group's feed columns that are not stored
+          tma_load_3d(w_dst + Cfg::kWStage, &tmX, kb * kGrK, row0, 0, fb);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
+      for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+        drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+  } else if (warp == 1) {
+    // ── MMA issuer ──
+    int s = 0, i = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    constexpr uint32_t kWStep = (FORM == kDx ? 32 : 2048) >> 4, kXStep = 32 >> 4, kWRun = Cfg::kWStage / 2 >> 4;
+    const uint64_t w0 = smem_desc(smem_u32(ring), FORM == kDx ? 16 : kGrK * 128, 1024);
+    const uint64_t x0 = smem_desc(smem_u32(ring) + Cfg::kWStage, 16, 1024);
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x, ++i) {
+      const int a = i & 1;
+      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
+      const uint32_t d = tmem + (uint32_t)(a * 2 * NT);
+      for (int kb = 0; ok && kb < kblocks; ++kb) {
+        ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
+#pragma unroll
+          for (int kk = 0; kk < kGrK / 16; ++kk)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              tc_mma(d + (uint32_t)(r * NT), w0 + off + r * kWRun + kk * kWStep, x0 + off + kk * kXStep, kIdesc, (kb | kk) != 0);
+          tc_commit(smem_u32(&sh->empty[s]));
+          if (kb + 1 == kblocks) tc_commit(smem_u32(&sh->tfull[a]));
+        }
+        __syncwarp();
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
+      tc_commit(smem_u32(&sh->drain));
+      drain_phase(smem_u32(&sh->drain), 0);
+    }
+  } else {
+    // ── epilogue: a warp has 32 columns of the output, run (warp - 2) / 4 ──
+    const int q = warp & 3, run = (warp - 2) / 4;
+    int i = 0;
+    for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++i) {
+      walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
+      const int a = i & 1, col = n0 + run * 128 + q * 32 + lane;
+      if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
+      tc_fence_after();
+      OUT* out = static_cast<OUT*>(p.out) + (int64_t)row0 * p.cols + col;
+#pragma unroll 1
+      for (int c = 0; c < NT; c += 16) {
+        if (c >= rows) break;
+        uint32_t r[16];
+        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * 2 + run) * NT + c), r);
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (c + v < rows && col < p.cols) {
+            if constexpr (sizeof(OUT) == 4)
+              out[(int64_t)(c + v) * p.cols] = __uint_as_float(r[v]);
+            else
+              out[(int64_t)(c + v) * p.cols] = __float2bfloat16_rn(__uint_as_float(r[v]));
+          }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
+}
+
 // ── host side ───────────────────────────────────────────────────────────────
 cudaError_t grouped_set_wait_limit(unsigned long long ns) { return set_wait_limit_this_file(ns); }
 int grouped_timeouts(bool reset) {
@@ -387,7 +559,7 @@ static mtl_status gr_check(const LaunchArgs& la, const uint64_t* bytes) {
       return fail(MTL_ERR_ARGUMENT, "%s: %s must be %u-byte aligned", who, what[FORM][i], align[i] + 1);
   }
   const int64_t rows = FORM == kDw ? (K + 127) / 128 * E : (T + 127) / 128 + E, cols = FORM == kDx ? K : N;
-  if (rows * ((cols + 127) / 128) > INT_MAX) return fail(MTL_ERR_UNSUPPORTED, "%s: more than 2^31 tiles", who);
+  if ((FORM == kDw ? rows : (T + 31) / 32 + E) * ((cols + 127) / 128) > INT_MAX) return fail(MTL_ERR_UNSUPPORTED, "%s: more than 2^31 tiles", who);
   return MTL_OK;
 }
 mtl_status gemm_grouped_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kFwd>(la, bytes); }
@@ -402,6 +574,16 @@ static cudaError_t gr_launch(const CUtensorMap& ta, const CUtensorMap& tb, const
   if (e != cudaSuccess) return e;
   const int grid = (int)std::min<int64_t>(tiles, la.sm_count);
   gemm_grouped_kernel<FORM, RUNS, BN, OUT><<<grid, kGrThreads, gr_smem<RUNS, BN>(), s>>>(ta, tb, p);
+  return cudaGetLastError();
+}
+
+template <int FORM, int NT, typename OUT>
+static cudaError_t gr_launch_slim(const CUtensorMap& tx, const CUtensorMap& tw, const GrArgs& p, int64_t tiles,
+                                  const LaunchArgs& la, cudaStream_t s) {
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(gemm_grouped_slim_kernel<FORM, NT, OUT>, slim_smem<NT>(), la.device, &done);
+  if (e != cudaSuccess) return e;
+  gemm_grouped_slim_kernel<FORM, NT, OUT><<<(int)std::min<int64_t>(tiles, la.sm_count), kGrThreads, slim_smem<NT>(), s>>>(tx, tw, p);
   return cudaGetLastError();
 }
 
@@ -426,10 +608,16 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   p.groups = E;
   p.vec = la.a[0].ptr % 16 == 0;  // N and K are multiples of 8
   const bool wide = false;
-  p.a_box = T / E >= kGrM ? kGrM : 32;
+  // Rows of a group in the MMA's N operand, 32 or 64 of them, while a group has up to 16
+  // or 40 on average and there are tiles for most SMs. Sustained, us, against tiles of 128
+  // rows: 2 rows a group (32 groups, 2048 x 4096) 81.7 and 89.5, 8 rows 83.1 and 90.8, 32
+  // rows (16 groups, 2048 x 2048) 25.5 with 64, 29.7 with 32 and 28.0, 64 rows 55 and 51.3.
+  const int64_t slim_tiles = (int64_t)E * ((cols + 255) / 256);
+  const int slim = FORM == kDw || slim_tiles * 4 < la.sm_count * 3 || T > 40 * (int64_t)E ? 0 : T <= 16 * (int64_t)E ? 32 : 64;
+  p.a_box = slim ? slim : T / E >= kGrM ? kGrM : 32;
   const void *A = reinterpret_cast<const void*>(la.a[1].ptr), *B = reinterpret_cast<const void*>(la.a[2].ptr);
   const int64_t row_tiles = FORM == kDw ? (int64_t)E * ((K + 127) / 128) : std::max<int64_t>(E, (T + 127) / 128);
-  const bool narrow = !wide && row_tiles * ((cols + 255) / 256) < la.sm_count;
+  const bool narrow = !wide && !slim && row_tiles * ((cols + 255) / 256) < la.sm_count;
   const int bn = narrow ? 128 : 256;
   p.chunked_a = FORM == kDw && K % 64 == 0;
   p.chunked_b = FORM != kDx && N % 64 == 0;
@@ -444,7 +632,17 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   const int64_t tile_m = wide ? 256 : 128;
   const int64_t tiles = (FORM == kDw ? (int64_t)E * ((K + tile_m - 1) / tile_m) : T / tile_m + E) * ((cols + bn - 1) / bn);
   cudaError_t e;
-  if (wide) {
+  if (slim) {
+    if constexpr (FORM != kDw) {
+      const int64_t n = ((int64_t)T / slim + E) * ((cols + 255) / 256);
+      if (slim == 32)
+        e = out ? gr_launch_slim<FORM, 32, __nv_bfloat16>(ta, tb, p, n, la, s) : gr_launch_slim<FORM, 32, float>(ta, tb, p, n, la, s);
+      else
+        e = out ? gr_launch_slim<FORM, 64, __nv_bfloat16>(ta, tb, p, n, la, s) : gr_launch_slim<FORM, 64, float>(ta, tb, p, n, la, s);
+    } else {
+      e = cudaErrorInvalidValue;
+    }
+  } else if (wide) {
     e = out ? gr_launch<FORM, 2, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 2, 256, float>(ta, tb, p, tiles, la, s);
   } else if (narrow) {
     e = out ? gr_launch<FORM, 1, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 1, 128, float>(ta, tb, p, tiles, la, s);

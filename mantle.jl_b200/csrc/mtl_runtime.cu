@@ -1041,6 +1041,7 @@ static mtl_status direct_args(int32_t kernel, const mtl_arg* args, int32_t nargs
   cudaGetLastError();
   la.sm_count = sms;
   la.device = dev;
+  la.a.reserve(nargs);
   for (int i = 0; i < nargs; ++i) {
     Arg x;
     const mtl_arg& m = args[i];

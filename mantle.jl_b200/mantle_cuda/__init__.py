@@ -30,6 +30,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import sys
 import threading
 from collections import deque
 from dataclasses import dataclass
@@ -517,6 +518,7 @@ class Kernel:
         nm, sig = C.c_char_p(), C.c_char_p()
         check(lib().mtl_kernel_info(self.id, C.byref(nm), C.byref(sig)))
         self.signature = sig.value.decode()
+        self.packed = _Packed(self) if name in _OPERANDS else None
 
     def __repr__(self) -> str:
         return f"Kernel({self.name}: {self.signature})"
@@ -612,61 +614,84 @@ def _operands(k: Kernel, args: Sequence) -> list:
     sizes, flag = _OPERANDS[k.name]
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"{k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
-    flat, device = [], None
-    for i, size in enumerate(sizes):
-        x = args[i]
-        if x is None:
-            flat += (L.ARG_NULL, 0, 0, 0)
-            continue
-        if size is _OUT:
-            kind = args[flag]
-            size = _OUT[kind] if kind in (0, 1) else 0  # the library refuses another type
-        if hasattr(x, "data_ptr"):
+    flat, device, tensor = [], None, _tensor_type()
+    for x, size in zip(args, sizes):
+        if tensor is not None and isinstance(x, tensor):
             if device is None:
-                import torch
-                device = torch.cuda.current_device() if torch.cuda.is_initialized() else 0
+                device = _current_device(x)
             if x.get_device() != device or not x.is_contiguous():
-                raise ArgumentError(L.ERR_ARGUMENT,
-                                    f"{k.name}: argument {i + 1} must be a contiguous CUDA tensor on the current device ({device})")
+                raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4 + 1} must be a contiguous CUDA tensor on the "
+                                    f"current device ({device})")
             got = x.element_size()
             flat += (L.ARG_PTR, 0, x.data_ptr(), x.numel() * got)
+        elif x is None:
+            flat += (L.ARG_NULL, 0, 0, 0)
+            continue
         elif isinstance(x, DevicePtr):
             flat += (L.ARG_PTR, 0, x.ptr, x.nbytes & 0xFFFFFFFFFFFFFFFF)
             continue
         else:
             x = x.resource if isinstance(x, UseHandle) else x
-            if not hasattr(x, "dtype"):
+            if not hasattr(x, "dtype") or hasattr(x, "data_ptr"):
                 raise ArgumentError(L.ERR_ARGUMENT, f"cannot pass {x!r} where the kernel takes a buffer")
             got = x.dtype.itemsize
             flat += (L.ARG_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
-        if got != size and size:
-            raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {i + 1} has elements of {got} bytes, expected {size}")
+        if size is _OUT:
+            kind = args[flag]
+            size = _OUT[kind] if kind in (0, 1) else got  # the library refuses another type
+        if got != size:
+            raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4} has elements of {got} bytes, expected {size}")
     return flat
 
 
-_packed = {}  # per kernel: the layout of its argument array, and the entry point taking it as bytes
+def _tensor_type():
+    """torch.Tensor where torch is loaded (no argument can be one where it is not)."""
+    torch = sys.modules.get("torch")
+    return getattr(torch, "Tensor", None)
 
 
-def _launch_packed(k: Kernel, args: Sequence, nd: tuple, stream: int) -> None:
-    """launch() of a kernel in _OPERANDS: the argument array is packed in one call (a
-    call costs the host 5 us instead of 25, and a decode step's kernel runs for 2 to 15)."""
-    flat = _operands(k, args)
-    if k.name not in _packed:
-        # every argument is {int32 kind, int32 rid, 8-byte value, uint64 bytes}
-        f = lib()["mtl_launch"]
-        f.restype = C.c_int32
-        f.argtypes = [C.c_int32, C.c_char_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
-        _packed[k.name] = (struct.Struct("<" + "".join("iiQQ" if s in "Bb" else "iii4xQ" for s in k.signature)), f)
-    layout, f = _packed[k.name]
-    for x in args[len(flat) // 4:]:
-        flat += (L.ARG_I32, 0, x, 0)
-    try:
-        packed = layout.pack(*flat)
-    except struct.error as e:
-        raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: a scalar argument is no Int32 ({e})") from None
-    status = f(k.id, packed, len(k.signature), struct.pack("<3q", *nd, *([1] * (3 - len(nd)))), len(nd), None, 0, stream)
-    if status:
-        check(status)
+def _current_device(x) -> int:
+    """The current CUDA device, asked for only where `x` is on one."""
+    return sys.modules["torch"].cuda.current_device() if x.get_device() >= 0 else 0
+
+
+class _Packed:
+    """How a kernel in _OPERANDS is launched: its argument array packed in one call
+    (each argument is {int32 kind, int32 rid, 8-byte value, uint64 bytes}), and the
+    entry point taking it as bytes. A launch costs the host 8 us this way and 25 with
+    an array of ctypes structures, and a decode step's kernel runs for 2 to 15."""
+
+    ndranges: dict = {}  # one-dimensional ranges as the entry point takes them
+
+    def __init__(self, k: Kernel):
+        self.kernel, self.nargs = k, len(k.signature)
+        self.pack = struct.Struct("<" + "".join("iiQQ" if s in "Bb" else "iii4xQ" for s in k.signature)).pack
+        self.entry = lib()["mtl_launch"]
+        self.entry.restype = C.c_int32
+        self.entry.argtypes = [C.c_int32, C.c_char_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
+        self.buffers = len(_OPERANDS[k.name][0])
+
+    def __call__(self, args: Sequence, ndrange, stream: int) -> None:
+        flat = _operands(self.kernel, args)
+        for x in args[self.buffers:]:
+            flat += (L.ARG_I32, 0, x, 0)
+        try:
+            packed = self.pack(*flat)
+        except struct.error as e:
+            raise ArgumentError(L.ERR_ARGUMENT, f"{self.kernel.name}: a scalar argument is no Int32 ({e})") from None
+        if type(ndrange) is int:
+            n = 1
+            range_ = self.ndranges.get(ndrange)
+            if range_ is None:
+                range_ = struct.pack("<3q", ndrange, 1, 1)
+                if len(self.ndranges) < 4096:
+                    self.ndranges[ndrange] = range_
+        else:
+            nd = _nd(ndrange)
+            n, range_ = len(nd), struct.pack("<3q", *nd, *([1] * (3 - len(nd))))
+        status = self.entry(self.kernel.id, packed, self.nargs, range_, n, None, 0, stream)
+        if status:
+            check(status)
 
 
 def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None:
@@ -690,9 +715,9 @@ def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None
 def launch(kernel, args: Sequence, ndrange, stream: int = 0, workspace=None) -> None:
     """Launch a built-in kernel outside any graph on `stream` (pointer args:
     Buffers, torch tensors or DevicePtr)."""
-    k = _kernel(kernel)
-    if k.name in _OPERANDS:
-        return _launch_packed(k, args, _nd(ndrange), stream)
+    k = kernel if isinstance(kernel, Kernel) else _kernel(kernel)
+    if k.packed is not None:
+        return k.packed(args, ndrange, stream)
     arr = (L.Arg * max(len(args), 1))(*[_arg(None, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))

@@ -297,6 +297,10 @@ def offsets_of(sizes, first=0):
     ([700, 20, 600], 0, 1320, 1024, 256, 0),
     ([2] * 40, 0, 80, 512, 640, 1),
     ([0, 0, 0], 0, 7, 64, 64, 0),
+    # many groups of a few rows (rows as the MMA's N operand), some of more than a tile's 32; N past a run of 128 and ragged
+    ([1, 0, 33, 5, 0, 2, 70, 16, 1, 1] * 3, 5, 400, 1000, 520, 0),
+    ([2] * 60, 0, 120, 515, 1300, 1),
+    ([0, 9, 15, 0, 31, 32, 1] * 6, 0, 530, 640, 130, 1),
 ])
 def test_gemm_grouped_fp8(dev, sizes, first, t, n, k, out):
     e = len(sizes)

@@ -86,6 +86,10 @@ SIZES = [
     ([0, 0, 0], 0, 5, 64, 64),
     ([1000, 1100], 0, 2100, 2056, 1032),
     ([300] * 6 + [0, 31], 0, 1831, 1024, 648),
+    # many groups of a few rows (rows as the MMA's N operand, 32 or 64 of them), some of more than a tile has
+    ([1, 0, 33, 5, 0, 2, 70, 16, 1, 1] * 3, 5, 400, 1032, 1000),
+    ([0, 9, 15, 0, 31, 32, 1] * 6, 0, 530, 640, 584),
+    ([20, 0, 65, 128, 3, 30, 31, 1] * 4, 2, 1120, 1024, 1096),
 ]
 
 
