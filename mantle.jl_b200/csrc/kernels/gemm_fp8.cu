@@ -259,8 +259,9 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     const uint64_t a0 = smem_desc(smem_u32(ring), 16, 1024), b0 = smem_desc(smem_u32(ring) + Cfg::kAStage, 16, 1024);
     for (int64_t t = t0; ok && t < ntiles; t += tstep) {
       for (int kb = kbeg; kb < kend; ++kb) {
-        ok = wait_warp(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts) &&
-             wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts);
+        // the loads were there long before; the accumulator is what the MMAs wait for
+        ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts) &&
+             wait_warp(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {

@@ -8,9 +8,8 @@
 //
 // Rows of no group keep what the output held; an empty group's dW is zeros.
 //
-// One persistent CTA per SM over tiles of RUNS x 128 rows by BN columns, the roles
-// and the ring of gemm_bf16: a TMA producer, a tcgen05.mma issuer, four epilogue
-// warps. No operand is transposed in memory: the forward product reads W N-major
+// One persistent CTA per SM over tiles of 128 rows by BN columns, the roles and the
+// ring of gemm_bf16: a TMA producer, a tcgen05.mma issuer, eight epilogue warps. No operand is transposed in memory: the forward product reads W N-major
 // (as it lies) and the input gradient reads the same memory K-major; the weight
 // gradient reads both X and dY "MN-major", a token a row of 128 bytes. The groups
 // start at any row, which TMA allows (only the inner coordinate is aligned).
@@ -38,14 +37,12 @@ namespace mtl {
 enum { kFwd = 0, kDx = 1, kDw = 2 };
 constexpr int kGrThreads = 320, kGrM = 128, kGrK = 64;
 
-template <int RUNS, int BN>
+template <int BN>
 struct GrCfg {
   static constexpr uint32_t kAStage = kGrM * kGrK * 2, kBStage = kGrK * BN * 2;
-  static constexpr uint32_t kStageBytes = RUNS * kAStage + kBStage;
+  static constexpr uint32_t kStageBytes = kAStage + kBStage;
   static constexpr int kStages = (int)(196608 / kStageBytes);
-  static constexpr int kAcc = RUNS * BN >= 512 ? 1 : 2;  // accumulator sets
-  static constexpr uint32_t kTmemCols = kAcc * RUNS * BN;
-  static constexpr int kTileM = RUNS * kGrM;
+  static constexpr uint32_t kTmemCols = 2 * BN;  // two accumulators
 };
 struct GrShared {
   uint4 stage[8][32 * 4];  // per epilogue warp: 64 bytes of 32 output rows
@@ -54,9 +51,9 @@ struct GrShared {
   int abort;
   GroupTable groups;
 };
-template <int RUNS, int BN>
+template <int BN>
 constexpr int gr_smem() {
-  return GrCfg<RUNS, BN>::kStages * (int)GrCfg<RUNS, BN>::kStageBytes + (int)sizeof(GrShared) + 1024;
+  return GrCfg<BN>::kStages * (int)GrCfg<BN>::kStageBytes + (int)sizeof(GrShared) + 1024;
 }
 
 struct GrArgs {
@@ -77,29 +74,28 @@ struct GrTile {
   int row0, depth;      // forward, dX: first row of A; dW: the group's first row and its row count
   int64_t crow;
 };
-template <int FORM, int RUNS, int BN>
+template <int FORM, int TM, int BN>  // TM rows a tile
 struct GrWalk {
   GroupWalk g;
   __device__ __forceinline__ GrTile find(const GrArgs& p, const GroupTable* groups, int t, int tiles_m, int tiles_n) {
-    constexpr int tm = RUNS * kGrM;
     GrTile c;
     if (FORM == kDw) {
       const int per = tiles_m * tiles_n, in = t % per;
       c.e = t / per;
-      c.m0 = in % tiles_m * tm;
+      c.m0 = in % tiles_m * TM;
       c.n0 = in / tiles_m * BN;
       c.rows = p.out_rows - c.m0;
       c.row0 = groups->lo[c.e];
       c.depth = groups->hi[c.e] - c.row0;
       c.crow = (int64_t)c.e * p.out_rows + c.m0;
     } else {
-      g.find(groups, t, tiles_n, tm, BN, &c.row0, &c.rows, &c.n0);
+      g.find(groups, t, tiles_n, TM, BN, &c.row0, &c.rows, &c.n0);
       c.e = g.e;
       c.m0 = 0;
       c.depth = p.depth;
       c.crow = c.row0;
     }
-    c.rows = min(c.rows, tm);
+    c.rows = min(c.rows, TM);
     return c;
   }
 };
@@ -107,11 +103,11 @@ struct GrWalk {
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16(addr, r); }
 
-template <int FORM, int RUNS, int BN, typename OUT>
+template <int FORM, int BN, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
-  using Cfg = GrCfg<RUNS, BN>;
-  constexpr int kStages = Cfg::kStages, kAcc = Cfg::kAcc;
+  using Cfg = GrCfg<BN>;
+  constexpr int kStages = Cfg::kStages;
   constexpr uint32_t kIdesc = idesc_bf16_f32(kGrM, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -125,7 +121,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       mbar_init(smem_u32(&sh->full[s]), 1);
       mbar_init(smem_u32(&sh->empty[s]), 1);
     }
-    for (int a = 0; a < kAcc; ++a) {
+    for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&sh->tfull[a]), 1);
       mbar_init(smem_u32(&sh->tempty[a]), 8);
     }
@@ -140,15 +136,15 @@ __global__ void __launch_bounds__(kGrThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  build_groups(&sh->groups, p.offsets, p.groups, p.T, Cfg::kTileM);
+  build_groups(&sh->groups, p.offsets, p.groups, p.T, kGrM);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
 
-  const int tiles_m = FORM == kDw ? (p.out_rows + Cfg::kTileM - 1) / Cfg::kTileM : 0, tiles_n = (p.cols + BN - 1) / BN;
+  const int tiles_m = FORM == kDw ? (p.out_rows + kGrM - 1) / kGrM : 0, tiles_n = (p.cols + BN - 1) / BN;
   const int ntiles = FORM == kDw ? tiles_m * tiles_n * p.groups : sh->groups.cum[p.groups] * tiles_n;  // checked by the host
-  GrWalk<FORM, RUNS, BN> walk;
+  GrWalk<FORM, kGrM, BN> walk;
 
   if (warp == 0) {
     // ── TMA producer (the whole warp waits, one lane issues) ──
@@ -162,7 +158,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         // a chunked operand comes in one box, zeros past its edges; other boxes that would
         // lie wholly past the output's rows or columns are not loaded:
         // what stale shared memory they leave feeds outputs that are not stored
-        const int a_boxes = FORM == kDw ? (p.chunked_a ? RUNS * kGrM / 64 : (c.rows + 63) / 64) : (c.rows + p.a_box - 1) / p.a_box;
+        const int a_boxes = FORM == kDw ? (p.chunked_a ? kGrM / 64 : (c.rows + 63) / 64) : (c.rows + p.a_box - 1) / p.a_box;
         const int b_boxes = FORM == kDx ? 1 : p.chunked_b ? BN / 64 : min(BN / 64, (p.cols - c.n0 + 63) / 64);
         const uint32_t bytes = (uint32_t)(a_boxes * (FORM == kDw ? kGrK * 128 : p.a_box * 128)) +
                                (FORM == kDx ? Cfg::kBStage : (uint32_t)(b_boxes * kGrK * 128));
@@ -173,7 +169,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           if (elect_one()) {
           const uint32_t fb = smem_u32(&sh->full[s]);
           mbar_expect_tx(fb, bytes);
-          const uint32_t a_dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes), b_dst = a_dst + RUNS * Cfg::kAStage;
+          const uint32_t a_dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes), b_dst = a_dst + Cfg::kAStage;
           if (FORM == kDw) {
             if (p.chunked_a)
               tma_load_4d(a_dst, &tmA, 0, c.row0 + kb * kGrK, c.m0 / 64, 0, fb);
@@ -219,15 +215,15 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     // bytes; K-major: rows of 128 bytes, a slice is 32 bytes further along the swizzled row
     constexpr uint32_t kAStep = (FORM == kDw ? 2048 : 32) >> 4, kBStep = (FORM == kDx ? 32 : 2048) >> 4;
     const uint64_t a0 = smem_desc(smem_u32(ring), FORM == kDw ? kGrK * 128 : 16, 1024);
-    const uint64_t b0 = smem_desc(smem_u32(ring) + RUNS * Cfg::kAStage, FORM == kDx ? 16 : kGrK * 128, 1024);
+    const uint64_t b0 = smem_desc(smem_u32(ring) + Cfg::kAStage, FORM == kDx ? 16 : kGrK * 128, 1024);
     for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const int kblocks = (c.depth + kGrK - 1) / kGrK;
       if (kblocks == 0) continue;
-      const int a = i % kAcc, runs = RUNS == 1 ? 1 : (c.rows + kGrM - 1) / kGrM;
-      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i / kAcc) & 1) ^ 1, abort, &g_grouped_timeouts);
+      const int a = i & 1;
+      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
       ++i;
-      const uint32_t d = tmem + (uint32_t)(a * RUNS * BN);
+      const uint32_t d = tmem + (uint32_t)(a * BN);
       for (int kb = 0; ok && kb < kblocks; ++kb) {
         ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
         if (!ok) break;
@@ -235,7 +231,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         if (FORM == kDw && c.depth - kb * kGrK < kGrK) {
           const int live = c.depth - kb * kGrK, end = (live + 15) / 16 * 16;
           steps = end / 16;
-          const int chunks = (RUNS * kGrM + BN) / 64, words = (end - live) * 8;  // 16-byte words a chunk
+          const int chunks = (kGrM + BN) / 64, words = (end - live) * 8;  // 16-byte words a chunk
           unsigned char* stage = ring + s * Cfg::kStageBytes;
           for (int w = lane; w < chunks * words; w += 32)
             *reinterpret_cast<uint4*>(stage + (w / words) * (kGrK * 128) + live * 128 + (w % words) * 16) =
@@ -246,18 +242,12 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
-          auto mmas = [&](int kk) {
-#pragma unroll
-            for (int r = 0; r < RUNS; ++r)
-              if (r < runs)
-                tc_mma(d + (uint32_t)(r * BN), a0 + off + (uint64_t)(r * (Cfg::kAStage >> 4) + kk * kAStep), b0 + off + kk * kBStep,
-                       kIdesc, (kb | kk) != 0);
-          };
+          auto mma = [&](int kk) { tc_mma(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, (kb | kk) != 0); };
           if (steps == kGrK / 16) {
 #pragma unroll
-            for (int kk = 0; kk < kGrK / 16; ++kk) mmas(kk);
+            for (int kk = 0; kk < kGrK / 16; ++kk) mma(kk);
           } else {
-            for (int kk = 0; kk < steps; ++kk) mmas(kk);
+            for (int kk = 0; kk < steps; ++kk) mma(kk);
           }
           tc_commit(smem_u32(&sh->empty[s]));
           if (kb + 1 == kblocks) tc_commit(smem_u32(&sh->tfull[a]));
@@ -280,18 +270,15 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const bool empty = c.depth == 0;
-      const int a = i % kAcc;
+      const int a = i & 1;
       if (!empty) {
-        if (!wait_warp(smem_u32(&sh->tfull[a]), (i / kAcc) & 1, abort, &g_grouped_timeouts)) break;
+        if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
         tc_fence_after();
         ++i;
       }
-#pragma unroll 1
-      for (int run = 0; run < RUNS; ++run) {
-        const int row = run * kGrM + q * 32;
-        if (row >= c.rows) break;  // uniform in the warp
-        OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
-        const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * RUNS + run) * BN);
+      if (q * 32 < c.rows) {  // uniform in the warp
+        OUT* out = static_cast<OUT*>(p.out) + (c.crow + q * 32) * (int64_t)p.cols;
+        const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
         constexpr int kW = 64 / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
 #pragma unroll 1
         for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
@@ -304,7 +291,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           } else {
             tmem_ld_row(tbase + ch * kW, r);
           }
-          store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
+          store_rows(sh->stage[warp - 2], lane, c.rows - q * 32, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
         }
       }
       if (!empty) {
@@ -493,6 +480,250 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kTmemCols) : "memory");
 }
 
+// ── the same on CTA pairs: 256 x 256 tiles ──────────────────────────────────
+// A pair loads 32 KiB a K block and CTA where one CTA a tile loads 48, which is less
+// traffic and, in a run held to its power, less of that; but a group's rows come in tiles
+// of 256. The weight gradient, whose rows are not a group's, gains most: its K loop is as
+// short as its groups while every tile leaves 128 to 256 KiB. A last K block with rows
+// behind the group lands on a barrier of each CTA's own; the CTA zeroes those rows and
+// then tells the even CTA, which issues the MMAs. Sustained, us, against one CTA a tile
+// (2048 x 4096): weight gradient of 16 groups of 8192 rows 181 and 210 (fp32), 145 and 173
+// (bf16; storing by TMA from two 4 KiB buffers a warp, with fewer stages for their room,
+// 158); forward with 4 groups 116 and 123, 8 groups 126 and 131, 16 groups 148 and 144.
+struct PairCfg {
+  static constexpr uint32_t kAStage = 128 * kGrK * 2, kStageBytes = 2 * kAStage;
+  static constexpr int kStages = 6, kBN = 256;
+};
+struct PairShared {
+  uint4 stage[8][kStageWords];  // per epilogue warp: 64 bytes of 32 output rows
+  // full, tempty: the even CTA's are used
+  uint64_t full[6], empty[6], tail[6], tfull[2], tempty[2], drain;
+  uint32_t tmem;
+  int abort;
+  GroupTable groups;
+};
+constexpr int kPairSmem = PairCfg::kStages * (int)PairCfg::kStageBytes + (int)sizeof(PairShared) + 1024;
+
+template <int FORM, typename OUT>
+__global__ void __launch_bounds__(kGrThreads, 1)
+    gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
+  using Cfg = PairCfg;
+  constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
+  constexpr uint32_t kIdesc = idesc_bf16_f32(256, BN, FORM == kDw, FORM != kDx);
+  extern __shared__ unsigned char gr_raw[];
+  unsigned char* ring =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gr_raw) + 1023) & ~uintptr_t(1023));
+  PairShared* sh = reinterpret_cast<PairShared*>(ring + kStages * Cfg::kStageBytes);
+  volatile int* abort = &sh->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = blockIdx.x & 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sh->full[s]), 2);
+      mbar_init(smem_u32(&sh->empty[s]), 1);
+      mbar_init(smem_u32(&sh->tail[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&sh->tfull[a]), 1);
+      mbar_init(smem_u32(&sh->tempty[a]), 16);
+    }
+    mbar_init(smem_u32(&sh->drain), 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  build_groups(&sh->groups, p.offsets, p.groups, p.T, 256);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are there
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem;
+
+  const int tiles_m = FORM == kDw ? (p.out_rows + 255) / 256 : 0, tiles_n = (p.cols + BN - 1) / BN;
+  const int ntiles = FORM == kDw ? tiles_m * tiles_n * p.groups : sh->groups.cum[p.groups] * tiles_n;
+  const int t0 = blockIdx.x / 2, tstep = gridDim.x / 2;
+  GrWalk<FORM, 256, BN> walk;
+
+  if (warp == 0) {
+    // ── TMA producer: this CTA's 128 rows of A and 128 columns of B ──
+    int s = 0;
+    uint32_t ph = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    for (int t = t0; ok && t < ntiles; t += tstep) {
+      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      const int m0 = c.m0 + rank * 128, n0 = c.n0 + rank * 128;
+      const int rows = min(max(c.rows - rank * 128, 0), 128), cols = min(max(p.cols - n0, 0), 128);
+      // boxes; what would lie wholly past the output's rows or columns is not loaded
+      const int a_boxes = FORM == kDw ? (rows + 63) / 64 : (rows + p.a_box - 1) / p.a_box;
+      const int b_boxes = FORM == kDx ? (cols > 0 ? 1 : 0) : (cols + 63) / 64;
+      const bool a_one = FORM == kDw && p.chunked_a && a_boxes, b_one = FORM != kDx && p.chunked_b && b_boxes;
+      const uint32_t a_bytes = FORM == kDw ? (uint32_t)((a_one ? 2 : a_boxes) * kGrK * 128) : (uint32_t)(a_boxes * p.a_box * 128);
+      const uint32_t bytes = a_bytes + (FORM == kDx ? (uint32_t)b_boxes * Cfg::kAStage : (uint32_t)((b_one ? 2 : b_boxes) * kGrK * 128));
+      const int kblocks = (c.depth + kGrK - 1) / kGrK;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts);
+        if (!ok) break;
+        if (elect_one()) {
+          const bool tail = FORM == kDw && c.depth - kb * kGrK < kGrK;
+          const uint32_t a_dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes), b_dst = a_dst + Cfg::kAStage;
+          const uint32_t fb = tail ? smem_u32(&sh->tail[s]) : map_rank(smem_u32(&sh->full[s]), 0);
+          if (tail)
+            mbar_expect_tx(fb, bytes);
+          else
+            mbar_expect_tx_cluster(fb, bytes);
+          if (FORM == kDw) {
+            const int row = c.row0 + kb * kGrK;
+            if (a_one)
+              tma_load_4d_pair(a_dst, &tmA, 0, row, m0 / 64, 0, fb);
+            else
+              for (int i = 0; i < a_boxes; ++i) tma_load_3d_pair(a_dst + i * (kGrK * 128), &tmA, m0 + i * 64, row, 0, fb);
+            if (b_one)
+              tma_load_4d_pair(b_dst, &tmB, 0, row, n0 / 64, 0, fb);
+            else
+              for (int i = 0; i < b_boxes; ++i) tma_load_3d_pair(b_dst + i * (kGrK * 128), &tmB, n0 + i * 64, row, 0, fb);
+          } else {
+            for (int i = 0; i < a_boxes; ++i)
+              tma_load_3d_pair(a_dst + i * p.a_box * 128, &tmA, kb * kGrK, c.row0 + rank * 128 + i * p.a_box, 0, fb);
+            if (FORM == kDx) {
+              if (b_boxes) tma_load_3d_pair(b_dst, &tmB, kb * kGrK, n0, c.e, fb);
+            } else if (b_one) {
+              tma_load_4d_pair(b_dst, &tmB, 0, kb * kGrK, n0 / 64, c.e, fb);
+            } else {
+              for (int i = 0; i < b_boxes; ++i)
+                tma_load_3d_pair(b_dst + i * (kGrK * 128), &tmB, n0 + i * 64, kb * kGrK, c.e, fb);
+            }
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0 && rank == 0)  // the loads in flight land before the CTAs leave
+      for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+        drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+  } else if (warp == 1) {
+    // ── MMA issuer (even CTA); both: a group's last K block made clean ──
+    int s = 0, i = 0;
+    uint32_t ph = 0, tph = 0;  // tph: a bit a stage
+    bool ok = true;
+    constexpr uint32_t kAStep = (FORM == kDw ? 2048 : 32) >> 4, kBStep = (FORM == kDx ? 32 : 2048) >> 4;
+    const uint64_t a0 = smem_desc(smem_u32(ring), FORM == kDw ? kGrK * 128 : 16, 1024);
+    const uint64_t b0 = smem_desc(smem_u32(ring) + Cfg::kAStage, FORM == kDx ? 16 : kGrK * 128, 1024);
+    // rows `live` .. up to a multiple of 16 of the stage zeroed, then the even CTA told
+    auto clean = [&](int st, int live) {
+      const bool here = wait_warp(smem_u32(&sh->tail[st]), tph >> st & 1, abort, &g_grouped_timeouts);
+      tph ^= 1u << st;
+      if (!here) return false;
+      const int end = (live + 15) / 16 * 16, words = (end - live) * 8;
+      unsigned char* stage = ring + st * Cfg::kStageBytes;
+      for (int w = lane; w < 4 * words; w += 32)
+        *reinterpret_cast<uint4*>(stage + (w / words) * (kGrK * 128) + live * 128 + (w % words) * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->full[st]), 0));
+      return true;
+    };
+    for (int t = t0; ok && t < ntiles; t += tstep) {
+      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      const int kblocks = (c.depth + kGrK - 1) / kGrK, live = FORM == kDw ? c.depth % kGrK : 0;
+      if (kblocks == 0) continue;
+      if (rank == 1) {
+        if (live) ok = clean((s + kblocks - 1) % kStages, live);
+        s = (s + kblocks) % kStages;
+        continue;
+      }
+      const int a = i & 1;
+      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
+      ++i;
+      const uint32_t d = tmem + (uint32_t)(a * BN);
+      for (int kb = 0; ok && kb < kblocks; ++kb) {
+        int steps = kGrK / 16;
+        if (live && kb + 1 == kblocks) {
+          steps = (live + 15) / 16;
+          ok = clean(s, live);
+          if (!ok) break;
+        }
+        ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
+          if (steps == kGrK / 16) {
+#pragma unroll
+            for (int kk = 0; kk < kGrK / 16; ++kk) tc_mma_pair(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, (kb | kk) != 0);
+          } else {
+            for (int kk = 0; kk < steps; ++kk) tc_mma_pair(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, (kb | kk) != 0);
+          }
+          tc_commit_pair(smem_u32(&sh->empty[s]));
+          if (kb + 1 == kblocks) tc_commit_pair(smem_u32(&sh->tfull[a]));
+        }
+        __syncwarp();
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && rank == 0 && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
+      tc_commit_pair(smem_u32(&sh->drain));
+      drain_phase(smem_u32(&sh->drain), 0);
+    }
+  } else {
+    // ── epilogue: this CTA's 128 rows; a warp 32 of them, half of the columns ──
+    const int q = warp & 3, half = (warp - 2) / 4;
+    int i = 0;
+    for (int t = t0; t < ntiles; t += tstep) {
+      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      const bool empty = c.depth == 0;
+      const int a = i & 1, row = rank * 128 + q * 32;
+      if (!empty) {
+        if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
+        tc_fence_after();
+        ++i;
+      }
+      if (row < c.rows) {
+        OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+        const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
+        constexpr int kW = 64 / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
+#pragma unroll 1
+        for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
+          const int col = c.n0 + ch * kW;
+          if (col >= p.cols) break;
+          uint32_t r[kW];
+          if (empty) {
+#pragma unroll
+            for (int v = 0; v < kW; ++v) r[v] = 0;
+          } else {
+            tmem_ld_row(tbase + ch * kW, r);
+          }
+          store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
+        }
+      }
+      if (!empty) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->tempty[a]), 0));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other's loads, MMAs or arrivals may reach it
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
 // ── host side ───────────────────────────────────────────────────────────────
 cudaError_t grouped_set_wait_limit(unsigned long long ns) { return set_wait_limit_this_file(ns); }
 int grouped_timeouts(bool reset) {
@@ -566,14 +797,14 @@ mtl_status gemm_grouped_check(const LaunchArgs& la, const uint64_t* bytes) { ret
 mtl_status gemm_grouped_dx_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kDx>(la, bytes); }
 mtl_status gemm_grouped_dw_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kDw>(la, bytes); }
 
-template <int FORM, int RUNS, int BN, typename OUT>
+template <int FORM, int BN, typename OUT>
 static cudaError_t gr_launch(const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
                              const LaunchArgs& la, cudaStream_t s) {
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(gemm_grouped_kernel<FORM, RUNS, BN, OUT>, gr_smem<RUNS, BN>(), la.device, &done);
+  cudaError_t e = allow_smem(gemm_grouped_kernel<FORM, BN, OUT>, gr_smem<BN>(), la.device, &done);
   if (e != cudaSuccess) return e;
   const int grid = (int)std::min<int64_t>(tiles, la.sm_count);
-  gemm_grouped_kernel<FORM, RUNS, BN, OUT><<<grid, kGrThreads, gr_smem<RUNS, BN>(), s>>>(ta, tb, p);
+  gemm_grouped_kernel<FORM, BN, OUT><<<grid, kGrThreads, gr_smem<BN>(), s>>>(ta, tb, p);
   return cudaGetLastError();
 }
 
@@ -585,6 +816,27 @@ static cudaError_t gr_launch_slim(const CUtensorMap& tx, const CUtensorMap& tw, 
   if (e != cudaSuccess) return e;
   gemm_grouped_slim_kernel<FORM, NT, OUT><<<(int)std::min<int64_t>(tiles, la.sm_count), kGrThreads, slim_smem<NT>(), s>>>(tx, tw, p);
   return cudaGetLastError();
+}
+
+template <int FORM, typename OUT>
+static cudaError_t gr_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
+                                  const LaunchArgs& la, cudaStream_t s) {
+  auto kernel = gemm_grouped_pair_kernel<FORM, OUT>;
+  static unsigned long long done = 0;
+  cudaError_t e = allow_smem(kernel, kPairSmem, la.device, &done);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, la.sm_count / 2)));
+  cfg.blockDim = dim3(kGrThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
 }
 
 template <int FORM>
@@ -607,34 +859,37 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   p.out_rows = K;
   p.groups = E;
   p.vec = la.a[0].ptr % 16 == 0;  // N and K are multiples of 8
-  const bool wide = false;
+  // Pairs where their 256-row tiles waste little (groups of 768 rows on average) and
+  // there is a tile for each.
+  const int64_t col_tiles = (cols + 255) / 256, pair_tiles = (FORM == kDw ? (int64_t)E * ((K + 255) / 256) : T / 256) * col_tiles;
+  const bool pair = pair_tiles >= la.sm_count / 2 && (FORM == kDw || T >= 768 * (int64_t)E);
   // Rows of a group in the MMA's N operand, 32 or 64 of them, while a group has up to 16
   // or 40 on average and there are tiles for most SMs. Sustained, us, against tiles of 128
   // rows: 2 rows a group (32 groups, 2048 x 4096) 81.7 and 89.5, 8 rows 83.1 and 90.8, 32
   // rows (16 groups, 2048 x 2048) 25.5 with 64, 29.7 with 32 and 28.0, 64 rows 55 and 51.3.
-  const int64_t slim_tiles = (int64_t)E * ((cols + 255) / 256);
+  const int64_t slim_tiles = (int64_t)E * col_tiles;
   const int slim = FORM == kDw || slim_tiles * 4 < la.sm_count * 3 || T > 40 * (int64_t)E ? 0 : T <= 16 * (int64_t)E ? 32 : 64;
   p.a_box = slim ? slim : T / E >= kGrM ? kGrM : 32;
   const void *A = reinterpret_cast<const void*>(la.a[1].ptr), *B = reinterpret_cast<const void*>(la.a[2].ptr);
   const int64_t row_tiles = FORM == kDw ? (int64_t)E * ((K + 127) / 128) : std::max<int64_t>(E, (T + 127) / 128);
-  const bool narrow = !wide && !slim && row_tiles * ((cols + 255) / 256) < la.sm_count;
-  const int bn = narrow ? 128 : 256;
+  const bool narrow = !pair && !slim && row_tiles * col_tiles < la.sm_count;
+  const int bn = narrow ? 128 : 256, box_n = pair ? 128 : bn;  // columns of B a tile, a box
   p.chunked_a = FORM == kDw && K % 64 == 0;
   p.chunked_b = FORM != kDx && N % 64 == 0;
   CUtensorMap ta, tb;
-  mtl_status st = p.chunked_a ? make_chunk_map(&ta, A, K, T, 1, kGrK, (wide ? 2 : 1) * kGrM / 64)
+  mtl_status st = p.chunked_a ? make_chunk_map(&ta, A, K, T, 1, kGrK, kGrM / 64)
                               : make_bf16_map(&ta, A, FORM == kDx ? N : K, T, 1, FORM == kDw ? kGrK : p.a_box);
   if (st) return st;
-  st = p.chunked_b ? make_chunk_map(&tb, B, N, FORM == kDw ? T : K, FORM == kDw ? 1 : E, kGrK, bn / 64)
+  st = p.chunked_b ? make_chunk_map(&tb, B, N, FORM == kDw ? T : K, FORM == kDw ? 1 : E, kGrK, box_n / 64)
        : FORM == kDw ? make_bf16_map(&tb, B, N, T, 1, kGrK)
-                     : make_bf16_map(&tb, B, N, K, E, FORM == kDx ? bn : kGrK);
+                     : make_bf16_map(&tb, B, N, K, E, FORM == kDx ? box_n : kGrK);
   if (st) return st;
-  const int64_t tile_m = wide ? 256 : 128;
+  const int64_t tile_m = pair ? 256 : 128;
   const int64_t tiles = (FORM == kDw ? (int64_t)E * ((K + tile_m - 1) / tile_m) : T / tile_m + E) * ((cols + bn - 1) / bn);
   cudaError_t e;
   if (slim) {
     if constexpr (FORM != kDw) {
-      const int64_t n = ((int64_t)T / slim + E) * ((cols + 255) / 256);
+      const int64_t n = ((int64_t)T / slim + E) * col_tiles;
       if (slim == 32)
         e = out ? gr_launch_slim<FORM, 32, __nv_bfloat16>(ta, tb, p, n, la, s) : gr_launch_slim<FORM, 32, float>(ta, tb, p, n, la, s);
       else
@@ -642,12 +897,12 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
     } else {
       e = cudaErrorInvalidValue;
     }
-  } else if (wide) {
-    e = out ? gr_launch<FORM, 2, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 2, 256, float>(ta, tb, p, tiles, la, s);
+  } else if (pair) {
+    e = out ? gr_launch_pair<FORM, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch_pair<FORM, float>(ta, tb, p, tiles, la, s);
   } else if (narrow) {
-    e = out ? gr_launch<FORM, 1, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 1, 128, float>(ta, tb, p, tiles, la, s);
+    e = out ? gr_launch<FORM, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 128, float>(ta, tb, p, tiles, la, s);
   } else {
-    e = out ? gr_launch<FORM, 1, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 1, 256, float>(ta, tb, p, tiles, la, s);
+    e = out ? gr_launch<FORM, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 256, float>(ta, tb, p, tiles, la, s);
   }
   return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }

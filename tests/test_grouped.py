@@ -90,6 +90,9 @@ SIZES = [
     ([1, 0, 33, 5, 0, 2, 70, 16, 1, 1] * 3, 5, 400, 1032, 1000),
     ([0, 9, 15, 0, 31, 32, 1] * 6, 0, 530, 640, 584),
     ([20, 0, 65, 128, 3, 30, 31, 1] * 4, 2, 1120, 1024, 1096),
+    # large groups, enough 256 x 256 tiles for CTA pairs in every form; chunked and ragged widths
+    ([2500, 0, 1800, 700], 3, 5010, 2056, 2104),
+    ([3001, 1999], 0, 5000, 2112, 1984),
 ]
 
 
@@ -141,6 +144,32 @@ def test_other_groups_rows_do_not_reach_a_group(dev, way):
         check(out[1], x[r].t(), dy[r], 0)
     else:
         check(out[r], *((x[r], w[1]) if way == "fwd" else (dy[r], w[1].t())), 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k,n", [(520, 264), (576, 320)])
+def test_other_groups_rows_do_not_reach_a_weight_gradient_of_many_groups(dev, k, n):
+    # enough tiles for CTA pairs; every other group and the rows of no group hold NaN and infinities
+    sizes = [(7 * i) % 131 for i in range(40)]
+    o = [4 + sum(sizes[:i]) for i in range(41)]
+    t = o[-1] + 9
+    x, dy = normal((t, k), 1), normal((t, n), 2)
+    bad = torch.ones(t, dtype=torch.bool)
+    for i in range(1, 40, 2):
+        bad[o[i]:o[i + 1]] = False
+    for v in (x, dy):
+        v[bad] = float("nan")
+        v[:2] = float("inf")
+    out = torch.full((40, k, n), 7.0, device="cuda")
+    launch("dw", out, x.cuda(), dy.cuda(), o, t, n, k, 40, 0)
+    torch.cuda.synchronize()
+    x, dy = x.double(), dy.double()
+    for i in range(1, 40, 2):
+        r = slice(o[i], o[i + 1])
+        check(out[i], x[r].t(), dy[r], 0)
+    for i in range(40):
+        if sizes[i] == 0:
+            assert float(out[i].abs().max()) == 0.0
 
 
 @pytest.mark.gpu
