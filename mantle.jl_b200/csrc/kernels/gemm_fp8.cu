@@ -974,6 +974,7 @@ static mtl_status fp8_check_common(const char* who, const LaunchArgs& la, const 
   const char* what[5] = {"C", "A", "A's scales", "B", "B's scales"};
   const unsigned align[5] = {out ? 1u : 3u, 15, 3, 15, 3};
   for (int i = 0; i < 5; ++i) {
+    if (!la.a[i].ptr && need[i]) return fail(MTL_ERR_ARGUMENT, "%s: %s must be a device buffer", who, what[i]);
     if (bytes[i] && bytes[i] < need[i])
       return fail(MTL_ERR_ARGUMENT, "%s: %s has %llu bytes, the launch touches %llu", who, what[i], (unsigned long long)bytes[i],
                   (unsigned long long)need[i]);
@@ -1002,7 +1003,7 @@ mtl_status gemm_grouped_fp8_check(const LaunchArgs& la, const uint64_t* bytes) {
                                        la.a[10].i32, la.a[11].i32))
     return st;
   if (la.a[8].i32 == 0) return fail(MTL_ERR_ARGUMENT, "gemm_grouped_fp8: K must be positive");
-  if ((bytes[5] && bytes[5] < (uint64_t)(groups + 1) * 4) || la.a[5].ptr % 4)
+  if (!la.a[5].ptr || (bytes[5] && bytes[5] < (uint64_t)(groups + 1) * 4) || la.a[5].ptr % 4)
     return fail(MTL_ERR_ARGUMENT, "gemm_grouped_fp8: the offsets are %lld 4-byte aligned Int32 values", (long long)groups + 1);
   return MTL_OK;
 }

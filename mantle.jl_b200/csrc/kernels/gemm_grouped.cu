@@ -783,6 +783,7 @@ static mtl_status gr_check(const LaunchArgs& la, const uint64_t* bytes) {
   const char* what[3][4] = {{"Y", "X", "W", "the offsets"}, {"dX", "dY", "W", "the offsets"}, {"dW", "X", "dY", "the offsets"}};
   const unsigned align[4] = {out ? 1u : 3u, 15, 15, 3};
   for (int i = 0; i < 4; ++i) {
+    if (!la.a[i].ptr && need[i]) return fail(MTL_ERR_ARGUMENT, "%s: %s must be a device buffer", who, what[FORM][i]);
     if (bytes[i] && bytes[i] < need[i])
       return fail(MTL_ERR_ARGUMENT, "%s: %s: %llu bytes, the launch touches %llu", who, what[FORM][i], (unsigned long long)bytes[i],
                   (unsigned long long)need[i]);

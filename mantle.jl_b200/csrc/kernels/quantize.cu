@@ -356,8 +356,8 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
   if (!gather && xrows != R)
     return fail(MTL_ERR_ARGUMENT, "quantize_fp8: without rows_of the input has as many rows as the output: %lld, got %lld", (long long)R,
                 (long long)xrows);
-  const bool q = la.a[0].ptr, s = la.a[1].ptr, qt = la.a[2].ptr, st = la.a[3].ptr;
-  if (q != s || qt != st || (!q && !qt))
+  const bool q = la.a[0].ptr, s = la.a[1].ptr, qt = la.a[2].ptr, st = la.a[3].ptr, none = batch == 0 || R == 0 || C == 0;
+  if (!none && (q != s || qt != st || (!q && !qt)))
     return fail(MTL_ERR_ARGUMENT, "quantize_fp8: give the codes and the scales of the row form, of the transposed form, or of both");
   const int64_t rb = (R + 127) / 128, cb = (C + 127) / 128, per = la.a[10].i32 ? 2 : 4;
   const bool square = block == 128;
@@ -366,6 +366,7 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
   const char* what[6] = {"the codes", "the scales", "the transposed codes", "the transposed scales", "the input", "rows_of"};
   const unsigned align[6] = {15, 3, 15, 3, la.a[10].i32 ? 1u : 3u, 3};
   for (int i = 0; i < 6; ++i) {
+    if (i == 4 && !la.a[i].ptr && need[i]) return fail(MTL_ERR_ARGUMENT, "quantize_fp8: the input must be a device buffer");
     if (!la.a[i].ptr) continue;
     if (bytes[i] && bytes[i] < need[i])
       return fail(MTL_ERR_ARGUMENT, "quantize_fp8: %s: %llu bytes, the launch touches %llu", what[i], (unsigned long long)bytes[i],

@@ -295,21 +295,21 @@ static KernelDesc g_kernels[] = {
     // values to 8-bit floating point, one scale per block of 128: q, s, transposed
     // q, transposed s, x, rows_of, R, C, rows of x, block (1 or 128), type of x (0
     // f32, 1 bf16), format (0 e4m3, 1 e5m2), power-of-two scales; ndrange = batch
-    {"quantize_fp8", "bbbbBbiiiiiii", false, 0b110000, 0b001111, quantize_check, nullptr, quantize_run, nullptr},
+    {"quantize_fp8", "bbbbBbiiiiiii", false, 0b110000, 0b001111, quantize_check, nullptr, quantize_run, nullptr, true},
     // C = A B^T of such values: C, A, A's scales, B, B's scales, M, N, K, rows per
     // scale of B (1 or 128), formats of A and B, output (0 f32, 1 bf16); ndrange = batch
-    {"gemm_fp8", "BBBBBiiiiiii", false, 0b11110, 0b1, gemm_fp8_check, nullptr, gemm_fp8_run, nullptr},
+    {"gemm_fp8", "BBBBBiiiiiii", false, 0b11110, 0b1, gemm_fp8_check, nullptr, gemm_fp8_run, nullptr, true},
     // the same by expert: Y, X, X's scales, W, W's scales, offsets, T, N, K, formats
     // of X and W, output; ndrange = groups
     {"gemm_grouped_fp8", "BBBBBBiiiiii", false, 0b111110, 0b1, gemm_grouped_fp8_check, nullptr, gemm_grouped_fp8_run,
-     nullptr},
+     nullptr, true},
     // bf16 products by expert and their gradients: Y, X, W / dX, dY, W / dW, X, dY;
     // offsets, T, N, K, output; ndrange = groups
-    {"gemm_grouped_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_check, nullptr, gemm_grouped_run, nullptr},
+    {"gemm_grouped_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_check, nullptr, gemm_grouped_run, nullptr, true},
     {"gemm_grouped_dx_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_dx_check, nullptr, gemm_grouped_dx_run,
-     nullptr},
+     nullptr, true},
     {"gemm_grouped_dw_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_dw_check, nullptr, gemm_grouped_dw_run,
-     nullptr},
+     nullptr, true},
     // NHWC bf16 convolution (implicit GEMM): out, in, w (HWIO), H, W, Cin, Cout,
     // k, stride, pad, relu, in_wpad, out_wpad; ndrange = images
     {"conv2d_bf16", "BBBiiiiiiiiii", false, 0b110, 0b001, conv_check, conv_workspace, conv_run, nullptr},
@@ -381,7 +381,7 @@ mtl_status launch_kernel(int kernel, const LaunchArgs& la, void* ws, uint64_t ws
   for (size_t i = 0; i < la.a.size(); ++i) {
     bytes[i] = la.a[i].bytes;
     char c = kd->sig[i];
-    if ((c == 'B') && (la.a[i].kind != MTL_ARG_PTR || la.a[i].ptr == 0))
+    if ((c == 'B') && (la.a[i].kind != MTL_ARG_PTR || (la.a[i].ptr == 0 && !kd->empties)))
       return fail(MTL_ERR_ARGUMENT, "%s: argument %zu must be a device buffer", kd->name, i + 1);
   }
   if (kd->check)

@@ -140,6 +140,9 @@ struct KernelDesc {
   // none); returns the register of each written argument through `out_reg`.
   int (*ew_emit)(const LaunchArgs&, std::vector<EwOp>& prog, int* slot, int* out_reg,
                  int* nregs);
+  // A buffer argument may be null in a direct launch that touches none of it (an
+  // empty batch's tensors have no address); the check refuses it otherwise.
+  bool empties = false;
 };
 const KernelDesc* kernel_desc(int id);
 int kernel_count();

@@ -592,38 +592,52 @@ def _nd(ndrange) -> tuple[int, ...]:
     return tuple(int(v) for v in ndrange) if isinstance(ndrange, (tuple, list)) else (int(ndrange),)
 
 
-# Bytes per element of the operands of the 8-bit and expert-grouped kernels, by
-# argument (a tuple indexed by the kernel's type argument where it decides), and
-# that argument's index. The library sees addresses and byte counts only, so what a
-# tensor or buffer says of itself is checked here.
-_OUT = (4, 2)
+# What the buffer arguments of the 8-bit and expert-grouped kernels hold, a letter each:
+# c codes (8 bits), f Float32, h bfloat16 (or its bits), i Int32, o f or h as the
+# kernel's type argument says, whose index follows. The library sees addresses and
+# byte counts only, so what a tensor or buffer says of itself is checked here.
 _OPERANDS = {
-    "quantize_fp8": ((1, 4, 1, 4, _OUT, 4), 10),
-    "gemm_fp8": ((_OUT, 1, 4, 1, 4), 11),
-    "gemm_grouped_fp8": ((_OUT, 1, 4, 1, 4, 4), 11),
-    "gemm_grouped_bf16": ((_OUT, 2, 2, 4), 7),
-    "gemm_grouped_dx_bf16": ((_OUT, 2, 2, 4), 7),
-    "gemm_grouped_dw_bf16": ((_OUT, 2, 2, 4), 7),
+    "quantize_fp8": ("cfcfoi", 10),
+    "gemm_fp8": ("ocfcf", 11),
+    "gemm_grouped_fp8": ("ocfcfi", 11),
+    "gemm_grouped_bf16": ("ohhi", 7),
+    "gemm_grouped_dx_bf16": ("ohhi", 7),
+    "gemm_grouped_dw_bf16": ("ohhi", 7),
 }
+_KINDS = {np.dtype(t): k for k, types in {"c": (np.uint8, np.int8), "f": (np.float32,), "h": (np.uint16, np.int16),
+                                          "i": (np.int32, np.uint32)}.items() for t in types}
+_KIND_NAMES = {"c": "8-bit codes", "f": "Float32", "h": "bfloat16", "i": "Int32"}
+_tensor = None  # torch.Tensor, once torch is loaded
+
+
+def _with_torch() -> None:
+    global _tensor
+    torch = sys.modules["torch"]
+    for kind, names in {"c": ("uint8", "int8", "float8_e4m3fn", "float8_e5m2"), "f": ("float32",),
+                        "h": ("bfloat16", "uint16", "int16"), "i": ("int32",)}.items():
+        _KINDS.update({getattr(torch, n): kind for n in names if hasattr(torch, n)})
+    _tensor = torch.Tensor
 
 
 def _operands(k: Kernel, args: Sequence) -> list:
     """(kind, rid, address, bytes) of each buffer argument of a kernel in _OPERANDS, in
-    one flat list, checked: element sizes, and for torch tensors contiguity and the
+    one flat list, checked: element types, and for torch tensors contiguity and the
     current CUDA device. A graph resource's address is its plan's and stays 0."""
-    sizes, flag = _OPERANDS[k.name]
+    kinds, flag = _OPERANDS[k.name]
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"{k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
-    flat, device, tensor = [], None, _tensor_type()
-    for x, size in zip(args, sizes):
-        if tensor is not None and isinstance(x, tensor):
+    if _tensor is None and "torch" in sys.modules:
+        _with_torch()
+    flat, device = [], None
+    for x, want in zip(args, kinds):
+        if _tensor is not None and isinstance(x, _tensor):
             if device is None:
-                device = _current_device(x)
+                device = sys.modules["torch"].cuda.current_device() if x.get_device() >= 0 else 0
             if x.get_device() != device or not x.is_contiguous():
                 raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4 + 1} must be a contiguous CUDA tensor on the "
                                     f"current device ({device})")
-            got = x.element_size()
-            flat += (L.ARG_PTR, 0, x.data_ptr(), x.numel() * got)
+            got = _KINDS.get(x.dtype)
+            flat += (L.ARG_PTR, 0, x.data_ptr(), x.nbytes)
         elif x is None:
             flat += (L.ARG_NULL, 0, 0, 0)
             continue
@@ -632,27 +646,16 @@ def _operands(k: Kernel, args: Sequence) -> list:
             continue
         else:
             x = x.resource if isinstance(x, UseHandle) else x
-            if not hasattr(x, "dtype") or hasattr(x, "data_ptr"):
+            if not isinstance(x, (Buffer, TransientBuffer, VirtualBuffer)):
                 raise ArgumentError(L.ERR_ARGUMENT, f"cannot pass {x!r} where the kernel takes a buffer")
-            got = x.dtype.itemsize
+            got = _KINDS.get(x.dtype)
             flat += (L.ARG_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
-        if size is _OUT:
+        if want == "o":
             kind = args[flag]
-            size = _OUT[kind] if kind in (0, 1) else got  # the library refuses another type
-        if got != size:
-            raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4} has elements of {got} bytes, expected {size}")
+            want = "fh"[kind] if kind in (0, 1) else got  # the library refuses another type
+        if got != want:
+            raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4} holds {x.dtype}, expected {_KIND_NAMES[want]}")
     return flat
-
-
-def _tensor_type():
-    """torch.Tensor where torch is loaded (no argument can be one where it is not)."""
-    torch = sys.modules.get("torch")
-    return getattr(torch, "Tensor", None)
-
-
-def _current_device(x) -> int:
-    """The current CUDA device, asked for only where `x` is on one."""
-    return sys.modules["torch"].cuda.current_device() if x.get_device() >= 0 else 0
 
 
 class _Packed:

@@ -136,9 +136,75 @@ def test_a_training_step_of_experts_in_a_graph(dev):
     torch.cuda.synchronize()
     assert np.array_equal(Y.array(), y.cpu().numpy().reshape(-1)) and np.array_equal(DX.array(), dx.cpu().numpy().reshape(-1))
     assert np.array_equal(DW.array().view(np.int16), dw.view(torch.int16).cpu().numpy().reshape(-1))
-    with pytest.raises(M.ArgumentError, match="elements of 4 bytes"):
+    with pytest.raises(M.ArgumentError, match="holds float32, expected bfloat16"):
         M.compute(graph, "bad", lambda p: M.dispatch(p, M.kernels.gemm_grouped_bf16, (
             Wr(p, Y), R(p, Y), R(p, W), R(p, O), t, n, k, 0), e))
+
+
+@pytest.mark.gpu
+def test_no_rows_at_all(dev):
+    # an empty batch's tensors have no address: every call is a no-op, but a weight gradient is zeros
+    e, k, n = 3, 64, 72
+    h = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    off, w = torch.zeros(e + 1, dtype=torch.int32, device="cuda"), h(e, k, n)
+    M.launch(M.kernels.gemm_grouped_bf16, (h(0, n), h(0, k), w, off, 0, n, k, 1), e, stream=stream())
+    M.launch(M.kernels.gemm_grouped_dx_bf16, (h(0, k), h(0, n), w, off, 0, n, k, 1), e, stream=stream())
+    dw = torch.full((e, k, n), 5.0, device="cuda")
+    M.launch(M.kernels.gemm_grouped_dw_bf16, (dw, h(0, k), h(0, n), off, 0, n, k, 0), e, stream=stream())
+    q, s = quantized(torch.zeros((1, 0, k), device="cuda"), 1)
+    qw, sw = quantized(torch.zeros((e, n, k), device="cuda"), 128)
+    M.launch(M.kernels.gemm_grouped_fp8, (h(0, n), q, s, qw, sw, off, 0, n, k, 0, 0, 1), e, stream=stream())
+    M.launch(M.kernels.gemm_fp8, (h(1, 0, n), q, s, qw, sw, 0, n, k, 128, 0, 0, 1), 1, stream=stream())
+    torch.cuda.synchronize()
+    assert float(dw.abs().max()) == 0.0
+    # but not where something would be touched
+    with pytest.raises(M.ArgumentError, match="X must be a device buffer"):
+        M.launch(M.kernels.gemm_grouped_bf16, (h(4, n), h(0, k), w, off, 4, n, k, 1), e, stream=stream())
+    with pytest.raises(M.ArgumentError, match="A must be a device buffer"):
+        M.launch(M.kernels.gemm_fp8, (h(1, 4, n), q, s, qw, sw, 4, n, k, 128, 0, 0, 1), 1, stream=stream())
+
+
+@pytest.mark.gpu
+def test_types_strides_and_devices_are_refused(dev):
+    e, t, k, n = 2, 16, 64, 72
+    x, w = (torch.zeros(s, dtype=torch.bfloat16, device="cuda") for s in ((t, k), (e, k, n)))
+    y, off = torch.zeros((t, n), device="cuda"), torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    go = lambda *a: M.launch(M.kernels.gemm_grouped_bf16, (*a, t, n, k, 0), e, stream=stream())  # noqa: E731
+    go(y, x, w, off)
+    go(torch.nn.Parameter(y, requires_grad=False), x, w, off)
+    for args, match in (((y, x.half(), w, off), "holds torch.float16, expected bfloat16"), ((y, x, w, off.long()), "expected Int32"),
+                        ((y, x, w, off.float()), "expected Int32"), ((y.bfloat16(), x, w, off), "expected Float32"),
+                        ((y, x.t().contiguous().t(), w, off), "contiguous"), ((y, x, w.cpu(), off), "current device"),
+                        ((y.cpu(), x, w, off), "contiguous CUDA tensor"), ((y, x, w, [0, 1, 2]), "takes a buffer")):
+        with pytest.raises(M.ArgumentError, match=match):
+            go(*args)
+    with pytest.raises(M.ArgumentError, match="no Int32"):
+        M.launch(M.kernels.gemm_grouped_bf16, (y, x, w, off, t, n, k, 1 << 40), e, stream=stream())
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_a_thousand_experts(dev):
+    e, k, n = 1024, 64, 72
+    sizes = np.arange(e) % 4
+    o = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    t = int(o[-1])
+    g = torch.Generator().manual_seed(2)
+    x, w = torch.randint(-3, 4, (t, k), generator=g).bfloat16(), torch.randint(-3, 4, (e, k, n), generator=g).bfloat16()
+    y, off = torch.zeros((t, n), device="cuda"), torch.from_numpy(o).cuda()
+    M.launch(M.kernels.gemm_grouped_bf16, (y, x.cuda(), w.cuda(), off, t, n, k, 0), e, stream=stream())
+    which = torch.from_numpy(np.repeat(np.arange(e), sizes))
+    want = torch.einsum("tk,tkn->tn", x.double(), w[which].double())  # whole numbers: exact
+    torch.cuda.synchronize()
+    assert torch.equal(y.double().cpu(), want)
+    qx, sx = quantized(x[None].cuda().float(), 1)
+    qw, sw = quantized(w.transpose(1, 2).contiguous().cuda().float(), 128)
+    M.launch(M.kernels.gemm_grouped_fp8, (y, qx, sx, qw, sw, off, t, n, k, 0, 0, 0), e, stream=stream())
+    torch.cuda.synchronize()
+    vx = values(qx[0].view(CODE[0]), sx[0], 1, k)
+    vw = torch.stack([values(qw[i].view(CODE[0]), sw[i], 128, k) for i in range(e)])[which]
+    tol = (128 * 2.0 ** -23 + 3 * 2.0 ** -24) * torch.einsum("tk,tnk->tn", vx.abs(), vw.abs())
+    assert ((y.double().cpu() - torch.einsum("tk,tnk->tn", vx, vw)).abs() <= tol).all()
 
 
 @pytest.mark.gpu
