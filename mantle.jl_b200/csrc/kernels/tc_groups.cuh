@@ -108,21 +108,31 @@ __device__ __forceinline__ void store_rows(uint4* stage, int lane, int rows, OUT
     stage[lane * 4 + (w ^ (lane >> 1 & 3))] = u;
   }
   __syncwarp();
-  const int w = lane & 3, c = col + w * kPer;
+  if (vec) {
+    const int w = lane & 3, c = col + w * kPer;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = i * 8 + lane / 4;
-    const uint4 u = stage[row * 4 + (w ^ (row >> 1 & 3))];
-    if (row < rows) {
-      OUT* dst = out + (int64_t)row * cols + c;
-      if (vec && c + kPer <= cols) {
-        *reinterpret_cast<uint4*>(dst) = u;
-      } else {
-        const OUT* e = reinterpret_cast<const OUT*>(&u);
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + lane / 4;
+      const uint4 u = stage[row * 4 + (w ^ (row >> 1 & 3))];
+      if (row < rows) {
+        OUT* dst = out + (int64_t)row * cols + c;
+        if (c + kPer <= cols) {
+          *reinterpret_cast<uint4*>(dst) = u;
+        } else {
+          const OUT* e = reinterpret_cast<const OUT*>(&u);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          if (c + k < cols) dst[k] = e[k];
+          for (int k = 0; k < kPer; ++k)
+            if (c + k < cols) dst[k] = e[k];
+        }
       }
+    }
+  } else {
+    // rows start anywhere: neighbouring lanes store neighbouring values
+    const int c = lane % COLS, w = c / kPer;
+#pragma unroll 4
+    for (int row = lane / COLS; row < 32; row += 32 / COLS) {
+      const OUT v = reinterpret_cast<const OUT*>(&stage[row * 4 + (w ^ (row >> 1 & 3))])[c % kPer];
+      if (row < rows && col + c < cols) out[(int64_t)row * cols + col + c] = v;
     }
   }
   __syncwarp();
