@@ -6,17 +6,19 @@
 // A: M rows of K codes, B: N rows of K codes (both e4m3 or e5m2, rows K rounded up
 // to 16 bytes apart, as quantize_fp8 writes them), sA: (K blocks, M), sB: one scale
 // per 128 x 128 block (N blocks, K blocks) or per row (K blocks, N); C fp32 or bf16.
-// The same kernel runs a batch of products and products grouped by expert
-// (gemm_grouped_fp8: rows offsets[e] .. offsets[e + 1] of A times B[e]).
+// The same kernels run a batch of products and products grouped by expert
+// (gemm_grouped_fp8: rows offsets[e] .. offsets[e + 1] of A times B[e]). Two forms for
+// few rows follow the tiles below.
 //
 // The scales are arbitrary fp32 values, so a block's products cannot simply
 // accumulate in tensor memory: each K block of 128 is one chain of four
 // tcgen05.mma (kind::f8f6f4, K = 32) into its own accumulator, and eight warps
 // read it back (tcgen05.ld), multiply by the scales and add to fp32 sums in
 // registers, rounding to nearest, while the tensor core runs the next K block
-// into another accumulator. A K block of a 128 x 256 tile is 512 cycles of MMAs;
-// its read-back and packed FMAs take about as many issue slots of the two warps
-// per scheduler.
+// into another accumulator. A K block of a 128 x 256 tile is 512 cycles of MMAs, but
+// the two accumulators that fit are handed back and forth in about 800 with nothing to
+// add, and the sums come to about 1050: 8192 cubed takes 545 us in a burst (2020
+// TFLOP/s) and 642 in a long run, which the power cap holds to that.
 //
 // One persistent CTA per SM, three warpgroups; the first gives registers up
 // (setmaxnreg) so that the sums of the other two stay in theirs:
@@ -64,8 +66,8 @@ struct F8None {};
 template <bool GROUPED, bool ROWB>
 struct F8Shared {
   uint4 stage[8][kStageWords];  // per warp of sums: output rows on their way out
-  alignas(16) float sa[kF8Scales][4][kF8M];              // K blocks' scales of the tile's rows of A
-  alignas(16) float sb[kF8Scales][4][ROWB ? 256 : 4];    // and of its rows of B, or of its 128-row blocks
+  alignas(16) float sa[kF8Scales][4][kF8M];            // K blocks' scales of the tile's rows of A
+  alignas(16) float sb[kF8Scales][4][ROWB ? 256 : 4];  // and of its rows of B, or of its 128-row blocks
   uint64_t full[8], empty[8], tfull[4], tempty[4], sfull[kF8Scales], sempty[kF8Scales], drain;
   uint32_t tmem;
   int abort;
@@ -217,117 +219,117 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
   // 384 threads start with 168 registers each: 128 x 56 + 256 x 224 = 384 x 168
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8FewRegs));
-  if (warp == 0) {
-    // ── TMA producer (the whole warp waits, one lane issues) ──
-    int s = 0;
-    uint32_t ph = 0;
-    int64_t issued = 0;
-    bool ok = true;
-    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
-      const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
-      const int boxes = (c.rows + p.a_box - 1) / p.a_box;
-      const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
-      for (int kb = kbeg; kb < kend; ++kb) {
-        ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts);
-        if (!ok) break;
-        if (elect_one()) {
-          const uint32_t fb = smem_u32(&sh->full[s]), dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes);
-          mbar_expect_tx(fb, bytes);
-          tma_load_3d(dst + Cfg::kAStage, &tmB, kb * kF8K, c.n0, c.b_b, fb);
-          for (int r = 0; r < boxes; ++r)
-            tma_load_3d(dst + r * p.a_box * kF8K, &tmA, kb * kF8K, c.a_row + r * p.a_box, c.a_b, fb);
-        }
-        __syncwarp();
-        ++issued;
-        if (++s == kStages) {
-          s = 0;
-          ph ^= 1;
-        }
-      }
-    }
-    if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
-      for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-        drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
-  } else if (warp == 1) {
-    // ── MMA issuer (the whole warp waits, one lane issues) ──
-    int s = 0, a = 0;
-    uint32_t ph = 0, aph = 0;
-    bool ok = true;
-    // both operands K-major: rows of 128 bytes, 8-row groups 1024 bytes apart; a K = 32
-    // slice is 32 bytes further along the swizzled row
-    const uint64_t a0 = smem_desc(smem_u32(ring), 16, 1024), b0 = smem_desc(smem_u32(ring) + Cfg::kAStage, 16, 1024);
-    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
-      for (int kb = kbeg; kb < kend; ++kb) {
-        // the loads were there long before; the accumulator is what the MMAs wait for
-        ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts) &&
-             wait_warp(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t d = tmem + (uint32_t)(a * BN);
-          const uint64_t ad = a0 + (uint64_t)(s * (Cfg::kStageBytes >> 4)), bd = b0 + (uint64_t)(s * (Cfg::kStageBytes >> 4));
-#pragma unroll
-          for (int kk = 0; kk < kF8K / 32; ++kk) tc_mma_f8(d, ad + kk * 2, bd + kk * 2, p.idesc, kk != 0);
-          tc_commit(smem_u32(&sh->empty[s]));
-          tc_commit(smem_u32(&sh->tfull[a]));
-        }
-        __syncwarp();
-        if (++s == kStages) {
-          s = 0;
-          ph ^= 1;
-        }
-        if (++a == kAcc) {
-          a = 0;
-          aph ^= 1;
-        }
-      }
-    }
-    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
-      tc_commit(smem_u32(&sh->drain));
-      drain_phase(smem_u32(&sh->drain), 0);
-    }
-  } else if (warp == 2) {
-    // ── scales: a K block's 128 + BN (or its 128-row blocks') into a ring of their own ──
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    for (int64_t t = t0; ok && t < ntiles; t += tstep) {
-      const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
-      const float* sa = p.sA + c.sa;
-      const float* sb = ROWB ? p.sB + (int64_t)c.b_b * p.kblocks * p.N + c.n0
-                             : p.sB + ((int64_t)c.b_b * p.nblocks + c.n0 / 128) * p.kblocks;
-      const int cols = min(BN, p.N - c.n0);
-      for (int kb0 = kbeg; kb0 < kend; kb0 += 4) {
-        ok = wait_warp(smem_u32(&sh->sempty[s]), ph ^ 1, abort, &g_fp8_timeouts);
-        if (!ok) break;
-        for (int j = 0; j < min(4, kend - kb0); ++j) {
-          const uint32_t da = smem_u32(sh->sa[s][j]), db = smem_u32(sh->sb[s][j]);
-          const int64_t kb = kb0 + j;
-#pragma unroll
-          for (int i = 0; i < kF8M / 32; ++i)
-            if (i * 32 + lane < c.rows) cp_async4(da + (i * 32 + lane) * 4, sa + kb * p.M + i * 32 + lane);
-          if (ROWB) {
-#pragma unroll
-            for (int i = 0; i < BN / 32; ++i)
-              if (i * 32 + lane < cols) cp_async4(db + (i * 32 + lane) * 4, sb + kb * p.N + i * 32 + lane);
-          } else if (lane * 128 < cols) {
-            cp_async4(db + lane * 4, sb + (int64_t)lane * p.kblocks + kb);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8FewRegs));
+    if (warp == 0) {
+      // ── TMA producer (the whole warp waits, one lane issues) ──
+      int s = 0;
+      uint32_t ph = 0;
+      int64_t issued = 0;
+      bool ok = true;
+      for (int64_t t = t0; ok && t < ntiles; t += tstep) {
+        const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
+        const int boxes = (c.rows + p.a_box - 1) / p.a_box;
+        const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
+        for (int kb = kbeg; kb < kend; ++kb) {
+          ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts);
+          if (!ok) break;
+          if (elect_one()) {
+            const uint32_t fb = smem_u32(&sh->full[s]), dst = smem_u32(ring) + (uint32_t)(s * Cfg::kStageBytes);
+            mbar_expect_tx(fb, bytes);
+            tma_load_3d(dst + Cfg::kAStage, &tmB, kb * kF8K, c.n0, c.b_b, fb);
+            for (int r = 0; r < boxes; ++r)
+              tma_load_3d(dst + r * p.a_box * kF8K, &tmA, kb * kF8K, c.a_row + r * p.a_box, c.a_b, fb);
+          }
+          __syncwarp();
+          ++issued;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
           }
         }
-        cp_async_arrive(smem_u32(&sh->sfull[s]));
-        if (++s == kF8Scales) {
-          s = 0;
-          ph ^= 1;
+      }
+      if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
+        for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+    } else if (warp == 1) {
+      // ── MMA issuer (the whole warp waits, one lane issues) ──
+      int s = 0, a = 0;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true;
+      // both operands K-major: rows of 128 bytes, 8-row groups 1024 bytes apart; a K = 32
+      // slice is 32 bytes further along the swizzled row
+      const uint64_t a0 = smem_desc(smem_u32(ring), 16, 1024), b0 = smem_desc(smem_u32(ring) + Cfg::kAStage, 16, 1024);
+      for (int64_t t = t0; ok && t < ntiles; t += tstep) {
+        for (int kb = kbeg; kb < kend; ++kb) {
+          // the loads were there long before; the accumulator is what the MMAs wait for
+          ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_fp8_timeouts) &&
+               wait_warp(smem_u32(&sh->tempty[a]), aph ^ 1, abort, &g_fp8_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t d = tmem + (uint32_t)(a * BN);
+            const uint64_t ad = a0 + (uint64_t)(s * (Cfg::kStageBytes >> 4)), bd = b0 + (uint64_t)(s * (Cfg::kStageBytes >> 4));
+#pragma unroll
+            for (int kk = 0; kk < kF8K / 32; ++kk) tc_mma_f8(d, ad + kk * 2, bd + kk * 2, p.idesc, kk != 0);
+            tc_commit(smem_u32(&sh->empty[s]));
+            tc_commit(smem_u32(&sh->tfull[a]));
+          }
+          __syncwarp();
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++a == kAcc) {
+            a = 0;
+            aph ^= 1;
+          }
         }
       }
+      if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
+        tc_commit(smem_u32(&sh->drain));
+        drain_phase(smem_u32(&sh->drain), 0);
+      }
+    } else if (warp == 2) {
+      // ── scales: a K block's 128 + BN (or its 128-row blocks') into a ring of their own ──
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int64_t t = t0; ok && t < ntiles; t += tstep) {
+        const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
+        const float* sa = p.sA + c.sa;
+        const float* sb = ROWB ? p.sB + (int64_t)c.b_b * p.kblocks * p.N + c.n0
+                               : p.sB + ((int64_t)c.b_b * p.nblocks + c.n0 / 128) * p.kblocks;
+        const int cols = min(BN, p.N - c.n0);
+        for (int kb0 = kbeg; kb0 < kend; kb0 += 4) {
+          ok = wait_warp(smem_u32(&sh->sempty[s]), ph ^ 1, abort, &g_fp8_timeouts);
+          if (!ok) break;
+          for (int j = 0; j < min(4, kend - kb0); ++j) {
+            const uint32_t da = smem_u32(sh->sa[s][j]), db = smem_u32(sh->sb[s][j]);
+            const int64_t kb = kb0 + j;
+#pragma unroll
+            for (int i = 0; i < kF8M / 32; ++i)
+              if (i * 32 + lane < c.rows) cp_async4(da + (i * 32 + lane) * 4, sa + kb * p.M + i * 32 + lane);
+            if (ROWB) {
+#pragma unroll
+              for (int i = 0; i < BN / 32; ++i)
+                if (i * 32 + lane < cols) cp_async4(db + (i * 32 + lane) * 4, sb + kb * p.N + i * 32 + lane);
+            } else if (lane * 128 < cols) {
+              cp_async4(db + lane * 4, sb + (int64_t)lane * p.kblocks + kb);
+            }
+          }
+          cp_async_arrive(smem_u32(&sh->sfull[s]));
+          if (++s == kF8Scales) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  }
-  if constexpr (SPLIT) {  // the two meetings of the cluster, see the other warps
-    cluster_sync();
-    cluster_sync();
-  }
+    if constexpr (SPLIT) {  // the two meetings of the cluster, see the other warps
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8ManyRegs));
     // ── scaled sums: warp reads TMEM lanes 32 q .. +32, columns half * kCols .. ──

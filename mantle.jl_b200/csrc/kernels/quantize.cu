@@ -19,8 +19,9 @@
 // 128 rows. Rows of codes start every 16 bytes rounded up (TMA's row stride) and
 // the bytes between are zeros.
 //
-// Both kernels are bound by HBM: a value is read once, kept in registers, and
-// written once per output. See the figures at each kernel.
+// A value is read once, kept in registers, and written once per output, so that HBM is
+// the bound to reach; the figures are at each kernel (a device-to-device copy reaches
+// 5.4 TB/s at these sizes).
 
 #include <cuda_runtime.h>
 
@@ -188,7 +189,10 @@ __device__ __forceinline__ int holder_of(int value) {  // the first lane that ho
 // ── row blocks, no transpose ────────────────────────────────────────────────
 // Sixteen lanes a block of 128 (eight values each), a CTA sixteen rows of U
 // neighbouring blocks: the U loads of a thread are in flight together, and the
-// scales of sixteen rows leave as one 64-byte run.
+// scales of sixteen rows leave as one 64-byte run. 8192 x 4096 bf16: 18.5 us, 5.4 TB/s
+// (26 with the two divisions of a scale in every lane). Rows that do not start on 16
+// bytes are loaded value by value: 8192 x 4095 30.5 us; aligned words around them,
+// shifted into place, took 28.6, and in fp32 38.7 instead of 36.3.
 constexpr int kQuantThreads = 256;
 template <typename T, int U, bool E5M2>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs a, unsigned row_tiles, unsigned col_tiles) {
@@ -228,7 +232,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
 // sixteen lanes of a row, column maxima over the CTA through shared memory. The
 // transposed codes go through a 16 KiB tile whose 8-byte chunks are placed by
 // chunk ^ (column / 8): the sixteen lanes that write one instruction's columns
-// hit all 32 banks, and so do the sixteen that read a transposed row.
+// hit all 32 banks, and so do the sixteen that read a transposed row. 8192 x 4096 bf16
+// both ways: 30 us, 4.5 TB/s, bound by instruction issue (52 with the scales' divisions
+// in every lane and 64-bit tile indexes, 35 with magnitudes compared one by one; 33 at
+// three CTAs an SM); 5001 x 4100 fp32 in squares 25.5 us, 4.8 TB/s.
 template <typename T, bool E5M2>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantize_tile_kernel(QuantArgs a, int square) {
   __shared__ alignas(16) uint32_t colmax[8][128];
