@@ -3,8 +3,9 @@
 //
 // Group e holds rows offsets[e] .. offsets[e + 1] of the row matrix. The
 // offsets live on the device, so the host cannot check them: each is clamped to
-// [the previous group's start, rows], and a group that ends before it starts is
-// empty. Whatever they hold, no access leaves the buffers.
+// [0, rows], and one below an earlier one counts as that one. So whatever they hold,
+// no access leaves the buffers, no row is in two groups, and the tiles are no more than
+// the host counted.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,13 +25,25 @@ struct GroupTable {
 // Every thread of the CTA calls this; `tile_m` rows a tile.
 __device__ __forceinline__ void build_groups(GroupTable* g, const int* __restrict__ offsets, int groups, int rows,
                                              int tile_m) {
+  int falls = 0;
   for (int e = threadIdx.x; e < groups; e += blockDim.x) {
-    const int lo = min(max(offsets[e], 0), rows), hi = min(max(offsets[e + 1], lo), rows);
+    const int lo = min(max(offsets[e], 0), rows), end = min(max(offsets[e + 1], 0), rows), hi = max(lo, end);
+    falls |= end < lo;
     g->lo[e] = lo;
     g->hi[e] = hi;
     g->cum[e + 1] = (hi - lo + tile_m - 1) / tile_m;
   }
-  __syncthreads();
+  if (__syncthreads_or(falls)) {  // not in order, which one thread mends
+    if (threadIdx.x == 0) {
+      int top = 0;
+      for (int e = 0; e < groups; ++e) {
+        g->lo[e] = top = max(top, g->lo[e]);
+        g->hi[e] = max(top, g->hi[e]);
+        g->cum[e + 1] = (g->hi[e] - top + tile_m - 1) / tile_m;
+      }
+    }
+    __syncthreads();
+  }
   if (threadIdx.x < 32) {
     int carry = 0;
     for (int base = 0; base < groups; base += 32) {

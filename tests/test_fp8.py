@@ -335,6 +335,6 @@ def test_gemm_grouped_fp8_bad_offsets_stay_in_bounds(dev):
     torch.cuda.synchronize()
     got, vx = guard.double().cpu(), values(qx[0], sx[0], 1, k)
     assert (got[t:] == 3.0).all()
-    for lo, hi, e in ((0, 20, 0), (90, 100, 3)):  # rows that one group alone holds
+    for lo, hi, e in ((0, 20, 0), (0, 40, 0), (40, 90, 2), (90, 100, 3)):  # an offset below an earlier one counts as that one
         vw = values(qw[e], sw[e], 128, k)
         check_product(got[lo:hi], vx[lo:hi] @ vw.t(), vx[lo:hi].abs() @ vw.abs().t(), 2, 0)

@@ -177,7 +177,7 @@ def test_other_groups_rows_do_not_reach_a_weight_gradient_of_many_groups(dev, k,
 def test_bad_offsets_stay_in_bounds(dev, way):
     t, n, k = 100, 136, 72
     x, dy, w = normal((t, k), 1).cuda(), normal((t, n), 2).cuda(), normal((4, k, n), 3).cuda()
-    off = [-5, 40, 20, 90, 1 << 30]  # clamped: 0..40, none, 20..90, 90..100
+    off = [-5, 40, 20, 90, 1 << 30]  # clamped: 0..40, none, 40..90, 90..100
     rows = {"fwd": (t, n), "dx": (t, k), "dw": (4 * k, n)}[way]
     guard = torch.full((rows[0] + 64, rows[1]), 3.0, device="cuda")
     a, b = {"fwd": (x, w), "dx": (dy, w), "dw": (x, dy)}[way]
@@ -185,12 +185,32 @@ def test_bad_offsets_stay_in_bounds(dev, way):
     torch.cuda.synchronize()
     assert (guard[rows[0]:] == 3.0).all() and torch.isfinite(guard).all()
     x, dy, w, got = x.double().cpu(), dy.double().cpu(), w.double().cpu(), guard.double().cpu()
-    for e, lo, hi in ((0, 0, 20), (3, 90, 100)):
+    for e, lo, hi in ((0, 0, 20), (0, 0, 40), (1, 40, 40), (2, 40, 90), (3, 90, 100)):
         if way == "dw":
-            if e == 3:
-                check(got[3 * k:4 * k], x[90:100].t(), dy[90:100], 0)
+            if (lo, hi) != (0, 20):
+                check(got[e * k:(e + 1) * k], x[lo:hi].t(), dy[lo:hi], 0)
         else:
             check(got[lo:hi], *((x[lo:hi], w[e]) if way == "fwd" else (dy[lo:hi], w[e].t())), 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("t", [100, 1600])
+def test_offsets_that_fall_give_no_row_to_two_groups(dev, way, t):
+    # 0, T, 0, T, ...: the first group has every row, the others none; with 100 rows as the MMA's N operand
+    e, n, k = 32, 1032, 1000
+    x, dy, w = normal((t, k), 1).cuda(), normal((t, n), 2).cuda(), normal((e, k, n), 3).cuda()
+    out = torch.full({"fwd": (t, n), "dx": (t, k), "dw": (e, k, n)}[way], 3.0, device="cuda")
+    a, b = {"fwd": (x, w), "dx": (dy, w), "dw": (x, dy)}[way]
+    launch(way, out, a, b, [0, t] * (e // 2) + [0], t, n, k, e, 0)
+    torch.cuda.synchronize()
+    x, dy, w = x.double().cpu(), dy.double().cpu(), w[0].double().cpu()
+    if way == "dw":
+        check(out[0], x.t(), dy, 0)
+        assert float(out[1:].abs().max()) == 0.0
+    else:
+        check(out, *((x, w) if way == "fwd" else (dy, w.t())), 0)
+    assert M.kernel_timeouts() == 0
 
 
 @pytest.mark.gpu
