@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   if (warp == 0) {
     // ── TMA producer: this CTA's 128 rows of A and 128 columns of B ──
     int s = 0;
-    uint32_t ph = 0;
+    uint32_t ph = 0, tails = 0, tph = 0;  // stages that tail was used for, the parity of its last use: a bit a stage
     int64_t issued = 0;
     bool ok = true;
     for (int t = t0; ok && t < ntiles; t += tstep) {
@@ -604,6 +604,10 @@ __global__ void __launch_bounds__(kGrThreads, 1)
             }
           }
         }
+        if (FORM == kDw && c.depth - kb * kGrK < kGrK) {
+          tph = tails >> s & 1 ? tph ^ 1u << s : tph;
+          tails |= 1u << s;
+        }
         __syncwarp();
         ++issued;
         if (++s == kStages) {
@@ -612,9 +616,14 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         }
       }
     }
-    if (!ok && lane == 0 && rank == 0)  // the loads in flight land before the CTAs leave
-      for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-        drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+    if (!ok && lane == 0) {  // the loads in flight land before the CTAs leave
+      if (FORM == kDw)
+        for (int i = 0; i < kStages; ++i)
+          if (tails >> i & 1) drain_phase(smem_u32(&sh->tail[i]), tph >> i & 1);
+      if (rank == 0)
+        for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+    }
   } else if (warp == 1) {
     // ── MMA issuer (even CTA); both: a group's last K block made clean ──
     int s = 0, i = 0;
