@@ -358,7 +358,7 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
   for (int i = 10; i < 13; ++i)
     if (la.a[i].i32 != 0 && la.a[i].i32 != 1)
       return fail(MTL_ERR_ARGUMENT, "quantize_fp8: argument %d must be 0 or 1, got %d", i + 1, la.a[i].i32);
-  const bool gather = la.a[5].kind == MTL_ARG_PTR && la.a[5].ptr;
+  const bool gather = la.a[5].kind == MTL_ARG_PTR;
   if (gather && batch > 1) return fail(MTL_ERR_UNSUPPORTED, "quantize_fp8: rows_of goes with a batch of one, got %lld", (long long)batch);
   if (!gather && xrows != R)
     return fail(MTL_ERR_ARGUMENT, "quantize_fp8: without rows_of the input has as many rows as the output: %lld, got %lld", (long long)R,
@@ -373,7 +373,8 @@ mtl_status quantize_check(const LaunchArgs& la, const uint64_t* bytes) {
   const char* what[6] = {"the codes", "the scales", "the transposed codes", "the transposed scales", "the input", "rows_of"};
   const unsigned align[6] = {15, 3, 15, 3, la.a[10].i32 ? 1u : 3u, 3};
   for (int i = 0; i < 6; ++i) {
-    if (i == 4 && !la.a[i].ptr && need[i]) return fail(MTL_ERR_ARGUMENT, "quantize_fp8: the input must be a device buffer");
+    if (la.a[i].kind == MTL_ARG_PTR && !la.a[i].ptr && need[i])  // given, but without an address: not the same as left out
+      return fail(MTL_ERR_ARGUMENT, "quantize_fp8: %s must be a device buffer", what[i]);
     if (!la.a[i].ptr) continue;
     if (bytes[i] && bytes[i] < need[i])
       return fail(MTL_ERR_ARGUMENT, "quantize_fp8: %s: %llu bytes, the launch touches %llu", what[i], (unsigned long long)bytes[i],

@@ -47,6 +47,11 @@ def q_args(r, c, block=1, both=False, kind=0, fmt=0, pow2=0, rows_of=None, xrows
     ([None] + q_args(4, 256)[1:], 1, "codes and the scales"),
     ([None, None] + q_args(4, 256)[2:], 1, "codes and the scales"),
     ([M.DevicePtr((1 << 20) + 8, 1 << 20)] + q_args(4, 256)[1:], 1, "16-byte aligned"),
+    # an empty tensor, which has no address, is not an argument left out
+    ([ptr(0, 0), ptr(0, 0)] + q_args(4, 256, both=True)[2:], 1, "the codes must be a device buffer"),
+    (q_args(4, 256, both=True)[:2] + [ptr(0, 0), ptr(0, 0)] + q_args(4, 256)[4:], 1, "the transposed codes must be"),
+    (q_args(4, 256, rows_of=ptr(0, 0)), 1, "rows_of must be a device buffer"),
+    (q_args(4, 256, xrows=9, rows_of=ptr(0, 0)), 1, "rows_of must be a device buffer"),
 ])
 def test_quantize_refuses(args, nd, match):
     with pytest.raises(M.MantleError, match=match):
