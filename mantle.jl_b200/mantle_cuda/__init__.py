@@ -619,10 +619,11 @@ def _with_torch() -> None:
     _tensor = torch.Tensor
 
 
-def _operands(k: Kernel, args: Sequence) -> list:
+def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
     """(kind, rid, address, bytes) of each buffer argument of a kernel in _OPERANDS, in
-    one flat list, checked: element types, and for torch tensors contiguity and the
-    current CUDA device. A graph resource's address is its plan's and stays 0."""
+    one flat list, checked: element types, for torch tensors contiguity and the current
+    CUDA device, for a launch's Buffers that device too where torch tells it. A graph's
+    resources have their plan's addresses, so only a graph takes them."""
     kinds, flag = _OPERANDS[k.name]
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"{k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
@@ -645,9 +646,15 @@ def _operands(k: Kernel, args: Sequence) -> list:
             flat += (L.ARG_PTR, 0, x.ptr, x.nbytes & 0xFFFFFFFFFFFFFFFF)
             continue
         else:
-            x = x.resource if isinstance(x, UseHandle) else x
-            if not isinstance(x, (Buffer, TransientBuffer, VirtualBuffer)):
+            x = x.resource if graph and isinstance(x, UseHandle) else x
+            if not isinstance(x, (Buffer, TransientBuffer, VirtualBuffer) if graph else Buffer):
                 raise ArgumentError(L.ERR_ARGUMENT, f"cannot pass {x!r} where the kernel takes a buffer")
+            if not graph and _tensor is not None:
+                if device is None:
+                    device = sys.modules["torch"].cuda.current_device()
+                if x.dev.ordinal != device:
+                    raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4 + 1} is a buffer on device {x.dev.ordinal}, "
+                                        f"the current one is {device}")
             got = _KINDS.get(x.dtype)
             flat += (L.ARG_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
         if want == "o":
@@ -703,7 +710,7 @@ def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"dispatch!: {k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
     if k.name in _OPERANDS:
-        _operands(k, args)
+        _operands(k, args, graph=True)
     arr = (L.Arg * max(len(args), 1))(*[_arg(p.graph, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))

@@ -369,7 +369,8 @@ def build_experts(dev, tokens: int = 4096, experts: int = 16, top: int = 2, widt
         src = Buffer.wrap(dev, w, dtype=np.float32)
         codes = Buffer(dev, np.uint8, experts * n * rows_of_codes(k))
         scales = Buffer(dev, np.float32, experts * -(-n // 128) * -(-k // 128))
-        launch(kernels.quantize_fp8, (codes, scales, None, None, src, None, n, k, n, 128, 0, 0, 0), experts, stream=dev.stream)
+        with torch.cuda.device(device):
+            launch(kernels.quantize_fp8, (codes, scales, None, None, src, None, n, k, n, 128, 0, 0, 0), experts, stream=dev.stream)
         dev.synchronize()
         weights[name], tensors[name] = (codes, scales), w
     x = Buffer.wrap(dev, x_t, dtype=np.uint16)
