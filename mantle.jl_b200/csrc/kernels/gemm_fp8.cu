@@ -892,10 +892,13 @@ static cudaError_t fp8_launch(const CUtensorMap& ta, const CUtensorMap& tb, cons
   cudaError_t e = allow_smem(kernel, smem, device, &done);
   if (e != cudaSuccess) return e;
   // the register split draws on what the block starts with: with less it would wait for good
-  static const int regs = [&] {
+  static int known = 0;  // registers a thread, once the runtime has said
+  int regs = __atomic_load_n(&known, __ATOMIC_RELAXED);
+  if (!regs) {
     cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, kernel) == cudaSuccess ? at.numRegs : 0;
-  }();
+    if ((e = cudaFuncGetAttributes(&at, kernel)) != cudaSuccess) return e;
+    __atomic_store_n(&known, regs = at.numRegs, __ATOMIC_RELAXED);
+  }
   if (regs * kF8Threads < 128 * kF8FewRegs + 256 * kF8ManyRegs) return cudaErrorLaunchOutOfResources;
   if constexpr (SPLIT) {
     cudaLaunchConfig_t cfg = {};
