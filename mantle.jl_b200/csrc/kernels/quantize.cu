@@ -47,9 +47,6 @@ struct QuantArgs {
 };
 
 // ── values ──────────────────────────────────────────────────────────────────
-struct Row8 {
-  float v[8];
-};
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 
@@ -77,9 +74,9 @@ struct Raw8<uint16_t> {
   // the fp32 bits of column c's magnitude, and of the largest in a word
   static __device__ __forceinline__ uint32_t column(const uint32_t (&m)[4], int c) { return c & 1 ? m[c / 2] & 0xffff0000u : m[c / 2] << 16; }
   static __device__ __forceinline__ uint32_t whole(uint32_t m) { return max(m & 0xffff0000u, m << 16); }
-  __device__ __forceinline__ Row8 get() const {
-    return Row8{{bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y), bf16_lo(u.z), bf16_hi(u.z), bf16_lo(u.w),
-                 bf16_hi(u.w)}};
+  __device__ __forceinline__ float2 pair(int i) const {  // values 2 i and 2 i + 1
+    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+    return make_float2(bf16_lo(w), bf16_hi(w));
   }
 };
 template <>
@@ -99,11 +96,16 @@ struct Raw8<float> {
     }
   }
   static constexpr int kWords = 8;
-  __device__ __forceinline__ uint32_t mag(int i) const { return __float_as_uint(get().v[i]) & 0x7fffffffu; }
+  __device__ __forceinline__ uint32_t mag(int i) const {
+    const float2 p = pair(i / 2);
+    return __float_as_uint(i & 1 ? p.y : p.x) & 0x7fffffffu;
+  }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
   static __device__ __forceinline__ uint32_t column(const uint32_t (&m)[8], int c) { return m[c]; }
   static __device__ __forceinline__ uint32_t whole(uint32_t m) { return m; }
-  __device__ __forceinline__ Row8 get() const { return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}}; }
+  __device__ __forceinline__ float2 pair(int i) const {
+    return i == 0 ? make_float2(a.x, a.y) : i == 1 ? make_float2(a.z, a.w) : i == 2 ? make_float2(b.x, b.y) : make_float2(b.z, b.w);
+  }
 };
 
 // The input row behind output row r: null where it is past the end or rows_of
@@ -148,12 +150,20 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
         : "f"(a), "f"(b), "f"(c), "f"(d));
   return u;
 }
-template <bool E5M2>
-__device__ __forceinline__ uint2 codes8(const Row8& v, float r) {
-  float x[8];
+// Two products an instruction, each rounded to the nearest as one alone is.
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  float2 z;
+  asm("{ .reg .b64 a, b; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 a, a, b; mov.b64 {%0, %1}, a; }"
+      : "=f"(z.x), "=f"(z.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return z;
+}
+template <bool E5M2, typename RAW>
+__device__ __forceinline__ uint2 codes8(const RAW& v, float r) {  // of a row
+  float2 x[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(v.v[i], r);
-  return make_uint2(codes4<E5M2>(x[0], x[1], x[2], x[3]), codes4<E5M2>(x[4], x[5], x[6], x[7]));
+  for (int i = 0; i < 4; ++i) x[i] = mul2(v.pair(i), make_float2(r, r));
+  return make_uint2(codes4<E5M2>(x[0].x, x[0].y, x[1].x, x[1].y), codes4<E5M2>(x[2].x, x[2].y, x[3].x, x[3].y));
 }
 
 // The maxima of N values over 16 lanes at once: a step halves the values a lane
@@ -189,7 +199,7 @@ __device__ __forceinline__ int holder_of(int value) {  // the first lane that ho
 // ── row blocks, no transpose ────────────────────────────────────────────────
 // Sixteen lanes a block of 128 (eight values each), a CTA sixteen rows of U
 // neighbouring blocks: the U loads of a thread are in flight together, and the
-// scales of sixteen rows leave as one 64-byte run. 8192 x 4096 bf16: 18.5 us, 5.4 TB/s
+// scales of sixteen rows leave as one 64-byte run. 8192 x 4096 bf16: 18.1 us, 5.6 TB/s
 // (26 with the two divisions of a scale in every lane). Rows that do not start on 16
 // bytes are loaded value by value: 8192 x 4095 30.5 us; aligned words around them,
 // shifted into place, took 28.6, and in fp32 38.7 instead of 36.3.
@@ -222,7 +232,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
     const float inv = __shfl_sync(0xffffffffu, sc.r, holder_of<U>(u), 16);
     const int64_t c = (kb0 + u) * 128 + lane16 * 8;
     if (r < a.R && c < a.Cp)
-      *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8<E5M2>(raw[u].get(), inv);
+      *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8<E5M2>(raw[u], inv);
   }
 }
 
@@ -233,14 +243,14 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
 // transposed codes go through a 16 KiB tile whose 8-byte chunks are placed by
 // chunk ^ (column / 8): the sixteen lanes that write one instruction's columns
 // hit all 32 banks, and so do the sixteen that read a transposed row. 8192 x 4096 bf16
-// both ways: 30 us, 4.5 TB/s, bound by instruction issue (52 with the scales' divisions
+// both ways: 29.9 us, 4.6 TB/s, bound by instruction issue (52 with the scales' divisions
 // in every lane and 64-bit tile indexes, 35 with magnitudes compared one by one; 33 at
-// three CTAs an SM); 5001 x 4100 fp32 in squares 25.5 us, 4.8 TB/s.
+// three CTAs an SM); 5001 x 4100 fp32 in squares 25.3 us, 4.8 TB/s.
 template <typename T, bool E5M2>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantize_tile_kernel(QuantArgs a, int square) {
   __shared__ alignas(16) uint32_t colmax[8][128];
   __shared__ uint2 turned[128 * 16];
-  __shared__ float inv[128];
+  __shared__ alignas(8) float inv[128];
   __shared__ uint32_t tilemax[8];
   const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4, warp = threadIdx.x >> 5;
   const unsigned cb = (unsigned)a.cb, tiles = (unsigned)a.rb * cb, b = blockIdx.x / tiles, in = blockIdx.x % tiles;
@@ -288,7 +298,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
 #pragma unroll
       for (int p = 0; p < 8; ++p)
         if (r0 + p < a.R && c < a.Cp)
-          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p].get(), sc.r);
+          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p], sc.r);
     }
     if (!a.qt) return;
     if (threadIdx.x < 128) inv[threadIdx.x] = sc.r;
@@ -301,7 +311,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
       for (int p = 0; p < 8; ++p) {
         const float rinv = __shfl_sync(0xffffffffu, sc.r, holder_of<8>(p), 16);
         if (r0 + p < a.R && c < a.Cp)
-          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p].get(), rinv);
+          *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p], rinv);
       }
     }
     if (!a.qt) return;
@@ -325,13 +335,16 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
     }
   }
   __syncthreads();
-  // columns as rows: eight codes down each of the thread's eight columns
+  // columns as rows: eight codes down each of the thread's eight columns, two columns at once
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    Row8 down;
+  for (int i = 0; i < 4; ++i) {
+    const float2 r = *reinterpret_cast<const float2*>(&inv[lane16 * 8 + 2 * i]);
+    float2 x[8];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) down.v[p] = raw[p].get().v[i];
-    turned[(lane16 * 8 + i) * 16 + (sub ^ lane16)] = codes8<E5M2>(down, inv[lane16 * 8 + i]);
+    for (int p = 0; p < 8; ++p) x[p] = mul2(raw[p].pair(i), r);
+    uint2* to = &turned[(lane16 * 8 + 2 * i) * 16 + (sub ^ lane16)];
+    to[0] = make_uint2(codes4<E5M2>(x[0].x, x[1].x, x[2].x, x[3].x), codes4<E5M2>(x[4].x, x[5].x, x[6].x, x[7].x));
+    to[16] = make_uint2(codes4<E5M2>(x[0].y, x[1].y, x[2].y, x[3].y), codes4<E5M2>(x[4].y, x[5].y, x[6].y, x[7].y));
   }
   __syncthreads();
 #pragma unroll
