@@ -607,12 +607,14 @@ _OPERANDS = {
 _KINDS = {np.dtype(t): k for k, types in {"c": (np.uint8, np.int8), "f": (np.float32,), "h": (np.uint16, np.int16),
                                           "i": (np.int32, np.uint32)}.items() for t in types}
 _KIND_NAMES = {"c": "8-bit codes", "f": "Float32", "h": "bfloat16", "i": "Int32"}
-_tensor = None  # torch.Tensor, once torch is loaded
+_PTR = L.ARG_PTR
+_tensor = _current_device = None  # torch.Tensor, torch.cuda.current_device, once torch is loaded
 
 
 def _with_torch() -> None:
-    global _tensor
+    global _tensor, _current_device
     torch = sys.modules["torch"]
+    _current_device = torch.cuda.current_device
     for kind, names in {"c": ("uint8", "int8", "float8_e4m3fn", "float8_e5m2"), "f": ("float32",),
                         "h": ("bfloat16", "uint16", "int16"), "i": ("int32",)}.items():
         _KINDS.update({getattr(torch, n): kind for n in names if hasattr(torch, n)})
@@ -629,21 +631,24 @@ def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
         raise ArgumentError(L.ERR_ARGUMENT, f"{k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
     if _tensor is None and "torch" in sys.modules:
         _with_torch()
+    out = args[flag]
+    if out == 0 or out == 1:  # the library refuses another type
+        kinds = kinds.replace("o", "fh"[out])
     flat, device = [], None
     for x, want in zip(args, kinds):
         if _tensor is not None and isinstance(x, _tensor):
+            on = x.get_device()
             if device is None:
-                device = sys.modules["torch"].cuda.current_device() if x.get_device() >= 0 else 0
-            if x.get_device() != device or not x.is_contiguous():
+                device = _current_device() if on >= 0 else 0
+            if on != device or not x.is_contiguous():
                 raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4 + 1} must be a contiguous CUDA tensor on the "
                                     f"current device ({device})")
-            got = _KINDS.get(x.dtype)
-            flat += (L.ARG_PTR, 0, x.data_ptr(), x.nbytes)
+            flat += (_PTR, 0, x.data_ptr(), x.nbytes)
         elif x is None:
             flat += (L.ARG_NULL, 0, 0, 0)
             continue
         elif isinstance(x, DevicePtr):
-            flat += (L.ARG_PTR, 0, x.ptr, x.nbytes & 0xFFFFFFFFFFFFFFFF)
+            flat += (_PTR, 0, x.ptr, x.nbytes & 0xFFFFFFFFFFFFFFFF)
             continue
         else:
             x = x.resource if graph and isinstance(x, UseHandle) else x
@@ -651,16 +656,12 @@ def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
                 raise ArgumentError(L.ERR_ARGUMENT, f"cannot pass {x!r} where the kernel takes a buffer")
             if not graph and _tensor is not None:
                 if device is None:
-                    device = sys.modules["torch"].cuda.current_device()
+                    device = _current_device()
                 if x.dev.ordinal != device:
                     raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4 + 1} is a buffer on device {x.dev.ordinal}, "
                                         f"the current one is {device}")
-            got = _KINDS.get(x.dtype)
-            flat += (L.ARG_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
-        if want == "o":
-            kind = args[flag]
-            want = "fh"[kind] if kind in (0, 1) else got  # the library refuses another type
-        if got != want:
+            flat += (_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
+        if _KINDS.get(x.dtype) != want != "o":
             raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4} holds {x.dtype}, expected {_KIND_NAMES[want]}")
     return flat
 
@@ -680,13 +681,13 @@ class _Packed:
         self.entry.restype = C.c_int32
         self.entry.argtypes = [C.c_int32, C.c_char_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
         self.buffers = len(_OPERANDS[k.name][0])
+        self.scalars = [L.ARG_I32, 0, 0, 0] * (self.nargs - self.buffers)
 
     def __call__(self, args: Sequence, ndrange, stream: int) -> None:
-        flat = _operands(self.kernel, args)
-        for x in args[self.buffers:]:
-            flat += (L.ARG_I32, 0, x, 0)
+        buffers, scalars = _operands(self.kernel, args), self.scalars.copy()
+        scalars[2::4] = args[self.buffers:]
         try:
-            packed = self.pack(*flat)
+            packed = self.pack(*buffers, *scalars)
         except struct.error as e:
             raise ArgumentError(L.ERR_ARGUMENT, f"{self.kernel.name}: a scalar argument is no Int32 ({e})") from None
         if type(ndrange) is int:

@@ -120,7 +120,8 @@ def test_a_launch_takes_buffers_of_the_current_device_only(monkeypatch):
     for x in (free, M.VirtualBuffer(np.uint8, 64), M.UseHandle(free, 1, 1)):
         with pytest.raises(M.ArgumentError, match="takes a buffer"):
             M.launch(M.kernels.quantize_fp8, [x, ptr(4 * 8)] + q_args(4, 256)[2:], 1)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    M._with_torch()
+    monkeypatch.setattr(M, "_current_device", lambda: 0)
     far = made(M.Buffer, dtype=np.dtype(np.uint8), n=1024, ptr=1 << 20, nbytes=1024, dev=made(M.Device, ordinal=1, handle=None), handle=None)
     with pytest.raises(M.ArgumentError, match="argument 1 is a buffer on device 1, the current one is 0"):
         M.launch(M.kernels.quantize_fp8, [far] + q_args(4, 256)[1:], 1)
