@@ -243,9 +243,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
 // transposed codes go through a 16 KiB tile whose 8-byte chunks are placed by
 // chunk ^ (column / 8): the sixteen lanes that write one instruction's columns
 // hit all 32 banks, and so do the sixteen that read a transposed row. 8192 x 4096 bf16
-// both ways: 29.9 us, 4.6 TB/s, bound by instruction issue (52 with the scales' divisions
-// in every lane and 64-bit tile indexes, 35 with magnitudes compared one by one; 33 at
-// three CTAs an SM); 5001 x 4100 fp32 in squares 25.3 us, 4.8 TB/s.
+// both ways: 29.9 us, 4.6 TB/s (52 with the scales' divisions in every lane and 64-bit
+// tile indexes, 35 with magnitudes compared one by one; 33 at three CTAs an SM); a
+// thousand rows more take 3.03 us, 5.5 TB/s and so the copy's rate, and 5 us are the
+// launch and the first and last tiles' time. 5001 x 4100 fp32 in squares 25.3 us, 4.8 TB/s.
 template <typename T, bool E5M2>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantize_tile_kernel(QuantArgs a, int square) {
   __shared__ alignas(16) uint32_t colmax[8][128];
