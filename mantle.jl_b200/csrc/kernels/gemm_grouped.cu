@@ -104,8 +104,30 @@ struct GrWalk {
   }
 };
 
-__device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
-__device__ __forceinline__ void tmem_ld_row(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16(addr, r); }
+// W columns of a row, or zeros.
+template <int W>
+__device__ __forceinline__ void tmem_ld_row(uint32_t addr, bool zero, uint32_t (&r)[W]) {
+  constexpr int kPart = W < 32 ? W : 32;
+  uint32_t part[W / kPart][kPart];
+  if (zero) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] = 0;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < W / kPart; ++i) {
+    if constexpr (kPart == 32)
+      tmem_ld32_nowait(addr + (uint32_t)(i * kPart), part[i]);
+    else
+      tmem_ld16_nowait(addr, part[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < W / kPart; ++i) {
+    tmem_wait_ld(part[i]);
+#pragma unroll
+    for (int j = 0; j < kPart; ++j) r[i * kPart + j] = part[i][j];
+  }
+}
 
 template <int FORM, int BN, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
@@ -289,12 +311,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           const int col = c.n0 + ch * kW;
           if (col >= p.cols) break;
           uint32_t r[kW];
-          if (empty) {
-#pragma unroll
-            for (int v = 0; v < kW; ++v) r[v] = 0;
-          } else {
-            tmem_ld_row(tbase + ch * kW, r);
-          }
+          tmem_ld_row(tbase + ch * kW, empty, r);
           store_rows(sh->stage[warp - 2], lane, c.rows - q * 32, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
         }
       }
@@ -494,30 +511,36 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 // (2048 x 4096): weight gradient of 16 groups of 8192 rows 181 and 210 (fp32), 145 and 173
 // (bf16; storing by TMA from two 4 KiB buffers a warp, with fewer stages for their room,
 // 158); forward with 4 groups 116 and 123, 8 groups 126 and 131, 16 groups 148 and 144.
+template <int FORM>
 struct PairCfg {
   static constexpr uint32_t kAStage = 128 * kGrK * 2, kStageBytes = 2 * kAStage;
-  static constexpr int kStages = 6, kBN = 256;
+  static constexpr int kStages = FORM == kDw ? 5 : 6, kBN = 256;
+  static constexpr int kPiece = FORM == kDw ? 128 : 64;  // bytes of an output row a store
 };
+template <int FORM>
 struct PairShared {
-  uint4 stage[8][kStageWords];  // per epilogue warp: 64 bytes of 32 output rows
+  uint4 stage[8][32 * PairCfg<FORM>::kPiece / 16];  // per epilogue warp: output rows on their way out
   // full, tempty: the even CTA's are used
   uint64_t full[6], empty[6], tail[6], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
   GroupTable groups;
 };
-constexpr int kPairSmem = PairCfg::kStages * (int)PairCfg::kStageBytes + (int)sizeof(PairShared) + 1024;
+template <int FORM>
+constexpr int pair_smem() {
+  return PairCfg<FORM>::kStages * (int)PairCfg<FORM>::kStageBytes + (int)sizeof(PairShared<FORM>) + 1024;
+}
 
 template <int FORM, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
-  using Cfg = PairCfg;
+  using Cfg = PairCfg<FORM>;
   constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
   constexpr uint32_t kIdesc = idesc_bf16_f32(256, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gr_raw) + 1023) & ~uintptr_t(1023));
-  PairShared* sh = reinterpret_cast<PairShared*>(ring + kStages * Cfg::kStageBytes);
+  auto* sh = reinterpret_cast<PairShared<FORM>*>(ring + kStages * Cfg::kStageBytes);
   volatile int* abort = &sh->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = blockIdx.x & 1;
 
@@ -707,18 +730,13 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       if (row < c.rows) {
         OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
         const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
-        constexpr int kW = 64 / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
+        constexpr int kW = Cfg::kPiece / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
 #pragma unroll 1
         for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
           const int col = c.n0 + ch * kW;
           if (col >= p.cols) break;
           uint32_t r[kW];
-          if (empty) {
-#pragma unroll
-            for (int v = 0; v < kW; ++v) r[v] = 0;
-          } else {
-            tmem_ld_row(tbase + ch * kW, r);
-          }
+          tmem_ld_row(tbase + ch * kW, empty, r);
           store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
         }
       }
@@ -837,12 +855,12 @@ static cudaError_t gr_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, 
                                   const LaunchArgs& la, cudaStream_t s) {
   auto kernel = gemm_grouped_pair_kernel<FORM, OUT>;
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(kernel, kPairSmem, la.device, &done);
+  cudaError_t e = allow_smem(kernel, pair_smem<FORM>(), la.device, &done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, la.sm_count / 2)));
   cfg.blockDim = dim3(kGrThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = pair_smem<FORM>();
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -94,20 +94,24 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// 64 bytes of each of 32 output rows, columns `col` on of `cols`, a lane holding its
-// row's sums in v and `rows` rows valid: through shared memory (2 KiB of the warp's
-// own), so that an instruction writes whole 64-byte pieces of eight rows. A lane that
-// stores its own row touches 32 of them with 16 bytes each: a 128 x 256 tile of fp32
-// took 13000 cycles to leave that way. 16-byte words are placed by word ^ (row / 2 %
-// 4): no bank is hit twice on either side. `vec`: output rows start on 16 bytes.
-constexpr int kStageWords = 32 * 4;
+// 64 or 128 bytes of each of 32 output rows, columns `col` on of `cols`, a lane holding
+// its row's sums in v and `rows` rows valid: through shared memory (2 or 4 KiB of the
+// warp's own), so that an instruction writes whole pieces of eight or four rows. A lane
+// that stores its own row touches 32 of them with 16 bytes each: a 128 x 256 tile of fp32
+// took 13000 cycles to leave that way. 128 bytes, whole lines where rows are aligned, leave
+// faster where there is the room: a weight gradient that is all stores (537 MB in fp32) took
+// 89 us against 115 with 64, and 102 with 128 bytes of sixteen rows at a time. 16-byte
+// words are placed by word ^ row: no bank is hit twice on either side. `vec`: output rows
+// start on 16 bytes.
+constexpr int kStageWords = 32 * 4;  // of 64-byte pieces
 template <typename OUT, int COLS>
 __device__ __forceinline__ void store_rows(uint4* stage, int lane, int rows, OUT* out, int cols, int col, int vec,
                                            const float (&v)[COLS]) {
-  static_assert(COLS * sizeof(OUT) == 64, "64 bytes a row");
-  constexpr int kPer = 16 / sizeof(OUT);  // values a word
+  constexpr int kPer = 16 / sizeof(OUT), kWords = COLS / kPer;  // values a word, words a row
+  static_assert(kWords == 4 || kWords == 8, "64 or 128 bytes a row");
+  auto at = [&](int row, int w) { return row * kWords + (w ^ (kWords == 8 ? row & 7 : row >> 1 & 3)); };
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kWords; ++w) {
     uint4 u;
     if constexpr (sizeof(OUT) == 4) {
       u = make_uint4(__float_as_uint(v[4 * w]), __float_as_uint(v[4 * w + 1]), __float_as_uint(v[4 * w + 2]),
@@ -118,15 +122,15 @@ __device__ __forceinline__ void store_rows(uint4* stage, int lane, int rows, OUT
       for (int i = 0; i < 4; ++i) b[i] = __floats2bfloat162_rn(v[8 * w + 2 * i], v[8 * w + 2 * i + 1]);
       u = *reinterpret_cast<uint4*>(b);
     }
-    stage[lane * 4 + (w ^ (lane >> 1 & 3))] = u;
+    stage[at(lane, w)] = u;
   }
   __syncwarp();
   if (vec) {
-    const int w = lane & 3, c = col + w * kPer;
+    const int w = lane % kWords, c = col + w * kPer;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = i * 8 + lane / 4;
-      const uint4 u = stage[row * 4 + (w ^ (row >> 1 & 3))];
+    for (int i = 0; i < kWords; ++i) {
+      const int row = i * (32 / kWords) + lane / kWords;
+      const uint4 u = stage[at(row, w)];
       if (row < rows) {
         OUT* dst = out + (int64_t)row * cols + c;
         if (c + kPer <= cols) {
@@ -141,12 +145,14 @@ __device__ __forceinline__ void store_rows(uint4* stage, int lane, int rows, OUT
     }
   } else {
     // rows start anywhere: neighbouring lanes store neighbouring values
-    const int c = lane % COLS, w = c / kPer;
+    constexpr int kLanes = COLS < 32 ? COLS : 32;  // lanes a row
 #pragma unroll 4
-    for (int row = lane / COLS; row < 32; row += 32 / COLS) {
-      const OUT v = reinterpret_cast<const OUT*>(&stage[row * 4 + (w ^ (row >> 1 & 3))])[c % kPer];
-      if (row < rows && col + c < cols) out[(int64_t)row * cols + col + c] = v;
-    }
+    for (int row = lane / kLanes; row < 32; row += 32 / kLanes)
+#pragma unroll
+      for (int c = lane % kLanes; c < COLS; c += kLanes) {
+        const OUT x = reinterpret_cast<const OUT*>(&stage[at(row, c / kPer)])[c % kPer];
+        if (row < rows && col + c < cols) out[(int64_t)row * cols + col + c] = x;
+      }
   }
   __syncwarp();
 }
