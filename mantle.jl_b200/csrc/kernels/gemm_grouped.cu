@@ -511,36 +511,41 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 // (2048 x 4096): weight gradient of 16 groups of 8192 rows 181 and 210 (fp32), 145 and 173
 // (bf16; storing by TMA from two 4 KiB buffers a warp, with fewer stages for their room,
 // 158); forward with 4 groups 116 and 123, 8 groups 126 and 131, 16 groups 148 and 144.
-template <int FORM>
+//
+// Weight gradients of short groups are stores for the most part, and take one stage of the
+// ring for rows leaving in pieces of 128 bytes instead of 64 (store_rows). Sustained, us,
+// 128 and 64 bytes, 16 groups, 2048 x 4096: 128 rows a group 111 and 128 (fp32), 75.5 and
+// 81.4 (bf16); 256 rows 132 and 148, 100.4 and 101; 384 rows 157 and 166, 126 and 123; 512
+// rows 185 and 186, 151 and 147.
+template <int PIECE>  // bytes of an output row a store
 struct PairCfg {
   static constexpr uint32_t kAStage = 128 * kGrK * 2, kStageBytes = 2 * kAStage;
-  static constexpr int kStages = FORM == kDw ? 5 : 6, kBN = 256;
-  static constexpr int kPiece = FORM == kDw ? 128 : 64;  // bytes of an output row a store
+  static constexpr int kStages = PIECE == 128 ? 5 : 6, kBN = 256;
 };
-template <int FORM>
+template <int PIECE>
 struct PairShared {
-  uint4 stage[8][32 * PairCfg<FORM>::kPiece / 16];  // per epilogue warp: output rows on their way out
+  uint4 stage[8][32 * PIECE / 16];  // per epilogue warp: output rows on their way out
   // full, tempty: the even CTA's are used
   uint64_t full[6], empty[6], tail[6], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
   GroupTable groups;
 };
-template <int FORM>
+template <int PIECE>
 constexpr int pair_smem() {
-  return PairCfg<FORM>::kStages * (int)PairCfg<FORM>::kStageBytes + (int)sizeof(PairShared<FORM>) + 1024;
+  return PairCfg<PIECE>::kStages * (int)PairCfg<PIECE>::kStageBytes + (int)sizeof(PairShared<PIECE>) + 1024;
 }
 
-template <int FORM, typename OUT>
+template <int FORM, int PIECE, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
-  using Cfg = PairCfg<FORM>;
+  using Cfg = PairCfg<PIECE>;
   constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
   constexpr uint32_t kIdesc = idesc_bf16_f32(256, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gr_raw) + 1023) & ~uintptr_t(1023));
-  auto* sh = reinterpret_cast<PairShared<FORM>*>(ring + kStages * Cfg::kStageBytes);
+  auto* sh = reinterpret_cast<PairShared<PIECE>*>(ring + kStages * Cfg::kStageBytes);
   volatile int* abort = &sh->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rank = blockIdx.x & 1;
 
@@ -730,7 +735,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       if (row < c.rows) {
         OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
         const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
-        constexpr int kW = Cfg::kPiece / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
+        constexpr int kW = PIECE / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
 #pragma unroll 1
         for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
           const int col = c.n0 + ch * kW;
@@ -850,17 +855,17 @@ static cudaError_t gr_launch_slim(const CUtensorMap& tx, const CUtensorMap& tw, 
   return cudaGetLastError();
 }
 
-template <int FORM, typename OUT>
+template <int FORM, int PIECE, typename OUT>
 static cudaError_t gr_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
                                   const LaunchArgs& la, cudaStream_t s) {
-  auto kernel = gemm_grouped_pair_kernel<FORM, OUT>;
+  auto kernel = gemm_grouped_pair_kernel<FORM, PIECE, OUT>;
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(kernel, pair_smem<FORM>(), la.device, &done);
+  cudaError_t e = allow_smem(kernel, pair_smem<PIECE>(), la.device, &done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, la.sm_count / 2)));
   cfg.blockDim = dim3(kGrThreads);
-  cfg.dynamicSmemBytes = pair_smem<FORM>();
+  cfg.dynamicSmemBytes = pair_smem<PIECE>();
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -930,7 +935,11 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
       e = cudaErrorInvalidValue;
     }
   } else if (pair) {
-    e = out ? gr_launch_pair<FORM, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch_pair<FORM, float>(ta, tb, p, tiles, la, s);
+    if (FORM == kDw && T <= (out ? 256 : 512) * (int64_t)E)
+      e = out ? gr_launch_pair<FORM, FORM == kDw ? 128 : 64, __nv_bfloat16>(ta, tb, p, tiles, la, s)
+              : gr_launch_pair<FORM, FORM == kDw ? 128 : 64, float>(ta, tb, p, tiles, la, s);
+    else
+      e = out ? gr_launch_pair<FORM, 64, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch_pair<FORM, 64, float>(ta, tb, p, tiles, la, s);
   } else if (narrow) {
     e = out ? gr_launch<FORM, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 128, float>(ta, tb, p, tiles, la, s);
   } else {
