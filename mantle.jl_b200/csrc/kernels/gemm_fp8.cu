@@ -54,9 +54,15 @@ constexpr int kF8Threads = 384, kF8M = 128, kF8K = 128;
 constexpr int kF8FewRegs = 56, kF8ManyRegs = 224;  // registers a thread of the first / the other warpgroups
 constexpr int kF8GroupM = 16;  // row tiles per raster group of a dense product
 
+// A stage less than there would be room for, so that rows leave in pieces of 128 bytes
+// (store_rows): the warps that store are the ones that sum, and every tile waits for them.
+// 4096 x 4096, us, this way, with the pieces of 64 bytes that leave room for the fourth
+// stage, and with those and three stages: K = 512 in fp32 27.6, 30.4 and 30.4, in bf16 21.8, 24.5
+// and 23.7; K = 2048 with row scales 69.4, 76.2 and 73.2; K = 4096 79.3, 81.6 and 80.3. With two
+// stages K = 4096 takes 92.
 template <int BN>
 struct F8Cfg {
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int kStages = BN == 256 ? 3 : BN == 128 ? 5 : 7;
   static constexpr int kAcc = BN == 256 ? 2 : 4;  // accumulators of BN columns
   static constexpr uint32_t kTmemCols = kAcc * BN;
   static constexpr uint32_t kAStage = kF8M * kF8K, kStageBytes = kAStage + BN * kF8K;
@@ -65,7 +71,7 @@ constexpr int kF8Scales = 2;  // groups of four K blocks whose scales are on the
 struct F8None {};
 template <bool GROUPED, bool ROWB>
 struct F8Shared {
-  uint4 stage[8][kStageWords];  // per warp of sums: output rows on their way out
+  uint4 stage[8][2 * kStageWords];  // per warp of sums: output rows on their way out
   alignas(16) float sa[kF8Scales][4][kF8M];            // K blocks' scales of the tile's rows of A
   alignas(16) float sb[kF8Scales][4][ROWB ? 256 : 4];  // and of its rows of B, or of its 128-row blocks
   uint64_t full[8], empty[8], tfull[4], tempty[4], sfull[kF8Scales], sempty[kF8Scales], drain;
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int i = 0; i < kCols; i += 4) part[i / 4 * kF8M] = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
         break;
       }
-      constexpr int kOut = 64 / sizeof(OUT);  // columns a piece
+      constexpr int kOut = kCols * sizeof(OUT) < 128 ? kCols : 128 / sizeof(OUT);  // columns a piece
       OUT* out = static_cast<OUT*>(p.C) + (c.crow + q * 32) * p.N;
 #pragma unroll
       for (int i = 0; i < kCols; i += kOut)
