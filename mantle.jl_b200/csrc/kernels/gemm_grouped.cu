@@ -104,6 +104,31 @@ struct GrWalk {
   }
 };
 
+// Terms an accumulator runs for. The tensor core drops what an addition shifts out of fp32
+// instead of rounding it, so the error grows with the terms (1352 of them: 1.4e-6 of the
+// result). Where an fp32 output is the sum of more than 768 terms (DEEP), sums of 768 are
+// added in registers, rounded to the nearest, and the error stays at 0.8e-6. (In a bf16
+// output its rounding, 2e-3, hides it.) A weight gradient's terms are its group's rows, of
+// which the host knows the average. Kernels of their own: in one, the registers for the
+// sums slowed tiles of a single run too, a weight gradient from 115 to 138 us; so, 8192 rows
+// over 16 groups forward in fp32 take 161 us, and 157 to 161 in one accumulator.
+constexpr int kRunTerms = 768;
+template <bool DEEP>
+constexpr int kRunBlocks = DEEP ? kRunTerms / kGrK : 1 << 28;
+
+// acc += W columns of a row of tensor memory, of which those from `cols` on are not wanted.
+template <int W>
+__device__ __forceinline__ void tmem_add(uint32_t addr, int cols, float (&acc)[W]) {
+#pragma unroll
+  for (int v = 0; v < W; v += 16) {  // 32 at a time leave too few registers
+    if (v >= cols) break;  // uniform in the warp
+    uint32_t r[16];
+    tmem_ld16(addr + (uint32_t)v, r);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[v + k] += __uint_as_float(r[k]);
+  }
+}
+
 // W columns of a row, or zeros.
 template <int W>
 __device__ __forceinline__ void tmem_ld_row(uint32_t addr, bool zero, uint32_t (&r)[W]) {
@@ -129,11 +154,11 @@ __device__ __forceinline__ void tmem_ld_row(uint32_t addr, bool zero, uint32_t (
   }
 }
 
-template <int FORM, int BN, typename OUT>
+template <int FORM, int BN, typename OUT, bool DEEP>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
   using Cfg = GrCfg<BN>;
-  constexpr int kStages = Cfg::kStages;
+  constexpr int kStages = Cfg::kStages, kRun = kRunBlocks<DEEP>;
   constexpr uint32_t kIdesc = idesc_bf16_f32(kGrM, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -246,11 +271,17 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const int kblocks = (c.depth + kGrK - 1) / kGrK;
       if (kblocks == 0) continue;
-      const int a = i & 1;
-      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
-      ++i;
-      const uint32_t d = tmem + (uint32_t)(a * BN);
+      int a = 0, in = 0;
       for (int kb = 0; ok && kb < kblocks; ++kb) {
+        const bool first = in == 0, last = ++in == kRun || kb + 1 == kblocks;  // of an accumulator's run
+        if (last) in = 0;
+        if (first) {
+          a = i & 1;
+          ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
+          ++i;
+          if (!ok) break;
+        }
+        const uint32_t d = tmem + (uint32_t)(a * BN);
         ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
         if (!ok) break;
         int steps = kGrK / 16;
@@ -268,7 +299,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
-          auto mma = [&](int kk) { tc_mma(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, (kb | kk) != 0); };
+          auto mma = [&](int kk) { tc_mma(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, !first || kk != 0); };
           if (steps == kGrK / 16) {
 #pragma unroll
             for (int kk = 0; kk < kGrK / 16; ++kk) mma(kk);
@@ -276,7 +307,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
             for (int kk = 0; kk < steps; ++kk) mma(kk);
           }
           tc_commit(smem_u32(&sh->empty[s]));
-          if (kb + 1 == kblocks) tc_commit(smem_u32(&sh->tfull[a]));
+          if (last) tc_commit(smem_u32(&sh->tfull[a]));
         }
         __syncwarp();
         if (++s == kStages) {
@@ -295,6 +326,34 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     int i = 0;
     for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      if constexpr (DEEP) {
+        // every run's sums into registers, which frees the accumulators before the rows are stored
+        const int kblocks = (c.depth + kGrK - 1) / kGrK, row = q * 32, from = c.n0 + half * (BN / 2);
+        constexpr int kW = 16;  // columns a piece
+        float acc[BN / 2];
+#pragma unroll
+        for (int v = 0; v < BN / 2; ++v) acc[v] = 0.0f;
+        bool ok = true;
+        for (int left = kblocks; left > 0; left -= kRun, ++i) {
+          const int a = i & 1;
+          ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          if (row < c.rows) tmem_add(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half * (BN / 2)), p.cols - from, acc);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+        }
+        if (!ok) break;
+        if (row < c.rows) {  // uniform in the warp
+          OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+#pragma unroll
+          for (int v = 0; v < BN / 2; v += kW)
+            if (from + v < p.cols)
+              store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, from + v, p.vec, reinterpret_cast<const float(&)[kW]>(acc[v]));
+        }
+        continue;
+      }
       const bool empty = c.depth == 0;
       const int a = i & 1;
       if (!empty) {
@@ -351,7 +410,7 @@ template <int FORM, int NT, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_slim_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const GrArgs p) {
   using Cfg = SlimCfg<NT>;
-  constexpr int kStages = Cfg::kStages, BN = 256;
+  constexpr int kStages = Cfg::kStages, BN = 256, kRun = kRunBlocks<sizeof(OUT) == 4>;
   constexpr uint32_t kIdesc = idesc_bf16_f32(128, NT, FORM != kDx, false);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -436,11 +495,18 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     constexpr uint32_t kWStep = (FORM == kDx ? 32 : 2048) >> 4, kXStep = 32 >> 4, kWRun = Cfg::kWStage / 2 >> 4;
     const uint64_t w0 = smem_desc(smem_u32(ring), FORM == kDx ? 16 : kGrK * 128, 1024);
     const uint64_t x0 = smem_desc(smem_u32(ring) + Cfg::kWStage, 16, 1024);
-    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x, ++i) {
-      const int a = i & 1;
-      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
-      const uint32_t d = tmem + (uint32_t)(a * 2 * NT);
+    for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+      int a = 0, in = 0;
       for (int kb = 0; ok && kb < kblocks; ++kb) {
+        const bool first = in == 0, last = ++in == kRun || kb + 1 == kblocks;  // of an accumulator's run
+        if (last) in = 0;
+        if (first) {
+          a = i & 1;
+          ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
+          ++i;
+          if (!ok) break;
+        }
+        const uint32_t d = tmem + (uint32_t)(a * 2 * NT);
         ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
         if (!ok) break;
         tc_fence_after();
@@ -450,9 +516,9 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           for (int kk = 0; kk < kGrK / 16; ++kk)
 #pragma unroll
             for (int r = 0; r < 2; ++r)
-              tc_mma(d + (uint32_t)(r * NT), w0 + off + r * kWRun + kk * kWStep, x0 + off + kk * kXStep, kIdesc, (kb | kk) != 0);
+              tc_mma(d + (uint32_t)(r * NT), w0 + off + r * kWRun + kk * kWStep, x0 + off + kk * kXStep, kIdesc, !first || kk != 0);
           tc_commit(smem_u32(&sh->empty[s]));
-          if (kb + 1 == kblocks) tc_commit(smem_u32(&sh->tfull[a]));
+          if (last) tc_commit(smem_u32(&sh->tfull[a]));
         }
         __syncwarp();
         if (++s == kStages) {
@@ -469,29 +535,40 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     // ── epilogue: a warp has 32 columns of the output, run (warp - 2) / 4 ──
     const int q = warp & 3, run = (warp - 2) / 4;
     int i = 0;
-    for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++i) {
+    bool ok = true;
+    for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
       walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
-      const int a = i & 1, col = n0 + run * 128 + q * 32 + lane;
-      if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
-      tc_fence_after();
-      OUT* out = static_cast<OUT*>(p.out) + (int64_t)row0 * p.cols + col;
-#pragma unroll 1
-      for (int c = 0; c < NT; c += 16) {
-        if (c >= rows) break;
-        uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * 2 + run) * NT + c), r);
+      const int col = n0 + run * 128 + q * 32 + lane;
+      float acc[NT];
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (c + v < rows && col < p.cols) {
-            if constexpr (sizeof(OUT) == 4)
-              out[(int64_t)(c + v) * p.cols] = __uint_as_float(r[v]);
-            else
-              out[(int64_t)(c + v) * p.cols] = __float2bfloat16_rn(__uint_as_float(r[v]));
-          }
+      for (int c = 0; c < NT; ++c) acc[c] = 0.0f;
+      for (int kb = 0; kb < kblocks; kb += kRun, ++i) {
+        const int a = i & 1;
+        ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < NT; c += 16) {
+          if (c >= rows) break;
+          uint32_t r[16];
+          tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * 2 + run) * NT + c), r);
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[c + v] += __uint_as_float(r[v]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+      if (!ok) break;
+      OUT* out = static_cast<OUT*>(p.out) + (int64_t)row0 * p.cols + col;
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+        if (c < rows && col < p.cols) {
+          if constexpr (sizeof(OUT) == 4)
+            out[(int64_t)c * p.cols] = acc[c];
+          else
+            out[(int64_t)c * p.cols] = __float2bfloat16_rn(acc[c]);
+        }
     }
   }
   tc_fence_before();
@@ -536,11 +613,11 @@ constexpr int pair_smem() {
   return PairCfg<PIECE>::kStages * (int)PairCfg<PIECE>::kStageBytes + (int)sizeof(PairShared<PIECE>) + 1024;
 }
 
-template <int FORM, int PIECE, typename OUT>
+template <int FORM, int PIECE, typename OUT, bool DEEP>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
   using Cfg = PairCfg<PIECE>;
-  constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
+  constexpr int kStages = Cfg::kStages, BN = Cfg::kBN, kRun = kRunBlocks<DEEP>;
   constexpr uint32_t kIdesc = idesc_bf16_f32(256, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -683,11 +760,17 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         s = (s + kblocks) % kStages;
         continue;
       }
-      const int a = i & 1;
-      ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
-      ++i;
-      const uint32_t d = tmem + (uint32_t)(a * BN);
+      int a = 0, in = 0;
       for (int kb = 0; ok && kb < kblocks; ++kb) {
+        const bool first = in == 0, last = ++in == kRun || kb + 1 == kblocks;  // of an accumulator's run
+        if (last) in = 0;
+        if (first) {
+          a = i & 1;
+          ok = wait_warp(smem_u32(&sh->tempty[a]), ((i >> 1) & 1) ^ 1, abort, &g_grouped_timeouts);
+          ++i;
+          if (!ok) break;
+        }
+        const uint32_t d = tmem + (uint32_t)(a * BN);
         int steps = kGrK / 16;
         if (live && kb + 1 == kblocks) {
           steps = (live + 15) / 16;
@@ -701,12 +784,12 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));
           if (steps == kGrK / 16) {
 #pragma unroll
-            for (int kk = 0; kk < kGrK / 16; ++kk) tc_mma_pair(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, (kb | kk) != 0);
+            for (int kk = 0; kk < kGrK / 16; ++kk) tc_mma_pair(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, !first || kk != 0);
           } else {
-            for (int kk = 0; kk < steps; ++kk) tc_mma_pair(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, (kb | kk) != 0);
+            for (int kk = 0; kk < steps; ++kk) tc_mma_pair(d, a0 + off + kk * kAStep, b0 + off + kk * kBStep, kIdesc, !first || kk != 0);
           }
           tc_commit_pair(smem_u32(&sh->empty[s]));
-          if (kb + 1 == kblocks) tc_commit_pair(smem_u32(&sh->tfull[a]));
+          if (last) tc_commit_pair(smem_u32(&sh->tfull[a]));
         }
         __syncwarp();
         if (++s == kStages) {
@@ -725,6 +808,34 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     int i = 0;
     for (int t = t0; t < ntiles; t += tstep) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+      if constexpr (DEEP) {
+        // every run's sums into registers, which frees the accumulators before the rows are stored
+        const int kblocks = (c.depth + kGrK - 1) / kGrK, row = rank * 128 + q * 32, from = c.n0 + half * (BN / 2);
+        constexpr int kW = PIECE / 4;  // columns a piece
+        float acc[BN / 2];
+#pragma unroll
+        for (int v = 0; v < BN / 2; ++v) acc[v] = 0.0f;
+        bool ok = true;
+        for (int left = kblocks; left > 0; left -= kRun, ++i) {
+          const int a = i & 1;
+          ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          if (row < c.rows) tmem_add(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half * (BN / 2)), p.cols - from, acc);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->tempty[a]), 0));
+        }
+        if (!ok) break;
+        if (row < c.rows) {  // uniform in the warp
+          OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+#pragma unroll
+          for (int v = 0; v < BN / 2; v += kW)
+            if (from + v < p.cols)
+              store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, from + v, p.vec, reinterpret_cast<const float(&)[kW]>(acc[v]));
+        }
+        continue;
+      }
       const bool empty = c.depth == 0;
       const int a = i & 1, row = rank * 128 + q * 32;
       if (!empty) {
@@ -834,14 +945,14 @@ mtl_status gemm_grouped_check(const LaunchArgs& la, const uint64_t* bytes) { ret
 mtl_status gemm_grouped_dx_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kDx>(la, bytes); }
 mtl_status gemm_grouped_dw_check(const LaunchArgs& la, const uint64_t* bytes) { return gr_check<kDw>(la, bytes); }
 
-template <int FORM, int BN, typename OUT>
+template <int FORM, int BN, typename OUT, bool DEEP>
 static cudaError_t gr_launch(const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
                              const LaunchArgs& la, cudaStream_t s) {
   static unsigned long long done = 0;
-  cudaError_t e = allow_smem(gemm_grouped_kernel<FORM, BN, OUT>, gr_smem<BN>(), la.device, &done);
+  cudaError_t e = allow_smem(gemm_grouped_kernel<FORM, BN, OUT, DEEP>, gr_smem<BN>(), la.device, &done);
   if (e != cudaSuccess) return e;
   const int grid = (int)std::min<int64_t>(tiles, la.sm_count);
-  gemm_grouped_kernel<FORM, BN, OUT><<<grid, kGrThreads, gr_smem<BN>(), s>>>(ta, tb, p);
+  gemm_grouped_kernel<FORM, BN, OUT, DEEP><<<grid, kGrThreads, gr_smem<BN>(), s>>>(ta, tb, p);
   return cudaGetLastError();
 }
 
@@ -855,10 +966,10 @@ static cudaError_t gr_launch_slim(const CUtensorMap& tx, const CUtensorMap& tw, 
   return cudaGetLastError();
 }
 
-template <int FORM, int PIECE, typename OUT>
+template <int FORM, int PIECE, typename OUT, bool DEEP>
 static cudaError_t gr_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
                                   const LaunchArgs& la, cudaStream_t s) {
-  auto kernel = gemm_grouped_pair_kernel<FORM, PIECE, OUT>;
+  auto kernel = gemm_grouped_pair_kernel<FORM, PIECE, OUT, DEEP>;
   static unsigned long long done = 0;
   cudaError_t e = allow_smem(kernel, pair_smem<PIECE>(), la.device, &done);
   if (e != cudaSuccess) return e;
@@ -899,6 +1010,7 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   // Pairs where their 256-row tiles waste little (groups of 768 rows on average) and
   // there is a tile for each.
   const int64_t col_tiles = (cols + 255) / 256, pair_tiles = (FORM == kDw ? (int64_t)E * ((K + 255) / 256) : T / 256) * col_tiles;
+  const bool deep = !out && (FORM == kDw ? T > kRunTerms * (int64_t)E : p.depth > kRunTerms);
   const bool pair = pair_tiles >= la.sm_count / 2 && (FORM == kDw || T >= 768 * (int64_t)E);
   // Rows of a group in the MMA's N operand, 32 or 64 of them, while a group has up to 16
   // or 40 on average and there are tiles for most SMs. Sustained, us, against tiles of 128
@@ -934,16 +1046,22 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
     } else {
       e = cudaErrorInvalidValue;
     }
+  } else if (pair && FORM == kDw && T <= (out ? 256 : 512) * (int64_t)E) {
+    constexpr int kPiece = FORM == kDw ? 128 : 64;
+    e = out ? gr_launch_pair<FORM, kPiece, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
+            : gr_launch_pair<FORM, kPiece, float, false>(ta, tb, p, tiles, la, s);
   } else if (pair) {
-    if (FORM == kDw && T <= (out ? 256 : 512) * (int64_t)E)
-      e = out ? gr_launch_pair<FORM, FORM == kDw ? 128 : 64, __nv_bfloat16>(ta, tb, p, tiles, la, s)
-              : gr_launch_pair<FORM, FORM == kDw ? 128 : 64, float>(ta, tb, p, tiles, la, s);
-    else
-      e = out ? gr_launch_pair<FORM, 64, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch_pair<FORM, 64, float>(ta, tb, p, tiles, la, s);
+    e = out    ? gr_launch_pair<FORM, 64, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
+        : deep ? gr_launch_pair<FORM, 64, float, true>(ta, tb, p, tiles, la, s)
+               : gr_launch_pair<FORM, 64, float, false>(ta, tb, p, tiles, la, s);
   } else if (narrow) {
-    e = out ? gr_launch<FORM, 128, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 128, float>(ta, tb, p, tiles, la, s);
+    e = out    ? gr_launch<FORM, 128, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
+        : deep ? gr_launch<FORM, 128, float, true>(ta, tb, p, tiles, la, s)
+               : gr_launch<FORM, 128, float, false>(ta, tb, p, tiles, la, s);
   } else {
-    e = out ? gr_launch<FORM, 256, __nv_bfloat16>(ta, tb, p, tiles, la, s) : gr_launch<FORM, 256, float>(ta, tb, p, tiles, la, s);
+    e = out    ? gr_launch<FORM, 256, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
+        : deep ? gr_launch<FORM, 256, float, true>(ta, tb, p, tiles, la, s)
+               : gr_launch<FORM, 256, float, false>(ta, tb, p, tiles, la, s);
   }
   return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }

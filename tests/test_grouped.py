@@ -214,6 +214,37 @@ def test_offsets_that_fall_give_no_row_to_two_groups(dev, way, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("way,sizes,n,k", [
+    ("fwd", [200], 136, 8192), ("dx", [200], 8192, 136), ("dw", [8200], 136, 200),      # one CTA a tile, 128 columns
+    ("fwd", [300] * 4, 2048, 4100 // 8 * 8), ("dw", [4100] * 20, 264, 200),               # 256 columns, and pairs
+    ("fwd", [2] * 40, 1024, 8192), ("dx", [33, 0, 5] * 14, 8192, 1032),                  # rows as the MMA's N operand
+    ("fwd", [2600, 2520], 1024, 8192), ("dx", [2600, 2520], 8192, 1024), ("dw", [8192, 8200], 1792, 1800),  # CTA pairs
+])
+def test_long_contractions_in_fp32(dev, way, sizes, n, k):
+    # An MMA of 16 products is off by up to 2^-23 of the sum it adds to. With terms of one size the sum after j MMAs
+    # is of size 4 sqrt(j), so the 48 of a run of 768 terms are off by sum 4 sqrt(j) 2^-23 = 900 * 2^-23 where its
+    # own size is sqrt(768): 32.5 * 2^-23 = 3.9e-6 of it at most, if all errors point one way. Runs are added with
+    # half a unit of rounding each, 11 of them 11 * 2^-24 = 0.7e-6 at most: 4.6e-6 in all, whatever the length. (One
+    # accumulator over 8192 terms may be off by ten times the first part, and is by 8e-6.)
+    e, t = len(sizes), sum(sizes)
+    o = [sum(sizes[:i]) for i in range(e + 1)]
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    a, b = ({"fwd": (t, k), "dx": (t, n), "dw": (t, k)}[way], {"fwd": (e, k, n), "dx": (e, k, n), "dw": (t, n)}[way])
+    a, b = (torch.randn(v, generator=g, device="cuda").to(torch.bfloat16) for v in (a, b))
+    out = torch.full({"fwd": (t, n), "dx": (t, k), "dw": (e, k, n)}[way], float("nan"), device="cuda")
+    launch(way, out, a, b, o, t, n, k, e, 0)
+    for i in range(e):
+        r = slice(o[i], o[i + 1])
+        if sizes[i] == 0:
+            continue
+        x, y = (a[r].double().t(), b[r].double()) if way == "dw" else (a[r].double(), b[i].double().t() if way == "dx" else b[i].double())
+        want = x @ y
+        off = (out[i] if way == "dw" else out[r]).double() - want
+        assert float(off.norm()) <= 4.6e-6 * float(want.norm())
+    assert M.kernel_timeouts() == 0
+
+
+@pytest.mark.gpu
 def test_the_gradients_are_the_products_derivatives(dev):
     # the directional derivative of L = sum(Y * dY) by central differences: L is linear in X and in W, so a step
     # of h along a direction D changes L by h <grad, D> exactly, up to the sums' rounding (fp32, S as above) and
