@@ -539,36 +539,44 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
       walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
       const int col = n0 + run * 128 + q * 32 + lane;
-      float acc[NT];
+      OUT* out = static_cast<OUT*>(p.out) + (int64_t)row0 * p.cols + col;
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(run * NT);
+      if constexpr (sizeof(OUT) == 4) {  // the sums of every run
+        float acc[NT];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) acc[c] = 0.0f;
-      for (int kb = 0; kb < kblocks; kb += kRun, ++i) {
-        const int a = i & 1;
-        ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+        for (int c = 0; c < NT; ++c) acc[c] = 0.0f;
+        for (int kb = 0; kb < kblocks; kb += kRun, ++i) {
+          const int a = i & 1;
+          ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          tmem_add(lanes + (uint32_t)(a * 2 * NT), rows, acc);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+        }
         if (!ok) break;
-        tc_fence_after();
 #pragma unroll
+        for (int c = 0; c < NT; ++c)
+          if (c < rows && col < p.cols) out[(int64_t)c * p.cols] = acc[c];
+      } else {
+        const int a = i & 1;
+        if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
+        tc_fence_after();
+#pragma unroll 1
         for (int c = 0; c < NT; c += 16) {
           if (c >= rows) break;
           uint32_t r[16];
-          tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((a * 2 + run) * NT + c), r);
+          tmem_ld16(lanes + (uint32_t)(a * 2 * NT + c), r);
 #pragma unroll
-          for (int v = 0; v < 16; ++v) acc[c + v] += __uint_as_float(r[v]);
+          for (int v = 0; v < 16; ++v)
+            if (c + v < rows && col < p.cols) out[(int64_t)(c + v) * p.cols] = __float2bfloat16_rn(__uint_as_float(r[v]));
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+        ++i;
       }
-      if (!ok) break;
-      OUT* out = static_cast<OUT*>(p.out) + (int64_t)row0 * p.cols + col;
-#pragma unroll
-      for (int c = 0; c < NT; ++c)
-        if (c < rows && col < p.cols) {
-          if constexpr (sizeof(OUT) == 4)
-            out[(int64_t)c * p.cols] = acc[c];
-          else
-            out[(int64_t)c * p.cols] = __float2bfloat16_rn(acc[c]);
-        }
     }
   }
   tc_fence_before();
