@@ -17,8 +17,8 @@
 // registers, rounding to nearest, while the tensor core runs the next K block
 // into another accumulator. A K block of a 128 x 256 tile is 512 cycles of MMAs, but
 // the two accumulators that fit are handed back and forth in about 800 with nothing to
-// add, and the sums come to about 1050: 8192 cubed takes 545 us in a burst (2020
-// TFLOP/s) and 642 in a long run, which the power cap holds to that.
+// add, and the sums come to about 1050: 8192 cubed takes 536 us in a burst (2050
+// TFLOP/s) and 622 to 635 in a long run, which the power cap holds to that.
 //
 // One persistent CTA per SM, three warpgroups; the first gives registers up
 // (setmaxnreg) so that the sums of the other two stay in theirs:
