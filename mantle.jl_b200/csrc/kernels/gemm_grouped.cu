@@ -78,14 +78,14 @@ struct GrTile {
   int row0, depth;      // forward, dX: first row of A; dW: the group's first row and its row count
   int64_t crow;
 };
-template <int FORM, int TM, int BN>  // TM rows a tile
+template <int FORM, int TM, int BN, bool DEEP>  // TM rows a tile
 struct GrWalk {
   GroupWalk g;
   __device__ __forceinline__ GrTile find(const GrArgs& p, const GroupTable* groups, int t, int tiles_m, int tiles_n) {
     GrTile c;
     if (FORM == kDw) {
       const int per = tiles_m * tiles_n, in = t % per;
-      c.e = t / per;
+      c.e = DEEP ? groups->cum[t / per] : t / per;  // DEEP: as order_groups left them
       c.m0 = in % tiles_m * TM;
       c.n0 = in / tiles_m * BN;
       c.rows = p.out_rows - c.m0;
@@ -108,13 +108,40 @@ struct GrWalk {
 // instead of rounding it, so the error grows with the terms (1352 of them: 1.4e-6 of the
 // result). Where an fp32 output is the sum of more than 768 terms (DEEP), sums of 768 are
 // added in registers, rounded to the nearest, and the error stays at 0.8e-6. (In a bf16
-// output its rounding, 2e-3, hides it.) A weight gradient's terms are its group's rows, of
-// which the host knows the average. Kernels of their own: in one, the registers for the
-// sums slowed tiles of a single run too, a weight gradient from 115 to 138 us; so, 8192 rows
-// over 16 groups forward in fp32 take 161 us, and 157 to 161 in one accumulator.
+// output its rounding, 2e-3, hides it.) Tiles of a single run are not to pay for the
+// registers that hold those sums: with both kinds of tile in one loop a weight gradient went
+// from 115 to 138 us. Forward and for the input gradient the terms are the same in every
+// tile, so these are kernels of their own (8192 rows over 16 groups forward in fp32 take 161
+// us, and 157 to 161 in one accumulator). A weight gradient's terms are its group's rows,
+// which only the device knows: there the groups of a single run come first (order_groups) and
+// the others after them, in a loop of their own. In this order the first loop costs 1 % for
+// the registers of the second (128 rows a group 114.6 -> 115.9 us), in the other one 7 %.
 constexpr int kRunTerms = 768;
 template <bool DEEP>
 constexpr int kRunBlocks = DEEP ? kRunTerms / kGrK : 1 << 28;
+
+// A DEEP weight gradient's groups, those of a single run first: cum[i] is the i-th of them,
+// cum[kMaxGroups] how many these are. Every thread of the CTA calls this, after build_groups,
+// whose sums of tiles a weight gradient does not need.
+__device__ __forceinline__ void order_groups(GroupTable* g, int groups) {
+  if (threadIdx.x < 32) {
+    const uint32_t below = (1u << threadIdx.x) - 1;
+    auto is_short = [&](int e) { return e < groups && g->hi[e] - g->lo[e] <= kRunTerms; };
+    int shorts = 0;
+    for (int base = 0; base < groups; base += 32) shorts += __popc(__ballot_sync(0xffffffffu, is_short(base + (int)threadIdx.x)));
+    int at = 0, rest = shorts;  // where the next of either goes
+    for (int base = 0; base < groups; base += 32) {
+      const int e = base + (int)threadIdx.x;
+      const bool one = is_short(e);
+      const uint32_t s = __ballot_sync(0xffffffffu, one), l = __ballot_sync(0xffffffffu, e < groups && !one);
+      if (e < groups) g->cum[one ? at + __popc(s & below) : rest + __popc(l & below)] = e;
+      at += __popc(s);
+      rest += __popc(l);
+    }
+    if (threadIdx.x == 0) g->cum[kMaxGroups] = shorts;
+  }
+  __syncthreads();
+}
 
 // acc += W columns of a row of tensor memory, of which those from `cols` on are not wanted.
 template <int W>
@@ -188,6 +215,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   build_groups(&sh->groups, p.offsets, p.groups, p.T, kGrM);
+  if constexpr (FORM == kDw && DEEP) order_groups(&sh->groups, p.groups);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -195,7 +223,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 
   const int tiles_m = FORM == kDw ? (p.out_rows + kGrM - 1) / kGrM : 0, tiles_n = (p.cols + BN - 1) / BN;
   const int ntiles = FORM == kDw ? tiles_m * tiles_n * p.groups : sh->groups.cum[p.groups] * tiles_n;  // checked by the host
-  GrWalk<FORM, kGrM, BN> walk;
+  GrWalk<FORM, kGrM, BN, DEEP> walk;
 
   if (warp == 0) {
     // ── TMA producer (the whole warp waits, one lane issues) ──
@@ -322,62 +350,68 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     }
   } else {
     // ── epilogue: warps 2..9 read TMEM lanes 32 (warp % 4) .. +32, half of the columns each ──
-    const int q = warp & 3, half = (warp - 2) / 4;
-    int i = 0;
-    for (int t = blockIdx.x; t < ntiles; t += gridDim.x) {
-      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
-      if constexpr (DEEP) {
-        // every run's sums into registers, which frees the accumulators before the rows are stored
-        const int kblocks = (c.depth + kGrK - 1) / kGrK, row = q * 32, from = c.n0 + half * (BN / 2);
-        constexpr int kW = 16;  // columns a piece
+    const int q = warp & 3, half = (warp - 2) / 4, row = q * 32;
+    int i = 0, t = blockIdx.x;
+    bool ok = true;
+    if constexpr (FORM == kDw || !DEEP) {
+      const int end = DEEP ? sh->groups.cum[kMaxGroups] * tiles_m * tiles_n : ntiles;
+      for (; ok && t < end; t += gridDim.x) {
+        const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+        const bool empty = c.depth == 0;
+        const int a = i & 1;
+        if (!empty) {
+          ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          ++i;
+        }
+        if (row < c.rows) {  // uniform in the warp
+          OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+          const uint32_t tbase = tmem + ((uint32_t)row << 16) + (uint32_t)(a * BN);
+          constexpr int kW = 64 / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
+#pragma unroll 1
+          for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
+            const int col = c.n0 + ch * kW;
+            if (col >= p.cols) break;
+            uint32_t r[kW];
+            tmem_ld_row(tbase + ch * kW, empty, r);
+            store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
+          }
+        }
+        if (!empty) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
+        }
+      }
+    }
+    if constexpr (DEEP) {
+      // tiles of several runs: every run's sums into registers, which frees the accumulators
+      // before the rows are stored
+      for (; ok && t < ntiles; t += gridDim.x) {
+        const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+        const int kblocks = (c.depth + kGrK - 1) / kGrK, from = c.n0 + half * (BN / 2);
+        constexpr int kW = 64 / sizeof(OUT);  // columns a piece
         float acc[BN / 2];
 #pragma unroll
         for (int v = 0; v < BN / 2; ++v) acc[v] = 0.0f;
-        bool ok = true;
         for (int left = kblocks; left > 0; left -= kRun, ++i) {
           const int a = i & 1;
           ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
           if (!ok) break;
           tc_fence_after();
-          if (row < c.rows) tmem_add(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half * (BN / 2)), p.cols - from, acc);
+          if (row < c.rows) tmem_add(tmem + ((uint32_t)row << 16) + (uint32_t)(a * BN + half * (BN / 2)), p.cols - from, acc);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
         }
-        if (!ok) break;
-        if (row < c.rows) {  // uniform in the warp
+        if (ok && row < c.rows) {  // uniform in the warp
           OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
 #pragma unroll
           for (int v = 0; v < BN / 2; v += kW)
             if (from + v < p.cols)
               store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, from + v, p.vec, reinterpret_cast<const float(&)[kW]>(acc[v]));
         }
-        continue;
-      }
-      const bool empty = c.depth == 0;
-      const int a = i & 1;
-      if (!empty) {
-        if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
-        tc_fence_after();
-        ++i;
-      }
-      if (q * 32 < c.rows) {  // uniform in the warp
-        OUT* out = static_cast<OUT*>(p.out) + (c.crow + q * 32) * (int64_t)p.cols;
-        const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
-        constexpr int kW = 64 / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
-#pragma unroll 1
-        for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
-          const int col = c.n0 + ch * kW;
-          if (col >= p.cols) break;
-          uint32_t r[kW];
-          tmem_ld_row(tbase + ch * kW, empty, r);
-          store_rows(sh->stage[warp - 2], lane, c.rows - q * 32, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
-        }
-      }
-      if (!empty) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->tempty[a]));
       }
     }
   }
@@ -655,6 +689,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   build_groups(&sh->groups, p.offsets, p.groups, p.T, 256);
+  if constexpr (FORM == kDw && DEEP) order_groups(&sh->groups, p.groups);
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are there
@@ -664,7 +699,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   const int tiles_m = FORM == kDw ? (p.out_rows + 255) / 256 : 0, tiles_n = (p.cols + BN - 1) / BN;
   const int ntiles = FORM == kDw ? tiles_m * tiles_n * p.groups : sh->groups.cum[p.groups] * tiles_n;
   const int t0 = blockIdx.x / 2, tstep = gridDim.x / 2;
-  GrWalk<FORM, 256, BN> walk;
+  GrWalk<FORM, 256, BN, DEEP> walk;
 
   if (warp == 0) {
     // ── TMA producer: this CTA's 128 rows of A and 128 columns of B ──
@@ -812,18 +847,51 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     }
   } else {
     // ── epilogue: this CTA's 128 rows; a warp 32 of them, half of the columns ──
-    const int q = warp & 3, half = (warp - 2) / 4;
-    int i = 0;
-    for (int t = t0; t < ntiles; t += tstep) {
-      const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
-      if constexpr (DEEP) {
-        // every run's sums into registers, which frees the accumulators before the rows are stored
-        const int kblocks = (c.depth + kGrK - 1) / kGrK, row = rank * 128 + q * 32, from = c.n0 + half * (BN / 2);
-        constexpr int kW = PIECE / 4;  // columns a piece
+    const int q = warp & 3, half = (warp - 2) / 4, row = rank * 128 + q * 32;
+    int i = 0, t = t0;
+    bool ok = true;
+    if constexpr (FORM == kDw || !DEEP) {
+      const int end = DEEP ? sh->groups.cum[kMaxGroups] * tiles_m * tiles_n : ntiles;
+      for (; ok && t < end; t += tstep) {
+        const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+        const bool empty = c.depth == 0;
+        const int a = i & 1;
+        if (!empty) {
+          ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
+          if (!ok) break;
+          tc_fence_after();
+          ++i;
+        }
+        if (row < c.rows) {
+          OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
+          const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
+          constexpr int kW = PIECE / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
+#pragma unroll 1
+          for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
+            const int col = c.n0 + ch * kW;
+            if (col >= p.cols) break;
+            uint32_t r[kW];
+            tmem_ld_row(tbase + ch * kW, empty, r);
+            store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
+          }
+        }
+        if (!empty) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->tempty[a]), 0));
+        }
+      }
+    }
+    if constexpr (DEEP) {
+      // tiles of several runs: every run's sums into registers, which frees the accumulators
+      // before the rows are stored
+      for (; ok && t < ntiles; t += tstep) {
+        const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
+        const int kblocks = (c.depth + kGrK - 1) / kGrK, from = c.n0 + half * (BN / 2);
+        constexpr int kW = 64 / sizeof(OUT);  // columns a piece; 128 bytes spill registers
         float acc[BN / 2];
 #pragma unroll
         for (int v = 0; v < BN / 2; ++v) acc[v] = 0.0f;
-        bool ok = true;
         for (int left = kblocks; left > 0; left -= kRun, ++i) {
           const int a = i & 1;
           ok = wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts);
@@ -834,40 +902,13 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->tempty[a]), 0));
         }
-        if (!ok) break;
-        if (row < c.rows) {  // uniform in the warp
+        if (ok && row < c.rows) {  // uniform in the warp
           OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
 #pragma unroll
           for (int v = 0; v < BN / 2; v += kW)
             if (from + v < p.cols)
               store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, from + v, p.vec, reinterpret_cast<const float(&)[kW]>(acc[v]));
         }
-        continue;
-      }
-      const bool empty = c.depth == 0;
-      const int a = i & 1, row = rank * 128 + q * 32;
-      if (!empty) {
-        if (!wait_warp(smem_u32(&sh->tfull[a]), (i >> 1) & 1, abort, &g_grouped_timeouts)) break;
-        tc_fence_after();
-        ++i;
-      }
-      if (row < c.rows) {
-        OUT* out = static_cast<OUT*>(p.out) + (c.crow + row) * (int64_t)p.cols;
-        const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
-        constexpr int kW = PIECE / sizeof(OUT), kChunks = BN / 2 / kW;  // columns a chunk, chunks a half
-#pragma unroll 1
-        for (int ch = half * kChunks; ch < (half + 1) * kChunks; ++ch) {
-          const int col = c.n0 + ch * kW;
-          if (col >= p.cols) break;
-          uint32_t r[kW];
-          tmem_ld_row(tbase + ch * kW, empty, r);
-          store_rows(sh->stage[warp - 2], lane, c.rows - row, out, p.cols, col, p.vec, reinterpret_cast<const float(&)[kW]>(r));
-        }
-      }
-      if (!empty) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->tempty[a]), 0));
       }
     }
   }
@@ -1018,7 +1059,7 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   // Pairs where their 256-row tiles waste little (groups of 768 rows on average) and
   // there is a tile for each.
   const int64_t col_tiles = (cols + 255) / 256, pair_tiles = (FORM == kDw ? (int64_t)E * ((K + 255) / 256) : T / 256) * col_tiles;
-  const bool deep = !out && (FORM == kDw ? T > kRunTerms * (int64_t)E : p.depth > kRunTerms);
+  const bool deep = !out && (FORM == kDw ? T : p.depth) > kRunTerms;  // a group has T rows at most
   const bool pair = pair_tiles >= la.sm_count / 2 && (FORM == kDw || T >= 768 * (int64_t)E);
   // Rows of a group in the MMA's N operand, 32 or 64 of them, while a group has up to 16
   // or 40 on average and there are tiles for most SMs. Sustained, us, against tiles of 128
@@ -1056,8 +1097,9 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
     }
   } else if (pair && FORM == kDw && T <= (out ? 256 : 512) * (int64_t)E) {
     constexpr int kPiece = FORM == kDw ? 128 : 64;
-    e = out ? gr_launch_pair<FORM, kPiece, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
-            : gr_launch_pair<FORM, kPiece, float, false>(ta, tb, p, tiles, la, s);
+    e = out    ? gr_launch_pair<FORM, kPiece, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
+        : deep ? gr_launch_pair<FORM, kPiece, float, true>(ta, tb, p, tiles, la, s)
+               : gr_launch_pair<FORM, kPiece, float, false>(ta, tb, p, tiles, la, s);
   } else if (pair) {
     e = out    ? gr_launch_pair<FORM, 64, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
         : deep ? gr_launch_pair<FORM, 64, float, true>(ta, tb, p, tiles, la, s)

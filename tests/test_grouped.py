@@ -245,6 +245,40 @@ def test_long_contractions_in_fp32(dev, way, sizes, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sizes,n,k", [
+    ([8192] + [0] * 15, 136, 200), ([12000] + [8] * 63, 136, 136),     # one CTA a tile
+    ([8192] + [0] * 15, 1792, 1800), ([12000] + [8] * 63, 520, 264),   # pairs, groups short on average
+    ([9000] + [100] * 15, 1800, 1800),                                  # pairs, longer ones
+    # a run and a little more or less, long groups between short and empty ones
+    ([700, 768, 769, 0, 5000, 832, 64, 1, 1536, 1537, 0, 767], 264, 200),
+    ([700, 768, 769, 0, 5000, 832, 64, 1, 1536, 1537, 0, 767], 776, 1032),
+    ([900, 0, 3] * 40, 264, 136),
+])
+def test_a_weight_gradients_long_groups_among_short_ones_in_fp32(dev, sizes, n, k):
+    # The bound of the test above, 3.9e-6 for a run of 768 terms and half a unit of rounding for each run that is
+    # added, for every group by its own length, whatever the others'. Groups of up to 16 rows are left to the bound of
+    # `check`: over few elements errors do not add up as the bound's root of the terms.
+    e, t = len(sizes), sum(sizes)
+    o = [sum(sizes[:i]) for i in range(e + 1)]
+    g = torch.Generator(device="cuda").manual_seed(n + k + e)
+    x, dy = (torch.randn(v, generator=g, device="cuda").to(torch.bfloat16) for v in ((t, k), (t, n)))
+    out = torch.full((2, e, k, n), float("nan"), device="cuda")
+    for i in range(2):
+        launch("dw", out[i], x, dy, o, t, n, k, e, 0)
+    assert torch.equal(out[0], out[1])
+    for i in range(e):
+        r = slice(o[i], o[i + 1])
+        a, b = x[r].double().t(), dy[r].double()
+        want = a @ b
+        if sizes[i] <= 16:
+            assert ((out[0, i].double() - want).abs() <= (sizes[i] + 16) * 2.0 ** -23 * (a.abs() @ b.abs())).all()
+        else:
+            runs = -(-sizes[i] // 768)
+            assert float((out[0, i].double() - want).norm()) <= (3.9e-6 + runs * 2.0 ** -24) * float(want.norm()), sizes[i]
+    assert M.kernel_timeouts() == 0
+
+
+@pytest.mark.gpu
 def test_the_gradients_are_the_products_derivatives(dev):
     # the directional derivative of L = sum(Y * dY) by central differences: L is linear in X and in W, so a step
     # of h along a direction D changes L by h <grad, D> exactly, up to the sums' rounding (fp32, S as above) and
