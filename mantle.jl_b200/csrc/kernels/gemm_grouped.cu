@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         *reinterpret_cast<uint4*>(stage + (w / words) * (kGrK * 128) + live * 128 + (w % words) * 16) = make_uint4(0, 0, 0, 0);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&sh->full[st]), 0));
+      if (lane == 0) mbar_arrive_release_cluster(map_rank(smem_u32(&sh->full[st]), 0));
       return true;
     };
     for (int t = t0; ok && t < ntiles; t += tstep) {
@@ -822,6 +822,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         }
         ok = wait_warp(smem_u32(&sh->full[s]), ph, abort, &g_grouped_timeouts);
         if (!ok) break;
+        if (live && kb + 1 == kblocks) mbar_acquire_cluster(smem_u32(&sh->full[s]), ph);  // the odd CTA's zeros, see clean
         tc_fence_after();
         if (elect_one()) {
           const uint64_t off = (uint64_t)(s * (Cfg::kStageBytes >> 4));

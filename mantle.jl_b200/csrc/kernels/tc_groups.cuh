@@ -160,10 +160,14 @@ __device__ __forceinline__ void store_rows(uint4* stage, int lane, int rows, OUT
 // ── CTA pairs ────────────────────────────────────────────────────────────────
 // Two CTAs of a cluster run one tcgen05.mma (cta_group::2) on both SMs: each holds 128
 // of the 256 rows of A and half of B's columns, and its tensor memory the sums of its
-// rows. The even CTA issues; its barriers are reached from both through mapa. The
+// rows. The even CTA issues; its barriers are reached from both through mapa. Most
 // barrier operations have no .cluster scope: what they order is the async proxy's and
 // tensor memory's, and a wait that acquires at cluster scope drops the L1 cache each
-// time (a grouped forward product took 259 us with it, 131 without).
+// time (a grouped forward product took 259 us with it, 131 without). Where a CTA stores to
+// its shared memory itself, for an MMA that the even CTA issues, a release and an acquire at
+// cluster scope order the two (mbar_arrive_release_cluster, mbar_acquire_cluster), restricted
+// to shared memory: so they cost nothing that was measured, and whole ones, once a tile, 8 to
+// 18 % (256 rows a group 140 -> 157 us).
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
@@ -174,6 +178,17 @@ __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t bar, uint32_t by
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar) {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// After a wait for this phase: what the threads that arrived so wrote to shared memory
+// before is visible.
+__device__ __forceinline__ void mbar_acquire_cluster(uint32_t bar, uint32_t parity) {
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.relaxed.cluster.shared::cta.b64 p, [%0], %1; }" ::"r"(bar), "r"(parity)
+               : "memory");
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
 }
 // Loads whose barrier may be the other CTA's.
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {

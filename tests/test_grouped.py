@@ -173,6 +173,27 @@ def test_other_groups_rows_do_not_reach_a_weight_gradient_of_many_groups(dev, k,
 
 
 @pytest.mark.gpu
+def test_rows_behind_a_group_stay_out_of_its_weight_gradient_every_time(dev):
+    # Groups of every length modulo 64 on CTA pairs, each CTA clearing its own half of a group's last rows. Groups of NaN
+    # lie between them and fill shared memory before and after; one launch that took a row uncleared would show it.
+    k, n = 320, 328
+    sizes = [m for i in range(64) for m in (64 + i, 70)]
+    o = [sum(sizes[:i]) for i in range(129)]
+    t = o[-1]
+    x, dy = normal((t, k), 5).cuda(), normal((t, n), 6).cuda()
+    for i in range(1, 128, 2):
+        x[o[i]:o[i + 1]], dy[o[i]:o[i + 1]] = float("nan"), float("inf")
+    out = torch.full((2, 128, k, n), 7.0, device="cuda")
+    for i in range(200):
+        launch("dw", out[int(i > 0)], x, dy, o, t, n, k, 128, 0)
+        if i:
+            assert torch.equal(out[0, ::2], out[1, ::2]), i
+    for i in range(0, 128, 2):
+        r = slice(o[i], o[i + 1])
+        check(out[0, i], x[r].double().cpu().t(), dy[r].double().cpu(), 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("way", WAYS)
 def test_bad_offsets_stay_in_bounds(dev, way):
     t, n, k = 100, 136, 72
