@@ -322,11 +322,13 @@ mtl_status mtl_kernel_timeouts(int32_t reset, int64_t* count);
  * refused. Tests shorten it to make a wait run out in milliseconds. */
 mtl_status mtl_set_wait_limit(uint64_t ns);
 /* Test hook for the same failure path (no counterpart in the reference): in
- * the next `launches` launches of the named kernel family ("gemm_bf16" is the
- * one that has the hook) CTA 0's producer issues no load, so that CTA's MMA
- * issuer waits on a stage that never fills until the limit runs out, counts a
- * timeout and winds down with nothing in flight; every other CTA computes its
- * tiles. 0 clears. */
+ * the next `launches` launches of the named kernel family CTA 0's producer issues
+ * no load ("gemm_bf16") or the loads of one K block ("gemm_fp8", for both 8-bit
+ * products, and "gemm_grouped_bf16", for the three products by expert), so that
+ * CTA's MMA issuer waits on a stage that never fills until the limit runs out,
+ * counts a timeout and winds down; every other CTA computes its tiles. A
+ * gemm_fp8 launch of up to 16 rows waits for nothing and is not counted. 0
+ * clears. */
 mtl_status mtl_inject_stall(const char* kernel, int32_t launches);
 
 /* Scatter-add / histogram that allocates nothing (no counterpart in the

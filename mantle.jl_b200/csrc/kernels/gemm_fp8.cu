@@ -95,6 +95,7 @@ struct F8Args {
   int a_box;  // rows per TMA box of A
   int vec;    // rows of C start on 16 bytes
   int splits;  // CTAs a tile (a cluster), SPLIT kernels
+  int stall;   // the CTA whose producer stops after one K block, see take_stall
 };
 
 __device__ int g_fp8_timeouts;
@@ -232,11 +233,13 @@ __global__ void __launch_bounds__(kF8Threads, 1)
       uint32_t ph = 0;
       int64_t issued = 0;
       bool ok = true;
+      const bool stalls = (int)blockIdx.x == p.stall;
       for (int64_t t = t0; ok && t < ntiles; t += tstep) {
         const F8Tile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n, BN);
         const int boxes = (c.rows + p.a_box - 1) / p.a_box;
         const uint32_t bytes = (uint32_t)(boxes * p.a_box * kF8K + BN * kF8K);
-        for (int kb = kbeg; kb < kend; ++kb) {
+        const int last = stalls ? min(kend, kbeg + 1) : kend;
+        for (int kb = kbeg; kb < last; ++kb) {
           ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts);
           if (!ok) break;
           if (elect_one()) {
@@ -253,6 +256,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             ph ^= 1;
           }
         }
+        if (stalls) ok = ok && issued == 0;
       }
       if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
         for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
@@ -291,10 +295,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           }
         }
       }
-      if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
-        tc_commit(smem_u32(&sh->drain));
-        drain_phase(smem_u32(&sh->drain), 0);
-      }
+      if (!ok) drain_mmas<false>(smem_u32(&sh->drain));
     } else if (warp == 2) {
       // ── scales: a K block's 128 + BN (or its 128-row blocks') into a ring of their own ──
       int s = 0;
@@ -426,14 +427,20 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
         next_scales(kb);
       }
-      if (!ok) break;
       if constexpr (SPLIT) {  // the ring is free: every load landed and every MMA is done
         // four columns of a row a word, the rows of a word's columns next to one another
         float4* part = reinterpret_cast<float4*>(ring) + (half * kCols / 4) * kF8M + row;
+        if (ok) {
 #pragma unroll
-        for (int i = 0; i < kCols; i += 4) part[i / 4 * kF8M] = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          for (int i = 0; i < kCols; i += 4) part[i / 4 * kF8M] = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        } else {  // a CTA that gave up: the tile is NaN, not part of a sum
+          const float lost = __int_as_float(0x7fc00000);
+#pragma unroll 1
+          for (int i = 0; i < kCols; i += 4) part[i / 4 * kF8M] = make_float4(lost, lost, lost, lost);
+        }
         break;
       }
+      if (!ok) break;
       constexpr int kOut = kCols * sizeof(OUT) < 128 ? kCols : 128 / sizeof(OUT);  // columns a piece
       OUT* out = static_cast<OUT*>(p.C) + (c.crow + q * 32) * p.N;
 #pragma unroll
@@ -556,9 +563,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     uint32_t ph = 0;
     int64_t issued = 0;
     bool ok = true;
+    const bool stalls = (int)blockIdx.x == p.stall;
     for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
       walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
-      for (int kb = 0; kb < p.kblocks; ++kb) {
+      const int last = stalls ? min(p.kblocks, 1) : p.kblocks;
+      for (int kb = 0; kb < last; ++kb) {
         ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_fp8_timeouts);
         if (!ok) break;
         if (elect_one()) {
@@ -575,6 +584,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
           ph ^= 1;
         }
       }
+      if (stalls) ok = ok && issued == 0;
     }
     if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
       for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
@@ -614,10 +624,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
       }
     }
-    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
-      tc_commit(smem_u32(&sh->drain));
-      drain_phase(smem_u32(&sh->drain), 0);
-    }
+    if (!ok) drain_mmas<false>(smem_u32(&sh->drain));
   } else if (warp == 2) {
     // ── scales, four K blocks at a time ──
     int s = 0;
@@ -875,6 +882,8 @@ static mtl_status make_code_map(CUtensorMap* map, const void* base, int64_t K, i
   return MTL_OK;
 }
 
+static std::atomic<int> g_fp8_stalls{0};
+void fp8_inject_stall(int launches) { g_fp8_stalls.store(launches > 0 ? launches : 0); }
 cudaError_t fp8_set_wait_limit(unsigned long long ns) { return set_wait_limit_this_file(ns); }
 int fp8_timeouts(bool reset) {
   int v = 0;
@@ -1078,6 +1087,7 @@ static mtl_status fp8_run(const char* who, const LaunchArgs& la, int M, int N, i
       return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     }
   }
+  p.stall = take_stall(g_fp8_stalls);  // of the kernels that wait
   if constexpr (GROUPED) {
     // Rows of a group in the MMA's N operand, 32 of them, while a group has up to 16 on
     // average and there are tiles for most SMs. Sustained, us, against tiles of 128 rows:

@@ -69,6 +69,7 @@ struct GrArgs {
   int a_box;  // rows per TMA box of A (forward, dX)
   int vec;    // rows of the output start on 16 bytes
   int chunked_a, chunked_b;  // MN-major operands loaded one box a K block
+  int stall;  // the CTA whose producer stops after one K block, see take_stall
 };
 
 __device__ int g_grouped_timeouts;
@@ -232,6 +233,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       int s = 0;
       uint32_t ph = 0;
       int64_t issued = 0;
+      const bool stalls = (int)blockIdx.x == p.stall;
       for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
         const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
         // a chunked operand comes in one box, zeros past its edges; other boxes that would
@@ -242,7 +244,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         const uint32_t bytes = (uint32_t)(a_boxes * (FORM == kDw ? kGrK * 128 : p.a_box * 128)) +
                                (FORM == kDx ? Cfg::kBStage : (uint32_t)(b_boxes * kGrK * 128));
         const int kblocks = (c.depth + kGrK - 1) / kGrK;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        const int last = stalls ? min(kblocks, 1) : kblocks;
+        for (int kb = 0; kb < last; ++kb) {
           ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts);
           if (!ok) break;
           if (elect_one()) {
@@ -280,6 +283,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
             ph ^= 1;
           }
         }
+        if (stalls) ok = ok && issued == 0;
       }
       if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
         for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
@@ -344,10 +348,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         }
       }
     }
-    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
-      tc_commit(smem_u32(&sh->drain));
-      drain_phase(smem_u32(&sh->drain), 0);
-    }
+    if (!ok) drain_mmas<false>(smem_u32(&sh->drain));
   } else {
     // ── epilogue: warps 2..9 read TMEM lanes 32 (warp % 4) .. +32, half of the columns each ──
     const int q = warp & 3, half = (warp - 2) / 4, row = q * 32;
@@ -490,11 +491,13 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     uint32_t ph = 0;
     int64_t issued = 0;
     bool ok = true;
+    const bool stalls = (int)blockIdx.x == p.stall;
     for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
       walk.find(&sh->groups, t, tiles_n, NT, BN, &row0, &rows, &n0);
       const int w_boxes = FORM == kDx ? 1 : p.chunked_b ? 4 : min(4, (p.cols - n0 + 63) / 64);
       const uint32_t bytes = Cfg::kXStage + (FORM == kDx ? Cfg::kWStage : (uint32_t)(w_boxes * kGrK * 128));
-      for (int kb = 0; kb < kblocks; ++kb) {
+      const int last = stalls ? min(kblocks, 1) : kblocks;
+      for (int kb = 0; kb < last; ++kb) {
         ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts);
         if (!ok) break;
         if (elect_one()) {
@@ -517,6 +520,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           ph ^= 1;
         }
       }
+      if (stalls) ok = ok && issued == 0;
     }
     if (!ok && lane == 0)  // the loads in flight land before the CTA leaves
       for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
@@ -561,10 +565,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         }
       }
     }
-    if (!ok && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
-      tc_commit(smem_u32(&sh->drain));
-      drain_phase(smem_u32(&sh->drain), 0);
-    }
+    if (!ok) drain_mmas<false>(smem_u32(&sh->drain));
   } else {
     // ── epilogue: a warp has 32 columns of the output, run (warp - 2) / 4 ──
     const int q = warp & 3, run = (warp - 2) / 4;
@@ -707,6 +708,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     uint32_t ph = 0, tails = 0, tph = 0;  // stages that tail was used for, the parity of its last use: a bit a stage
     int64_t issued = 0;
     bool ok = true;
+    const bool stalls = (int)blockIdx.x == p.stall;
     for (int t = t0; ok && t < ntiles; t += tstep) {
       const GrTile c = walk.find(p, &sh->groups, t, tiles_m, tiles_n);
       const int m0 = c.m0 + rank * 128, n0 = c.n0 + rank * 128;
@@ -718,7 +720,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       const uint32_t a_bytes = FORM == kDw ? (uint32_t)((a_one ? 2 : a_boxes) * kGrK * 128) : (uint32_t)(a_boxes * p.a_box * 128);
       const uint32_t bytes = a_bytes + (FORM == kDx ? (uint32_t)b_boxes * Cfg::kAStage : (uint32_t)((b_one ? 2 : b_boxes) * kGrK * 128));
       const int kblocks = (c.depth + kGrK - 1) / kGrK;
-      for (int kb = 0; kb < kblocks; ++kb) {
+      const int last = stalls ? min(kblocks, 1) : kblocks;
+      for (int kb = 0; kb < last; ++kb) {
         ok = wait_warp(smem_u32(&sh->empty[s]), ph ^ 1, abort, &g_grouped_timeouts);
         if (!ok) break;
         if (elect_one()) {
@@ -763,14 +766,19 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           ph ^= 1;
         }
       }
+      if (stalls) ok = ok && issued == 0;
     }
     if (!ok && lane == 0) {  // the loads in flight land before the CTAs leave
       if (FORM == kDw)
         for (int i = 0; i < kStages; ++i)
           if (tails >> i & 1) drain_phase(smem_u32(&sh->tail[i]), tph >> i & 1);
-      if (rank == 0)
+      if (rank == 0) {
         for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
           drain_phase(smem_u32(&sh->full[i % kStages]), (uint32_t)(i / kStages) & 1);
+      } else {  // its loads count on the even CTA's barriers, which it cannot wait on: many times what a load takes
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 1000000) __nanosleep(10000);
+      }
     }
   } else if (warp == 1) {
     // ── MMA issuer (even CTA); both: a group's last K block made clean ──
@@ -842,10 +850,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         }
       }
     }
-    if (!ok && rank == 0 && lane == 0) {  // the MMAs in flight finish before the tensor memory is freed
-      tc_commit_pair(smem_u32(&sh->drain));
-      drain_phase(smem_u32(&sh->drain), 0);
-    }
+    if (!ok && rank == 0) drain_mmas<true>(smem_u32(&sh->drain));
   } else {
     // ── epilogue: this CTA's 128 rows; a warp 32 of them, half of the columns ──
     const int q = warp & 3, half = (warp - 2) / 4, row = rank * 128 + q * 32;
@@ -922,6 +927,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
+static std::atomic<int> g_grouped_stalls{0};
+void grouped_inject_stall(int launches) { g_grouped_stalls.store(launches > 0 ? launches : 0); }
 cudaError_t grouped_set_wait_limit(unsigned long long ns) { return set_wait_limit_this_file(ns); }
 int grouped_timeouts(bool reset) {
   int v = 0;
@@ -1056,6 +1063,7 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   p.depth = FORM == kFwd ? K : N;
   p.out_rows = K;
   p.groups = E;
+  p.stall = take_stall(g_grouped_stalls);
   p.vec = la.a[0].ptr % 16 == 0;  // N and K are multiples of 8
   // Pairs where their 256-row tiles waste little (groups of 768 rows on average) and
   // there is a tile for each.

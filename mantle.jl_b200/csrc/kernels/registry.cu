@@ -80,6 +80,8 @@ cudaError_t conv_set_wait_limit(unsigned long long ns);
 cudaError_t fp8_set_wait_limit(unsigned long long ns);
 cudaError_t grouped_set_wait_limit(unsigned long long ns);
 void gemm_inject_stall(int launches);
+void fp8_inject_stall(int launches);
+void grouped_inject_stall(int launches);
 
 // ── checks ──────────────────────────────────────────────────────────────────
 static int64_t nd_total(const LaunchArgs& la) {
@@ -435,10 +437,16 @@ mtl_status mtl_set_wait_limit(uint64_t ns) {
 
 mtl_status mtl_inject_stall(const char* kernel, int32_t launches) {
   if (!kernel) return mtl::fail(MTL_ERR_ARGUMENT, "mtl_inject_stall: NULL kernel name");
-  if (std::strcmp(kernel, "gemm_bf16") != 0)
-    return mtl::fail(MTL_ERR_UNSUPPORTED, "mtl_inject_stall: only gemm_bf16 has a stall hook, not %s", kernel);
-  mtl::gemm_inject_stall(launches);
-  return MTL_OK;
+  const struct {
+    const char* name;
+    void (*hook)(int);
+  } hooks[] = {{"gemm_bf16", mtl::gemm_inject_stall}, {"gemm_fp8", mtl::fp8_inject_stall}, {"gemm_grouped_bf16", mtl::grouped_inject_stall}};
+  for (const auto& h : hooks)
+    if (std::strcmp(kernel, h.name) == 0) {
+      h.hook(launches);
+      return MTL_OK;
+    }
+  return mtl::fail(MTL_ERR_UNSUPPORTED, "mtl_inject_stall: gemm_bf16, gemm_fp8 and gemm_grouped_bf16 have a stall hook, not %s", kernel);
 }
 
 }  // extern "C"

@@ -10,6 +10,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "tc_common.cuh"
 
 namespace mtl {
@@ -217,11 +219,34 @@ __device__ __forceinline__ void tc_mma_pair(uint32_t d, uint64_t a, uint64_t b, 
       : "memory");
 }
 
+// The MMAs in flight finish before a CTA that gives up frees its tensor memory: a whole
+// converged warp calls this, for a commit covers the MMAs of the thread that makes it and
+// they were issued by the lane that elect_one chooses.
+template <bool PAIR>
+__device__ __forceinline__ void drain_mmas(uint32_t bar) {
+  if (elect_one()) {
+    if (PAIR)
+      tc_commit_pair(bar);
+    else
+      tc_commit(bar);
+    drain_phase(bar, 0);
+  }
+  __syncwarp();
+}
+
 // Every thread of every CTA of the cluster; what each wrote to its shared memory before
 // is there for the others after.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The launches left whose CTA 0 loads one K block and stops (mtl_inject_stall), so that its
+// waits run out; the CTA to stop in this one, or -1.
+static inline int take_stall(std::atomic<int>& launches) {
+  for (int left = launches.load(std::memory_order_relaxed); left > 0;)
+    if (launches.compare_exchange_weak(left, left - 1)) return 0;
+  return -1;
 }
 
 // A kernel's dynamic shared memory above 48 KiB, allowed once per device.

@@ -1037,9 +1037,10 @@ def set_wait_limit(ns: int = 0) -> None:
 
 
 def inject_stall(kernel: str, launches: int = 1) -> None:
-    """In the next `launches` launches of `kernel` ("gemm_bf16"), CTA 0's
-    producer loads nothing, so that CTA's waits run out (a test of the
-    bounded-wait path); 0 clears."""
+    """In the next `launches` launches of `kernel` ("gemm_bf16"; "gemm_fp8" for
+    the 8-bit products, "gemm_grouped_bf16" for the products by expert), CTA 0's
+    producer stops, so that CTA's waits run out (a test of the bounded-wait
+    path); 0 clears."""
     check(lib().mtl_inject_stall(kernel.encode(), launches))
 
 

@@ -293,3 +293,66 @@ def test_buffers_past_two_to_the_31(dev):
     vx, vw = values(qx[0, t - 200:].view(CODE[0]), sx[0][:, t - 200:], 1, c), values(qw[1].view(CODE[0]), sw[1], 128, c).t()
     assert ((y[t - 200:t - 7].double().cpu() - (vx @ vw)[:193]).abs() <= bound(vx, vw, False)[:193]).all()
     assert (y[t - 7:] == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,ran_out,m,groups,n,k,out", [
+    ("fp8", 1, 512, 0, 1024, 384, 0),              # tiles of 128 rows
+    ("fp8", 1, 512, 0, 1024, 384, 1),
+    ("fp8", 1, 200, 0, 1024, 4096, 0),             # the K blocks split over a cluster
+    ("fp8 grouped", 1, 1100, 3, 1500, 640, 0),
+    ("fp8 grouped", 1, 120, 60, 515, 1300, 1),     # rows as the MMA's N operand
+    ("fwd", 1, 1100, 3, 2048, 320, 1), ("fwd", 1, 1100, 3, 1096, 1600, 0), ("dx", 1, 1100, 3, 320, 1096, 0), ("dw", 1, 5000, 3, 264, 520, 0),
+    ("fwd", 1, 2000, 4, 2560, 320, 1),
+    ("fwd", 1, 80, 40, 640, 512, 0), ("dx", 1, 1100, 40, 512, 640, 1),  # rows as the MMA's N operand
+    ("fwd", 2, 5120, 2, 776, 520, 1), ("dx", 2, 5120, 2, 1600, 776, 0), ("dw", 2, 4000, 8, 776, 520, 0), ("dw", 2, 9001, 3, 1288, 1032, 1),  # CTA pairs
+])
+def test_a_wait_that_runs_out_ends_the_launch(dev, form, ran_out, m, groups, n, k, out):
+    # The first CTA loads one K block and stops, with the limit of a wait at 20 ms. The launch returns, the CTA (a pair's
+    # two) is counted, its tiles (two at most in each case) are not written, or NaN, and every other one has the bits of a
+    # launch without the stop; so has the next launch everywhere.
+    import time
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    dt = torch.bfloat16 if out else torch.float32
+    if form == "fp8":
+        a, b, c = quantized(rand(1, m, k), 1), quantized(rand(1, n, k), 128), torch.empty((1, m, n), dtype=dt, device="cuda")
+        go = lambda: M.launch(M.kernels.gemm_fp8, (c, *a, *b, m, n, k, 128, 0, 0, out), 1, stream=stream())  # noqa: E731
+    else:
+        off = torch.linspace(0, m, groups + 1).int().cuda()
+        if form == "fp8 grouped":
+            a, b, c = quantized(rand(1, m, k), 1), quantized(rand(groups, n, k), 128), torch.empty((1, m, n), dtype=dt, device="cuda")
+            go = lambda: M.launch(M.kernels.gemm_grouped_fp8, (c, *a, *b, off, m, n, k, 0, 0, out), groups, stream=stream())  # noqa: E731
+        else:
+            x, dy, w = (v.to(torch.bfloat16) for v in (rand(m, k), rand(m, n), rand(groups, k, n)))
+            kernel, a, b, shape = {"fwd": (M.kernels.gemm_grouped_bf16, x, w, (1, m, n)), "dx": (M.kernels.gemm_grouped_dx_bf16, dy, w, (1, m, k)),
+                                   "dw": (M.kernels.gemm_grouped_dw_bf16, x, dy, (groups, k, n))}[form]
+            c = torch.empty(shape, dtype=dt, device="cuda")
+            go = lambda: M.launch(kernel, (c, a, b, off, m, n, k, out), groups, stream=stream())  # noqa: E731
+    go()
+    torch.cuda.synchronize()
+    want = c.clone()
+    assert torch.isfinite(want).all()
+    c.fill_(float("nan"))
+    torch.cuda.synchronize()
+    M.kernel_timeouts(reset=True)
+    hook = "gemm_fp8" if form.startswith("fp8") else "gemm_grouped_bf16"
+    try:
+        M.set_wait_limit(20_000_000)
+        M.inject_stall(hook, 1)
+        t0 = time.perf_counter()
+        go()
+        torch.cuda.synchronize()
+        took = time.perf_counter() - t0
+    finally:
+        M.inject_stall(hook, 0)
+        M.set_wait_limit(0)
+    assert M.kernel_timeouts(reset=True) == ran_out
+    assert took < 1.0
+    lost = torch.isnan(c)
+    assert bool(lost[0, 0, 0]) and int(lost.sum()) <= 2 * 256 * 256 and int(lost.sum()) < lost.numel()
+    assert torch.equal(c[~lost], want[~lost])
+    c.fill_(float("nan"))
+    go()
+    torch.cuda.synchronize()
+    assert torch.equal(c, want) and M.kernel_timeouts() == 0
