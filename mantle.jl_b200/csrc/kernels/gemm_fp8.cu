@@ -985,6 +985,7 @@ static mtl_status fp8_check_common(const char* who, const LaunchArgs& la, const 
                                    int64_t N, int64_t K, int64_t rows, int bblock, int fa, int fb, int out) {
   if (la.ndim != 1) return fail(MTL_ERR_ARGUMENT, "%s: ndrange must be one-dimensional", who);
   if (M < 0 || N < 0 || K < 0) return fail(MTL_ERR_ARGUMENT, "%s: negative dimension", who);
+  if (std::max({M, N, K}) > kMaxSize) return fail(MTL_ERR_UNSUPPORTED, "%s: a dimension above 2^31 - 256", who);
   if (bblock != 1 && bblock != 128)
     return fail(MTL_ERR_ARGUMENT, "%s: B's scales cover 1 or 128 rows each, got %d", who, bblock);
   if ((fa | fb | out) & ~1)

@@ -972,6 +972,7 @@ static mtl_status gr_check(const LaunchArgs& la, const uint64_t* bytes) {
   const int64_t E = la.nd[0], T = la.a[4].i32, N = la.a[5].i32, K = la.a[6].i32;
   const int out = la.a[7].i32;
   if (T < 0 || N < 0 || K < 0) return fail(MTL_ERR_ARGUMENT, "%s: negative dimension", who);
+  if (std::max({T, N, K}) > kMaxSize) return fail(MTL_ERR_UNSUPPORTED, "%s: a dimension above 2^31 - 256", who);
   if (N % 8 || K % 8)
     return fail(MTL_ERR_UNSUPPORTED, "%s: N and K must be multiples of 8 (16-byte rows), got N=%lld K=%lld", who, (long long)N,
                 (long long)K);

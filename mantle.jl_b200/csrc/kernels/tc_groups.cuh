@@ -17,6 +17,9 @@
 namespace mtl {
 
 constexpr int kMaxGroups = 1024;
+// The largest size of a product: the kernels round sizes and coordinates up to tiles of 256
+// in 32 bits.
+constexpr int kMaxSize = 0x7fffffff - 255;
 
 struct GroupTable {
   int lo[kMaxGroups];       // first row

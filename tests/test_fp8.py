@@ -103,6 +103,19 @@ def test_gemm_grouped_fp8_refuses(args, groups, match):
         M.launch(M.kernels.gemm_grouped_fp8, args, groups)
 
 
+@pytest.mark.parametrize("m,n,k", [(2**31 - 1, 1, 1), (1, 2**31 - 1, 1), (1, 1, 2**31 - 1), (1, 1, 2**31 - 255)])
+def test_sizes_that_tiles_would_round_past_32_bits_are_refused(m, n, k):
+    # buffers of unknown extent (0 bytes), so that the sizes alone decide
+    any_, off = ptr(0), ptr(0)
+    with pytest.raises(M.MantleError, match="above 2\\^31 - 256"):
+        M.launch(M.kernels.gemm_fp8, [any_] * 5 + [m, n, k, 128, 0, 0, 0], 1)
+    with pytest.raises(M.MantleError, match="above 2\\^31 - 256"):
+        M.launch(M.kernels.gemm_grouped_fp8, [any_] * 5 + [off, m, n, k, 0, 0, 0], 1)
+    for kernel in (M.kernels.gemm_grouped_bf16, M.kernels.gemm_grouped_dx_bf16, M.kernels.gemm_grouped_dw_bf16):
+        with pytest.raises(M.MantleError, match="above 2\\^31 - 256"):
+            M.launch(kernel, [any_] * 3 + [off, m, n, k, 0], 1)
+
+
 def test_tensors_are_checked_before_the_call():
     with pytest.raises(M.ArgumentError, match="contiguous CUDA tensor"):
         M.launch(M.kernels.gemm_fp8, [torch.zeros(20)] + g_args(1, 4, 5, 64)[1:], 1)
