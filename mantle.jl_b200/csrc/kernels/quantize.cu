@@ -166,6 +166,14 @@ __device__ __forceinline__ uint2 codes8(const RAW& v, float r) {  // of a row
   return make_uint2(codes4<E5M2>(x[0].x, x[0].y, x[1].x, x[1].y), codes4<E5M2>(x[2].x, x[2].y, x[3].x, x[3].y));
 }
 
+// What lies between rows of codes is zeros times an inverse, so zeros but where the inverse
+// is NaN. There the thread that wrote the eight codes at `at` of a row clears those that are
+// not below `end`, the row's length; with a test in every write 8192 x 4096 rows took 18.2 us
+// instead of 17.2.
+__device__ __forceinline__ void clear_padding(uint8_t* codes, int64_t at, int64_t end) {
+  for (int64_t i = at > end ? at : end; i < at + 8; ++i) codes[i - at] = 0;
+}
+
 // The maxima of N values over 16 lanes at once: a step halves the values a lane
 // keeps, so N values take N + log2(16 / N) shuffles where N separate reductions take
 // 4 N, and each lane ends with one value's maximum: value held_by(lane). The two
@@ -205,7 +213,7 @@ __device__ __forceinline__ int holder_of(int value) {  // the first lane that ho
 // shifted into place, took 28.6, and in fp32 38.7 instead of 36.3.
 constexpr int kQuantThreads = 256;
 template <typename T, int U, bool E5M2>
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs a, unsigned row_tiles, unsigned col_tiles) {
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 6 : 4) quantize_rows_kernel(QuantArgs a, unsigned row_tiles, unsigned col_tiles) {
   const int lane16 = threadIdx.x & 15, sub = threadIdx.x >> 4;
   const unsigned b = blockIdx.x / (row_tiles * col_tiles), in = blockIdx.x % (row_tiles * col_tiles);
   const int64_t batch = b, r = in / col_tiles * 16 + sub, kb0 = in % col_tiles * U;
@@ -234,6 +242,11 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(QuantArgs 
     if (r < a.R && c < a.Cp)
       *reinterpret_cast<uint2*>(a.q + (batch * a.R + r) * a.Cp + c) = codes8<E5M2>(raw[u], inv);
   }
+  if (__any_sync(0xffffffffu, isnan(sc.r)))
+    for (int u = 0; u < U; ++u) {
+      const int64_t c = (kb0 + u) * 128 + lane16 * 8;
+      if (r < a.R && c < a.Cp) clear_padding(a.q + (batch * a.R + r) * a.Cp + c, c, a.C);
+    }
 }
 
 // ── 128 x 128 tiles: square blocks, transposed outputs ──────────────────────
@@ -279,6 +292,12 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
     }
     rm[p] = Raw::whole(row);
   }
+  bool bad = false;  // an inverse is NaN: there is a NaN in the tile, so one of a row and one of a column are
+  auto clear_rows = [&]() {
+#pragma unroll 1
+    for (int p = 0; p < 8; ++p)
+      if (r0 + p < a.R && c < a.Cp) clear_padding(a.q + (batch * a.R + r0 + p) * a.Cp + c, c, a.C);
+  };
   if (square) {
     uint32_t m = 0;
 #pragma unroll
@@ -301,7 +320,11 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
         if (r0 + p < a.R && c < a.Cp)
           *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p], sc.r);
     }
-    if (!a.qt) return;
+    bad = isnan(sc.r);
+    if (!a.qt) {  // row blocks alone are the other kernel's
+      if (bad) clear_rows();
+      return;
+    }
     if (threadIdx.x < 128) inv[threadIdx.x] = sc.r;
   } else {
     if (a.q) {
@@ -315,7 +338,6 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
           *reinterpret_cast<uint2*>(a.q + (batch * a.R + r0 + p) * a.Cp + c) = codes8<E5M2>(raw[p], rinv);
       }
     }
-    if (!a.qt) return;
 #pragma unroll
     for (int i = 0; i < Raw::kWords; ++i) cm[i] = Raw::larger(cm[i], __shfl_xor_sync(0xffffffffu, cm[i], 16));
     if ((threadIdx.x & 31) < 16) {
@@ -331,11 +353,12 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
       for (int w = 0; w < 8; ++w) m = max(m, colmax[w][threadIdx.x]);
       const Scale sc = scale_of<E5M2>(m, a.pow2);
       inv[threadIdx.x] = sc.r;
+      bad = isnan(sc.r);
       const int64_t col = kb * 128 + threadIdx.x;
       if (col < a.C) a.st[(batch * a.rb + rblk) * a.C + col] = sc.s;
     }
   }
-  __syncthreads();
+  bad = __syncthreads_or(bad);
   // columns as rows: eight codes down each of the thread's eight columns, two columns at once
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -354,6 +377,14 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 3) quantiz
     const int64_t at = rblk * 128 + lane16 * 8;
     if (kb * 128 + col < a.C && at < a.Rp)
       *reinterpret_cast<uint2*>(a.qt + (batch * a.C + kb * 128 + col) * a.Rp + at) = turned[col * 16 + (lane16 ^ sub)];
+  }
+  if (bad) {
+    if (a.q) clear_rows();
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const int64_t col = kb * 128 + sub * 8 + i, at = rblk * 128 + lane16 * 8;
+      if (col < a.C && at < a.Rp) clear_padding(a.qt + (batch * a.C + col) * a.Rp + at, at, a.R);
+    }
   }
 }
 

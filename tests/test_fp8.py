@@ -216,6 +216,23 @@ def test_quantize_special_values(dev, block, pow2, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("r,c", [(260, 405), (1, 1), (7, 15), (133, 8), (129, 1161), (2000, 523)])
+def test_quantize_pads_blocks_of_nan_with_zeros(dev, block, kind, r, c):
+    # NaN and infinities in the last block of rows and of columns: what lies between the rows of codes is zeros all the same
+    x = inputs((r, c), kind, r + c)
+    x[0, c - 1], x[r - 1, 0], x[r - 1, c - 1] = float("nan"), float("nan"), float("nan")
+    x[r // 2, c - 1], x[r - 1, c // 2] = float("inf"), float("nan")
+    q, s, qt, st = gpu_quantize(x[None].cuda(), block, 0, 0, both=True)
+    q1, s1, _, _ = gpu_quantize(x[None].cuda(), block, 0, 0)
+    for got, want in ((q, quantize(x, block, 0, 0)[0]), (q1, quantize(x, block, 0, 0)[0]), (qt, quantize(x.t(), block, 0, 0)[0])):
+        same(got[0], want)
+    for codes, n in ((q, c), (q1, c), (qt, r)):
+        assert int(codes.view(torch.uint8)[0, :, n:].max() if up16(n) > n else 0) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("block", [1, 128])
 def test_quantize_gathers_rows(dev, block):
     x = inputs((70, 300), torch.bfloat16, 5)
