@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import struct
 import sys
 import threading
@@ -518,7 +519,10 @@ class Kernel:
         nm, sig = C.c_char_p(), C.c_char_p()
         check(lib().mtl_kernel_info(self.id, C.byref(nm), C.byref(sig)))
         self.signature = sig.value.decode()
-        self.packed = _Packed(self) if name in _OPERANDS else None
+        self.packed = None
+        if name in _OPERANDS:
+            self.wanted, self.flags = {}, operator.itemgetter(*_OPERANDS[name][1].values())  # see _wanted
+            self.packed = _Packed(self)
 
     def __repr__(self) -> str:
         return f"Kernel({self.name}: {self.signature})"
@@ -593,20 +597,23 @@ def _nd(ndrange) -> tuple[int, ...]:
 
 
 # What the buffer arguments of the 8-bit and expert-grouped kernels hold, a letter each:
-# c codes (8 bits), f Float32, h bfloat16 (or its bits), i Int32, o f or h as the
-# kernel's type argument says, whose index follows. The library sees addresses and
-# byte counts only, so what a tensor or buffer says of itself is checked here.
+# f Float32, h bfloat16 (or its bits), i Int32, o f or h as the kernel's type argument
+# says, p and q 8-bit codes in the formats that its first and second format argument
+# say; behind them those arguments' indexes. The library sees addresses and byte counts
+# only, so what a tensor or buffer says of itself is checked here.
 _OPERANDS = {
-    "quantize_fp8": ("cfcfoi", 10),
-    "gemm_fp8": ("ocfcf", 11),
-    "gemm_grouped_fp8": ("ocfcfi", 11),
-    "gemm_grouped_bf16": ("ohhi", 7),
-    "gemm_grouped_dx_bf16": ("ohhi", 7),
-    "gemm_grouped_dw_bf16": ("ohhi", 7),
+    "quantize_fp8": ("pfpfoi", {"o": 10, "p": 11}),
+    "gemm_fp8": ("opfqf", {"o": 11, "p": 9, "q": 10}),
+    "gemm_grouped_fp8": ("opfqfi", {"o": 11, "p": 9, "q": 10}),
+    "gemm_grouped_bf16": ("ohhi", {"o": 7}),
+    "gemm_grouped_dx_bf16": ("ohhi", {"o": 7}),
+    "gemm_grouped_dw_bf16": ("ohhi", {"o": 7}),
 }
-_KINDS = {np.dtype(t): k for k, types in {"c": (np.uint8, np.int8), "f": (np.float32,), "h": (np.uint16, np.int16),
-                                          "i": (np.int32, np.uint32)}.items() for t in types}
-_KIND_NAMES = {"c": "8-bit codes", "f": "Float32", "h": "bfloat16", "i": "Int32"}
+# What an element type can stand for; 4 and 5 are codes in e4m3 and e5m2, which plain bytes
+# may be either of, and * is what no test follows for.
+_KINDS = {np.dtype(t): k + "*" for k, types in {"45": (np.uint8, np.int8), "f": (np.float32,), "h": (np.uint16, np.int16),
+                                                "i": (np.int32, np.uint32)}.items() for t in types}
+_KIND_NAMES = {"4": "8-bit codes in e4m3", "5": "8-bit codes in e5m2", "f": "Float32", "h": "bfloat16", "i": "Int32"}
 _PTR = L.ARG_PTR
 _tensor = _current_device = None  # torch.Tensor, torch.cuda.current_device, once torch is loaded
 
@@ -615,10 +622,22 @@ def _with_torch() -> None:
     global _tensor, _current_device
     torch = sys.modules["torch"]
     _current_device = torch.cuda.current_device
-    for kind, names in {"c": ("uint8", "int8", "float8_e4m3fn", "float8_e5m2"), "f": ("float32",),
+    for kind, names in {"45": ("uint8", "int8"), "4": ("float8_e4m3fn",), "5": ("float8_e5m2",), "f": ("float32",),
                         "h": ("bfloat16", "uint16", "int16"), "i": ("int32",)}.items():
-        _KINDS.update({getattr(torch, n): kind for n in names if hasattr(torch, n)})
+        _KINDS.update({getattr(torch, n): kind + "*" for n in names if hasattr(torch, n)})
     _tensor = torch.Tensor
+
+
+def _wanted(k: Kernel, args: Sequence) -> str:
+    """_OPERANDS' letters of a kernel with o, p and q resolved by the call's type and
+    format arguments, kept for calls of the same; * for one that the library refuses."""
+    kinds, flags = _OPERANDS[k.name]
+    for letter, i in flags.items():
+        valid = isinstance(args[i], (int, np.integer)) and args[i] in (0, 1)
+        kinds = kinds.replace(letter, ("fh" if letter == "o" else "45")[int(args[i])] if valid else "*")
+    if "*" not in kinds:
+        k.wanted[k.flags(args)] = kinds
+    return kinds
 
 
 def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
@@ -626,14 +645,14 @@ def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
     one flat list, checked: element types, for torch tensors contiguity and the current
     CUDA device, for a launch's Buffers that device too where torch tells it. A graph's
     resources have their plan's addresses, so only a graph takes them."""
-    kinds, flag = _OPERANDS[k.name]
     if len(args) != len(k.signature):
         raise ArgumentError(L.ERR_ARGUMENT, f"{k.name} takes {len(k.signature)} arguments ({k.signature}), got {len(args)}")
     if _tensor is None and "torch" in sys.modules:
         _with_torch()
-    out = args[flag]
-    if out == 0 or out == 1:  # the library refuses another type
-        kinds = kinds.replace("o", "fh"[out])
+    try:
+        kinds = k.wanted[k.flags(args)]
+    except (KeyError, TypeError):
+        kinds = _wanted(k, args)
     flat, device = [], None
     for x, want in zip(args, kinds):
         if _tensor is not None and isinstance(x, _tensor):
@@ -661,7 +680,7 @@ def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
                     raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4 + 1} is a buffer on device {x.dev.ordinal}, "
                                         f"the current one is {device}")
             flat += (_PTR, 0, getattr(x, "ptr", 0), getattr(x, "nbytes", 0))
-        if _KINDS.get(x.dtype) != want != "o":
+        if want not in _KINDS.get(x.dtype, "*"):
             raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: argument {len(flat) // 4} holds {x.dtype}, expected {_KIND_NAMES[want]}")
     return flat
 

@@ -140,6 +140,39 @@ def test_a_launch_takes_buffers_of_the_current_device_only(monkeypatch):
         M.launch(M.kernels.quantize_fp8, [far] + q_args(4, 256)[1:], 1)
 
 
+def test_codes_of_another_format_are_refused(monkeypatch):
+    # tensors that say which format their codes are in: the call's format has to be that one
+    class Codes:
+        def __init__(self, dtype, nbytes=1 << 16):
+            self.dtype, self.nbytes = dtype, nbytes
+        get_device = lambda self: 0  # noqa: E731
+        is_contiguous = lambda self: True  # noqa: E731
+        data_ptr = lambda self: 1 << 20  # noqa: E731
+    M._with_torch()
+    monkeypatch.setattr(M, "_tensor", Codes)
+    monkeypatch.setattr(M, "_current_device", lambda: 0)
+    e4, e5, u8 = torch.float8_e4m3fn, torch.float8_e5m2, torch.uint8
+    quantize_, gemm, grouped = M.kernels.quantize_fp8, M.kernels.gemm_fp8, M.kernels.gemm_grouped_fp8
+    name = {0: "e4m3", 1: "e5m2"}
+    for fa in (0, 1):
+        right, wrong = (e4, e5)[fa], (e5, e4)[fa]
+        for kernel, args, at in ((quantize_, q_args(4, 256, both=True, fmt=fa), (0, 2)), (gemm, g_args(1, 4, 5, 64, fa=fa, fb=1 - fa), (1,)),
+                                 (gemm, g_args(1, 4, 5, 64, fa=1 - fa, fb=fa), (3,)),
+                                 (grouped, e_args(3, 10, 40, 64)[:9] + [fa, 1 - fa, 0], (1,)), (grouped, e_args(3, 10, 40, 64)[:9] + [1 - fa, fa, 0], (3,))):
+            for i in at:
+                for good in (right, u8):
+                    args[i] = Codes(good)
+                    assert len(M._operands(kernel, args)) % 4 == 0
+                args[i] = Codes(wrong)
+                with pytest.raises(M.ArgumentError, match=f"argument {i + 1} holds {wrong}, expected 8-bit codes in {name[fa]}"):
+                    M.launch(kernel, args, 1)
+                args[i] = ptr(1 << 16)
+    for kernel, args, flag in ((gemm, g_args(1, 4, 5, 64), 9), (quantize_, q_args(4, 256), 11)):  # a format that is none: the library's refusal
+        args[flag], args[1 if kernel is gemm else 0] = 2, Codes(e5)
+        with pytest.raises(M.MantleError, match="formats|must be 0 or 1"):
+            M.launch(kernel, args, 1)
+
+
 # ── on the GPU ───────────────────────────────────────────────────────────────
 def stream():
     return torch.cuda.current_stream().cuda_stream
