@@ -108,8 +108,7 @@ struct GrWalk {
 // Terms an accumulator runs for. The tensor core drops what an addition shifts out of fp32
 // instead of rounding it, so the error grows with the terms (1352 of them: 1.4e-6 of the
 // result). Where an fp32 output is the sum of more than 768 terms (DEEP), sums of 768 are
-// added in registers, rounded to the nearest, and the error stays at 0.8e-6. (In a bf16
-// output its rounding, 2e-3, hides it.) Tiles of a single run are not to pay for the
+// added in registers, rounded to the nearest, and the error stays at 0.8e-6. Tiles of a single run are not to pay for the
 // registers that hold those sums: with both kinds of tile in one loop a weight gradient went
 // from 115 to 138 us. Forward and for the input gradient the terms are the same in every
 // tile, so these are kernels of their own (8192 rows over 16 groups forward in fp32 take 161
@@ -117,17 +116,24 @@ struct GrWalk {
 // which only the device knows: there the groups of a single run come first (order_groups) and
 // the others after them, in a loop of their own. In this order the first loop costs 1 % for
 // the registers of the second (128 rows a group 114.6 -> 115.9 us), in the other one 7 %.
-constexpr int kRunTerms = 768;
-template <bool DEEP>
-constexpr int kRunBlocks = DEEP ? kRunTerms / kGrK : 1 << 28;
+//
+// A bf16 output is DEEP above 32768 terms: by the same growth a run is off by 3.4e-5 of the
+// result, and 8 million terms in one accumulator would be by 8e-3, more than the rounding to
+// bf16. It also keeps every wait for an accumulator far below the limit, which the sums of a
+// billion terms in one would pass.
+template <typename OUT>
+constexpr int kRunTerms = sizeof(OUT) == 4 ? 768 : 32768;
+template <typename OUT, bool DEEP>
+constexpr int kRunBlocks = DEEP ? kRunTerms<OUT> / kGrK : 1 << 28;
 
 // A DEEP weight gradient's groups, those of a single run first: cum[i] is the i-th of them,
 // cum[kMaxGroups] how many these are. Every thread of the CTA calls this, after build_groups,
 // whose sums of tiles a weight gradient does not need.
+template <typename OUT>
 __device__ __forceinline__ void order_groups(GroupTable* g, int groups) {
   if (threadIdx.x < 32) {
     const uint32_t below = (1u << threadIdx.x) - 1;
-    auto is_short = [&](int e) { return e < groups && g->hi[e] - g->lo[e] <= kRunTerms; };
+    auto is_short = [&](int e) { return e < groups && g->hi[e] - g->lo[e] <= kRunTerms<OUT>; };
     int shorts = 0;
     for (int base = 0; base < groups; base += 32) shorts += __popc(__ballot_sync(0xffffffffu, is_short(base + (int)threadIdx.x)));
     int at = 0, rest = shorts;  // where the next of either goes
@@ -186,7 +192,7 @@ template <int FORM, int BN, typename OUT, bool DEEP>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
   using Cfg = GrCfg<BN>;
-  constexpr int kStages = Cfg::kStages, kRun = kRunBlocks<DEEP>;
+  constexpr int kStages = Cfg::kStages, kRun = kRunBlocks<OUT, DEEP>;
   constexpr uint32_t kIdesc = idesc_bf16_f32(kGrM, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   build_groups(&sh->groups, p.offsets, p.groups, p.T, kGrM);
-  if constexpr (FORM == kDw && DEEP) order_groups(&sh->groups, p.groups);
+  if constexpr (FORM == kDw && DEEP) order_groups<OUT>(&sh->groups, p.groups);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -445,7 +451,7 @@ template <int FORM, int NT, typename OUT>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_slim_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const GrArgs p) {
   using Cfg = SlimCfg<NT>;
-  constexpr int kStages = Cfg::kStages, BN = 256, kRun = kRunBlocks<sizeof(OUT) == 4>;
+  constexpr int kStages = Cfg::kStages, BN = 256, kRun = kRunBlocks<OUT, sizeof(OUT) == 4>;
   constexpr uint32_t kIdesc = idesc_bf16_f32(128, NT, FORM != kDx, false);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -660,7 +666,7 @@ template <int FORM, int PIECE, typename OUT, bool DEEP>
 __global__ void __launch_bounds__(kGrThreads, 1)
     gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GrArgs p) {
   using Cfg = PairCfg<PIECE>;
-  constexpr int kStages = Cfg::kStages, BN = Cfg::kBN, kRun = kRunBlocks<DEEP>;
+  constexpr int kStages = Cfg::kStages, BN = Cfg::kBN, kRun = kRunBlocks<OUT, DEEP>;
   constexpr uint32_t kIdesc = idesc_bf16_f32(256, BN, FORM == kDw, FORM != kDx);
   extern __shared__ unsigned char gr_raw[];
   unsigned char* ring =
@@ -690,7 +696,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   build_groups(&sh->groups, p.offsets, p.groups, p.T, 256);
-  if constexpr (FORM == kDw && DEEP) order_groups(&sh->groups, p.groups);
+  if constexpr (FORM == kDw && DEEP) order_groups<OUT>(&sh->groups, p.groups);
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are there
@@ -1045,6 +1051,22 @@ static cudaError_t gr_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, 
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
 }
 
+template <int FORM, int BN>
+static cudaError_t gr_launch_by(bool bf16, bool deep, const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
+                                const LaunchArgs& la, cudaStream_t s) {
+  if (bf16)
+    return deep ? gr_launch<FORM, BN, __nv_bfloat16, true>(ta, tb, p, tiles, la, s) : gr_launch<FORM, BN, __nv_bfloat16, false>(ta, tb, p, tiles, la, s);
+  return deep ? gr_launch<FORM, BN, float, true>(ta, tb, p, tiles, la, s) : gr_launch<FORM, BN, float, false>(ta, tb, p, tiles, la, s);
+}
+template <int FORM, int PIECE>
+static cudaError_t gr_launch_pair_by(bool bf16, bool deep, const CUtensorMap& ta, const CUtensorMap& tb, const GrArgs& p, int64_t tiles,
+                                     const LaunchArgs& la, cudaStream_t s) {
+  if (bf16)
+    return deep ? gr_launch_pair<FORM, PIECE, __nv_bfloat16, true>(ta, tb, p, tiles, la, s)
+                : gr_launch_pair<FORM, PIECE, __nv_bfloat16, false>(ta, tb, p, tiles, la, s);
+  return deep ? gr_launch_pair<FORM, PIECE, float, true>(ta, tb, p, tiles, la, s) : gr_launch_pair<FORM, PIECE, float, false>(ta, tb, p, tiles, la, s);
+}
+
 template <int FORM>
 static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   const char* who = kGrName[FORM];
@@ -1069,14 +1091,15 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   // Pairs where their 256-row tiles waste little (groups of 768 rows on average) and
   // there is a tile for each.
   const int64_t col_tiles = (cols + 255) / 256, pair_tiles = (FORM == kDw ? (int64_t)E * ((K + 255) / 256) : T / 256) * col_tiles;
-  const bool deep = !out && (FORM == kDw ? T : p.depth) > kRunTerms;  // a group has T rows at most
+  // a group has T rows at most
+  const bool deep = (FORM == kDw ? T : p.depth) > (out ? kRunTerms<__nv_bfloat16> : kRunTerms<float>);
   const bool pair = pair_tiles >= la.sm_count / 2 && (FORM == kDw || T >= 768 * (int64_t)E);
   // Rows of a group in the MMA's N operand, 32 or 64 of them, while a group has up to 16
   // or 40 on average and there are tiles for most SMs. Sustained, us, against tiles of 128
   // rows: 2 rows a group (32 groups, 2048 x 4096) 81.7 and 89.5, 8 rows 83.1 and 90.8, 32
   // rows (16 groups, 2048 x 2048) 25.5 with 64, 29.7 with 32 and 28.0, 64 rows 55 and 51.3.
   const int64_t slim_tiles = (int64_t)E * col_tiles;
-  const int slim = FORM == kDw || slim_tiles * 4 < la.sm_count * 3 || T > 40 * (int64_t)E ? 0 : T <= 16 * (int64_t)E ? 32 : 64;
+  const int slim = FORM == kDw || (out && deep) || slim_tiles * 4 < la.sm_count * 3 || T > 40 * (int64_t)E ? 0 : T <= 16 * (int64_t)E ? 32 : 64;
   p.a_box = slim ? slim : T / E >= kGrM ? kGrM : 32;
   const void *A = reinterpret_cast<const void*>(la.a[1].ptr), *B = reinterpret_cast<const void*>(la.a[2].ptr);
   const int64_t row_tiles = FORM == kDw ? (int64_t)E * ((K + 127) / 128) : std::max<int64_t>(E, (T + 127) / 128);
@@ -1107,21 +1130,13 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
     }
   } else if (pair && FORM == kDw && T <= (out ? 256 : 512) * (int64_t)E) {
     constexpr int kPiece = FORM == kDw ? 128 : 64;
-    e = out    ? gr_launch_pair<FORM, kPiece, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
-        : deep ? gr_launch_pair<FORM, kPiece, float, true>(ta, tb, p, tiles, la, s)
-               : gr_launch_pair<FORM, kPiece, float, false>(ta, tb, p, tiles, la, s);
+    e = gr_launch_pair_by<FORM, kPiece>(out, deep, ta, tb, p, tiles, la, s);
   } else if (pair) {
-    e = out    ? gr_launch_pair<FORM, 64, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
-        : deep ? gr_launch_pair<FORM, 64, float, true>(ta, tb, p, tiles, la, s)
-               : gr_launch_pair<FORM, 64, float, false>(ta, tb, p, tiles, la, s);
+    e = gr_launch_pair_by<FORM, 64>(out, deep, ta, tb, p, tiles, la, s);
   } else if (narrow) {
-    e = out    ? gr_launch<FORM, 128, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
-        : deep ? gr_launch<FORM, 128, float, true>(ta, tb, p, tiles, la, s)
-               : gr_launch<FORM, 128, float, false>(ta, tb, p, tiles, la, s);
+    e = gr_launch_by<FORM, 128>(out, deep, ta, tb, p, tiles, la, s);
   } else {
-    e = out    ? gr_launch<FORM, 256, __nv_bfloat16, false>(ta, tb, p, tiles, la, s)
-        : deep ? gr_launch<FORM, 256, float, true>(ta, tb, p, tiles, la, s)
-               : gr_launch<FORM, 256, float, false>(ta, tb, p, tiles, la, s);
+    e = gr_launch_by<FORM, 256>(out, deep, ta, tb, p, tiles, la, s);
   }
   return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }

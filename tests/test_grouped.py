@@ -300,6 +300,42 @@ def test_a_weight_gradients_long_groups_among_short_ones_in_fp32(dev, sizes, n, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("way,sizes,n,k", [
+    ("dw", [8_000_000], 16, 16), ("fwd", [16], 16, 8_000_000), ("dx", [16], 8_000_000, 16),  # one CTA a tile
+    ("dw", [3_000_000, 40, 32768, 0, 32769], 136, 72), ("fwd", [500] * 4, 2560, 40_000),
+    ("dw", [1_000_000, 5, 40_000], 1288, 1032), ("dw", [33_000] + [35] * 200, 264, 136), ("fwd", [5120], 1024, 40_000), ("dx", [5120], 40_000, 1024),  # pairs
+    ("fwd", [2] * 40, 1024, 40_000),                                                         # few rows a group
+])
+def test_very_long_contractions_in_bf16(dev, way, sizes, n, k):
+    # Sums of more than 32768 terms are added run by run. As above, the 2048 MMAs of a run are off by sum 4 sqrt(j) 2^-23
+    # = 2.5e5 * 2^-23 at most where the run's own size is 181: 1.63e-4 of it. Runs are added with half a unit of fp32
+    # each, and the result is rounded to bf16: 2^-8 of the value. No wait takes as long as the sum: the limit is 10 ms
+    # here, and the 8 million terms of a tile take longer.
+    e, t = len(sizes), sum(sizes)
+    o = [sum(sizes[:i]) for i in range(e + 1)]
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    a, b = ({"fwd": (t, k), "dx": (t, n), "dw": (t, k)}[way], {"fwd": (e, k, n), "dx": (e, k, n), "dw": (t, n)}[way])
+    a, b = (torch.randn(v, generator=g, device="cuda", dtype=torch.bfloat16) for v in (a, b))
+    out = torch.full({"fwd": (t, n), "dx": (t, k), "dw": (e, k, n)}[way], float("nan"), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    try:
+        M.set_wait_limit(10_000_000)
+        launch(way, out, a, b, o, t, n, k, e, 1)
+        torch.cuda.synchronize()
+    finally:
+        M.set_wait_limit(0)
+    assert M.kernel_timeouts(reset=True) == 0
+    for i in range(e):
+        r = slice(o[i], o[i + 1])
+        x, y = (a[r].t(), b[r]) if way == "dw" else (a[r], b[i].t() if way == "dx" else b[i])
+        want = torch.zeros((x.shape[0], y.shape[1]), dtype=torch.float64, device="cuda")
+        for c in range(0, x.shape[1], 1 << 18):
+            want += x[:, c:c + (1 << 18)].double() @ y[c:c + (1 << 18)].double()
+        off = (out[i] if way == "dw" else out[r]).double() - want
+        assert float(off.norm()) <= (2.0 ** -8 + 1.63e-4 + -(-x.shape[1] // 32768) * 2.0 ** -24) * float(want.norm())
+
+
+@pytest.mark.gpu
 def test_the_gradients_are_the_products_derivatives(dev):
     # the directional derivative of L = sum(Y * dY) by central differences: L is linear in X and in W, so a step
     # of h along a direction D changes L by h <grad, D> exactly, up to the sums' rounding (fp32, S as above) and
