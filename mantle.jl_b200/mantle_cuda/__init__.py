@@ -702,6 +702,12 @@ class _Packed:
         self.buffers = len(_OPERANDS[k.name][0])
         self.scalars = [L.ARG_I32, 0, 0, 0] * (self.nargs - self.buffers)
 
+    def range_of(self, nd: tuple) -> bytes:
+        try:
+            return struct.pack("<3q", *nd, *([1] * (3 - len(nd))))
+        except struct.error as e:
+            raise ArgumentError(L.ERR_ARGUMENT, f"{self.kernel.name}: no ndrange: {nd} ({e})") from None
+
     def __call__(self, args: Sequence, ndrange, stream: int) -> None:
         buffers, scalars = _operands(self.kernel, args), self.scalars.copy()
         scalars[2::4] = args[self.buffers:]
@@ -713,12 +719,12 @@ class _Packed:
             n = 1
             range_ = self.ndranges.get(ndrange)
             if range_ is None:
-                range_ = struct.pack("<3q", ndrange, 1, 1)
+                range_ = self.range_of((ndrange,))
                 if len(self.ndranges) < 4096:
                     self.ndranges[ndrange] = range_
         else:
             nd = _nd(ndrange)
-            n, range_ = len(nd), struct.pack("<3q", *nd, *([1] * (3 - len(nd))))
+            n, range_ = len(nd), self.range_of(nd)
         status = self.entry(self.kernel.id, packed, self.nargs, range_, n, None, 0, stream)
         if status:
             check(status)

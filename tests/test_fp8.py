@@ -123,6 +123,12 @@ def test_tensors_are_checked_before_the_call():
         M.launch(M.kernels.gemm_fp8, g_args(1, 4, 5, 64)[:-1], 1)
 
 
+@pytest.mark.parametrize("nd,match", [(1 << 70, "no ndrange"), ((1, 1, 1, 1), "no ndrange"), ((1, 1), "one-dimensional"), (-1, "negative"), ((), "1-3 dimensions")])
+def test_an_ndrange_that_is_none_is_refused(nd, match):
+    with pytest.raises(M.MantleError, match=match):
+        M.launch(M.kernels.gemm_fp8, g_args(1, 4, 5, 64), nd)
+
+
 def test_a_launch_takes_buffers_of_the_current_device_only(monkeypatch):
     # a graph's transients have no address of their own; another device's memory may not be reachable
     def made(cls, **fields):
