@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 template <int NT>
 struct SlimCfg {
   static constexpr uint32_t kWStage = 256 * kGrK * 2, kXStage = NT * kGrK * 2, kStageBytes = kWStage + kXStage;
-  static constexpr int kStages = 196608 / (int)kStageBytes;  // 5
+  static constexpr int kStages = 196608 / (int)kStageBytes;  // 5, or 4 with 64 rows
   static constexpr uint32_t kTmemCols = 4 * NT < 32 ? 32 : 4 * NT;  // two accumulators of two runs
 };
 template <int NT>
@@ -1103,6 +1103,7 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   p.a_box = slim ? slim : T / E >= kGrM ? kGrM : 32;
   const void *A = reinterpret_cast<const void*>(la.a[1].ptr), *B = reinterpret_cast<const void*>(la.a[2].ptr);
   const int64_t row_tiles = FORM == kDw ? (int64_t)E * ((K + 127) / 128) : std::max<int64_t>(E, (T + 127) / 128);
+  // always so for a weight gradient: without a pair tile for every two SMs it has less than one of 128 rows for each
   const bool narrow = !pair && !slim && row_tiles * col_tiles < la.sm_count;
   const int bn = narrow ? 128 : 256, box_n = pair ? 128 : bn;  // columns of B a tile, a box
   p.chunked_a = FORM == kDw && K % 64 == 0;
@@ -1136,7 +1137,10 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
   } else if (narrow) {
     e = gr_launch_by<FORM, 128>(out, deep, ta, tb, p, tiles, la, s);
   } else {
-    e = gr_launch_by<FORM, 256>(out, deep, ta, tb, p, tiles, la, s);
+    if constexpr (FORM != kDw)
+      e = gr_launch_by<FORM, 256>(out, deep, ta, tb, p, tiles, la, s);
+    else
+      e = cudaErrorInvalidValue;
   }
   return e == cudaSuccess ? MTL_OK : fail(MTL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }
