@@ -429,3 +429,39 @@ def test_gemm_grouped_fp8_bad_offsets_stay_in_bounds(dev):
     for lo, hi, e in ((0, 20, 0), (0, 40, 0), (40, 90, 2), (90, 100, 3)):  # an offset below an earlier one counts as that one
         vw = values(qw[e], sw[e], 128, k)
         check_product(got[lo:hi], vx[lo:hi] @ vw.t(), vx[lo:hi].abs() @ vw.abs().t(), 2, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fa,fb", [(1, 0), (0, 1), (1, 1)])
+@pytest.mark.parametrize("sizes,t,n,k,out", [
+    ([130, 0, 64, 1], 200, 264, 384, 1), ([700, 20, 600], 1320, 1024, 250, 0),  # tiles
+    ([2] * 60, 120, 515, 1300, 1), ([33, 0, 5, 1] * 20, 790, 640, 130, 0),      # rows as the MMA's N operand
+])
+def test_gemm_grouped_fp8_in_both_formats(dev, sizes, t, n, k, out, fa, fb):
+    # gradients in e5m2 times weight codes in e4m3, and the other pairs
+    e, o = len(sizes), offsets_of(sizes)
+    qx, sx, _, _ = gpu_quantize(inputs((1, t, k), torch.float32, t).cuda(), 1, fa, 0)
+    qw, sw, _, _ = gpu_quantize(inputs((e, n, k), torch.float32, n).cuda(), 128, fb, 0)
+    y = torch.full((t, n), 3.0, dtype=torch.bfloat16 if out else torch.float32, device="cuda")
+    M.launch(M.kernels.gemm_grouped_fp8, (y, qx, sx, qw, sw, torch.tensor(o, dtype=torch.int32, device="cuda"), t, n, k, fa, fb, out),
+             e, stream=stream())
+    torch.cuda.synchronize()
+    vx, got = values(qx[0], sx[0], 1, k), y.double().cpu()
+    for i in range(e):
+        r, vw = slice(o[i], o[i + 1]), values(qw[i], sw[i], 128, k)
+        if sizes[i]:
+            check_product(got[r], vx[r] @ vw.t(), vx[r].abs() @ vw.abs().t(), -(-k // 128), out)
+    assert (got[o[-1]:] == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bblock", [128, 1])
+@pytest.mark.parametrize("m,n,k,fa,fb,out", [
+    (1, 264, 700, 1, 1, 0), (5, 300, 1300, 1, 1, 1), (9, 136, 2050, 1, 1, 0), (16, 520, 640, 1, 0, 1), (12, 72, 300, 0, 1, 0),  # few rows
+    (200, 1000, 3000, 1, 1, 0), (2100, 1100, 300, 1, 1, 1), (40, 500, 2200, 0, 1, 0)])
+def test_gemm_fp8_in_both_formats(dev, bblock, m, n, k, fa, fb, out):
+    qa, sa, qb, sb, va, vb = operands(1, m, n, k, bblock, fa, fb, m + n)
+    c = torch.full((1, m, n), float("nan"), dtype=torch.bfloat16 if out else torch.float32, device="cuda")
+    M.launch(M.kernels.gemm_fp8, (c, qa, sa, qb, sb, m, n, k, bblock, fa, fb, out), 1, stream=stream())
+    torch.cuda.synchronize()
+    check_product(c, va @ vb.transpose(1, 2), va.abs() @ vb.abs().transpose(1, 2), -(-k // 128), out)

@@ -357,3 +357,21 @@ def test_the_gradients_are_the_products_derivatives(dev):
     # whole numbers below 2^24 throughout: every product and sum is exact
     assert float((loss(x + h * dirx, w) - loss(x - h * dirx, w)) / (2 * h)) == float((dx.double() * dirx.double()).sum())
     assert float((loss(x, w + h * dirw) - loss(x, w - h * dirw)) / (2 * h)) == float((dw.double() * dirw.double()).sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [0, 1])
+def test_weight_gradients_of_a_thousand_groups(dev, kind):
+    # as many groups as there may be, two of them of several runs, among empty ones; whole numbers: exact in fp32
+    e, k, n = 1024, 64, 72
+    sizes = [i % 4 for i in range(e)]
+    sizes[5], sizes[1023] = 900, 2000
+    o = [sum(sizes[:i]) for i in range(e + 1)]
+    g = torch.Generator().manual_seed(3)
+    x, dy = (torch.randint(-3, 4, s, generator=g).to(torch.bfloat16) for s in ((o[-1], k), (o[-1], n)))
+    out = torch.full((e, k, n), float("nan"), dtype=torch.bfloat16 if kind else torch.float32, device="cuda")
+    launch("dw", out, x.cuda(), dy.cuda(), o, o[-1], n, k, e, kind)
+    torch.cuda.synchronize()
+    for i in range(e):
+        want = x[o[i]:o[i + 1]].float().t() @ dy[o[i]:o[i + 1]].float()
+        assert torch.equal(out[i].cpu(), want.to(out.dtype)), i
