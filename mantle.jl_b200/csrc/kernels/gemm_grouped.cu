@@ -634,15 +634,15 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 // short as its groups while every tile leaves 128 to 256 KiB. A last K block with rows
 // behind the group lands on a barrier of each CTA's own; the CTA zeroes those rows and
 // then tells the even CTA, which issues the MMAs. Sustained, us, against one CTA a tile
-// (2048 x 4096): weight gradient of 16 groups of 8192 rows 181 and 210 (fp32), 145 and 173
+// (2048 x 4096): weight gradient of 8192 rows in 16 groups 181 and 210 (fp32), 145 and 173
 // (bf16; storing by TMA from two 4 KiB buffers a warp, with fewer stages for their room,
 // 158); forward with 4 groups 116 and 123, 8 groups 126 and 131, 16 groups 148 and 144.
 //
 // Weight gradients of short groups are stores for the most part, and take one stage of the
 // ring for rows leaving in pieces of 128 bytes instead of 64 (store_rows). Sustained, us,
-// 128 and 64 bytes, 16 groups, 2048 x 4096: 128 rows a group 111 and 128 (fp32), 75.5 and
-// 81.4 (bf16); 256 rows 132 and 148, 100.4 and 101; 384 rows 157 and 166, 126 and 123; 512
-// rows 185 and 186, 151 and 147.
+// 128 and 64 bytes, 16 groups (half to one and a half times as long each), 2048 x 4096: 128
+// rows a group 107 and 129 (fp32), 72 and 80 (bf16); 256 rows 130 and 147, 104 and 104; 384
+// rows 165 and 170, 129 and 125; 512 rows 197 and 189, 156 and 148.
 template <int PIECE>  // bytes of an output row a store
 struct PairCfg {
   static constexpr uint32_t kAStage = 128 * kGrK * 2, kStageBytes = 2 * kAStage;
@@ -1129,7 +1129,7 @@ static mtl_status gr_run(const LaunchArgs& la, cudaStream_t s) {
     } else {
       e = cudaErrorInvalidValue;
     }
-  } else if (pair && FORM == kDw && T <= (out ? 256 : 512) * (int64_t)E) {
+  } else if (pair && FORM == kDw && T <= (out ? 256 : 448) * (int64_t)E) {
     constexpr int kPiece = FORM == kDw ? 128 : 64;
     e = gr_launch_pair_by<FORM, kPiece>(out, deep, ta, tb, p, tiles, la, s);
   } else if (pair) {
