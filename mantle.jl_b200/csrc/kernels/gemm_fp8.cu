@@ -16,9 +16,9 @@
 // read it back (tcgen05.ld), multiply by the scales and add to fp32 sums in
 // registers, rounding to nearest, while the tensor core runs the next K block
 // into another accumulator. A K block of a 128 x 256 tile is 512 cycles of MMAs, but
-// the two accumulators that fit are handed back and forth in about 800 with nothing to
-// add, and the sums come to about 1050: 8192 cubed takes 536 us in a burst (2050
-// TFLOP/s) and 622 to 635 in a long run, which the power cap holds to that.
+// with its loads and the hand-offs of the two accumulators that fit it takes about 860
+// with nothing to add, and with the sums about 1050: 8192 cubed takes 536 us in a burst
+// (2050 TFLOP/s) and 622 to 635 in a long run, which the power cap holds to that.
 //
 // One persistent CTA per SM, three warpgroups; the first gives registers up
 // (setmaxnreg) so that the sums of the other two stay in theirs:
@@ -51,7 +51,9 @@
 namespace mtl {
 
 constexpr int kF8Threads = 384, kF8M = 128, kF8K = 128;
-constexpr int kF8FewRegs = 56, kF8ManyRegs = 224;  // registers a thread of the first / the other warpgroups
+// Registers a thread of the first / the other warpgroups. The kernels are compiled for the
+// 168 that both start with: those of 256 columns spill 8 to 60 bytes a thread.
+constexpr int kF8FewRegs = 56, kF8ManyRegs = 224;
 constexpr int kF8GroupM = 16;  // row tiles per raster group of a dense product
 
 // A stage less than there would be room for, so that rows leave in pieces of 128 bytes

@@ -110,6 +110,28 @@ def test_a_linear_layer_forward_and_backward(dev, m, n, k, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sizes,n,k", [([70, 0, 130, 3], 264, 200), ([3] * 50, 515, 1100)])
+def test_an_input_gradient_by_expert_in_8_bits(dev, sizes, n, k):
+    # dX = dY W[e]: gradients in e5m2 times the weights' transposed codes, which the quantizer makes with the others
+    e, t = len(sizes), sum(sizes)
+    o = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    g = torch.Generator().manual_seed(n)
+    w, dy = torch.randn((e, n, k), generator=g), torch.randn((1, t, n), generator=g)
+    _, _, wqt, wst = quantized(w.cuda(), 128, both=True)
+    dq, ds = quantized(dy.cuda().to(torch.bfloat16), 1, fmt=1)
+    dx = torch.full((t, k), float("nan"), device="cuda")
+    M.launch(M.kernels.gemm_grouped_fp8, (dx, dq, ds, wqt, wst, torch.from_numpy(o).cuda(), t, k, n, 1, 0, 0), e, stream=stream())
+    torch.cuda.synchronize()
+    vd = values(dq[0].view(CODE[1]), ds[0], 1, n)
+    for i in range(e):
+        r, vw = slice(int(o[i]), int(o[i + 1])), values(wqt[i].view(CODE[0]), wst[i], 128, n).t()
+        if sizes[i]:
+            assert ((dx[r].double().cpu() - vd[r] @ vw).abs() <= bound(vd[r], vw, False)).all()
+            # the codes stand for the weights: off by 2^-4 of a value, or of the block's smallest normal one
+            assert ((vw - w[i].double()).abs() <= 2.0 ** -4 * w[i].double().abs() + 2.0 ** -10 * wst[i].max().item()).all()
+
+
+@pytest.mark.gpu
 def test_a_training_step_of_experts_in_a_graph(dev):
     # forward and both gradients as passes of one plan, replayed, against the same launches outside it
     t, e, k, n = 300, 5, 136, 264
