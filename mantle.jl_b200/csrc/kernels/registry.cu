@@ -28,7 +28,14 @@ LM_DECL(gemm_grouped_fp8)
 LM_DECL(gemm_grouped)
 LM_DECL(gemm_grouped_dx)
 LM_DECL(gemm_grouped_dw)
+LM_DECL(rms_norm)
+LM_DECL(rms_norm_grad)
+LM_DECL(route_experts)
+LM_DECL(route_experts_grad)
+LM_DECL(combine_experts)
+LM_DECL(combine_experts_grad)
 #undef LM_DECL
+uint64_t rms_norm_grad_workspace(const LaunchArgs& la);
 mtl_status conv_check(const LaunchArgs& la, const uint64_t* bytes);
 mtl_status conv_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream);
 mtl_status nchwconv_check(const LaunchArgs& la, const uint64_t* bytes);
@@ -312,6 +319,28 @@ static KernelDesc g_kernels[] = {
      nullptr, true},
     {"gemm_grouped_dw_bf16", "BBBBiiii", false, 0b1110, 0b1, gemm_grouped_dw_check, nullptr, gemm_grouped_dw_run,
      nullptr, true},
+    // h = x + residual, y = h / rms(h) * w by row: y, q, s (8-bit codes of y and scales),
+    // h, x, residual, w, C, type, type of w (0 f32, 1 bf16), format, power-of-two scales,
+    // eps; ndrange = rows
+    {"rms_norm", "bbbbBbBiiiiif", false, 0b1110000, 0b0001111, rms_norm_check, nullptr, rms_norm_run, nullptr, true},
+    // its gradient: dx, dw, dy, h, w, the residual path's gradient, C, types, eps; ndrange = rows
+    {"rms_norm_grad", "BbBBBbiiif", false, 0b111100, 0b000011, rms_norm_grad_check, rms_norm_grad_workspace,
+     rms_norm_grad_run, nullptr, true},
+    // routing to experts: ids, weights, offsets, rows_of, row_at, logits, bias, live, E,
+    // top, groups, top_groups, best, score (0 softmax, 1 sigmoid), renorm, type, scale;
+    // ndrange = tokens
+    {"route_experts", "BBbbbBbbiiiiiiiif", false, 0b11100000, 0b00011111, route_experts_check, nullptr,
+     route_experts_run, nullptr, true},
+    // its gradient: dlogits, dweights, logits, ids, E, top, score, renorm, type, scale
+    {"route_experts_grad", "BBBBiiiiif", false, 0b1110, 0b0001, route_experts_grad_check, nullptr,
+     route_experts_grad_run, nullptr, true},
+    // the experts' rows back to their tokens: y, rows, weights, row_at, base, R, C, top,
+    // type of the rows, type of y; ndrange = tokens
+    {"combine_experts", "BBbBbiiiii", false, 0b11110, 0b00001, combine_experts_check, nullptr, combine_experts_run,
+     nullptr, true},
+    // its gradient: drows, dweights, dy, rows, weights, row_at, rows_of, R, C, top, types
+    {"combine_experts_grad", "BbBbbBBiiiii", false, 0b1111100, 0b0000011, combine_experts_grad_check, nullptr,
+     combine_experts_grad_run, nullptr, true},
     // NHWC bf16 convolution (implicit GEMM): out, in, w (HWIO), H, W, Cin, Cout,
     // k, stride, pad, relu, in_wpad, out_wpad; ndrange = images
     {"conv2d_bf16", "BBBiiiiiiiiii", false, 0b110, 0b001, conv_check, conv_workspace, conv_run, nullptr},

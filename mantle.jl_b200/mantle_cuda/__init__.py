@@ -596,10 +596,10 @@ def _nd(ndrange) -> tuple[int, ...]:
     return tuple(int(v) for v in ndrange) if isinstance(ndrange, (tuple, list)) else (int(ndrange),)
 
 
-# What the buffer arguments of the 8-bit and expert-grouped kernels hold, a letter each:
-# f Float32, h bfloat16 (or its bits), i Int32, o f or h as the kernel's type argument
-# says, p and q 8-bit codes in the formats that its first and second format argument
-# say; behind them those arguments' indexes. The library sees addresses and byte counts
+# What the buffer arguments of the 8-bit and expert-grouped kernels, and of those around
+# them, hold, a letter each: f Float32, h bfloat16 (or its bits), i Int32, o and t f or h as
+# the kernel's first and second type argument say, p and q 8-bit codes in the formats that
+# its first and second format argument say; behind them those arguments' indexes. The library sees addresses and byte counts
 # only, so what a tensor or buffer says of itself is checked here.
 _OPERANDS = {
     "quantize_fp8": ("pfpfoi", {"o": 10, "p": 11}),
@@ -608,6 +608,12 @@ _OPERANDS = {
     "gemm_grouped_bf16": ("ohhi", {"o": 7}),
     "gemm_grouped_dx_bf16": ("ohhi", {"o": 7}),
     "gemm_grouped_dw_bf16": ("ohhi", {"o": 7}),
+    "rms_norm": ("opfooot", {"o": 8, "t": 9, "p": 10}),
+    "rms_norm_grad": ("ofooto", {"o": 7, "t": 8}),
+    "route_experts": ("ifiiiofi", {"o": 15}),
+    "route_experts_grad": ("ofoi", {"o": 8}),
+    "combine_experts": ("tofit", {"o": 8, "t": 9}),
+    "combine_experts_grad": ("oftofii", {"o": 10, "t": 11}),
 }
 # What an element type can stand for; 4 and 5 are codes in e4m3 and e5m2, which plain bytes
 # may be either of, and * is what no test follows for.
@@ -629,12 +635,12 @@ def _with_torch() -> None:
 
 
 def _wanted(k: Kernel, args: Sequence) -> str:
-    """_OPERANDS' letters of a kernel with o, p and q resolved by the call's type and
+    """_OPERANDS' letters of a kernel with o, t, p and q resolved by the call's type and
     format arguments, kept for calls of the same; * for one that the library refuses."""
     kinds, flags = _OPERANDS[k.name]
     for letter, i in flags.items():
         valid = isinstance(args[i], (int, np.integer)) and args[i] in (0, 1)
-        kinds = kinds.replace(letter, ("fh" if letter == "o" else "45")[int(args[i])] if valid else "*")
+        kinds = kinds.replace(letter, ("fh" if letter in "ot" else "45")[int(args[i])] if valid else "*")
     if "*" not in kinds:
         k.wanted[k.flags(args)] = kinds
     return kinds
@@ -685,6 +691,19 @@ def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
     return flat
 
 
+def _scratch(k: Kernel, x) -> tuple[int, int]:
+    """Address and bytes of a launch's scratch, with an operand's checks but for the type."""
+    if isinstance(x, DevicePtr):
+        return x.ptr, x.nbytes
+    on, ordered = (x.get_device(), x.is_contiguous()) if _tensor is not None and isinstance(x, _tensor) else (
+        x.dev.ordinal if isinstance(x, Buffer) else None, True)
+    if on is None:
+        raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: cannot pass {x!r} as scratch")
+    if not ordered or (_tensor is not None and on != (_current_device() if on >= 0 else 0)):
+        raise ArgumentError(L.ERR_ARGUMENT, f"{k.name}: the scratch must be contiguous and on the current device")
+    return (x.ptr, x.nbytes) if isinstance(x, Buffer) else (x.data_ptr(), x.nbytes)
+
+
 class _Packed:
     """How a kernel in _OPERANDS is launched: its argument array packed in one call
     (each argument is {int32 kind, int32 rid, 8-byte value, uint64 bytes}), and the
@@ -695,12 +714,12 @@ class _Packed:
 
     def __init__(self, k: Kernel):
         self.kernel, self.nargs = k, len(k.signature)
-        self.pack = struct.Struct("<" + "".join("iiQQ" if s in "Bb" else "iii4xQ" for s in k.signature)).pack
+        self.pack = struct.Struct("<" + "".join("iiQQ" if s in "Bb" else "iif4xQ" if s == "f" else "iii4xQ" for s in k.signature)).pack
         self.entry = lib()["mtl_launch"]
         self.entry.restype = C.c_int32
         self.entry.argtypes = [C.c_int32, C.c_char_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
         self.buffers = len(_OPERANDS[k.name][0])
-        self.scalars = [L.ARG_I32, 0, 0, 0] * (self.nargs - self.buffers)
+        self.scalars = [v for s in k.signature[self.buffers:] for v in (L.ARG_F32 if s == "f" else L.ARG_I32, 0, 0, 0)]
 
     def range_of(self, nd: tuple) -> bytes:
         try:
@@ -708,13 +727,13 @@ class _Packed:
         except struct.error as e:
             raise ArgumentError(L.ERR_ARGUMENT, f"{self.kernel.name}: no ndrange: {nd} ({e})") from None
 
-    def __call__(self, args: Sequence, ndrange, stream: int) -> None:
+    def __call__(self, args: Sequence, ndrange, stream: int, workspace=None) -> None:
         buffers, scalars = _operands(self.kernel, args), self.scalars.copy()
         scalars[2::4] = args[self.buffers:]
         try:
             packed = self.pack(*buffers, *scalars)
-        except struct.error as e:
-            raise ArgumentError(L.ERR_ARGUMENT, f"{self.kernel.name}: a scalar argument is no Int32 ({e})") from None
+        except (struct.error, OverflowError) as e:
+            raise ArgumentError(L.ERR_ARGUMENT, f"{self.kernel.name}: a scalar argument is no Int32 or no Float32 ({e})") from None
         if type(ndrange) is int:
             n = 1
             range_ = self.ndranges.get(ndrange)
@@ -725,7 +744,8 @@ class _Packed:
         else:
             nd = _nd(ndrange)
             n, range_ = len(nd), self.range_of(nd)
-        status = self.entry(self.kernel.id, packed, self.nargs, range_, n, None, 0, stream)
+        scratch, size = (None, 0) if workspace is None else _scratch(self.kernel, workspace)
+        status = self.entry(self.kernel.id, packed, self.nargs, range_, n, scratch, size, stream)
         if status:
             check(status)
 
@@ -750,10 +770,11 @@ def dispatch(p: PassHandle, kernel, args: Sequence, ndrange, group=None) -> None
 
 def launch(kernel, args: Sequence, ndrange, stream: int = 0, workspace=None) -> None:
     """Launch a built-in kernel outside any graph on `stream` (pointer args:
-    Buffers, torch tensors or DevicePtr)."""
+    Buffers, torch tensors or DevicePtr). `workspace`: the scratch that
+    workspace_bytes asks for, not shared by launches that may run at once."""
     k = kernel if isinstance(kernel, Kernel) else _kernel(kernel)
     if k.packed is not None:
-        return k.packed(args, ndrange, stream)
+        return k.packed(args, ndrange, stream, workspace)
     arr = (L.Arg * max(len(args), 1))(*[_arg(None, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
     nda = (C.c_int64 * 3)(*nd, *([1] * (3 - len(nd))))

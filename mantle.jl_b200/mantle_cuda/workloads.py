@@ -348,6 +348,24 @@ def route_to_experts(tokens: int, experts: int, top: int, seed: int):
     return (order // top).astype(np.int32), offsets
 
 
+def _experts_in_8_bits(dev, experts: int, width: int, hidden: int, gen):
+    """Both layers' weights drawn by `gen` and quantized in 128 x 128 blocks: name ->
+    (codes, scales) Buffers, and name -> the tensor before."""
+    import torch
+    device = f"cuda:{dev.ordinal}"
+    tensors, weights = {}, {}
+    for name, n, k in (("up", hidden, width), ("down", width, hidden)):
+        w = torch.randn((experts, n, k), generator=gen, device=device) / float(np.sqrt(k))
+        src = Buffer.wrap(dev, w, dtype=np.float32)
+        codes = Buffer(dev, np.uint8, experts * n * rows_of_codes(k))
+        scales = Buffer(dev, np.float32, experts * -(-n // 128) * -(-k // 128))
+        with torch.cuda.device(device):
+            launch(kernels.quantize_fp8, (codes, scales, None, None, src, None, n, k, n, 128, 0, 0, 0), experts, stream=dev.stream)
+        dev.synchronize()
+        weights[name], tensors[name] = (codes, scales), w
+    return weights, tensors
+
+
 def build_experts(dev, tokens: int = 4096, experts: int = 16, top: int = 2, width: int = 2048, hidden: int = 4096,
                   seed: int = 12, **plan_kw) -> ExpertsWorkload:
     """Two layers of experts in 8 bits as one graph: the tokens' rows gathered into
@@ -363,16 +381,8 @@ def build_experts(dev, tokens: int = 4096, experts: int = 16, top: int = 2, widt
     rows_of, offsets = route_to_experts(tokens, experts, top, seed)
     T = tokens * top
     x_t = torch.randn((tokens, width), generator=gen, device=device).to(torch.bfloat16)
-    tensors, weights = {"x": x_t}, {}
-    for name, n, k in (("up", hidden, width), ("down", width, hidden)):
-        w = torch.randn((experts, n, k), generator=gen, device=device) / float(np.sqrt(k))
-        src = Buffer.wrap(dev, w, dtype=np.float32)
-        codes = Buffer(dev, np.uint8, experts * n * rows_of_codes(k))
-        scales = Buffer(dev, np.float32, experts * -(-n // 128) * -(-k // 128))
-        with torch.cuda.device(device):
-            launch(kernels.quantize_fp8, (codes, scales, None, None, src, None, n, k, n, 128, 0, 0, 0), experts, stream=dev.stream)
-        dev.synchronize()
-        weights[name], tensors[name] = (codes, scales), w
+    weights, tensors = _experts_in_8_bits(dev, experts, width, hidden, gen)
+    tensors["x"] = x_t
     x = Buffer.wrap(dev, x_t, dtype=np.uint16)
     rows, off = Buffer(dev, rows_of), Buffer(dev, offsets)
     y = Buffer(dev, np.uint16, T * width)
@@ -395,6 +405,82 @@ def build_experts(dev, tokens: int = 4096, experts: int = 16, top: int = 2, widt
         experts))
     plan = Plan(g, **plan_kw)
     return ExpertsWorkload(tokens, experts, top, width, hidden, x, y, rows_of, offsets, weights, g, plan, tensors)
+
+
+@dataclass
+class MoeWorkload:
+    tokens: int
+    experts: int
+    top: int
+    width: int
+    hidden: int
+    x: Buffer
+    y: Buffer
+    ids: Buffer           # (tokens * top,) the experts of each token
+    routes: Buffer        # (tokens * top,) their weights
+    offsets: Buffer       # (experts + 1,) the rows of each expert
+    rows_of: Buffer       # (tokens * top,) the token of each row
+    row_at: Buffer        # (tokens * top,) the row of each token's experts
+    weights: dict         # name -> (codes, scales) Buffers
+    graph: Graph
+    plan: Plan
+    tensors: dict
+
+    @property
+    def flops_step(self) -> int:
+        return 4 * self.tokens * self.top * self.width * self.hidden + 2 * self.tokens * self.width * self.experts
+
+
+def build_moe(dev, tokens: int = 4096, experts: int = 16, top: int = 2, width: int = 2048, hidden: int = 4096,
+              seed: int = 13, eps: float = 1e-6, **plan_kw) -> MoeWorkload:
+    """A whole mixture-of-experts layer as one graph, routed on the device: the tokens
+    normalised, their logits against the router's weights, the choice of `top` experts
+    and the rows' order, the two layers of experts of build_experts, and the rows back
+    to their tokens, weighted, on top of x. `experts` is a multiple of 8 (the router's
+    product). Inputs are drawn on the device by torch's generator (seed)."""
+    import torch
+    device = f"cuda:{dev.ordinal}"
+    gen = torch.Generator(device=device)
+    gen.manual_seed(seed)
+    T = tokens * top
+    x_t = torch.randn((tokens, width), generator=gen, device=device).to(torch.bfloat16)
+    scale_t = 1 + 0.1 * torch.randn(width, generator=gen, device=device)
+    router_t = (torch.randn((width, experts), generator=gen, device=device) / float(np.sqrt(width))).to(torch.bfloat16)
+    weights, tensors = _experts_in_8_bits(dev, experts, width, hidden, gen)
+    tensors.update(x=x_t, scale=scale_t, router=router_t)
+    x, router = Buffer.wrap(dev, x_t, dtype=np.uint16), Buffer.wrap(dev, router_t, dtype=np.uint16)
+    scale = Buffer.wrap(dev, scale_t, dtype=np.float32)
+    ids, rows_of, row_at = (Buffer(dev, np.int32, T) for _ in range(3))
+    routes, offsets = Buffer(dev, np.float32, T), Buffer(dev, np.int32, experts + 1)
+    y = Buffer(dev, np.uint16, tokens * width)
+    g = Graph(dev)
+    R = lambda p, b: use(p, b, read=True)  # noqa: E731
+    W = lambda p, b: use(p, b, write=True)  # noqa: E731
+    codes_of = lambda n: (Transient.Buffer(g, np.uint8, T * rows_of_codes(n)), Transient.Buffer(g, np.float32, T * -(-n // 128)))  # noqa: E731
+    normed, logits = Transient.Buffer(g, np.uint16, tokens * width), Transient.Buffer(g, np.float32, tokens * experts)
+    q1, s1 = codes_of(width)
+    h, rows = Transient.Buffer(g, np.uint16, T * hidden), Transient.Buffer(g, np.uint16, T * width)
+    q2, s2 = codes_of(hidden)
+    (up, up_s), (down, down_s) = weights["up"], weights["down"]
+    compute(g, "norm", lambda p: dispatch(p, kernels.rms_norm, (
+        W(p, normed), None, None, None, R(p, x), None, R(p, scale), width, 1, 0, 0, 0, eps), tokens))
+    compute(g, "logits", lambda p: dispatch(p, kernels.gemm_bf16, (
+        W(p, logits), R(p, normed), R(p, router), tokens, experts, width), 1))
+    compute(g, "route", lambda p: dispatch(p, kernels.route_experts, (
+        W(p, ids), W(p, routes), W(p, offsets), W(p, rows_of), W(p, row_at), R(p, logits), None, None,
+        experts, top, 1, 1, 1, 0, 1, 0, 1.0), tokens))
+    compute(g, "quantize x", lambda p: dispatch(p, kernels.quantize_fp8, (
+        W(p, q1), W(p, s1), None, None, R(p, normed), R(p, rows_of), T, width, tokens, 1, 1, 0, 0), 1))
+    compute(g, "up", lambda p: dispatch(p, kernels.gemm_grouped_fp8, (
+        W(p, h), R(p, q1), R(p, s1), R(p, up), R(p, up_s), R(p, offsets), T, hidden, width, 0, 0, 1), experts))
+    compute(g, "quantize h", lambda p: dispatch(p, kernels.quantize_fp8, (
+        W(p, q2), W(p, s2), None, None, R(p, h), None, T, hidden, T, 1, 1, 0, 0), 1))
+    compute(g, "down", lambda p: dispatch(p, kernels.gemm_grouped_fp8, (
+        W(p, rows), R(p, q2), R(p, s2), R(p, down), R(p, down_s), R(p, offsets), T, width, hidden, 0, 0, 1), experts))
+    compute(g, "combine", lambda p: dispatch(p, kernels.combine_experts, (
+        W(p, y), R(p, rows), R(p, routes), R(p, row_at), R(p, x), T, width, top, 1, 1), tokens))
+    plan = Plan(g, **plan_kw)
+    return MoeWorkload(tokens, experts, top, width, hidden, x, y, ids, routes, offsets, rows_of, row_at, weights, g, plan, tensors)
 
 
 # ── CNN inference ───────────────────────────────────────────────────────────

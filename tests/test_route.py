@@ -1,0 +1,408 @@
+"""Routing to experts against a plain restatement in 64 bits: the choice and the rows'
+order exactly, weights and gradients within the roundings of 32 bits.
+
+u = 2^-24, D the largest difference of two logits of a token. exp of a difference is off by
+2 units of its result (2 u each) and by u D from the rounded difference; a sum of positive
+terms adds u for each of at most 37 additions, a quotient and the scale u each. A score is
+thus off by (D + 4 + D + 4 + 37 + 3) u of itself at most, one over the chosen's sum by
+less: (2 D + 64) u covers both, and so it does sigmoid's score (D replaced by |l|, whose
+exp has no difference to round).
+
+The gradient's factors are such scores, and 1 - s likewise; with e = (2 D + 64) u, and
+S = |g| + sum |g| u, its terms are off by 4 e of c u S at most.
+"""
+import numpy as np
+import pytest
+import torch
+
+import mantle_cuda as M
+
+u = 2.0 ** -24
+F, H = torch.float32, torch.bfloat16
+SOFTMAX, SIGMOID = 0, 1
+ptr = lambda n, at=1 << 20: M.DevicePtr(at, n)  # noqa: E731
+BIG = ptr(1 << 40)
+
+
+# ── the restatement ──────────────────────────────────────────────────────────
+def scores(l, score):
+    l = l.astype(np.float64)
+    with np.errstate(all="ignore"):
+        if score == SIGMOID:
+            return 1 / (1 + np.exp(-l))
+        m = l.max()
+        if m == -np.inf:
+            return np.zeros_like(l)
+        p = np.exp(l - m)
+        return p / p.sum()
+
+
+def choose(l, top, score, bias=None, groups=1, top_groups=1, best=1):
+    """The chosen experts of one token's logits, or None for a token that is not a number."""
+    if np.isnan(l).any() or (bias is not None and np.isnan(bias).any()) or (score == SOFTMAX and l.max() == np.inf):
+        return None
+    s = scores(l, score)
+    key = l.astype(np.float64) if bias is None else s + bias.astype(np.float64)
+    for_groups = s if bias is None else key
+    key, for_groups = (np.where(l == -np.inf, -np.inf, v) for v in (key, for_groups))
+    E = len(l)
+    if groups > 1:
+        per = E // groups
+        if bias is None and best == 1:
+            for_groups = key
+        value = np.array([sum(x for i, x in enumerate(sorted(for_groups[g * per:(g + 1) * per], reverse=True)[:best]) if i == 0 or x > -np.inf)
+                          for g in range(groups)])
+        keep = sorted(range(groups), key=lambda g: (-value[g], g))[:top_groups]
+        key = np.array([key[e] if e // per in keep else -np.inf for e in range(E)])
+    order = sorted(range(E), key=lambda e: (-key[e], e))[:top]
+    return [e for e in order if key[e] > -np.inf]
+
+
+def routed(logits, top, score, renorm, scale=1.0, bias=None, live=None, **groups):
+    """ids (T, top) and weights (T, top) in 64 bits."""
+    T = len(logits)
+    ids, w = np.full((T, top), -1), np.zeros((T, top))
+    for t in range(T):
+        if live is not None and not live[t]:
+            continue
+        c = choose(logits[t], top, score, bias, **groups)
+        if c is None:
+            w[t] = np.nan
+            continue
+        if not c:
+            continue
+        ids[t, :len(c)] = c
+        l = logits[t].astype(np.float64)
+        if renorm:  # relative to the largest, so that no sum underflows
+            if score == SOFTMAX:
+                x = np.exp(l[c] - l[c].max())
+            else:
+                x = np.exp(np.minimum(l[c], 0) - min(l[c].max(), 0)) / (1 + np.exp(-np.abs(l[c])))
+            w[t, :len(c)] = x / x.sum() * scale
+        else:
+            w[t, :len(c)] = scores(l, score)[c] * scale
+    return ids, w
+
+
+def ordered(ids, E):
+    """offsets, rows_of, row_at of the chosen slots by expert, then slot."""
+    T, top = ids.shape
+    flat = ids.reshape(-1)
+    rows = [s for e in range(E) for s in np.flatnonzero(flat == e)]
+    offsets = np.concatenate([[0], np.cumsum(np.bincount(flat[flat >= 0], minlength=E))])
+    rows_of, row_at = np.full(T * top, -1), np.full(T * top, -1)
+    rows_of[:len(rows)] = np.array(rows, dtype=int) // top
+    row_at[rows] = np.arange(len(rows))
+    return offsets, rows_of, row_at
+
+
+def test_the_restatement():
+    l = np.array([[1.0, 3.0, 3.0, -np.inf, 2.0, 0.0]], np.float32)
+    assert routed(l, 3, SOFTMAX, True)[0].tolist() == [[1, 2, 4]]
+    assert routed(l, 6, SOFTMAX, False)[0].tolist() == [[1, 2, 4, 0, 5, -1]]
+    assert routed(l, 2, SIGMOID, True, bias=np.array([1, 0, 0, 9, 0, 0.9]))[0].tolist() == [[0, 5]]
+    assert routed(l, 2, SIGMOID, True, groups=3, top_groups=1)[0].tolist() == [[1, 0]]  # groups 0 and 1 tie
+    assert ordered(np.array([[1, 0], [-1, 1]]), 3)[1].tolist() == [0, 0, 1, -1]
+
+
+# ── refusals (no launch) ─────────────────────────────────────────────────────
+def r_args(t=4, E=8, top=2, groups=1, top_groups=1, best=1, score=0, renorm=0, kind=0, scale=1.0, **change):
+    n = 4 * t * top
+    a = dict(ids=ptr(n), w=ptr(n), off=ptr(4 * (E + 1)), rows=ptr(n), at=ptr(n), l=ptr(t * E * (2 if kind == 1 else 4)), bias=None, live=None)
+    a.update(change)
+    return [*a.values(), E, top, groups, top_groups, best, score, renorm, kind, scale]
+
+
+@pytest.mark.parametrize("args,nd,match", [
+    (r_args(ids=ptr(31)), 4, "ids"), (r_args(w=ptr(31)), 4, "the weights"), (r_args(off=ptr(35)), 4, "offsets"),
+    (r_args(rows=ptr(31)), 4, "rows_of"), (r_args(at=ptr(31)), 4, "row_at"), (r_args(l=ptr(127)), 4, "the logits"),
+    (r_args(kind=1, l=ptr(63)), 4, "the logits"), (r_args(bias=ptr(31)), 4, "the bias"), (r_args(live=ptr(15)), 4, "live"),
+    (r_args(), 5, "ids"), (r_args(off=None), 4, "go together"), (r_args(rows=None), 4, "go together"), (r_args(at=None), 4, "go together"),
+    (r_args(top=0), 4, "top must be"), (r_args(top=9), 4, "top must be"), (r_args(E=64, top=33), 4, "top must be"),
+    (r_args(E=0), 4, "no experts"), (r_args(E=1025), 4, "more than 1024 experts"),
+    (r_args(groups=3), 4, "divide the experts"), (r_args(groups=0), 4, "divide the experts"), (r_args(groups=16), 4, "divide the experts"),
+    (r_args(groups=4, top_groups=5), 4, "top_groups"), (r_args(groups=4, top_groups=0), 4, "top_groups"),
+    (r_args(groups=4, best=3), 4, "best two"), (r_args(groups=8, best=2), 4, "best two"), (r_args(best=0), 4, "best two"),
+    (r_args(score=2), 4, "must be 0 or 1"), (r_args(renorm=-1), 4, "must be 0 or 1"), (r_args(kind=2), 4, "must be 0 or 1"),
+    (r_args(scale=float("nan")), 4, "finite"), (r_args(scale=float("inf")), 4, "finite"),
+    (r_args(ids=BIG, w=BIG, rows=BIG, at=BIG, l=BIG), 1 << 30, "slots"), (r_args(), (4, 1), "one-dimensional"),
+    (r_args(l=ptr(1 << 20, (1 << 20) + 2)), 4, "4-byte aligned"), (r_args(bias=ptr(0, 0)), 4, "the bias must be a device buffer"),
+    (r_args(live=ptr(0, 0)), 4, "live must be a device buffer"), (r_args(ids=ptr(0, 0)), 4, "ids must be a device buffer"),
+])
+def test_route_refuses(args, nd, match):
+    with pytest.raises(M.MantleError, match=match):
+        M.launch(M.kernels.route_experts, args, nd)
+
+
+def d_args(t=4, E=8, top=2, score=0, renorm=0, kind=0, scale=1.0, **change):
+    per = 2 if kind == 1 else 4
+    a = dict(dl=ptr(t * E * per), dw=ptr(4 * t * top), l=ptr(t * E * per), ids=ptr(4 * t * top))
+    a.update(change)
+    return [*a.values(), E, top, score, renorm, kind, scale]
+
+
+@pytest.mark.parametrize("args,nd,match", [
+    (d_args(dl=ptr(127)), 4, "dlogits"), (d_args(dw=ptr(31)), 4, "the weights' gradient"), (d_args(l=ptr(127)), 4, "the logits"),
+    (d_args(ids=ptr(31)), 4, "ids"), (d_args(), 5, "dlogits"), (d_args(top=9), 4, "top must be"), (d_args(score=3), 4, "must be 0 or 1"),
+    (d_args(renorm=3), 4, "must be 0 or 1"), (d_args(kind=3), 4, "must be 0 or 1"), (d_args(scale=float("inf")), 4, "finite"),
+    (d_args(E=2000), 4, "more than 1024"), (d_args(ids=ptr(0, 0)), 4, "ids must be a device buffer"),
+])
+def test_route_grad_refuses(args, nd, match):
+    with pytest.raises(M.MantleError, match=match):
+        M.launch(M.kernels.route_experts_grad, args, nd)
+
+
+# ── on the device ────────────────────────────────────────────────────────────
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def route(logits, top, score, renorm, scale=1.0, bias=None, live=None, groups=1, top_groups=1, best=1, order=True):
+    T, E = logits.shape
+    i = lambda n: torch.full((n,), -7, dtype=torch.int32, device="cuda")  # noqa: E731
+    ids, w = i(T * top), torch.full((T * top,), -7.0, device="cuda")
+    rest = (i(E + 1), i(T * top), i(T * top)) if order else (None, None, None)
+    args = (ids, w, *rest, logits, bias, live, E, top, groups, top_groups, best, score, renorm, int(logits.dtype == H), scale)
+    need = M.workspace_bytes(M.kernels.route_experts, args, T)
+    M.launch(M.kernels.route_experts, args, T, stream=stream(), workspace=torch.empty(need, dtype=torch.uint8, device="cuda") if need else None)
+    torch.cuda.synchronize()
+    return ids.view(T, top), w.view(T, top), rest
+
+
+def check(logits, top, score, renorm, scale=1.0, bias=None, live=None, **groups):
+    ids, w, rest = route(logits.cuda(), top, score, renorm, scale, None if bias is None else bias.cuda(), None if live is None else live.cuda(), **groups)
+    l = logits.float().numpy()
+    want, weights = routed(l, top, score, renorm, scale, None if bias is None else bias.numpy(), None if live is None else live.numpy(), **groups)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    got = w.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(weights))
+    fine = ~np.isnan(weights)
+    with np.errstate(invalid="ignore"):
+        finite = np.where(np.isfinite(l), l, 0).astype(np.float64)
+        D = (finite.max(1) - finite.min(1) + np.abs(finite).max(1))[:, None] * np.ones((1, top))
+    assert (np.abs(got - weights)[fine] <= ((2 * D + 64) * u * np.abs(weights) + 1e-44)[fine]).all()
+    for a, b in zip(rest, ordered(want, logits.shape[1])):
+        assert np.array_equal(a.cpu().numpy(), b)
+    alone = route(logits.cuda(), top, score, renorm, scale, None if bias is None else bias.cuda(), None if live is None else live.cuda(), order=False, **groups)
+    assert torch.equal(alone[0], ids) and torch.equal(alone[1].nan_to_num(9), w.nan_to_num(9))
+
+
+def normal(*shape, seed=0, kind=F):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(kind)
+
+
+SHAPES = [(1, 1, 1), (1, 8, 2), (5, 7, 3), (33, 32, 4), (70, 64, 6), (3, 100, 32), (31, 160, 6), (257, 256, 8), (9, 384, 8), (12, 1000, 5), (4, 1024, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("t,e,top", SHAPES)
+def test_route(dev, t, e, top, score, renorm, kind):
+    l = 2 * normal(t, e, seed=t, kind=kind)  # in bfloat16 many logits are equal
+    check(l, top, score, renorm)
+    check(l, top, score, renorm, 2.5, bias=0.1 * normal(e, seed=3))
+    check(l, top, score, renorm, bias=torch.zeros(e))
+    check(l, top, score, renorm, -0.5, live=(torch.arange(t) % 3 != 1).to(torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("t,e,top,groups,top_groups,best", [
+    (40, 256, 8, 8, 4, 2), (40, 64, 6, 8, 3, 1), (33, 160, 6, 8, 3, 1), (20, 96, 4, 6, 2, 2), (7, 16, 2, 16, 4, 1), (9, 1024, 8, 32, 5, 2),
+    (5, 1024, 8, 1024, 9, 1), (5, 1000, 8, 200, 3, 2), (6, 8, 8, 4, 2, 2), (50, 256, 8, 4, 4, 2)])
+def test_route_in_groups(dev, t, e, top, groups, top_groups, best, score, kind):
+    g = dict(groups=groups, top_groups=top_groups, best=best)
+    l = 2 * normal(t, e, seed=e, kind=kind)
+    check(l, top, score, 1, **g)
+    check(l, top, score, 0, 2.5, bias=0.1 * normal(e, seed=3), **g)
+    l[::2, : e // groups] = float("-inf")  # a whole group masked
+    l[1::2, ::2] = float("-inf")
+    check(l, top, score, 1, bias=0.1 * normal(e, seed=4), **g)
+    check(l, top, score, 1, **g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("bias", [False, True])
+def test_masks_and_values_that_are_not_numbers(dev, score, bias):
+    inf, nan = float("inf"), float("nan")
+    l = normal(12, 40)
+    l[0] = -inf                      # nothing left
+    l[1, 3:] = -inf                  # fewer than asked for
+    l[2, 7] = nan
+    l[3] = nan
+    l[4, 9] = inf                    # first under sigmoid, no number under softmax
+    l[5] = -3.0e38                   # the type's lowest values
+    l[6] = torch.where(torch.arange(40) % 2 == 0, -3.4e38, -inf)
+    l[7] = 0
+    l[8, :20], l[8, 20:] = 3.4e38, -3.4e38
+    l[9] = -200.0                    # scores that are zeros in 32 bits
+    l[9, 5] = -199.0
+    l[10, 0], l[10, 1] = 0.0, -0.0
+    b = None if not bias else 0.01 * normal(40, seed=2)
+    for renorm in (0, 1):
+        check(l, 6, score, renorm, bias=b)
+        check(l, 6, score, renorm, bias=b, groups=5, top_groups=2, best=2)
+        if bias:
+            b2 = b.clone()
+            b2[:36] = -inf
+            check(l[[5, 7, 10, 11]], 6, score, renorm, bias=b2)
+            b2[0] = nan
+            check(l[[5, 7, 10, 11]], 6, score, renorm, bias=b2)
+    # dead tokens count for nothing, whatever they hold
+    check(l, 6, score, 1, bias=b, live=torch.zeros(12, dtype=torch.int32))
+
+
+@pytest.mark.gpu
+def test_keys_that_32_bits_do_not_tell_apart(dev):
+    # scores plus biases that are equal or next to one another in 32 bits, and not in 64
+    E, T = 64, 40
+    l = normal(1, E, seed=1).expand(T, E).clone()
+    s = torch.sigmoid(l[0].double())
+    b = (0.75 - s).float()  # every key 0.75 but for the bias's own rounding, 2^-25 at most
+    for t in range(T):
+        l[t, t] += 2e-7
+    check(l, 8, SIGMOID, 1, bias=b)
+    check(l, 8, SIGMOID, 1, bias=b, groups=8, top_groups=3, best=2)
+    p = torch.softmax(l[0].double(), 0)
+    check(l, 8, SOFTMAX, 0, bias=(0.03 - p).float())
+    check(l, 8, SOFTMAX, 0, bias=(0.03 - p).float(), groups=4, top_groups=2, best=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,top", [(0, 8, 2), (1, 1, 1), (3000, 8, 2), (2049, 16, 8), (1500, 300, 32), (9000, 1024, 2), (40000, 256, 8), (70000, 3, 1)])
+def test_rows_in_order(dev, t, e, top):
+    # slots in order within an expert, experts of very different sizes, some empty, and dead tokens between
+    l = normal(t, e, seed=t) + torch.linspace(0, 4, e)
+    live = (normal(t, seed=5) < 1).to(torch.int32)
+    ids, w, rest = route(l.cuda(), top, SOFTMAX, 1, live=live.cuda())
+    ids = ids.cpu().numpy()
+    assert ((ids >= 0).all(1) == (live.numpy() != 0)).all() and (ids < e).all()
+    for a, b in zip(rest, ordered(ids, e)):
+        assert np.array_equal(a.cpu().numpy(), b)
+
+
+def grad(logits, ids, g, score, renorm, scale):
+    T, E = logits.shape
+    dl = torch.full_like(logits, float("nan"))
+    M.launch(M.kernels.route_experts_grad, (dl, g, logits, ids, E, ids.shape[1], score, renorm, int(logits.dtype == H), scale), T, stream=stream())
+    torch.cuda.synchronize()
+    return dl
+
+
+def exact_grad(l, ids, g, score, renorm, scale):
+    """(gradient, the magnitudes that its roundings go by) in 64 bits, of torch tensors."""
+    l, g = l.double(), g.double()
+    valid = ids >= 0
+    at, g = ids.clamp(min=0).long(), torch.where(valid, g, 0.0)
+    s = torch.softmax(l, 1).nan_to_num() if score == SOFTMAX else torch.sigmoid(l)
+    c = torch.where(valid, s.gather(1, at), 0.0)
+    if renorm:
+        c = c / c.sum(1, keepdim=True).clamp(min=1e-300)
+    mean = (g * c).sum(1, keepdim=True) if renorm or score == SOFTMAX else torch.zeros(len(l), 1, dtype=torch.float64)
+    most = (g.abs() * c).sum(1, keepdim=True)
+    d, m = c * (g - mean), c * (g.abs() + most)
+    if score == SIGMOID:
+        rest = torch.sigmoid(-l).gather(1, at)
+        d, m = d * rest, m * rest
+    out, mag = torch.zeros_like(l), torch.zeros_like(l)
+    if score == SOFTMAX and not renorm:
+        out, mag = -s * mean, s * most
+        d = c * g
+    return scale * out.scatter_add(1, at, torch.where(valid, d, 0.0)), abs(scale) * mag.scatter_add(1, at, torch.where(valid, m, 0.0))
+
+
+def check_grad(l, ids, g, score, renorm, scale):
+    dl = grad(l.cuda(), ids.cuda(), g.cuda(), score, renorm, scale).double().cpu()
+    want, mag = exact_grad(l, ids, g, score, renorm, scale)
+    finite = torch.where(l.double().isfinite(), l.double(), 0.0)
+    D = (finite.amax(1) - finite.amin(1) + finite.abs().amax(1))[:, None]
+    tol = 4 * (2 * D + 64) * u * mag + 1e-40
+    assert ((dl - want).abs() <= tol + (2.0 ** -8 if l.dtype == H else u) * (want.abs() + tol)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("t,e,top", SHAPES)
+def test_route_grad(dev, t, e, top, score, renorm, kind):
+    l, g = 2 * normal(t, e, seed=t, kind=kind), normal(t, top, seed=9)
+    ids = l.float().argsort(1, descending=True)[:, :top].to(torch.int32)
+    check_grad(l, ids, g, score, renorm, 1.0)
+    ids[::2, top // 2:] = -1
+    check_grad(l, ids, g, score, renorm, -2.5)
+    if e > 1:
+        l[1::2, 0] = float("-inf")
+        ids = torch.where(l.gather(1, ids.clamp(min=0).long()) == float("-inf"), -1, ids)
+        check_grad(l, ids.to(torch.int32), g, score, renorm, 1.0)
+    check_grad(l, torch.full_like(ids, -1), g, score, renorm, 1.0)
+    same = torch.zeros_like(ids) + e - 1  # one expert in every slot: the slots' gradients together
+    check_grad(l, same.to(torch.int32), g, score, renorm, 1.0)
+    outside = torch.full((t, top), e, dtype=torch.int32)
+    assert torch.equal(grad(l.cuda(), outside.cuda(), g.cuda(), score, renorm, 1.0), torch.zeros_like(l).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+def test_route_grad_against_differences(dev, score, renorm):
+    # 64-bit central differences of sum(g w) with a step of 1e-5, at ids held still
+    l, g, e = normal(2, 12, seed=1), normal(2, 4, seed=2), 1e-5
+    ids = l.argsort(1, descending=True)[:, :4]
+
+    def loss(x):
+        s = torch.softmax(x, 1) if score == SOFTMAX else torch.sigmoid(x)
+        w = s.gather(1, ids)
+        return (g.double() * (w / w.sum(1, keepdim=True) if renorm else w)).sum().item() * 1.5
+
+    dl = grad(l.cuda(), ids.to(torch.int32).cuda(), g.cuda(), score, renorm, 1.5)
+    for t in range(2):
+        for i in range(12):
+            step = torch.zeros(2, 12, dtype=torch.float64)
+            step[t, i] = e
+            assert abs((loss(l.double() + step) - loss(l.double() - step)) / (2 * e) - dl[t, i].item()) < 1e-5
+
+
+@pytest.mark.gpu
+def test_types_are_refused(dev):
+    l = normal(4, 8).cuda()
+    ids, w = torch.empty((4, 2), dtype=torch.int32, device="cuda"), torch.empty((4, 2), device="cuda")
+    go = lambda i, ww, ll, kind=0, bias=None, live=None: M.launch(M.kernels.route_experts, (  # noqa: E731
+        i, ww, None, None, None, ll, bias, live, 8, 2, 1, 1, 1, 0, 0, kind, 1.0), 4, stream=stream())
+    go(ids, w, l)
+    for args, match in (((ids.long(), w, l), "expected Int32"), ((ids, w.to(H), l), "expected Float32"), ((ids, w, l.to(H)), "expected Float32"),
+                        ((ids, w, l, 1), "expected bfloat16"), ((ids, w, l, 0, l[0].to(H).contiguous()), "expected Float32"),
+                        ((ids, w, l, 0, None, torch.ones(4, dtype=torch.bool, device="cuda")), "expected Int32"),
+                        ((ids, w, l.t().contiguous().t()), "contiguous")):
+        with pytest.raises(M.ArgumentError, match=match):
+            go(*args)
+
+
+@pytest.mark.gpu
+def test_captured_and_at_once(dev):
+    l = normal(3000, 64).cuda()
+    want = route(l, 4, SOFTMAX, 1)
+    fresh = lambda: (torch.zeros(12000, dtype=torch.int32, device="cuda"), torch.zeros(12000, device="cuda"),  # noqa: E731
+                     *(torch.zeros(n, dtype=torch.int32, device="cuda") for n in (65, 12000, 12000)))
+    args = lambda o: (*o, l, None, None, 64, 4, 1, 1, 1, 0, 1, 0, 1.0)  # noqa: E731
+    need = M.workspace_bytes(M.kernels.route_experts, args(fresh()), 3000)
+    scratch = lambda: torch.empty(need, dtype=torch.uint8, device="cuda") if need else None  # noqa: E731
+    outs, graphs, sides, kept = [fresh(), fresh()], [], [torch.cuda.Stream() for _ in range(2)], [scratch(), scratch()]
+    torch.cuda.synchronize()
+    for o, side, ws in zip(outs, sides, kept):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            M.launch(M.kernels.route_experts, args(o), 3000, stream=stream(), workspace=ws)
+        graphs.append(g)
+    for _ in range(3):
+        for g, side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o[0].view(3000, 4), want[0]) and torch.equal(o[1].view(3000, 4), want[1])
+        assert all(torch.equal(a, b) for a, b in zip(o[2:], want[2]))
