@@ -26,11 +26,19 @@
 
 #include "../mtl_internal.hpp"
 #include "rows.cuh"
+#include "tc_common.cuh"
 
 namespace mtl {
 
 // A row lies in the registers of one CTA, 32 values a thread at most.
 constexpr int kNormColumns = 32768;
+
+// The eights of columns that a row may touch: one more where its rows start off 16 bytes.
+static int eights_of(int C) { return (C + 7) / 8 + (C % 8 && C <= kNormColumns - 8 ? 1 : 0); }
+// Whether tensors whose rows start off 16 bytes are read in chunks all the same: `base` is
+// their phase. (Rows of a multiple of eight that start off 16 bytes, all of them, and the
+// longest rows, which the threads have no chunk more for, are read value by value.)
+static bool cut_in_chunks(int C, int base) { return C % 8 ? C <= kNormColumns - 8 : base == 0; }
 
 struct NormArgs {
   void* y;
@@ -69,21 +77,27 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// B threads a row: a warp each (several rows a CTA) up to 1024 columns, a CTA above.
+// B threads a row: a warp each (several rows a CTA) up to 1024 columns, a CTA above; N
+// eights a thread, which stay in registers between the sum and the outputs, so each value
+// is read once. Bound by HBM: 8192 x 4096 bf16 with the residual, h, y and codes (303 MB)
+// 49.5 us, 6.1 TB/s, 93 % of a plain copy's rate. Rows off 16 bytes are bound by the
+// instructions of going value by value: 5001 x 4013 float 33 us, 4.9 TB/s, 8192 x 4095 bf16
+// with the residual 77 us.
 template <typename T, int B, int N, bool VEC>
 __global__ void __launch_bounds__(B == 32 ? 128 : B) rms_norm_kernel(NormArgs a) {
   __shared__ float part[B == 32 ? 1 : B / 32];
-  __shared__ uint32_t blockmax[VEC ? 1 : B == 32 ? 4 * 2 * N : B * N / 16];
   const int tid = threadIdx.x;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (B == 32 && row >= a.R) return;
   const int C = a.C;
   const int64_t at = row * C;
   float v[N][8];
-  load_row<B, N, VEC>(v, static_cast<const T*>(a.x) + at, C, tid);
+#pragma unroll
+  for (int u = 0; u < N; ++u) load_part<B, VEC>(v[u], static_cast<const T*>(a.x) + at, C, tid, u);
   if (a.res) {
     float o[N][8];
-    load_row<B, N, VEC>(o, static_cast<const T*>(a.res) + at, C, tid);
+#pragma unroll
+    for (int u = 0; u < N; ++u) load_part<B, VEC>(o[u], static_cast<const T*>(a.res) + at, C, tid, u);
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -137,14 +151,19 @@ __global__ void __launch_bounds__(B == 32 ? 128 : B) rms_norm_kernel(NormArgs a)
       if (c < a.Cp) *reinterpret_cast<uint2*>(q + c) = c < C ? codes : make_uint2(0, 0);
     }
   } else {
-    // a block is four runs of 32 neighbouring columns, each one access of a warp
-    uint32_t* most = B == 32 ? blockmax + threadIdx.y * 2 * N : blockmax;
+    // A block is four runs of 32 neighbouring columns, each one access of a warp. Its scale is
+    // made once, and the inverse left where the maximum was.
     constexpr int kBlocks = B * N / 16;
+    __shared__ uint32_t blockmax[(B == 32 ? 4 : 1) * kBlocks];
+    uint32_t* most = blockmax + (B == 32 ? threadIdx.y * kBlocks : 0);
+    const auto meet = [] {
+      if constexpr (B == 32)
+        __syncwarp();
+      else
+        __syncthreads();
+    };
     for (int b = tid; b < kBlocks; b += B) most[b] = 0;
-    if constexpr (B == 32)
-      __syncwarp();
-    else
-      __syncthreads();
+    meet();
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -152,27 +171,40 @@ __global__ void __launch_bounds__(B == 32 ? 128 : B) rms_norm_kernel(NormArgs a)
         const uint32_t m = __reduce_max_sync(0xffffffffu, magnitude(v[u][i]));
         if ((tid & 31) == 0) atomicMax(most + ((u * 8 + i) * B + tid) / 128, m);
       }
-    if constexpr (B == 32)
-      __syncwarp();
-    else
-      __syncthreads();
+    meet();
+    for (int b = tid; b < a.cb; b += B) {
+      const Scale sc = a.e5m2 ? scale_of<true>(most[b], a.pow2) : scale_of<false>(most[b], a.pow2);
+      a.s[(int64_t)b * a.R + row] = sc.s;
+      most[b] = __float_as_uint(sc.r);
+    }
+    meet();
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = (u * 8 + i) * B + tid;
-        if (c >= a.Cp) continue;
-        const Scale sc = a.e5m2 ? scale_of<true>(most[c / 128], a.pow2) : scale_of<false>(most[c / 128], a.pow2);
-        if (c % 128 == 0 && c < C) a.s[(int64_t)(c / 128) * a.R + row] = sc.s;
-        const float x = v[u][i] * sc.r;
-        q[c] = c < C ? (uint8_t)(a.e5m2 ? codes4<true>(x, 0.0f, 0.0f, 0.0f) : codes4<false>(x, 0.0f, 0.0f, 0.0f)) : 0;
+        const float x = v[u][i] * __uint_as_float(most[c / 128]);
+        if (c < a.Cp) q[c] = c < C ? (uint8_t)(a.e5m2 ? codes4<true>(x, 0.0f, 0.0f, 0.0f) : codes4<false>(x, 0.0f, 0.0f, 0.0f)) : 0;
       }
   }
 }
 
 template <typename T, bool VEC>
-static void norm_launch(const NormArgs& a, cudaStream_t st) {
+static void norm_launch(const NormArgs& a, int sms, cudaStream_t st) {
   const unsigned rows = (unsigned)a.R, four = (unsigned)((a.R + 3) / 4);
+  // Few rows: one eight a thread, so that a row takes the least time (32 x 4096 with codes
+  // 3.7 -> 2.7 us, 400 x 4096 4.6 -> 4.1; 800 x 4096 6.1, and 7.5 this way).
+  if (a.R < 4 * (int64_t)sms && a.C > 256 && a.C <= 8192) {
+    if (a.C <= 1024)
+      rms_norm_kernel<T, 128, 1, VEC><<<rows, 128, 0, st>>>(a);
+    else if (a.C <= 2048)
+      rms_norm_kernel<T, 256, 1, VEC><<<rows, 256, 0, st>>>(a);
+    else if (a.C <= 4096)
+      rms_norm_kernel<T, 512, 1, VEC><<<rows, 512, 0, st>>>(a);
+    else
+      rms_norm_kernel<T, 1024, 1, VEC><<<rows, 1024, 0, st>>>(a);
+    return;
+  }
   if (a.C <= 256)
     rms_norm_kernel<T, 32, 1, VEC><<<four, dim3(32, 4), 0, st>>>(a);
   else if (a.C <= 512)
@@ -200,126 +232,243 @@ struct NormGradArgs {
   const void* w;
   const void* dres;
   int64_t R;
-  int C, wbf16;
+  int C, wbf16, stages, base, vec;  // base: the tensors' phase; vec: they have one
   float eps;
 };
 
+// The CTAs that an SM holds: the registers are dealt out for as many.
+constexpr int grad_residents(int most, int N) { return most == 32 ? (N == 4 ? 3 : N == 2 ? 5 : 8) : most == 128 ? 4 : most == 256 ? 2 : most == 384 ? 2 : 1; }
+
+// The sums of two values over the row's threads, in a fixed order. `part`: two slots a warp.
+template <bool WARP>
+__device__ __forceinline__ float2 row_sums(float x, float y, float* part) {
+  const int lane = threadIdx.x & 31;
+  // half the lanes go on with one value, half with the other
+  float keep = lane & 16 ? y : x;
+  keep += __shfl_xor_sync(0xffffffffu, lane & 16 ? x : y, 16);
+#pragma unroll
+  for (int d = 8; d; d >>= 1) keep += __shfl_xor_sync(0xffffffffu, keep, d);
+  if constexpr (WARP) {
+    return make_float2(__shfl_sync(0xffffffffu, keep, 0), __shfl_sync(0xffffffffu, keep, 16));
+  } else {
+    const int warps = blockDim.x >> 5;
+    if ((lane & 15) == 0) part[(threadIdx.x >> 5) * 2 + (lane >> 4)] = keep;
+    __syncthreads();
+    float2 sum = make_float2(0.0f, 0.0f);
+    const float2* p = reinterpret_cast<const float2*>(part);
+    if (warps <= 8) {
+      for (int w = 0; w < warps; ++w) sum.x += p[w].x, sum.y += p[w].y;
+    } else {
+      if (lane < warps) sum = p[lane];
+      sum = make_float2(warp_sum(sum.x), warp_sum(sum.y));
+    }
+    return sum;
+  }
+}
+
+// Bound by HBM, and by instruction issue behind that: 8192 x 4096 bf16 with dres (268 MB)
+// 51 us, 5.3 TB/s, 8192 x 2048 float 47 us, 5.7 TB/s. CTAs that load, add and write in
+// turn, value by value, took 95 us; with the ring and
+// two values an instruction (fma.rn.f32x2) 51. Three CTAs an SM instead of two leave 80
+// registers, and the spills take 60 us.
+//
 // CTAs stay and walk over the rows, so that a thread has the same columns in each and
-// keeps their sums of dw in registers.
-template <typename T, int B, int N, bool VEC>
-__global__ void __launch_bounds__(B == 32 ? 128 : B) rms_norm_grad_kernel(NormGradArgs a) {
-  __shared__ float part[2][2][B == 32 ? 1 : B / 32];
-  __shared__ float meet[B == 32 ? 4 * 256 * N : 1];
-  const int tid = threadIdx.x, C = a.C;
-  float dw[N][8];
+// keeps their weights and their sums of dw in registers: rows that start off 16 bytes are
+// taken a multiple of eight apart, whose chunks are cut alike. With RING the next rows are
+// on their way into a ring of `stages` in shared memory while one is worked on; each thread
+// waits for its own copies alone. Without, rows are loaded when their turn comes.
+// N: its eights of values a thread.
+template <typename T, int N, int MOST, bool PHASED, bool RING>
+__global__ void __launch_bounds__(MOST == 32 ? 128 : MOST, grad_residents(MOST, N)) rms_norm_grad_kernel(NormGradArgs a) {
+  constexpr bool WARP = MOST == 32;  // rows of a warp each
+  constexpr int K = N * 8 / kWide<T>, P = kPairs<T>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(8) float part[2][WARP ? 2 : MOST / 16];
+  const int tid = threadIdx.x, B = WARP ? 32 : blockDim.x, C = a.C;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.y, total = a.R * C;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const int phase = PHASED && a.vec ? (int)((row * C + a.base) % (16 / (int)sizeof(T))) : 0;
+  const auto chunk = [&](int u) { return chunk_of<T>(u * B + tid, phase, C); };
+  pdl_trigger();  // every CTA is resident: the sums' kernel may wait beside them
+  float2 dw[K][P], w[K][P];
 #pragma unroll
-  for (int u = 0; u < N; ++u)
+  for (int u = 0; u < K; ++u) {
+    if (a.wbf16)
+      load_each(w[u], static_cast<const uint16_t*>(a.w), chunk(u), C);
+    else
+      load_each(w[u], static_cast<const float*>(a.w), chunk(u), C);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[u][i] = 0.0f;
-  int turn = 0;
+    for (int i = 0; i < P; ++i) dw[u][i] = make_float2(0.0f, 0.0f);
+  }
   const float over = __fdiv_rn(1.0f, (float)C);
-  for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < a.R; row += (int64_t)gridDim.x * blockDim.y, turn ^= 1) {
-    const int64_t at = row * C;
-    float h[N][8], g[N][8];
-    load_row<B, N, VEC>(h, static_cast<const T*>(a.h) + at, C, tid);
-    load_row<B, N, VEC>(g, static_cast<const T*>(a.dy) + at, C, tid);
-    float hh = 0.0f, ah = 0.0f;
+  const int image = B * K * 16, stage_bytes = image * (a.dres ? 3 : 2);
+  uint8_t* mine = ring + threadIdx.y * a.stages * stage_bytes;
+  const T *hs = static_cast<const T*>(a.h), *gs = static_cast<const T*>(a.dy), *ds = static_cast<const T*>(a.dres);
+  const auto fetch = [&](int64_t r, int stage) {
+    if constexpr (RING) {
+      if (r < a.R) {
+        uint8_t* to = mine + stage * stage_bytes;
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      float w[8];
-      load_weights<B, VEC>(w, a.w, a.wbf16, C, tid, u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        hh = fmaf(h[u][i], h[u][i], hh);
-        ah = fmaf(g[u][i] * w[i], h[u][i], ah);
+        for (int u = 0; u < K; ++u) {
+          const int j = u * B + tid;
+          copy_chunk<PHASED>(to, j, hs, r, chunk(u), C, total);
+          copy_chunk<PHASED>(to + image, j, gs, r, chunk(u), C, total);
+          if (ds) copy_chunk<PHASED>(to + 2 * image, j, ds, r, chunk(u), C, total);
+        }
       }
+      copies_commit();
     }
-    hh = warp_sum(hh);
-    ah = warp_sum(ah);
-    if constexpr (B > 32) {
-      // written again two rows on, behind the next row's barrier
-      const int lane = tid & 31;
-      if (lane == 0) part[turn][0][tid >> 5] = hh, part[turn][1][tid >> 5] = ah;
-      __syncthreads();
-      hh = warp_sum(lane < B / 32 ? part[turn][0][lane] : 0.0f);
-      ah = warp_sum(lane < B / 32 ? part[turn][1][lane] : 0.0f);
-    }
-    const float r = __frsqrt_rn(hh * over + a.eps), k = ah * over * r * r;
+  };
+  for (int s = 0; s + 1 < a.stages; ++s) fetch(row + s * stride, s);
+  for (int turn = 0, stage = 0; row < a.R; row += stride, turn ^= 1) {
+    const uint8_t* from = mine + stage * stage_bytes;
+    if constexpr (RING) copies_wait(a.stages - 2);
+    const auto take = [&](float2 (&v)[P], int array, const T* p, int u) {
+      if constexpr (RING)
+        chunk_in<T>(v, from + array * image, u * B + tid);
+      else
+        load_chunk<PHASED>(v, p, row, chunk(u), C, total, a.vec);
+    };
+    float2 hh = make_float2(0.0f, 0.0f), ah = hh;
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      float w[8], d[8];
-      load_weights<B, VEC>(w, a.w, a.wbf16, C, tid, u);
-      if (a.dres) {
-        load_part<B, VEC>(d, static_cast<const T*>(a.dres) + at, C, tid, u);
+    for (int u = 0; u < K; ++u) {
+      float2 h[P], g[P];
+      take(h, 0, hs, u);
+      take(g, 1, gs, u);
+      // a chunk that is partly or wholly outside the row: no part of the sums. Its later
+      // values are not stored.
+      if (RING && (PHASED ? chunk(u).edge : !chunk(u).on)) only_inside(h, chunk(u), C), only_inside(g, chunk(u), C);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        hh = fma2(h[i], h[i], hh);
+        ah = fma2(mul2(g[i], w[u][i]), h[i], ah);
+      }
+      asm volatile("" ::: "memory");
+    }
+    // the slots are written again two rows on, behind the next row's barrier
+    const float2 sums = row_sums<WARP>(hh.x + hh.y, ah.x + ah.y, part[turn]);
+    // into the stage of the row before, whose last reads are behind this row's barrier
+    // (or a warp's sum)
+    fetch(row + (a.stages - 1) * stride, stage ? stage - 1 : a.stages - 1);
+    const float r = __frsqrt_rn(sums.x * over + a.eps);
+    const float2 r2 = both(r), k2 = both(-sums.y * over * r * r);
+    // the row once more, from where it lies: kept in registers over the barrier it would
+    // leave room for fewer threads
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      float2 h[P], g[P], d[P];
+      take(h, 0, hs, u);
+      take(g, 1, gs, u);
+      if (ds) {
+        take(d, 2, ds, u);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = 0.0f;
+        for (int i = 0; i < P; ++i) d[i] = make_float2(0.0f, 0.0f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dw[u][i] = fmaf(g[u][i], h[u][i] * r, dw[u][i]);
-        d[i] = fmaf(r, fmaf(-h[u][i], k, g[u][i] * w[i]), d[i]);
+      for (int i = 0; i < P; ++i) {
+        dw[u][i] = fma2(g[i], mul2(h[i], r2), dw[u][i]);
+        d[i] = fma2(r2, fma2(h[i], k2, mul2(g[i], w[u][i])), d[i]);
       }
-      store_part<B, VEC>(static_cast<T*>(a.dx) + at, d, C, tid, u);
+      store_chunk<PHASED>(static_cast<T*>(a.dx), row, d, chunk(u), C, a.vec);
+      asm volatile("" ::: "memory");  // one chunk after the other: the registers of one
     }
+    stage = stage + 1 == a.stages ? 0 : stage + 1;
   }
+  copies_wait(0);
   if (!a.part) return;
-  if constexpr (B == 32) {  // the CTA's warps' sums together
+  if constexpr (WARP) {  // the CTA's warps' sums together
+    __shared__ float meet[4][256 * N];
 #pragma unroll
-    for (int u = 0; u < N; ++u)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) meet[threadIdx.y * 256 * N + (u * 8 + i) * 32 + tid] = dw[u][i];
+    for (int u = 0; u < K; ++u) {
+      if (chunk(u).on) store_each(meet[threadIdx.y], dw[u], chunk(u), C);
+    }
     __syncthreads();
-    if (threadIdx.y) return;
-    for (unsigned y = 1; y < blockDim.y; ++y)
+    for (int c = threadIdx.y * 32 + tid; c < C; c += 128)
+      a.part[(int64_t)blockIdx.x * C + c] = meet[0][c] + meet[1][c] + meet[2][c] + meet[3][c];
+  } else {
 #pragma unroll
-      for (int u = 0; u < N; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dw[u][i] += meet[y * 256 * N + (u * 8 + i) * 32 + tid];
+    for (int u = 0; u < K; ++u)
+      if (chunk(u).on) store_each(a.part + (int64_t)blockIdx.x * C, dw[u], chunk(u), C);
   }
-#pragma unroll
-  for (int u = 0; u < N; ++u) store_part<B, VEC>(a.part + (int64_t)blockIdx.x * C, dw[u], C, tid, u);
 }
 
-// dw = the CTAs' sums, in their order: 32 columns a CTA, sixteen threads a column.
-__global__ void __launch_bounds__(512) rms_norm_dw_kernel(float* __restrict__ dw, const float* __restrict__ part, int parts, int C) {
-  __shared__ float sums[16][32];
+// dw = the CTAs' sums, in a fixed order: 32 columns a CTA, 32 threads a column, each with
+// every 32nd sum, eight loads in flight.
+__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(float* __restrict__ dw, const float* __restrict__ part, int parts, int C) {
+  __shared__ float sums[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float sum = 0.0f;
-  if (c < C)
-    for (int p = threadIdx.y; p < parts; p += 16) sum += part[(int64_t)p * C + c];
+  pdl_wait();  // the sums are the gradient kernel's
+  for (int p = threadIdx.y; p < parts; p += 256) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c < C && p + 32 * i < parts ? part[(int64_t)(p + 32 * i) * C + c] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i];
+  }
   sums[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
-  if (threadIdx.y == 0 && c < C) {
-    for (int y = 1; y < 16; ++y) sum += sums[y][threadIdx.x];
-    dw[c] = sum;
+  sum = warp_sum(sums[threadIdx.x][threadIdx.y]);
+  const int mine = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && mine < C) dw[mine] = sum;
+}
+
+// How a launch is laid out: CTAs of `threads` a row, `rows` rows at once a CTA, `N` eights of
+// values a thread, and the ring's stages (none: rows are loaded when their turn comes, for rows
+// too long for two stages).
+constexpr size_t kRing = 204 * 1024;  // of an SM's 227 KiB, for all its CTAs together
+struct GradShape {
+  int threads, rows, N, most, per_sm, stages, device;
+  int64_t ctas;
+  size_t stage_bytes;
+};
+static GradShape grad_shape(int64_t R, int C, int size, bool dres, int sms) {
+  GradShape g = {};
+  const int eights = eights_of(C);
+  g.rows = eights <= 128 ? 4 : 1;
+  g.N = eights <= 32 ? 1 : eights <= 64 ? 2 : eights <= 128 ? 4 : eights <= 2048 ? 2 : 4;
+  g.threads = g.rows == 4 ? 32 : (eights + 32 * g.N - 1) / (32 * g.N) * 32;
+  g.most = g.threads;
+  for (int most : {32, 128, 256, 384, 512, 1024})
+    if (g.threads <= most) {
+      g.most = most;
+      break;
+    }
+  g.per_sm = grad_residents(g.most, g.N);
+  g.stage_bytes = (size_t)g.threads * g.N * 8 * size * (dres ? 3 : 2);
+  while (g.per_sm > 1 && 2 * g.stage_bytes * g.rows * g.per_sm > kRing) --g.per_sm;
+  g.stages = (int)std::min<size_t>(8, kRing / (g.stage_bytes * g.rows * g.per_sm));
+  if (g.stages < 2) g.stages = 0;
+  g.ctas = (R + g.rows - 1) / g.rows;
+  if (g.ctas > g.per_sm * (int64_t)sms) g.ctas = std::max(8, g.per_sm * sms / 8 * 8);
+  return g;
+}
+
+template <typename T, int N, int MOST, bool PHASED, bool RING>
+static cudaError_t norm_grad_go(NormGradArgs a, const GradShape& g, cudaStream_t st) {
+  a.stages = RING ? g.stages : 0;
+  const size_t smem = RING ? g.stage_bytes * g.rows * g.stages : 0;
+  const auto kernel = rms_norm_grad_kernel<T, N, MOST, PHASED, RING>;
+  if constexpr (RING) {
+    static unsigned long long done;
+    if (const cudaError_t e = allow_shared(kernel, (int)kRing, g.device, &done)) return e;
   }
+  kernel<<<(unsigned)g.ctas, dim3(g.threads, g.rows), smem, st>>>(a);
+  return cudaSuccess;
 }
-
-// The CTAs of a launch: what an SM holds of them, and no more than there are rows.
-static int64_t grad_ctas(int64_t R, int C, int sms) {
-  if (C <= 1024) return std::min<int64_t>((R + 3) / 4, 4 * (int64_t)sms);
-  return std::min<int64_t>(R, (C <= 4096 ? 4 : C <= 8192 ? 2 : 1) * (int64_t)sms);
-}
-
-template <typename T, bool VEC>
-static void norm_grad_launch(const NormGradArgs& a, unsigned ctas, cudaStream_t st) {
-  if (a.C <= 256)
-    rms_norm_grad_kernel<T, 32, 1, VEC><<<ctas, dim3(32, 4), 0, st>>>(a);
-  else if (a.C <= 512)
-    rms_norm_grad_kernel<T, 32, 2, VEC><<<ctas, dim3(32, 4), 0, st>>>(a);
-  else if (a.C <= 1024)
-    rms_norm_grad_kernel<T, 32, 4, VEC><<<ctas, dim3(32, 4), 0, st>>>(a);
-  else if (a.C <= 2048)
-    rms_norm_grad_kernel<T, 128, 2, VEC><<<ctas, 128, 0, st>>>(a);
-  else if (a.C <= 4096)
-    rms_norm_grad_kernel<T, 256, 2, VEC><<<ctas, 256, 0, st>>>(a);
-  else if (a.C <= 8192)
-    rms_norm_grad_kernel<T, 512, 2, VEC><<<ctas, 512, 0, st>>>(a);
-  else if (a.C <= 16384)
-    rms_norm_grad_kernel<T, 1024, 2, VEC><<<ctas, 1024, 0, st>>>(a);
-  else
-    rms_norm_grad_kernel<T, 1024, 4, VEC><<<ctas, 1024, 0, st>>>(a);
+template <typename T, bool PHASED, bool RING>
+static cudaError_t norm_grad_launch(const NormGradArgs& a, const GradShape& g, cudaStream_t st) {
+  if (g.rows == 4)
+    return g.N == 1   ? norm_grad_go<T, 1, 32, PHASED, RING>(a, g, st)
+           : g.N == 2 ? norm_grad_go<T, 2, 32, PHASED, RING>(a, g, st)
+                      : norm_grad_go<T, 4, 32, PHASED, RING>(a, g, st);
+  if (g.N == 4) return norm_grad_go<T, 4, 1024, PHASED, false>(a, g, st);
+  if (g.most == 128) return norm_grad_go<T, 2, 128, PHASED, RING>(a, g, st);
+  if (g.most == 256) return norm_grad_go<T, 2, 256, PHASED, RING>(a, g, st);
+  if (g.most == 384) return norm_grad_go<T, 2, 384, PHASED, RING>(a, g, st);
+  if (g.most == 512) return norm_grad_go<T, 2, 512, PHASED, RING>(a, g, st);
+  return norm_grad_go<T, 2, 1024, PHASED, RING>(a, g, st);
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
@@ -376,9 +525,9 @@ mtl_status rms_norm_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
   const bool vec = (la.a[0].ptr | la.a[3].ptr | la.a[4].ptr | la.a[5].ptr | la.a[6].ptr) % 16 == 0 && a.C % 8 == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (la.a[8].i32)
-    vec ? norm_launch<uint16_t, true>(a, st) : norm_launch<uint16_t, false>(a, st);
+    vec ? norm_launch<uint16_t, true>(a, la.sm_count, st) : norm_launch<uint16_t, false>(a, la.sm_count, st);
   else
-    vec ? norm_launch<float, true>(a, st) : norm_launch<float, false>(a, st);
+    vec ? norm_launch<float, true>(a, la.sm_count, st) : norm_launch<float, false>(a, la.sm_count, st);
   return launched("rms_norm");
 }
 
@@ -403,7 +552,7 @@ mtl_status rms_norm_grad_check(const LaunchArgs& la, const uint64_t* bytes) {
 uint64_t rms_norm_grad_workspace(const LaunchArgs& la) {
   const int64_t R = la.nd[0], C = la.a[6].i32;
   if (la.a[1].kind != MTL_ARG_PTR || R <= 0 || C <= 0 || C > kNormColumns) return 0;
-  return bytes_of({grad_ctas(R, (int)C, la.sm_count), C, 4});
+  return bytes_of({grad_shape(R, (int)C, la.a[7].i32 ? 2 : 4, given(la, 5), la.sm_count).ctas, C, 4});
 }
 
 mtl_status rms_norm_grad_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, void* stream) {
@@ -424,16 +573,29 @@ mtl_status rms_norm_grad_run(const LaunchArgs& la, void* ws, uint64_t ws_bytes, 
   if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
     return fail(MTL_ERR_ARGUMENT, "rms_norm_grad: dw needs %llu bytes of scratch on 16 bytes (mtl_kernel_workspace), got %llu",
                 (unsigned long long)need, (unsigned long long)(ws ? ws_bytes : 0));
-  const int ctas = a.R ? (int)grad_ctas(a.R, a.C, la.sm_count) : 0;
   a.part = dw ? static_cast<float*>(ws) : nullptr;
-  const bool vec = (la.a[0].ptr | la.a[2].ptr | la.a[3].ptr | la.a[4].ptr | la.a[5].ptr) % 16 == 0 && a.C % 8 == 0;
-  if (ctas) {
-    if (la.a[7].i32)
-      vec ? norm_grad_launch<uint16_t, true>(a, ctas, st) : norm_grad_launch<uint16_t, false>(a, ctas, st);
+  const bool bf16 = la.a[7].i32;
+  const int size = bf16 ? 2 : 4;
+  a.base = phase_of(la.a[0].ptr, size);
+  a.vec = cut_in_chunks(a.C, a.base);
+  for (int i : {2, 3, 5}) a.vec &= !given(la, i) || phase_of(la.a[i].ptr, size) == a.base;
+  GradShape g = grad_shape(a.R, a.C, size, given(la, 5), la.sm_count);
+  g.device = la.device;
+  const bool phased = !a.vec || a.C % 8, ring = a.vec && g.stages;
+  if (a.R) {
+    cudaError_t e;
+    if (bf16)
+      e = !phased ? (ring ? norm_grad_launch<uint16_t, false, true>(a, g, st) : norm_grad_launch<uint16_t, false, false>(a, g, st))
+                  : (ring ? norm_grad_launch<uint16_t, true, true>(a, g, st) : norm_grad_launch<uint16_t, true, false>(a, g, st));
     else
-      vec ? norm_grad_launch<float, true>(a, ctas, st) : norm_grad_launch<float, false>(a, ctas, st);
+      e = !phased ? (ring ? norm_grad_launch<float, false, true>(a, g, st) : norm_grad_launch<float, false, false>(a, g, st))
+                  : (ring ? norm_grad_launch<float, true, true>(a, g, st) : norm_grad_launch<float, true, false>(a, g, st));
+    if (e != cudaSuccess) return fail(MTL_ERR_CUDA, "rms_norm_grad: %s", cudaGetErrorString(e));
   }
-  if (dw) rms_norm_dw_kernel<<<(a.C + 31) / 32, dim3(32, 16), 0, st>>>(dw, a.part, ctas, a.C);
+  if (dw) {
+    const cudaError_t e = launch_pdl(rms_norm_dw_kernel, dim3((a.C + 31) / 32), dim3(32, 32), 0, st, dw, (const float*)a.part, (int)g.ctas, a.C);
+    if (e != cudaSuccess) return fail(MTL_ERR_CUDA, "rms_norm_grad: %s", cudaGetErrorString(e));
+  }
   return launched("rms_norm_grad");
 }
 

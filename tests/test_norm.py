@@ -179,6 +179,34 @@ def test_norm(dev, r, c, kind, wkind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("r,c", [(5, 1), (9, 127), (17, 264), (3, 1000), (4, 1024), (9, 2047), (17, 4096), (2, 8192), (3, 8193), (1, 32767), (2, 32768)])
+def test_tensors_that_all_start_off_16_bytes(dev, r, c, kind):
+    # every tensor as far behind 16 bytes as the others, the outputs among them, and nothing written around them
+    w = (1 + 0.3 * rows(1, c, F, 5)[0]).to(kind)
+    for at in (1, 3):
+        x, res, dy = (rows(r, c, kind, k, at) for k in (1, 2, 3))
+        flat = [torch.full((r * c + at + 9,), 7.0, dtype=kind, device="cuda") for _ in range(3)]
+        y, h, dx = (f[at:at + r * c].view(r, c) for f in flat)
+        _, _, q, s = norm(x, w, res, out=y, h=h, fmt=0)
+        want = exact(x, w, res)
+        check_y(h, want[0], 0)
+        check_y(y, want[1])
+        check_codes(q, s, want[1], 0, 0)
+        dw = grad(dy, h, w, res, dx=dx)[1]
+        dx2, dw2 = grad(*(v.clone() for v in (dy, h, w, res)))
+        # cut elsewhere, so summed in another order: each within the bounds of test_norm_grad of the exact value
+        a = dy.double() * w.double()
+        rr = 1 / torch.sqrt((h.double() ** 2).mean(1, keepdim=True) + 1e-6)
+        m = rr * rr * (a * h.double()).abs().mean(1, keepdim=True)
+        tol = 256 * u * rr * (a.abs() + h.double().abs() * m) + 4 * u * (dx2.double().abs() + res.double().abs())
+        assert ((dx.double() - dx2.double()).abs() <= tol + 2 * HALF[kind] * dx2.double().abs()).all()
+        assert ((dw.double() - dw2.double()).abs() <= 2 * (28 + r) * u * (dy.double() * h.double() * rr).abs().sum(0)).all()
+        for f in flat:
+            assert (f[:at] == 7).all() and (f[at + r * c:] == 7).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("pow2", [0, 1])
 @pytest.mark.parametrize("fmt", [0, 1])
 @pytest.mark.parametrize("kind", [F, H])
