@@ -63,6 +63,34 @@ def compile_one(src: Path, force: bool) -> Path:
     return obj
 
 
+LAUNCH_SRC, LAUNCH_OUT = CSRC / "python" / "launch.cpp", HERE / "mantle_cuda" / "_launch.so"
+
+
+def build_launch(force: bool = False) -> None:
+    """The Python host's short way to a launch with torch tensors (mantle_cuda/_launch.so),
+    against the torch that is installed; the library itself does without either."""
+    newest_dep = max(LAUNCH_SRC.stat().st_mtime, (ROOT / "include" / "mantle_cuda.h").stat().st_mtime)
+    if not force and LAUNCH_OUT.exists() and LAUNCH_OUT.stat().st_mtime >= newest_dep:
+        return
+    import sysconfig
+
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths
+    except ImportError:
+        return
+    if not torch.version.cuda:
+        return
+    lib = Path(torch.__file__).parent / "lib"
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    cmd = ["g++", "-O2", "-std=c++20", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{d}" for d in (*include_paths(), sysconfig.get_paths()["include"], cuda)], str(LAUNCH_SRC), "-o", str(LAUNCH_OUT),
+           f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     srcs = sources()
@@ -76,6 +104,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    build_launch(force)
     if verbose:
         print(OUT)
     return OUT

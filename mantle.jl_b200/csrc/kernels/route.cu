@@ -41,6 +41,7 @@
 
 #include "../mtl_internal.hpp"
 #include "rows.cuh"
+#include "tc_common.cuh"
 
 namespace mtl {
 
@@ -59,167 +60,284 @@ struct RouteArgs {
   float scale;
 };
 
-// 64-bit keys as integers of the same order.
-__device__ __forceinline__ unsigned long long ordered(double v) {
-  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);  // -0 as 0
-  return u >> 63 ? ~u : u | 0x8000000000000000ull;
-}
-constexpr unsigned long long kNoKey = 0x000fffffffffffffull;  // ordered(-infinity)
-
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, d);
-    v = o > v ? o : v;
+// Keys as integers of the same order, -0 as 0.
+template <typename K>
+struct Key;
+template <>
+struct Key<uint32_t> {
+  static constexpr uint32_t kNone = 0x007fffffu;  // -infinity's
+  static __device__ __forceinline__ uint32_t of(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return u >> 31 ? ~u : u | 0x80000000u;
   }
-  return v;
-}
+  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
+  static __device__ __forceinline__ uint32_t most(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
+};
+template <>
+struct Key<unsigned long long> {
+  static constexpr unsigned long long kNone = 0x000fffffffffffffull;
+  static __device__ __forceinline__ unsigned long long of(double v) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+  }
+  static __device__ __forceinline__ double value(unsigned long long k) {
+    return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
+  }
+  // of the warp's, the upper halves first
+  static __device__ __forceinline__ unsigned long long most(unsigned long long k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return (unsigned long long)hi << 32 | lo;
+  }
+};
+using Key32 = Key<uint32_t>;
+using Key64 = Key<unsigned long long>;
+
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
+__device__ __forceinline__ float warp_most(float v) { return Key32::value(Key32::most(Key32::of(v))); }
+
+// e^x for x <= 0 to 1e-15: x = n ln 2 + r with |r| <= 0.35, the series of e^r up to r^12 / 12!
+// (the next term is below 2e-16), and 2^n in two factors, so that small results are denormal
+// as they should be. exp() of the library decides the same and takes twice the instructions.
+__device__ __forceinline__ double exp_down(double x) {
+  x = fmax(x, -746.0);
+  const double n = rint(x * 1.4426950408889634);
+  const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, x));
+  double y = 1.0 / 479001600.0;
+  y = fma(y, r, 1.0 / 39916800.0);
+  y = fma(y, r, 1.0 / 3628800.0);
+  y = fma(y, r, 1.0 / 362880.0);
+  y = fma(y, r, 1.0 / 40320.0);
+  y = fma(y, r, 1.0 / 5040.0);
+  y = fma(y, r, 1.0 / 720.0);
+  y = fma(y, r, 1.0 / 120.0);
+  y = fma(y, r, 1.0 / 24.0);
+  y = fma(y, r, 1.0 / 6.0);
+  y = fma(y, r, 0.5);
+  y = fma(y, r, 1.0);
+  y = fma(y, r, 1.0);
+  const int k = (int)n, half = k / 2;
+  const auto power = [](int i) { return __longlong_as_double((long long)(i + 1023) << 52); };
+  return y * power(half) * power(k - half);
+}
+// A score in 64 bits, softmax's up to the factor 1 / (sum over the experts).
+__device__ __forceinline__ double score_64(float l, int sigmoid, float most) {
+  if (!sigmoid) return exp_down((double)l - (double)most);
+  const double e = exp_down(-fabs((double)l)), r = __drcp_rn(1.0 + e);
+  return l < 0.0f ? e * r : r;
 }
 
-// The weights of a token's chosen experts: lane j has slot j's logit, or -inf for none.
+// The weights of a token's chosen experts: lane j has slot j's logit.
 __device__ __forceinline__ float weight_of(float l, bool valid, float most, float total, int sigmoid, int renorm, float scale) {
   float s;
   if (!renorm) {
     s = sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - most) / total;
   } else if (sigmoid) {
     // s_i up to a common factor: e^min(l, 0) / (1 + e^-|l|)
-    const float m = fminf(warp_max(valid ? l : -INFINITY), 0.0f);
+    const float m = fminf(warp_most(valid ? l : -INFINITY), 0.0f);
     s = valid ? expf(fminf(l, 0.0f) - m) / (1.0f + expf(-fabsf(l))) : 0.0f;
     s = s / warp_sum(s);
   } else {
-    const float m = warp_max(valid ? l : -INFINITY);
+    const float m = warp_most(valid ? l : -INFINITY);
     s = valid ? expf(l - m) : 0.0f;
     s = s / warp_sum(s);
   }
   return valid ? s * scale : 0.0f;
 }
 
-// A warp a token; lane i holds experts i, i + 32, ...: P of them.
-template <typename T, int P>
-__global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
-  extern __shared__ unsigned long long group_keys[];  // a warp's groups x 2
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = (int64_t)blockIdx.x * 4 + warp;
-  if (t >= a.T) return;
-  const int E = a.E;
-  const T* logits = static_cast<const T*>(a.logits) + t * E;
-  float l[P];
-  bool bad = false;
-  float most = -INFINITY;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int e = p * 32 + lane;
-    l[p] = e < E ? to_f32(logits[e]) : -INFINITY;
-    bad |= isnan(l[p]) || (a.bias && e < E && isnan(a.bias[e]));
-    most = fmaxf(most, l[p]);
+// The two largest of keys seen so far.
+template <typename K>
+struct Best {
+  K one = Key<K>::kNone, two = Key<K>::kNone;
+  __device__ __forceinline__ void add(K k) {
+    two = max(two, min(one, k));
+    one = max(one, k);
   }
-  most = warp_max(most);
-  bad = __any_sync(0xffffffffu, bad || (!a.sigmoid && most == INFINITY));
-  const bool none = most == -INFINITY || (a.live && !a.live[t]);
-  if (bad || none) {
-    if (lane < a.top) {
-      a.ids[t * a.top + lane] = -1;
-      a.weights[t * a.top + lane] = none && a.live && !a.live[t] ? 0.0f : bad ? NAN : 0.0f;
+  __device__ __forceinline__ void add(const Best& o) {
+    two = max(max(two, o.two), min(one, o.one));
+    one = max(one, o.one);
+  }
+};
+
+// Puts kNone in the place of the keys whose groups do not stay. Lane i holds experts i P
+// .. + P. `worth`: a key's score (plus bias), which group values are sums of. `values`: the
+// warp's place for its groups' values.
+template <int P, typename K, typename F>
+__device__ __forceinline__ void keep_groups(const RouteArgs& a, K (&key)[P], unsigned long long* values, F worth) {
+  const int lane = threadIdx.x & 31, first = lane * P, size = a.E / a.groups, lanes = size / P;
+  const auto value_of = [&](const Best<K>& b) -> unsigned long long {
+    if (a.best == 1 || b.one == Key<K>::kNone) return b.one == Key<K>::kNone ? 0 : b.one;
+    return Key64::of(worth(b.one) + (b.two != Key<K>::kNone ? worth(b.two) : 0.0));
+  };
+  if (size == lanes * P && (lanes & (lanes - 1)) == 0 && lanes >= 1) {
+    // a group is `lanes` lanes
+    Best<K> b;
+#pragma unroll
+    for (int p = 0; p < P; ++p) b.add(key[p]);
+    for (int d = 1; d < lanes; d *= 2) {
+      Best<K> o;
+      o.one = __shfl_xor_sync(0xffffffffu, b.one, d);
+      o.two = __shfl_xor_sync(0xffffffffu, b.two, d);
+      b.add(o);
+    }
+    const unsigned long long mine = value_of(b);
+    const int g = lane / lanes;
+    int ahead = 0;
+    for (int o = 0; o < a.groups; ++o) {
+      const unsigned long long other = __shfl_sync(0xffffffffu, mine, o * lanes);
+      ahead += other > mine || (other == mine && o < g);
+    }
+    if (ahead >= a.top_groups) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) key[p] = Key<K>::kNone;
     }
     return;
   }
-  float total = 0.0f;
-  if (!a.sigmoid) {
+  for (int g = 0; g < a.groups; ++g) {
+    Best<K> b;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (first + p >= g * size && first + p < (g + 1) * size) b.add(key[p]);
+    const K one = Key<K>::most(b.one);
+    const int holder = __ffs(__ballot_sync(0xffffffffu, b.one == one)) - 1;
+    b.two = Key<K>::most(lane == holder ? b.two : b.one);
+    b.one = one;
+    if (lane == 0) values[g] = value_of(b);
+  }
+  __syncwarp();
+  // a lane a group: does it stay? Said in the value's last place, once all are read.
+  constexpr int kMost = kMaxExperts / 32;
+  uint32_t stays = 0;
+  for (int i = 0; i < kMost && i * 32 < a.groups; ++i) {
+    const int g = i * 32 + lane;
+    if (g >= a.groups) break;
+    const unsigned long long mine = values[g];
+    int ahead = 0;
+    for (int o = 0; o < a.groups; ++o) ahead += values[o] > mine || (values[o] == mine && o < g);
+    stays |= (uint32_t)(ahead < a.top_groups) << i;
+  }
+  __syncwarp();
+  for (int i = 0; i < kMost && i * 32 + lane < a.groups; ++i) values[i * 32 + lane] = stays >> i & 1;
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (first + p < a.E && !values[(first + p) / size]) key[p] = Key<K>::kNone;
+  __syncwarp();
+}
+
+// The expert of slot `lane`: one choice after the other, the largest key, its lowest index.
+template <int P, typename K>
+__device__ __forceinline__ int choose(int top, K (&key)[P]) {
+  const int lane = threadIdx.x & 31, first = lane * P;
+  K mine = Key<K>::kNone;
+#pragma unroll
+  for (int p = 0; p < P; ++p) mine = max(mine, key[p]);
+  int id = -1;
+  for (int j = 0; j < top; ++j) {
+    const K k = Key<K>::most(mine);
+    if (k == Key<K>::kNone) break;
+    const int from = __ffs(__ballot_sync(0xffffffffu, mine == k)) - 1;
+    int e = first;
+    if (lane == from) {  // it gives its first such key and looks for its next
+      bool given = false;
+      mine = Key<K>::kNone;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        if (!given && key[p] == k) key[p] = Key<K>::kNone, given = true, e = first + p;
+        mine = max(mine, key[p]);
+      }
+    }
+    e = __shfl_sync(0xffffffffu, e, from);
+    if (lane == j) id = e;
+  }
+  return id;
+}
+
+// A token by a warp: lane i holds experts i P .. + P. `vec`: rows of logits on 16 bytes.
+template <typename T, int P>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsigned long long* values, bool vec) {
+  const int lane = threadIdx.x & 31, E = a.E, first = lane * P;
+  const T* logits = static_cast<const T*>(a.logits) + t * E;
+  float l[P];
+  if (vec && P * sizeof(T) >= 16 && first + P <= E) {
+    constexpr int kEach = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < P / kEach; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(logits + first)[i];
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if constexpr (sizeof(T) == 4)
+          l[i * kEach + j] = __uint_as_float(w[j]);
+        else
+          l[i * kEach + j] = j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p) l[p] = first + p < E ? to_f32(logits[first + p]) : -INFINITY;
+  }
+  float b[P];
+  if (a.bias) {
+    if (reinterpret_cast<uintptr_t>(a.bias) % 16 == 0 && P >= 4 && first + P <= E) {
+#pragma unroll
+      for (int i = 0; i < P / 4; ++i) {
+        const float4 f = reinterpret_cast<const float4*>(a.bias + first)[i];
+        b[4 * i] = f.x, b[4 * i + 1] = f.y, b[4 * i + 2] = f.z, b[4 * i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < P; ++p) b[p] = first + p < E ? a.bias[first + p] : 0.0f;
+    }
+  }
+  const bool live = !a.live || a.live[t];
+  bool bad = false;
+  uint32_t key[P], most_key = Key32::kNone;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    bad |= isnan(l[p]) || (a.bias && isnan(b[p]));
+    key[p] = Key32::of(l[p]);
+    most_key = max(most_key, key[p]);
+  }
+  const float most = Key32::value(Key32::most(most_key));
+  bad = __any_sync(0xffffffffu, bad || (!a.sigmoid && most == INFINITY));
+  if (bad || !live || most == -INFINITY) {
+    if (lane < a.top) {
+      a.ids[t * a.top + lane] = -1;
+      a.weights[t * a.top + lane] = bad && live ? NAN : 0.0f;
+    }
+    return;
+  }
+  float total = 1.0f;
+  if (!a.sigmoid && !a.renorm) {
+    total = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p) total += expf(l[p] - most);
     total = warp_sum(total);
   }
-  unsigned long long key[P];
+  int id;
   if (a.bias) {
-    double s[P], all = 0.0;
+    unsigned long long wide[P];
+    double s[P], over = 1.0;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      s[p] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)l[p])) : exp((double)l[p] - (double)most);
-      all += s[p];
-    }
+    for (int p = 0; p < P; ++p) s[p] = score_64(l[p], a.sigmoid, most);
     if (!a.sigmoid) {
-      all = warp_sum(all);
+      over = 0.0;
 #pragma unroll
-      for (int p = 0; p < P; ++p) s[p] /= all;
+      for (int p = 0; p < P; ++p) over += s[p];
+      over = __drcp_rn(warp_sum(over));
     }
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int e = p * 32 + lane;
-      key[p] = e < E && l[p] != -INFINITY ? ordered(s[p] + (double)a.bias[e]) : kNoKey;
-    }
+    for (int p = 0; p < P; ++p) wide[p] = l[p] == -INFINITY ? Key64::kNone : Key64::of(fma(s[p], over, (double)b[p]));
+    if (a.groups > 1) keep_groups<P>(a, wide, values, [](unsigned long long k) { return Key64::value(k); });
+    id = choose<P>(a.top, wide);
   } else {
-#pragma unroll
-    for (int p = 0; p < P; ++p) key[p] = ordered((double)l[p]);
-  }
-  if (a.groups > 1) {
-    // each group's best keys, one group after the other
-    const int per = E / a.groups;
-    unsigned long long* value = group_keys + warp * a.groups;
-    for (int g = 0; g < a.groups; ++g) {
-      const int lo = g * per, hi = lo + per;
-      unsigned long long first = kNoKey, second = kNoKey;
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const int e = p * 32 + lane;
-        const unsigned long long k = e >= lo && e < hi ? key[p] : kNoKey;
-        second = max(second, min(first, k));
-        first = max(first, k);
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        const unsigned long long f = __shfl_xor_sync(0xffffffffu, first, d), s = __shfl_xor_sync(0xffffffffu, second, d);
-        second = max(max(second, s), min(first, f));
-        first = max(first, f);
-      }
-      if (a.best > 1 && first != kNoKey) {
-        // without a bias the keys are logits: their scores, up to softmax's common factor
-        const auto score = [&](unsigned long long k) {
-          const double v = __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
-          return a.bias ? v : a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)most);
-        };
-        first = ordered(score(first) + (second != kNoKey ? score(second) : 0.0));
-      }
-      if (lane == 0) value[g] = first;
-    }
-    __syncwarp();
-    // a group stays if fewer than top_groups are ahead of it
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int e = p * 32 + lane;
-      if (e < E) {
-        const int g = e / per;
-        int ahead = 0;
-        for (int o = 0; o < a.groups; ++o) ahead += value[o] > value[g] || (value[o] == value[g] && o < g);
-        if (ahead >= a.top_groups) key[p] = kNoKey;
-      }
-    }
-  }
-  // one choice after the other: the largest key, its lowest index
-  int id = -1;
-  for (int j = 0; j < a.top; ++j) {
-    unsigned long long k = kNoKey;
-#pragma unroll
-    for (int p = 0; p < P; ++p) k = max(k, key[p]);
-    k = warp_max(k);
-    if (k == kNoKey) break;
-    int e = INT_MAX;
-#pragma unroll
-    for (int p = P - 1; p >= 0; --p)
-      if (key[p] == k) e = p * 32 + lane;
-    e = __reduce_min_sync(0xffffffffu, e);
-    if (lane == j) id = e;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (e == p * 32 + lane) key[p] = kNoKey;
+    if (a.groups > 1) keep_groups<P>(a, key, values, [&](uint32_t k) { return score_64(Key32::value(k), a.sigmoid, most); });
+    id = choose<P>(a.top, key);
   }
   const float chosen = id >= 0 ? to_f32(logits[id]) : -INFINITY;
   const float w = weight_of(chosen, id >= 0, most, total, a.sigmoid, a.renorm, a.scale);
@@ -243,29 +361,37 @@ struct OrderArgs {
   int64_t n;
   int E, top;
 };
+static size_t order_shared(int E) { return sizeof(int) * ((kOrderWarps + 2) * (size_t)E + 32); }
 
-__global__ void __launch_bounds__(kOrderWarps * 32) order_rows_kernel(OrderArgs a) {
+// The CTA's slots are lo .. hi. Several clusters (`parts`) may do this at once: each counts
+// all slots, and places the `part`-th share of every warp's.
+__device__ __forceinline__ void order_rows(const OrderArgs& a, int* shared, int64_t lo, int64_t hi, int part, int parts) {
   namespace cg = cooperative_groups;
-  extern __shared__ int order_smem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int E = a.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  int* count = order_smem;                // [warp][expert]
-  int* total = count + kOrderWarps * E;   // this CTA's rows of each expert
-  int* start = total + E;                 // the first row of each expert that is this CTA's
-  int* sums = start + E;                  // [32] of the scan, and the number of rows
-  for (int i = threadIdx.x; i < kOrderWarps * E; i += blockDim.x) count[i] = 0;
-  const int64_t steps = (a.n + 31) / 32, per = (steps + (int64_t)ctas * kOrderWarps - 1) / ((int64_t)ctas * kOrderWarps) * 32;
-  const int64_t lo = min(a.n, ((int64_t)rank * kOrderWarps + warp) * per), hi = min(a.n, lo + per);
-  __syncthreads();
+  int* count = shared;                   // [warp][expert]
+  int* total = count + kOrderWarps * E;  // this CTA's rows of each expert
+  int* start = total + E;                // the first row of each expert that is this CTA's
+  int* sums = start + E;                 // [32] of the scan, and the number of rows
+  const int64_t per = ((hi - lo + 31) / 32 + kOrderWarps - 1) / kOrderWarps * 32;
+  const int64_t from = min(hi, lo + warp * per), to = min(hi, from + per);
   int* mine = count + warp * E;
-  for (int64_t s = lo + lane; s < hi; s += 32) {
-    const int id = a.ids[s];
-    if ((unsigned)id < (unsigned)E) atomicAdd(mine + id, 1);
+  for (int i = lane; i < E; i += 32) mine[i] = 0;
+  __syncwarp();
+  constexpr int kAhead = 8;  // loads in flight
+  for (int64_t s = from; s < to; s += 32 * kAhead) {
+    int id[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) id[i] = s + i * 32 + lane < to ? a.ids[s + i * 32 + lane] : -1;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if ((unsigned)id[i] < (unsigned)E) atomicAdd(mine + id[i], 1);
   }
   __syncthreads();
   const int e = threadIdx.x;
   if (e < E) {
     int run = 0;
+#pragma unroll 8
     for (int w = 0; w < kOrderWarps; ++w) {
       const int c = count[w * E + e];
       count[w * E + e] = run;
@@ -276,6 +402,7 @@ __global__ void __launch_bounds__(kOrderWarps * 32) order_rows_kernel(OrderArgs 
   cluster.sync();
   int before = 0, all = 0;
   if (e < E)
+#pragma unroll 8
     for (int r = 0; r < ctas; ++r) {
       const int c = cluster.map_shared_rank(total, r)[e];
       if (r < rank) before += c;
@@ -302,28 +429,78 @@ __global__ void __launch_bounds__(kOrderWarps * 32) order_rows_kernel(OrderArgs 
   const int first = scan - all + (warp ? sums[warp - 1] : 0), rows = sums[31];
   if (e < E) {
     start[e] = first + before;
-    if (rank == 0) {
+    if (rank == 0 && part == 0) {
       a.offsets[e] = first;
       if (e == E - 1) a.offsets[E] = rows;
     }
   }
   cluster.sync();  // nobody leaves while its totals are read
-  for (int64_t s = lo + lane; s - lane < hi; s += 32) {
-    const int id = s < hi ? a.ids[s] : -1;
-    const bool valid = (unsigned)id < (unsigned)E;
-    const unsigned peers = __match_any_sync(0xffffffffu, valid ? id : -1);
-    if (valid) {
-      const int at = start[id] + mine[id] + __popc(peers & ((1u << lane) - 1));
-      a.rows_of[at] = (int)((uint32_t)s / (uint32_t)a.top);
-      a.row_at[s] = at;
-    } else if (s < hi) {
-      a.row_at[s] = -1;
-    }
-    __syncwarp();
-    if (valid && (peers & ((1u << lane) - 1)) == 0) mine[id] += __popc(peers);
-    __syncwarp();
+  const int64_t steps = (to - from + 31) / 32, begin = from + steps * part / parts * 32, end = min(to, from + steps * (part + 1) / parts * 32);
+  for (int64_t s = from; s < begin; s += 32 * kAhead) {  // the shares before
+    int id[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) id[i] = s + i * 32 < begin ? a.ids[s + i * 32 + lane] : -1;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if ((unsigned)id[i] < (unsigned)E) atomicAdd(mine + id[i], 1);
   }
-  for (int64_t r = rows + (int64_t)rank * blockDim.x + threadIdx.x; r < a.n; r += (int64_t)ctas * blockDim.x) a.rows_of[r] = -1;
+  __syncwarp();
+  for (int64_t s = begin; s < end; s += 32 * kAhead) {
+    int id[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) id[i] = s + i * 32 + lane < end ? a.ids[s + i * 32 + lane] : -1;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t slot = s + i * 32 + lane;
+      if (slot - lane >= end) break;
+      const bool valid = (unsigned)id[i] < (unsigned)E;
+      const unsigned peers = __match_any_sync(0xffffffffu, valid ? id[i] : -1), below = peers & ((1u << lane) - 1);
+      if (valid) {
+        const int at = start[id[i]] + mine[id[i]] + __popc(below);
+        a.rows_of[at] = (int)((uint32_t)slot / (uint32_t)a.top);
+        a.row_at[slot] = at;
+      } else if (slot < end) {
+        a.row_at[slot] = -1;
+      }
+      __syncwarp();
+      if (valid && below == 0) mine[id[i]] += __popc(peers);
+      __syncwarp();
+    }
+  }
+  for (int64_t r = rows + ((int64_t)part * ctas + rank) * blockDim.x + threadIdx.x; r < a.n; r += (int64_t)parts * ctas * blockDim.x) a.rows_of[r] = -1;
+}
+
+// ── the kernels ─────────────────────────────────────────────────────────────
+// The choice alone, four tokens a CTA.
+template <typename T, int P>
+__global__ void __launch_bounds__(128) route_kernel(RouteArgs a, bool vec) {
+  extern __shared__ __align__(16) unsigned long long values[];  // of a warp's groups
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5;
+  const int64_t t = (int64_t)blockIdx.x * 4 + warp;
+  if (t < a.T) route_token<T, P>(a, t, values + warp * (a.groups > 1 ? a.groups : 0), vec);
+}
+// The order alone, by one cluster, behind it.
+__global__ void __launch_bounds__(kOrderWarps * 32) order_rows_kernel(OrderArgs a) {
+  extern __shared__ __align__(16) int shared[];
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int64_t steps = (a.n + 31) / 32, per = (steps + cluster.num_blocks() - 1) / cluster.num_blocks() * 32;
+  const int64_t lo = min(a.n, (int64_t)cluster.block_rank() * per), hi = min(a.n, lo + per);
+  pdl_wait();
+  order_rows(a, shared, lo, hi, blockIdx.x / cluster.num_blocks(), gridDim.x / cluster.num_blocks());
+}
+// Both by one cluster, for few tokens.
+template <typename T, int P>
+__global__ void __launch_bounds__(kOrderWarps * 32) route_and_order_kernel(RouteArgs a, OrderArgs o, bool vec) {
+  extern __shared__ __align__(16) int shared[];
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int warp = threadIdx.x >> 5;
+  unsigned long long* values = reinterpret_cast<unsigned long long*>(shared) + warp * (a.groups > 1 ? a.groups : 0);
+  const int64_t per = (a.T + cluster.num_blocks() - 1) / cluster.num_blocks();
+  const int64_t lo = min(a.T, (int64_t)cluster.block_rank() * per), hi = min(a.T, lo + per);
+  for (int64_t t = lo + warp; t < hi; t += kOrderWarps) route_token<T, P>(a, t, values, vec);
+  __syncthreads();  // the ids are this CTA's own
+  order_rows(o, shared, lo * a.top, hi * a.top, 0, 1);
 }
 
 // ── the gradient ────────────────────────────────────────────────────────────
@@ -359,7 +536,7 @@ __global__ void __launch_bounds__(128) route_grad_kernel(RouteGradArgs a) {
       p[i] = e < E ? to_f32(logits[e]) : -INFINITY;
       most = fmaxf(most, p[i]);
     }
-    most = warp_max(most);
+    most = warp_most(most);
     if (most == -INFINITY) most = 0.0f;  // every expert masked: all of p is 0
     total = 0.0f;
 #pragma unroll
@@ -449,22 +626,63 @@ mtl_status route_experts_check(const LaunchArgs& la, const uint64_t* bytes) {
                          {"live", bytes_of({T, 4}), 4}});
 }
 
+constexpr int kRouteShared = 160 * 1024;  // more than order_shared() and the groups' values ask for
+
+template <typename... K, typename... A>
+static cudaError_t cluster_launch(void (*kernel)(K...), unsigned ctas, unsigned clusters, size_t shared, bool behind, int device, unsigned long long* done, cudaStream_t st, A... args) {
+  if (const cudaError_t e = allow_shared(kernel, kRouteShared, device, done)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas * clusters);
+  cfg.blockDim = dim3(kOrderWarps * 32);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = behind ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// One cluster chooses and orders up to this many tokens; beyond it more SMs' work on the
+// choice is worth a launch of its own for the order.
+#ifndef RFUSED
+#define RFUSED 256
+#endif
+constexpr int64_t kFewTokens = RFUSED;
+#ifndef RCLUST
+#define RCLUST 8
+#endif
+#ifndef RORDER
+#define RORDER 8
+#endif
+
+static bool few_tokens(const RouteArgs& a) {
+  return a.T > 0 && a.T <= kFewTokens && (a.groups == 1 || kOrderWarps * sizeof(unsigned long long) * a.groups <= kRouteShared);
+}
+
+template <typename T, int P>
+static cudaError_t route_go(const RouteArgs& a, const OrderArgs* o, bool vec, int device, cudaStream_t st) {
+  const size_t values = a.groups > 1 ? sizeof(unsigned long long) * a.groups : 0;
+  if (o && few_tokens(a)) {
+    static unsigned long long done;
+    const unsigned ctas = (unsigned)std::min<int64_t>(8, (a.T + kOrderWarps - 1) / kOrderWarps);
+    return cluster_launch(route_and_order_kernel<T, P>, ctas, 1, std::max(order_shared(a.E), kOrderWarps * values), false, device, &done, st, a, *o, vec);
+  }
+  if (a.T) route_kernel<T, P><<<(unsigned)((a.T + 3) / 4), 128, 4 * values, st>>>(a, vec);
+  return cudaSuccess;
+}
 template <typename T>
-static void route_launch(const RouteArgs& a, cudaStream_t st) {
-  const unsigned grid = (unsigned)((a.T + 3) / 4);
-  const size_t smem = a.groups > 1 ? 4 * sizeof(unsigned long long) * a.groups : 0;
-  if (a.E <= 32)
-    route_kernel<T, 1><<<grid, 128, smem, st>>>(a);
-  else if (a.E <= 64)
-    route_kernel<T, 2><<<grid, 128, smem, st>>>(a);
-  else if (a.E <= 128)
-    route_kernel<T, 4><<<grid, 128, smem, st>>>(a);
-  else if (a.E <= 256)
-    route_kernel<T, 8><<<grid, 128, smem, st>>>(a);
-  else if (a.E <= 512)
-    route_kernel<T, 16><<<grid, 128, smem, st>>>(a);
-  else
-    route_kernel<T, 32><<<grid, 128, smem, st>>>(a);
+static cudaError_t route_launch(const RouteArgs& a, const OrderArgs* o, bool vec, int device, cudaStream_t st) {
+  if (a.E <= 32) return route_go<T, 1>(a, o, vec, device, st);
+  if (a.E <= 64) return route_go<T, 2>(a, o, vec, device, st);
+  if (a.E <= 128) return route_go<T, 4>(a, o, vec, device, st);
+  if (a.E <= 256) return route_go<T, 8>(a, o, vec, device, st);
+  if (a.E <= 512) return route_go<T, 16>(a, o, vec, device, st);
+  return route_go<T, 32>(a, o, vec, device, st);
 }
 
 mtl_status route_experts_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
@@ -484,23 +702,23 @@ mtl_status route_experts_run(const LaunchArgs& la, void*, uint64_t, void* stream
   a.renorm = la.a[14].i32;
   a.scale = la.a[16].f32;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a.T) la.a[15].i32 ? route_launch<uint16_t>(a, st) : route_launch<float>(a, st);
-  if (given(la, 2)) {
-    OrderArgs o = {};
-    o.ids = a.ids;
-    o.offsets = reinterpret_cast<int*>(la.a[2].ptr);
-    o.rows_of = reinterpret_cast<int*>(la.a[3].ptr);
-    o.row_at = reinterpret_cast<int*>(la.a[4].ptr);
-    o.n = a.T * a.top;
-    o.E = a.E;
-    o.top = a.top;
-    const size_t smem = sizeof(int) * ((kOrderWarps + 2) * (size_t)a.E + 32);
-    if (smem > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(order_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return fail(MTL_ERR_CUDA, "route_experts: %s", cudaGetErrorString(e));
-    }
-    order_rows_kernel<<<1, kOrderWarps * 32, smem, st>>>(o);
+  const bool bf16 = la.a[15].i32, vec = la.a[5].ptr % 16 == 0 && (int64_t)a.E * (bf16 ? 2 : 4) % 16 == 0, ordering = given(la, 2);
+  OrderArgs o = {};
+  o.ids = a.ids;
+  o.offsets = reinterpret_cast<int*>(la.a[2].ptr);
+  o.rows_of = reinterpret_cast<int*>(la.a[3].ptr);
+  o.row_at = reinterpret_cast<int*>(la.a[4].ptr);
+  o.n = a.T * a.top;
+  o.E = a.E;
+  o.top = a.top;
+  cudaError_t e = bf16 ? route_launch<uint16_t>(a, ordering ? &o : nullptr, vec, la.device, st) : route_launch<float>(a, ordering ? &o : nullptr, vec, la.device, st);
+  if (e == cudaSuccess && ordering && !few_tokens(a)) {
+    static unsigned long long done;
+    // as many clusters as a warp has steps of 32 slots, so that each places one or few
+    const unsigned ctas = a.T ? RORDER : 1, clusters = (unsigned)std::max<int64_t>(1, std::min<int64_t>(RCLUST, o.n / (32 * kOrderWarps * ctas)));
+    e = cluster_launch(order_rows_kernel, ctas, clusters, order_shared(a.E), a.T > 0, la.device, &done, st, o);
   }
+  if (e != cudaSuccess) return fail(MTL_ERR_CUDA, "route_experts: %s", cudaGetErrorString(e));
   return launched("route_experts");
 }
 

@@ -28,6 +28,7 @@ everything else. Nothing here falls back to a CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 import math
 import operator
 import struct
@@ -622,6 +623,7 @@ _KINDS = {np.dtype(t): k + "*" for k, types in {"45": (np.uint8, np.int8), "f": 
 _KIND_NAMES = {"4": "8-bit codes in e4m3", "5": "8-bit codes in e5m2", "f": "Float32", "h": "bfloat16", "i": "Int32"}
 _PTR = L.ARG_PTR
 _tensor = _current_device = None  # torch.Tensor, torch.cuda.current_device, once torch is loaded
+_short_launch = _short_plan = None  # of _launch.so, where it was built
 
 
 def _with_torch() -> None:
@@ -632,6 +634,12 @@ def _with_torch() -> None:
                         "h": ("bfloat16", "uint16", "int16"), "i": ("int32",)}.items():
         _KINDS.update({getattr(torch, n): kind + "*" for n in names if hasattr(torch, n)})
     _tensor = torch.Tensor
+    try:
+        short = importlib.import_module("._launch", __name__)
+    except ImportError:  # launches with tensors cost the host more, and that is all
+        return
+    global _short_launch, _short_plan
+    _short_launch, _short_plan = short.launch, short.plan
 
 
 def _wanted(k: Kernel, args: Sequence) -> str:
@@ -691,6 +699,15 @@ def _operands(k: Kernel, args: Sequence, graph: bool = False) -> list:
     return flat
 
 
+def _short(k: Kernel):
+    """What _launch.launch checks of a launch of `k` with tensors (csrc/python/launch.cpp):
+    _OPERANDS' letters, and the argument that each of o, t, p and q goes by."""
+    letters, flags = _OPERANDS[k.name]
+    p = k.packed
+    p.short = _short_plan(C.cast(p.entry, C.c_void_p).value, k.id, k.signature, letters, tuple(flags.get(c, -1) for c in letters))
+    return p.short
+
+
 def _scratch(k: Kernel, x) -> tuple[int, int]:
     """Address and bytes of a launch's scratch, with an operand's checks but for the type."""
     if isinstance(x, DevicePtr):
@@ -719,6 +736,7 @@ class _Packed:
         self.entry.restype = C.c_int32
         self.entry.argtypes = [C.c_int32, C.c_char_p, C.c_int32, C.c_char_p, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
         self.buffers = len(_OPERANDS[k.name][0])
+        self.short = None  # see _short
         self.scalars = [v for s in k.signature[self.buffers:] for v in (L.ARG_F32 if s == "f" else L.ARG_I32, 0, 0, 0)]
 
     def range_of(self, nd: tuple) -> bytes:
@@ -774,6 +792,12 @@ def launch(kernel, args: Sequence, ndrange, stream: int = 0, workspace=None) -> 
     workspace_bytes asks for, not shared by launches that may run at once."""
     k = kernel if isinstance(kernel, Kernel) else _kernel(kernel)
     if k.packed is not None:
+        if _short_launch is not None:
+            status = _short_launch(k.packed.short or _short(k), args, ndrange, stream, workspace)
+            if status == 0:
+                return
+            if status is not None:
+                check(status)
         return k.packed(args, ndrange, stream, workspace)
     arr = (L.Arg * max(len(args), 1))(*[_arg(None, x, s) for x, s in zip(args, k.signature)])
     nd = _nd(ndrange)
