@@ -58,6 +58,7 @@ struct RouteArgs {
   int E, top, groups, top_groups, best;
   int sigmoid, renorm;
   float scale;
+  int cut, lanes, each;  // route_token: the runs that lie on lanes, the lanes of one, the experts of a lane
 };
 
 // Keys as integers of the same order, -0 as 0.
@@ -230,9 +231,10 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, K (&key)[P], uns
 }
 
 // The expert of slot `lane`: one choice after the other, the largest key, its lowest index.
+// This lane holds experts first, first + 1, ..., later lanes later ones.
 template <int P, typename K>
-__device__ __forceinline__ int choose(int top, K (&key)[P]) {
-  const int lane = threadIdx.x & 31, first = lane * P;
+__device__ __forceinline__ int choose(int top, K (&key)[P], int first) {
+  const int lane = threadIdx.x & 31;
   K mine = Key<K>::kNone;
 #pragma unroll
   for (int p = 0; p < P; ++p) mine = max(mine, key[p]);
@@ -257,13 +259,77 @@ __device__ __forceinline__ int choose(int top, K (&key)[P]) {
   return id;
 }
 
-// A token by a warp: lane i holds experts i P .. + P. `vec`: rows of logits on 16 bytes.
+// The choice with every key in 64 bits (or, without a bias, of logits): the expert of slot
+// `lane`. For the tokens that route_token's shorter way does not decide.
 template <typename T, int P>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsigned long long* values, bool vec) {
-  const int lane = threadIdx.x & 31, E = a.E, first = lane * P;
-  const T* logits = static_cast<const T*>(a.logits) + t * E;
+__device__ __noinline__ int choose_long(const RouteArgs& a, const T* logits, float most, unsigned long long* values) {
+  const int first = (threadIdx.x & 31) * P;
   float l[P];
-  if (vec && P * sizeof(T) >= 16 && first + P <= E) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) l[p] = first + p < a.E ? to_f32(logits[first + p]) : -INFINITY;
+  if (!a.bias) {
+    uint32_t key[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) key[p] = Key32::of(l[p]);
+    if (a.groups > 1) keep_groups<P>(a, key, values, [&](uint32_t k) { return score_64(Key32::value(k), a.sigmoid, most); });
+    return choose<P>(a.top, key, first);
+  }
+  unsigned long long key[P];
+  double s[P], over = 1.0;
+#pragma unroll
+  for (int p = 0; p < P; ++p) s[p] = score_64(l[p], a.sigmoid, most);
+  if (!a.sigmoid) {
+    over = 0.0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) over += s[p];
+    over = __drcp_rn(warp_sum(over));
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) key[p] = l[p] == -INFINITY ? Key64::kNone : Key64::of(fma(s[p], over, (double)a.bias[first + p]));
+  if (a.groups > 1) keep_groups<P>(a, key, values, [](unsigned long long k) { return Key64::value(k); });
+  return choose<P>(a.top, key, first);
+}
+
+// A score for the choice, with the fast exponential and reciprocal. With x its argument the
+// exponential is off by (2 + 1.2 |x|) 2^-23 of itself. A sigmoid s moves by s (1 - s) as much, where
+// s (1 - s) |x| <= 0.23, and by 1.5 2^-23 of itself for the sum and the reciprocal: 2.3 2^-23 in all. A
+// probability p = e^-D / total moves by (2 + 1.7 D) 2^-23 of itself, where D p <= 0.4 pmax, and with
+// its total, which is off by 34 2^-23 of itself (the mean of D is below ln E, and 37 additions).
+__device__ __forceinline__ float quick_score(float l, int sigmoid, float most, float part) {
+  return sigmoid ? __frcp_rn(1.0f + __expf(-l)) : __expf(l - most) * part;
+}
+// How far a key in 32 bits may then be from its 64-bit value, with the rounding of its sum
+// with a bias of up to bmax. pmax is `part`.
+__device__ __forceinline__ float key_bound(int sigmoid, float part, float bmax) { return (sigmoid ? 0x1p-21f : 0x1p-17f * part) + 0x1p-23f * bmax; }
+
+// softmax's 1 / (sum over the experts) in 64 bits, for score_64; 1 for sigmoid.
+template <typename T>
+__device__ __noinline__ double over_of(const RouteArgs& a, const T* logits, int first, int per, float most) {
+  if (a.sigmoid) return 1.0;
+  double sum = 0.0;
+#pragma unroll 1
+  for (int e = first; e < first + per; ++e) sum += score_64(to_f32(logits[e]), 0, most);
+  return __drcp_rn(warp_sum(sum));
+}
+
+// A token by a warp. A group lies on a.lanes lanes, a power of two, each with a.each of its
+// experts or fewer, P at most; where there are more groups than lanes all experts lie so as one
+// (a.cut). `vec`: rows of logits on 16 bytes.
+//
+// Without a bias keys are logits, and exact. With one they are 32-bit at first, off by `off`.
+// At least `top` of them are no less than the top-th largest of the lanes' largest, so
+// those that are, or are 2 off below, ten or so, are all that the choice can turn on: a lane
+// each, ranked by comparing each with all, and where two are within 2 off in 64 bits (a few
+// tokens of a thousand). Groups are compared likewise. With more candidates than lanes, or
+// groups, choose_long. One choice after the other with all keys in
+// 64 bits took 30 us for 8192 tokens of 256 experts, a third of it 64-bit arithmetic; this 17.
+template <typename T, int P>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsigned long long* values, int* candidates, bool vec) {
+  const int lane = threadIdx.x & 31, size = a.E / a.cut, g = lane / a.lanes, from = lane % a.lanes * a.each;
+  const int first = g * size + from, own = g < a.cut ? min(size - from, a.each) : 0;  // (own may be below 0)
+  const T* logits = static_cast<const T*>(a.logits) + t * a.E;
+  float l[P];
+  if (vec && P * sizeof(T) >= 16 && a.each == P && own == P && first % P == 0) {
     constexpr int kEach = 16 / (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < P / kEach; ++i) {
@@ -279,11 +345,12 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
     }
   } else {
 #pragma unroll
-    for (int p = 0; p < P; ++p) l[p] = first + p < E ? to_f32(logits[first + p]) : -INFINITY;
+    for (int p = 0; p < P; ++p) l[p] = p < own ? to_f32(logits[first + p]) : -INFINITY;
   }
-  float b[P];
+  float b[P], bmax = 0.0f;
+  bool bad = false;
   if (a.bias) {
-    if (reinterpret_cast<uintptr_t>(a.bias) % 16 == 0 && P >= 4 && first + P <= E) {
+    if (reinterpret_cast<uintptr_t>(a.bias) % 16 == 0 && P >= 4 && own == P && first % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < P / 4; ++i) {
         const float4 f = reinterpret_cast<const float4*>(a.bias + first)[i];
@@ -291,65 +358,205 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
       }
     } else {
 #pragma unroll
-      for (int p = 0; p < P; ++p) b[p] = first + p < E ? a.bias[first + p] : 0.0f;
+      for (int p = 0; p < P; ++p) b[p] = p < own ? a.bias[first + p] : 0.0f;
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      bad |= isnan(b[p]);
+      if (fabsf(b[p]) < INFINITY) bmax = fmaxf(bmax, fabsf(b[p]));
     }
   }
   const bool live = !a.live || a.live[t];
-  bool bad = false;
   uint32_t key[P], most_key = Key32::kNone;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    bad |= isnan(l[p]) || (a.bias && isnan(b[p]));
+    bad |= isnan(l[p]);
     key[p] = Key32::of(l[p]);
     most_key = max(most_key, key[p]);
   }
   const float most = Key32::value(Key32::most(most_key));
   bad = __any_sync(0xffffffffu, bad || (!a.sigmoid && most == INFINITY));
+  int* ids = a.ids + t * a.top;
+  float* weights = a.weights + t * a.top;
   if (bad || !live || most == -INFINITY) {
     if (lane < a.top) {
-      a.ids[t * a.top + lane] = -1;
-      a.weights[t * a.top + lane] = bad && live ? NAN : 0.0f;
+      ids[lane] = -1;
+      weights[lane] = bad && live ? NAN : 0.0f;
     }
     return;
   }
-  float total = 1.0f;
-  if (!a.sigmoid && !a.renorm) {
+  const bool sums = a.groups > 1 && a.best > 1;  // group values are sums of scores
+  float total = 1.0f, part = 1.0f, off = 0.0f;
+  if (!a.sigmoid && (a.bias || sums || !a.renorm)) {
     total = 0.0f;
 #pragma unroll
-    for (int p = 0; p < P; ++p) total += expf(l[p] - most);
+    for (int p = 0; p < P; ++p) total += a.renorm ? __expf(l[p] - most) : expf(l[p] - most);
     total = warp_sum(total);
+    part = 1.0f / total;
   }
-  int id;
+  if (a.bias || sums) {
+    if (a.bias) bmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bmax)));
+    off = key_bound(a.sigmoid, part, bmax);
+  }
   if (a.bias) {
-    unsigned long long wide[P];
-    double s[P], over = 1.0;
 #pragma unroll
-    for (int p = 0; p < P; ++p) s[p] = score_64(l[p], a.sigmoid, most);
-    if (!a.sigmoid) {
-      over = 0.0;
+    for (int p = 0; p < P; ++p) key[p] = l[p] == -INFINITY ? Key32::kNone : Key32::of(quick_score(l[p], a.sigmoid, most, part) + b[p]);
+  }
+  bool sure = true;
+  if (a.groups > 1) {
+    const int lanes = a.lanes;
+    sure = a.cut == a.groups;
+    if (sure) {
+      Best<uint32_t> best;
 #pragma unroll
-      for (int p = 0; p < P; ++p) over += s[p];
-      over = __drcp_rn(warp_sum(over));
+      for (int p = 0; p < P; ++p) best.add(key[p]);
+      for (int d = 1; d < lanes; d *= 2) {
+        Best<uint32_t> o;
+        o.one = __shfl_xor_sync(0xffffffffu, best.one, d);
+        o.two = __shfl_xor_sync(0xffffffffu, best.two, d);
+        best.add(o);
+      }
+      uint32_t mine = best.one;
+      if (sums && mine != Key32::kNone) {
+        const auto worth = [&](uint32_t k) { return a.bias ? Key32::value(k) : quick_score(Key32::value(k), a.sigmoid, most, part); };
+        mine = Key32::of(worth(best.one) + (best.two != Key32::kNone ? worth(best.two) : 0.0f));
+      }
+      int ahead = 0;
+      for (int o = 0; o < a.groups; ++o) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, o * lanes);
+        ahead += other > mine || (other == mine && o < g);
+      }
+      bool stays = ahead < a.top_groups;
+      if (a.bias || sums) {
+        // a sum of two is off by twice as much, and by its own rounding
+        const uint32_t kept = __reduce_min_sync(0xffffffffu, stays ? mine : 0xffffffffu);
+        const uint32_t dropped = __reduce_max_sync(0xffffffffu, stays || g >= a.groups ? Key32::kNone : mine);
+        if (dropped != Key32::kNone && Key32::value(kept) - Key32::value(dropped) <= 5.0f * off) {
+          // the keys that may be a group's best, in 64 bits, and the groups compared so
+          const uint32_t last = sums ? best.two : best.one;
+          const uint32_t least = last == Key32::kNone ? last + 1 : Key32::of(Key32::value(last) - (a.bias ? 2.0f * off : 0.0f));
+          uint32_t which = 0;
+#pragma unroll
+          for (int p = 0; p < P; ++p) which |= (uint32_t)(key[p] >= least && key[p] != Key32::kNone) << p;
+          const double over = a.bias ? over_of(a, logits, first, own, most) : 1.0;
+          Best<unsigned long long> wide;
+          while (__any_sync(0xffffffffu, which)) {
+            if (which) {
+              const int e = first + __ffs(which) - 1;
+              const float x = to_f32(logits[e]);
+              wide.add(Key64::of(a.bias ? fma(score_64(x, a.sigmoid, most), over, (double)a.bias[e]) : (double)x));
+              which &= which - 1;
+            }
+          }
+          for (int d = 1; d < lanes; d *= 2) {
+            Best<unsigned long long> o;
+            o.one = __shfl_xor_sync(0xffffffffu, wide.one, d);
+            o.two = __shfl_xor_sync(0xffffffffu, wide.two, d);
+            wide.add(o);
+          }
+          unsigned long long value = wide.one;
+          if (sums && value != Key64::kNone) {
+            const auto worth = [&](unsigned long long k) { return a.bias ? Key64::value(k) : score_64((float)Key64::value(k), a.sigmoid, most); };
+            value = Key64::of(worth(wide.one) + (wide.two != Key64::kNone ? worth(wide.two) : 0.0));
+          }
+          ahead = 0;
+          for (int o = 0; o < a.groups; ++o) {
+            const unsigned long long other = __shfl_sync(0xffffffffu, value, o * lanes);
+            ahead += other > value || (other == value && o < g);
+          }
+          stays = ahead < a.top_groups;
+        }
+      }
+      if (!stays) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) key[p] = Key32::kNone;
+      }
     }
+  }
+  int id = -1, place = lane, count = 0;
+  if (sure && !a.bias) {  // keys are exact
+    id = choose<P>(a.top, key, first);
+    count = __popc(__ballot_sync(0xffffffffu, id >= 0));
+  } else if (sure) {
+    // the top-th largest of the lanes' largest: a bitonic sort of them, the largest first
+    uint32_t sorted = Key32::kNone;
 #pragma unroll
-    for (int p = 0; p < P; ++p) wide[p] = l[p] == -INFINITY ? Key64::kNone : Key64::of(fma(s[p], over, (double)b[p]));
-    if (a.groups > 1) keep_groups<P>(a, wide, values, [](unsigned long long k) { return Key64::value(k); });
-    id = choose<P>(a.top, wide);
-  } else {
-    if (a.groups > 1) keep_groups<P>(a, key, values, [&](uint32_t k) { return score_64(Key32::value(k), a.sigmoid, most); });
-    id = choose<P>(a.top, key);
+    for (int p = 0; p < P; ++p) sorted = max(sorted, key[p]);
+#pragma unroll
+    for (int run = 2; run <= 32; run *= 2)
+#pragma unroll
+      for (int d = run / 2; d; d /= 2) {
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, sorted, d);
+        const bool larger = !(lane & d) == !(lane & run);
+        sorted = larger ? max(sorted, o) : min(sorted, o);
+      }
+    uint32_t least = __shfl_sync(0xffffffffu, sorted, a.top - 1);
+    if (least != Key32::kNone) least = Key32::of(Key32::value(least) - 2.0f * off);
+    least = max(least, Key32::kNone + 1);
+    int mine = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) mine += key[p] >= least;
+    int before = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before += o;
+    }
+    count = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine;
+    sure = count <= 32;
+    if (sure) {
+      // candidate i is lane i's, by rising index
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (key[p] >= least) {
+          candidates[before] = first + p;
+          candidates[32 + before++] = (int)key[p];
+        }
+      __syncwarp();
+      if (lane < count) id = candidates[lane];
+      const uint32_t k = lane < count ? (uint32_t)candidates[32 + lane] : Key32::kNone;
+      __syncwarp();
+      const float chosen = id >= 0 ? to_f32(logits[id]) : -INFINITY, bias = id >= 0 ? a.bias[id] : 0.0f, value = Key32::value(k);
+      place = 0;
+      bool close = false;
+      for (int o = 0; o < count; ++o) {
+        const uint32_t other = __shfl_sync(0xffffffffu, k, o);
+        place += other > k || (other == k && o < lane);
+        close |= fabsf(Key32::value(other) - value) <= 2.0f * off && o != lane;
+      }
+      if (__any_sync(0xffffffffu, close && id >= 0)) {
+        const double over = over_of(a, logits, first, own, most);
+        const unsigned long long wide = id >= 0 ? Key64::of(fma(score_64(chosen, a.sigmoid, most), over, (double)bias)) : Key64::kNone;
+        place = 0;
+        for (int o = 0; o < count; ++o) {
+          const unsigned long long other = __shfl_sync(0xffffffffu, wide, o);
+          place += other > wide || (other == wide && o < lane);
+        }
+      }
+      if (place >= a.top) id = -1;
+    }
+  }
+  if (!sure) {
+    id = choose_long<T, P>(a, logits, most, values);
+    place = lane;
+    count = __popc(__ballot_sync(0xffffffffu, id >= 0));
   }
   const float chosen = id >= 0 ? to_f32(logits[id]) : -INFINITY;
   const float w = weight_of(chosen, id >= 0, most, total, a.sigmoid, a.renorm, a.scale);
-  if (lane < a.top) {
-    a.ids[t * a.top + lane] = id;
-    a.weights[t * a.top + lane] = w;
+  if (id >= 0) {
+    ids[place] = id;
+    weights[place] = w;
+  }
+  if (lane >= count && lane < a.top) {  // fewer than asked for
+    ids[lane] = -1;
+    weights[lane] = 0.0f;
   }
 }
 
 // ── the rows' order ─────────────────────────────────────────────────────────
-// A counting sort by one cluster. Each warp has a run of slots and a counter for each
-// expert; the counters' prefix sums over warps, then over CTAs (whose totals the others
+// A counting sort by a cluster. Each warp has a run of slots and a counter for each expert;
+// the counters' prefix sums over warps, then over CTAs (whose totals the others
 // read in their shared memory), then over experts give each warp where its rows of each
 // expert start. So the order is that of the slots whatever the warps' timing.
 constexpr int kOrderWarps = 32;
@@ -475,10 +682,11 @@ __device__ __forceinline__ void order_rows(const OrderArgs& a, int* shared, int6
 template <typename T, int P>
 __global__ void __launch_bounds__(128) route_kernel(RouteArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned long long values[];  // of a warp's groups
+  __shared__ int candidates[4][64];
   pdl_trigger();
   const int warp = threadIdx.x >> 5;
   const int64_t t = (int64_t)blockIdx.x * 4 + warp;
-  if (t < a.T) route_token<T, P>(a, t, values + warp * (a.groups > 1 ? a.groups : 0), vec);
+  if (t < a.T) route_token<T, P>(a, t, values + warp * (a.groups > 1 ? a.groups : 0), candidates[warp], vec);
 }
 // The order alone, by one cluster, behind it.
 __global__ void __launch_bounds__(kOrderWarps * 32) order_rows_kernel(OrderArgs a) {
@@ -493,12 +701,13 @@ __global__ void __launch_bounds__(kOrderWarps * 32) order_rows_kernel(OrderArgs 
 template <typename T, int P>
 __global__ void __launch_bounds__(kOrderWarps * 32) route_and_order_kernel(RouteArgs a, OrderArgs o, bool vec) {
   extern __shared__ __align__(16) int shared[];
+  __shared__ int candidates[kOrderWarps][64];
   const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const int warp = threadIdx.x >> 5;
   unsigned long long* values = reinterpret_cast<unsigned long long*>(shared) + warp * (a.groups > 1 ? a.groups : 0);
   const int64_t per = (a.T + cluster.num_blocks() - 1) / cluster.num_blocks();
   const int64_t lo = min(a.T, (int64_t)cluster.block_rank() * per), hi = min(a.T, lo + per);
-  for (int64_t t = lo + warp; t < hi; t += kOrderWarps) route_token<T, P>(a, t, values, vec);
+  for (int64_t t = lo + warp; t < hi; t += kOrderWarps) route_token<T, P>(a, t, values, candidates[warp], vec);
   __syncthreads();  // the ids are this CTA's own
   order_rows(o, shared, lo * a.top, hi * a.top, 0, 1);
 }
@@ -647,18 +856,13 @@ static cudaError_t cluster_launch(void (*kernel)(K...), unsigned ctas, unsigned 
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// One cluster chooses and orders up to this many tokens; beyond it more SMs' work on the
-// choice is worth a launch of its own for the order.
-#ifndef RFUSED
-#define RFUSED 256
-#endif
-constexpr int64_t kFewTokens = RFUSED;
-#ifndef RCLUST
-#define RCLUST 8
-#endif
-#ifndef RORDER
-#define RORDER 8
-#endif
+// One cluster chooses and orders up to this many tokens: one launch, which costs the host less
+// and an otherwise idle GPU no more (128 tokens of 64 experts 9.4 us, 7.4 in two; of 256
+// tokens and experts 13.7 and 10.1).
+constexpr int64_t kFewTokens = 128;
+// Else the order is made by clusters of eight CTAs, as many as a warp has steps of 32 slots,
+// so that each places one or few (65536 slots 16.8 us by one cluster, 10.8 by eight).
+constexpr unsigned kOrderCtas = 8, kOrderClusters = 8;
 
 static bool few_tokens(const RouteArgs& a) {
   return a.T > 0 && a.T <= kFewTokens && (a.groups == 1 || kOrderWarps * sizeof(unsigned long long) * a.groups <= kRouteShared);
@@ -669,19 +873,25 @@ static cudaError_t route_go(const RouteArgs& a, const OrderArgs* o, bool vec, in
   const size_t values = a.groups > 1 ? sizeof(unsigned long long) * a.groups : 0;
   if (o && few_tokens(a)) {
     static unsigned long long done;
-    const unsigned ctas = (unsigned)std::min<int64_t>(8, (a.T + kOrderWarps - 1) / kOrderWarps);
+    const unsigned ctas = (unsigned)std::min<int64_t>(kOrderCtas, (a.T + kOrderWarps - 1) / kOrderWarps);
     return cluster_launch(route_and_order_kernel<T, P>, ctas, 1, std::max(order_shared(a.E), kOrderWarps * values), false, device, &done, st, a, *o, vec);
   }
   if (a.T) route_kernel<T, P><<<(unsigned)((a.T + 3) / 4), 128, 4 * values, st>>>(a, vec);
   return cudaSuccess;
 }
 template <typename T>
-static cudaError_t route_launch(const RouteArgs& a, const OrderArgs* o, bool vec, int device, cudaStream_t st) {
-  if (a.E <= 32) return route_go<T, 1>(a, o, vec, device, st);
-  if (a.E <= 64) return route_go<T, 2>(a, o, vec, device, st);
-  if (a.E <= 128) return route_go<T, 4>(a, o, vec, device, st);
-  if (a.E <= 256) return route_go<T, 8>(a, o, vec, device, st);
-  if (a.E <= 512) return route_go<T, 16>(a, o, vec, device, st);
+static cudaError_t route_launch(RouteArgs a, const OrderArgs* o, bool vec, int device, cudaStream_t st) {
+  a.cut = a.groups;
+  a.lanes = 1;
+  while (a.lanes * 2 * a.cut <= 32) a.lanes *= 2;
+  a.each = (a.E / a.cut + a.lanes - 1) / a.lanes;
+  if (a.cut > 32 || a.each > 32) a.cut = 1, a.lanes = 32, a.each = (a.E + 31) / 32;
+  const int most = std::max(a.each, (a.E + 31) / 32);  // of a lane, choose_long's among them
+  if (most <= 1) return route_go<T, 1>(a, o, vec, device, st);
+  if (most <= 2) return route_go<T, 2>(a, o, vec, device, st);
+  if (most <= 4) return route_go<T, 4>(a, o, vec, device, st);
+  if (most <= 8) return route_go<T, 8>(a, o, vec, device, st);
+  if (most <= 16) return route_go<T, 16>(a, o, vec, device, st);
   return route_go<T, 32>(a, o, vec, device, st);
 }
 
@@ -714,8 +924,7 @@ mtl_status route_experts_run(const LaunchArgs& la, void*, uint64_t, void* stream
   cudaError_t e = bf16 ? route_launch<uint16_t>(a, ordering ? &o : nullptr, vec, la.device, st) : route_launch<float>(a, ordering ? &o : nullptr, vec, la.device, st);
   if (e == cudaSuccess && ordering && !few_tokens(a)) {
     static unsigned long long done;
-    // as many clusters as a warp has steps of 32 slots, so that each places one or few
-    const unsigned ctas = a.T ? RORDER : 1, clusters = (unsigned)std::max<int64_t>(1, std::min<int64_t>(RCLUST, o.n / (32 * kOrderWarps * ctas)));
+    const unsigned ctas = a.T ? kOrderCtas : 1, clusters = (unsigned)std::max<int64_t>(1, std::min<int64_t>(kOrderClusters, o.n / (32 * kOrderWarps * ctas)));
     e = cluster_launch(order_rows_kernel, ctas, clusters, order_shared(a.E), a.T > 0, la.device, &done, st, o);
   }
   if (e != cudaSuccess) return fail(MTL_ERR_CUDA, "route_experts: %s", cudaGetErrorString(e));

@@ -212,7 +212,8 @@ def test_route(dev, t, e, top, score, renorm, kind):
 @pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
 @pytest.mark.parametrize("t,e,top,groups,top_groups,best", [
     (40, 256, 8, 8, 4, 2), (40, 64, 6, 8, 3, 1), (33, 160, 6, 8, 3, 1), (20, 96, 4, 6, 2, 2), (7, 16, 2, 16, 4, 1), (9, 1024, 8, 32, 5, 2),
-    (5, 1024, 8, 1024, 9, 1), (5, 1000, 8, 200, 3, 2), (6, 8, 8, 4, 2, 2), (50, 256, 8, 4, 4, 2)])
+    (5, 1024, 8, 1024, 9, 1), (5, 1000, 8, 200, 3, 2), (6, 8, 8, 4, 2, 2), (50, 256, 8, 4, 4, 2), (40, 148, 5, 4, 2, 2),
+    (9, 1023, 7, 31, 4, 2), (9, 992, 7, 31, 4, 1), (30, 33, 3, 11, 3, 2), (12, 24, 2, 3, 1, 1)])
 def test_route_in_groups(dev, t, e, top, groups, top_groups, best, score, kind):
     g = dict(groups=groups, top_groups=top_groups, best=best)
     l = 2 * normal(t, e, seed=e, kind=kind)
