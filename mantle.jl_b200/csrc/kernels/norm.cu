@@ -236,8 +236,9 @@ struct NormGradArgs {
   float eps;
 };
 
-// The CTAs that an SM holds: the registers are dealt out for as many.
-constexpr int grad_residents(int most, int N) { return most == 32 ? (N == 4 ? 3 : N == 2 ? 5 : 8) : most == 128 ? 4 : most == 256 ? 2 : most == 384 ? 2 : 1; }
+// The CTAs that an SM holds: the registers are dealt out for as many, about a hundred a
+// thread (at 80 the spills took 1023 x 5001 float from 20 to 22 us, 4092 rows from 48 to 61).
+constexpr int grad_residents(int most, int N) { return most == 32 ? (N == 4 ? 3 : N == 2 ? 5 : 8) : most == 128 ? 4 : most <= 320 ? 2 : 1; }
 
 // The sums of two values over the row's threads, in a fixed order. `part`: two slots a warp.
 template <bool WARP>
@@ -430,7 +431,7 @@ static GradShape grad_shape(int64_t R, int C, int size, bool dres, int sms) {
   g.N = eights <= 32 ? 1 : eights <= 64 ? 2 : eights <= 128 ? 4 : eights <= 2048 ? 2 : 4;
   g.threads = g.rows == 4 ? 32 : (eights + 32 * g.N - 1) / (32 * g.N) * 32;
   g.most = g.threads;
-  for (int most : {32, 128, 256, 384, 512, 1024})
+  for (int most : {32, 128, 256, 320, 512, 640, 1024})
     if (g.threads <= most) {
       g.most = most;
       break;
@@ -466,8 +467,9 @@ static cudaError_t norm_grad_launch(const NormGradArgs& a, const GradShape& g, c
   if (g.N == 4) return norm_grad_go<T, 4, 1024, PHASED, false>(a, g, st);
   if (g.most == 128) return norm_grad_go<T, 2, 128, PHASED, RING>(a, g, st);
   if (g.most == 256) return norm_grad_go<T, 2, 256, PHASED, RING>(a, g, st);
-  if (g.most == 384) return norm_grad_go<T, 2, 384, PHASED, RING>(a, g, st);
+  if (g.most == 320) return norm_grad_go<T, 2, 320, PHASED, RING>(a, g, st);
   if (g.most == 512) return norm_grad_go<T, 2, 512, PHASED, RING>(a, g, st);
+  if (g.most == 640) return norm_grad_go<T, 2, 640, PHASED, RING>(a, g, st);
   return norm_grad_go<T, 2, 1024, PHASED, RING>(a, g, st);
 }
 
