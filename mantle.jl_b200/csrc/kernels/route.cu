@@ -132,6 +132,10 @@ __device__ __forceinline__ double score_64(float l, int sigmoid, float most) {
   return l < 0.0f ? e * r : r;
 }
 
+// The score's sum with the bias, each rounded for itself: where the bias is so large that it
+// decides by rounding, scores that differ less than that are one.
+__device__ __forceinline__ double biased(double score, float bias) { return __dadd_rn(score, (double)bias); }
+
 // The weights of a token's chosen experts: lane j has slot j's logit.
 __device__ __forceinline__ float weight_of(float l, bool valid, float most, float total, int sigmoid, int renorm, float scale) {
   float s;
@@ -285,7 +289,7 @@ __device__ __noinline__ int choose_long(const RouteArgs& a, const T* logits, flo
     over = __drcp_rn(warp_sum(over));
   }
 #pragma unroll
-  for (int p = 0; p < P; ++p) key[p] = l[p] == -INFINITY ? Key64::kNone : Key64::of(fma(s[p], over, (double)a.bias[first + p]));
+  for (int p = 0; p < P; ++p) key[p] = l[p] == -INFINITY ? Key64::kNone : Key64::of(biased(s[p] * over, a.bias[first + p]));
   if (a.groups > 1) keep_groups<P>(a, key, values, [](unsigned long long k) { return Key64::value(k); });
   return choose<P>(a.top, key, first);
 }
@@ -444,7 +448,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
             if (which) {
               const int e = first + __ffs(which) - 1;
               const float x = to_f32(logits[e]);
-              wide.add(Key64::of(a.bias ? fma(score_64(x, a.sigmoid, most), over, (double)a.bias[e]) : (double)x));
+              wide.add(Key64::of(a.bias ? biased(score_64(x, a.sigmoid, most) * over, a.bias[e]) : (double)x));
               which &= which - 1;
             }
           }
@@ -527,7 +531,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
       }
       if (__any_sync(0xffffffffu, close && id >= 0)) {
         const double over = over_of(a, logits, first, own, most);
-        const unsigned long long wide = id >= 0 ? Key64::of(fma(score_64(chosen, a.sigmoid, most), over, (double)bias)) : Key64::kNone;
+        const unsigned long long wide = id >= 0 ? Key64::of(biased(score_64(chosen, a.sigmoid, most) * over, bias)) : Key64::kNone;
         place = 0;
         for (int o = 0; o < count; ++o) {
           const unsigned long long other = __shfl_sync(0xffffffffu, wide, o);
@@ -755,6 +759,7 @@ __global__ void __launch_bounds__(128) route_grad_kernel(RouteGradArgs a) {
   }
   const float u = weight_of(l, valid, most, total, a.sigmoid, a.renorm, 1.0f);
   const float mean = a.sigmoid && !a.renorm ? 0.0f : warp_sum(g * u);
+  __syncwarp();  // the row is read: dlogits may be the logits' own memory
   float d;
   if (dense) {
     // an expert named twice: its slots' gradients together

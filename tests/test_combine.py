@@ -217,8 +217,48 @@ def test_nothing_to_combine(dev):
     combine(e(6, 0), e(3, 2), i(3, 2), None, 0, F)
     assert (combine(e(0, 64), torch.ones(3, 2, device="cuda"), i(3, 2), None, 64, F) == 0).all()
     grad(e(0, 64), e(6, 64), e(0, 2), i(0, 2), i(6))
+    _, dw = grad(e(3, 64), e(0, 64), e(3, 2), i(3, 2), i(0))  # no rows at all
+    assert (dw == 0).all()
     _, dw = grad(e(3, 0), e(6, 0), e(3, 2), i(3, 2), i(6))
     assert (dw == 0).all()
+
+
+@pytest.mark.gpu
+def test_captured_and_at_once(dev):
+    t, top, c = 500, 3, 1160
+    at, of = places(t, top, 1, 0.1)
+    rows, w, dy = values((t * top, c), H, 1), values((t, top), F, 2), values((t, c), H, 3)
+    want, (drows, dw) = combine(rows, w, at, dy, c, H), grad(dy, rows, w, at, of)
+    outs = [(torch.zeros_like(want), torch.full_like(drows, 7.0), torch.zeros_like(dw)) for _ in range(2)]
+    graphs, sides = [], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for (y, d, e), side in zip(outs, sides):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            M.launch(M.kernels.combine_experts, (y, rows, w, at, dy, t * top, c, top, 1, 1), t, stream=stream())
+            M.launch(M.kernels.combine_experts_grad, (d, e, dy, rows, w, at, of, t * top, c, top, 1, 1), t, stream=stream())
+        graphs.append(g)
+    for _ in range(3):
+        for g, side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for y, d, e in outs:
+        assert torch.equal(y, want) and torch.equal(d, drows) and torch.equal(e, dw)
+
+
+@pytest.mark.gpu
+def test_types_and_scratch_are_refused(dev):
+    at, of = places(4, 2, 1)
+    rows, w, y = values((8, 64), F, 1), values((4, 2), F, 2), torch.empty((4, 64), device="cuda")
+    go = lambda *a, kind=0, ykind=0: M.launch(M.kernels.combine_experts, (*a, 8, 64, 2, kind, ykind), 4, stream=stream())  # noqa: E731
+    go(y, rows, w, at, None)
+    for args, kw, match in (((y, rows.to(H), w, at, None), {}, "expected Float32"), ((y, rows, w, at, None), {"kind": 1}, "expected bfloat16"),
+                            ((y, rows, w, at, None), {"ykind": 1}, "expected bfloat16"), ((y, rows, w.to(H), at, None), {}, "expected Float32"),
+                            ((y, rows, w, at.long(), None), {}, "expected Int32"), ((y, rows, w, at, y.to(H)), {}, "expected Float32"),
+                            ((y, rows.t().contiguous().t(), w, at, None), {}, "contiguous"), ((y, rows, w, at.cpu(), None), {}, "current device")):
+        with pytest.raises(M.ArgumentError, match=match):
+            go(*args, **kw)
 
 
 @pytest.mark.gpu

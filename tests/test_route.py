@@ -274,6 +274,36 @@ def test_keys_that_32_bits_do_not_tell_apart(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+def test_biases_that_are_large_or_infinite(dev, score):
+    l = normal(130, 48, seed=3)
+    b = 0.05 * normal(48, seed=4)
+    for change in ({3: float("inf")}, {3: float("inf"), 40: float("inf")}, {5: float("-inf"), 6: float("inf")}, {i: 1e30 for i in range(0, 48, 2)},
+                   {i: 4096.0 for i in range(10)}, {i: -3e38 for i in range(44)}):
+        x = b.clone()
+        for i, v in change.items():
+            x[i] = v
+        check(l, 6, score, 1, bias=x)
+        check(l, 6, score, 0, bias=x, groups=4, top_groups=2, best=2)
+        check(l, 6, score, 0, bias=x, groups=4, top_groups=2, best=1)
+    check(l, 32, score, 1, bias=b)  # a slot for every lane
+    check(l.to(H), 32, score, 1, bias=torch.zeros(48))  # and many ties
+    check(torch.zeros(5, 700), 32, score, 1, bias=torch.zeros(700))  # more equal keys than lanes
+    check(torch.zeros(5, 700), 32, score, 1, bias=torch.zeros(700), groups=7, top_groups=3, best=2)
+    check(torch.zeros(5, 700), 32, score, 1, groups=7, top_groups=3, best=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [32, 33, 127, 128, 129, 1023, 1025])
+def test_few_tokens_and_many_are_one(dev, t):
+    # one launch or two, one cluster or several: the same, token by token
+    l, b = normal(t, 40, seed=1), 0.1 * normal(40, seed=2)
+    check(l, 5, SIGMOID, 1, 2.5, bias=b, groups=5, top_groups=3, best=2)
+    live = (torch.arange(t) % 5 != 2).to(torch.int32)
+    check(l, 5, SOFTMAX, 0, live=live)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t,e,top", [(0, 8, 2), (1, 1, 1), (3000, 8, 2), (2049, 16, 8), (1500, 300, 32), (9000, 1024, 2), (40000, 256, 8), (70000, 3, 1)])
 def test_rows_in_order(dev, t, e, top):
     # slots in order within an expert, experts of very different sizes, some empty, and dead tokens between
@@ -343,6 +373,12 @@ def test_route_grad(dev, t, e, top, score, renorm, kind):
     check_grad(l, torch.full_like(ids, -1), g, score, renorm, 1.0)
     same = torch.zeros_like(ids) + e - 1  # one expert in every slot: the slots' gradients together
     check_grad(l, same.to(torch.int32), g, score, renorm, 1.0)
+    for way in ((l, ids.to(torch.int32)), (l.to(F), torch.zeros_like(ids).to(torch.int32))):  # over the logits themselves
+        x, i = way[0].cuda(), way[1].cuda()
+        want = grad(x, i, g.cuda(), score, renorm, 1.5)
+        M.launch(M.kernels.route_experts_grad, (x, g.cuda(), x, i, e, top, score, renorm, int(x.dtype == H), 1.5), t, stream=stream())
+        # (rows whose chosen experts are masked, every one, are 0 / 0 over their sum)
+        assert torch.equal(x.nan_to_num(9), want.nan_to_num(9))
     outside = torch.full((t, top), e, dtype=torch.int32)
     assert torch.equal(grad(l.cuda(), outside.cuda(), g.cuda(), score, renorm, 1.0), torch.zeros_like(l).cuda())
 
