@@ -81,8 +81,8 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(
 // eights a thread, which stay in registers between the sum and the outputs, so each value
 // is read once. Bound by HBM: 8192 x 4096 bf16 with the residual, h, y and codes (303 MB)
 // 49.5 us, 6.1 TB/s, 93 % of a plain copy's rate. Rows off 16 bytes are bound by the
-// instructions of going value by value: 5001 x 4013 float 33 us, 4.9 TB/s, 8192 x 4095 bf16
-// with the residual 77 us.
+// instructions of going value by value: 5001 x 4013 float 29 us, 5.6 TB/s, 8192 x 4095 bf16
+// with the residual 63 us.
 template <typename T, int B, int N, bool VEC>
 __global__ void __launch_bounds__(B == 32 ? 128 : B) rms_norm_kernel(NormArgs a) {
   __shared__ float part[B == 32 ? 1 : B / 32];
@@ -205,6 +205,10 @@ static void norm_launch(const NormArgs& a, int sms, cudaStream_t st) {
       rms_norm_kernel<T, 1024, 1, VEC><<<rows, 1024, 0, st>>>(a);
     return;
   }
+  // Four eights a thread on 16 bytes; two off them, where four take a hundred registers and
+  // leave too few threads (5001 x 4013 float 33 -> 29 us, 8192 x 4095 bf16 with the residual
+  // 77 -> 63, with codes 112 -> 86; on 16 bytes two take 34 us for four's 31 of 8192 x 4096 float
+  // to codes).
   if (a.C <= 256)
     rms_norm_kernel<T, 32, 1, VEC><<<four, dim3(32, 4), 0, st>>>(a);
   else if (a.C <= 512)
@@ -214,9 +218,9 @@ static void norm_launch(const NormArgs& a, int sms, cudaStream_t st) {
   else if (a.C <= 2048)
     rms_norm_kernel<T, 128, 2, VEC><<<rows, 128, 0, st>>>(a);
   else if (a.C <= 4096)
-    rms_norm_kernel<T, 128, 4, VEC><<<rows, 128, 0, st>>>(a);
+    rms_norm_kernel<T, VEC ? 128 : 256, VEC ? 4 : 2, VEC><<<rows, VEC ? 128 : 256, 0, st>>>(a);
   else if (a.C <= 8192)
-    rms_norm_kernel<T, 256, 4, VEC><<<rows, 256, 0, st>>>(a);
+    rms_norm_kernel<T, VEC ? 256 : 512, VEC ? 4 : 2, VEC><<<rows, VEC ? 256 : 512, 0, st>>>(a);
   else if (a.C <= 16384)
     rms_norm_kernel<T, 512, 4, VEC><<<rows, 512, 0, st>>>(a);
   else
