@@ -445,8 +445,13 @@ static GradShape grad_shape(int64_t R, int C, int size, bool dres, int sms) {
   while (g.per_sm > 1 && 2 * g.stage_bytes * g.rows * g.per_sm > kRing) --g.per_sm;
   g.stages = (int)std::min<size_t>(8, kRing / (g.stage_bytes * g.rows * g.per_sm));
   if (g.stages < 2) g.stages = 0;
+  // no more CTAs than the turns that the longest takes need: fewer sums of dw to add up
   g.ctas = (R + g.rows - 1) / g.rows;
-  if (g.ctas > g.per_sm * (int64_t)sms) g.ctas = std::max(8, g.per_sm * sms / 8 * 8);
+  const int64_t most = std::max(8, g.per_sm * sms / 8 * 8);
+  if (g.ctas > most) {
+    const int64_t turns = (g.ctas + most - 1) / most;
+    g.ctas = ((g.ctas + turns - 1) / turns + 7) / 8 * 8;
+  }
   return g;
 }
 

@@ -294,13 +294,22 @@ __device__ __noinline__ int choose_long(const RouteArgs& a, const T* logits, flo
   return choose<P>(a.top, key, first);
 }
 
-// A score for the choice, with the fast exponential and reciprocal. With x its argument the
+// A score for the choice, with the approximate exponential (2^-22 of itself) and reciprocal
+// (2^-23). With x its argument, whose product with log2 e and that constant are rounded, the
 // exponential is off by (2 + 1.2 |x|) 2^-23 of itself. A sigmoid s moves by s (1 - s) as much, where
 // s (1 - s) |x| <= 0.23, and by 1.5 2^-23 of itself for the sum and the reciprocal: 2.3 2^-23 in all. A
 // probability p = e^-D / total moves by (2 + 1.7 D) 2^-23 of itself, where D p <= 0.4 pmax, and with
 // its total, which is off by 34 2^-23 of itself (the mean of D is below ln E, and 37 additions).
+__device__ __forceinline__ float quick_exp(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+  return y;
+}
 __device__ __forceinline__ float quick_score(float l, int sigmoid, float most, float part) {
-  return sigmoid ? __frcp_rn(1.0f + __expf(-l)) : __expf(l - most) * part;
+  if (!sigmoid) return quick_exp(l - most) * part;
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + quick_exp(-l)));
+  return y;
 }
 // How far a key in 32 bits may then be from its 64-bit value, with the rounding of its sum
 // with a bias of up to bmax. pmax is `part`.
@@ -326,7 +335,8 @@ __device__ __noinline__ double over_of(const RouteArgs& a, const T* logits, int 
 // each, ranked by comparing each with all, and where two are within 2 off in 64 bits (a few
 // tokens of a thousand). Groups are compared likewise. With more candidates than lanes, or
 // groups, choose_long. One choice after the other with all keys in
-// 64 bits took 30 us for 8192 tokens of 256 experts, a third of it 64-bit arithmetic; this 17.
+// 64 bits took 30 us for 8192 tokens of 256 experts, a third of it 64-bit arithmetic; this 13:
+// 1150 instructions a token, whose issue bounds it.
 template <typename T, int P>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsigned long long* values, int* candidates, bool vec) {
   const int lane = threadIdx.x & 31, size = a.E / a.cut, g = lane / a.lanes, from = lane % a.lanes * a.each;
@@ -364,21 +374,29 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
 #pragma unroll
       for (int p = 0; p < P; ++p) b[p] = p < own ? a.bias[first + p] : 0.0f;
     }
+    // the largest magnitude, by its bits: a NaN is above infinity
+    uint32_t bits = 0;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      bad |= isnan(b[p]);
-      if (fabsf(b[p]) < INFINITY) bmax = fmaxf(bmax, fabsf(b[p]));
+    for (int p = 0; p < P; ++p) bits = max(bits, __float_as_uint(b[p]) & 0x7fffffffu);
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    bad = bits > 0x7f800000u;
+    if (bits == 0x7f800000u) {  // of the finite ones
+      bits = 0;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (fabsf(b[p]) < INFINITY) bits = max(bits, __float_as_uint(b[p]) & 0x7fffffffu);
+      bits = __reduce_max_sync(0xffffffffu, bits);
     }
+    bmax = __uint_as_float(bits);
   }
   const bool live = !a.live || a.live[t];
-  uint32_t key[P], most_key = Key32::kNone;
+  float most = -INFINITY;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     bad |= isnan(l[p]);
-    key[p] = Key32::of(l[p]);
-    most_key = max(most_key, key[p]);
+    most = fmaxf(most, l[p]);
   }
-  const float most = Key32::value(Key32::most(most_key));
+  most = warp_most(most);
   bad = __any_sync(0xffffffffu, bad || (!a.sigmoid && most == INFINITY));
   int* ids = a.ids + t * a.top;
   float* weights = a.weights + t * a.top;
@@ -394,15 +412,16 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
   if (!a.sigmoid && (a.bias || sums || !a.renorm)) {
     total = 0.0f;
 #pragma unroll
-    for (int p = 0; p < P; ++p) total += a.renorm ? __expf(l[p] - most) : expf(l[p] - most);
+    for (int p = 0; p < P; ++p) total += a.renorm ? quick_exp(l[p] - most) : expf(l[p] - most);
     total = warp_sum(total);
     part = 1.0f / total;
   }
-  if (a.bias || sums) {
-    if (a.bias) bmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bmax)));
-    off = key_bound(a.sigmoid, part, bmax);
-  }
-  if (a.bias) {
+  if (a.bias || sums) off = key_bound(a.sigmoid, part, bmax);
+  uint32_t key[P];
+  if (!a.bias) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) key[p] = Key32::of(l[p]);
+  } else {
 #pragma unroll
     for (int p = 0; p < P; ++p) key[p] = l[p] == -INFINITY ? Key32::kNone : Key32::of(quick_score(l[p], a.sigmoid, most, part) + b[p]);
   }
@@ -482,19 +501,14 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, unsig
     id = choose<P>(a.top, key, first);
     count = __popc(__ballot_sync(0xffffffffu, id >= 0));
   } else if (sure) {
-    // the top-th largest of the lanes' largest: a bitonic sort of them, the largest first
-    uint32_t sorted = Key32::kNone;
+    // The top-th largest of the lanes' largest, or (equal ones go together) a lower one.
+    uint32_t left = Key32::kNone, least = Key32::kNone;
 #pragma unroll
-    for (int p = 0; p < P; ++p) sorted = max(sorted, key[p]);
-#pragma unroll
-    for (int run = 2; run <= 32; run *= 2)
-#pragma unroll
-      for (int d = run / 2; d; d /= 2) {
-        const uint32_t o = __shfl_xor_sync(0xffffffffu, sorted, d);
-        const bool larger = !(lane & d) == !(lane & run);
-        sorted = larger ? max(sorted, o) : min(sorted, o);
-      }
-    uint32_t least = __shfl_sync(0xffffffffu, sorted, a.top - 1);
+    for (int p = 0; p < P; ++p) left = max(left, key[p]);
+    for (int j = 0; j < a.top; ++j) {
+      least = Key32::most(left);
+      if (left == least) left = Key32::kNone;
+    }
     if (least != Key32::kNone) least = Key32::of(Key32::value(least) - 2.0f * off);
     least = max(least, Key32::kNone + 1);
     int mine = 0;
