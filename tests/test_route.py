@@ -291,6 +291,8 @@ def test_biases_that_are_large_or_infinite(dev, score):
     check(torch.zeros(5, 700), 32, score, 1, bias=torch.zeros(700))  # more equal keys than lanes
     check(torch.zeros(5, 700), 32, score, 1, bias=torch.zeros(700), groups=7, top_groups=3, best=2)
     check(torch.zeros(5, 700), 32, score, 1, groups=7, top_groups=3, best=2)
+    check(torch.zeros(5, 256), 8, score, 1, bias=torch.zeros(256), groups=8, top_groups=3, best=2)
+    check(torch.zeros(5, 256), 8, score, 1, bias=torch.zeros(256), groups=8, top_groups=3, best=1)
 
 
 @pytest.mark.gpu
