@@ -1,5 +1,6 @@
 """The short way of a launch with torch tensors (mantle_cuda/_launch): it takes plain calls alone, and
 leaves the rest to the long way, which says what is wrong."""
+import numpy as np
 import pytest
 import torch
 
@@ -92,3 +93,30 @@ def test_a_tensor_without_storage_is_refused(dev):
     with FakeTensorMode():
         fake = torch.empty(4, 64, device="cuda")
     assert short(M.kernels.rms_norm, norm_args(fake, x, w), 4, stream()) is None
+
+
+@pytest.mark.gpu
+def test_buffers_take_the_long_way_to_the_same_results(dev):
+    r, c = 70, 333
+    h, dy, w = torch.randn(r, c, device="cuda"), torch.randn(r, c, device="cuda"), torch.randn(c, device="cuda")
+    dx, dw = torch.empty_like(h), torch.empty_like(w)
+    k = M.kernels.rms_norm_grad
+    args = (dx, dw, dy, h, w, None, c, 0, 0, 1e-6)
+    need = M.workspace_bytes(k, args, r)
+    M.launch(k, args, r, stream=stream(), workspace=torch.empty(need, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    B = lambda t: M.Buffer(dev, t.cpu().numpy().reshape(-1))  # noqa: E731
+    DX, DW, ws = M.Buffer(dev, np.float32, r * c), M.Buffer(dev, np.float32, c), M.Buffer(dev, np.uint8, need)
+    bufs = (DX, DW, B(dy), B(h), B(w), None, c, 0, 0, 1e-6)
+    assert M.workspace_bytes(k, bufs, r) == need
+    M.launch(k, bufs, r, stream=dev.stream, workspace=ws)
+    dev.synchronize()
+    assert np.array_equal(DX.array(), dx.cpu().numpy().reshape(-1)) and np.array_equal(DW.array(), dw.cpu().numpy())
+    with pytest.raises(M.ArgumentError, match="of scratch"):
+        M.launch(k, bufs, r, stream=dev.stream)
+    with pytest.raises(M.ArgumentError, match="of scratch"):
+        M.launch(k, bufs, r, stream=dev.stream, workspace=M.Buffer(dev, np.uint8, need - 4))
+    with pytest.raises(M.ArgumentError, match="h: "):
+        M.launch(k, (DX, DW, B(dy), DW, B(w), None, c, 0, 0, 1e-6), r, stream=dev.stream, workspace=ws)
+    with pytest.raises(M.ArgumentError, match="expected Float32"):
+        M.launch(k, (DX, ws, B(dy), B(h), B(w), None, c, 0, 0, 1e-6), r, stream=dev.stream, workspace=ws)
