@@ -409,6 +409,16 @@ def test_captured_on_other_streams_and_in_a_graph(dev):
         M.run(plan)
     dev.synchronize()
     bits = lambda t: t.view(torch.int16).cpu().numpy().view(np.uint16).reshape(-1)  # noqa: E731
+    # a plan of the gradient alone, which is two kernels
+    H2, DX2, DW2, G2 = B(h, np.uint16), M.Buffer(dev, np.uint16, r * c), M.Buffer(dev, np.float32, c), M.Graph(dev)
+    M.compute(G2, "grad", lambda p: M.dispatch(p, M.kernels.rms_norm_grad, (
+        Wr(p, DX2), Wr(p, DW2), R(p, DY), R(p, H2), R(p, Wt), R(p, DY), c, 1, 0, 1e-6), r))
+    alone = M.Plan(G2)
+    for _ in range(3):
+        M.run(alone)
+        M.run(plan)
+    dev.synchronize()
+    assert np.array_equal(DX2.array(), bits(dx)) and np.array_equal(DW2.array(), dw.cpu().numpy())
     assert np.array_equal(Y.array(), bits(y)) and np.array_equal(DX.array(), bits(dx)) and np.array_equal(DW.array(), dw.cpu().numpy())
 
 

@@ -445,3 +445,29 @@ def test_captured_and_at_once(dev):
     for o in outs:
         assert torch.equal(o[0].view(3000, 4), want[0]) and torch.equal(o[1].view(3000, 4), want[1])
         assert all(torch.equal(a, b) for a, b in zip(o[2:], want[2]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [60, 3000])
+def test_as_a_plan(dev, t):
+    E, top = 64, 4
+    l = normal(t, E).cuda()
+    want = route(l, top, SIGMOID, 1, 2.5, groups=8, top_groups=4, best=2)
+    L, n = M.Buffer.wrap(dev, l, dtype=np.float32), t * top
+    ids, rows_of, row_at, off, w = (M.Buffer(dev, d, k) for d, k in ((np.int32, n), (np.int32, n), (np.int32, n), (np.int32, E + 1), (np.float32, n)))
+    dw, dl = M.Buffer(dev, normal(t, top, seed=2).numpy().reshape(-1)), M.Buffer(dev, np.float32, t * E)
+    g = M.Graph(dev)
+    R, W = (lambda p, b: M.use(p, b, read=True)), (lambda p, b: M.use(p, b, write=True))
+    M.compute(g, "route", lambda p: M.dispatch(p, M.kernels.route_experts, (
+        W(p, ids), W(p, w), W(p, off), W(p, rows_of), W(p, row_at), R(p, L), None, None, E, top, 8, 4, 2, 1, 1, 0, 2.5), t))
+    alone = M.Plan(g)
+    M.compute(g, "grad", lambda p: M.dispatch(p, M.kernels.route_experts_grad, (
+        W(p, dl), R(p, dw), R(p, L), R(p, ids), E, top, 1, 1, 0, 2.5), t))
+    both = M.Plan(g)
+    for plan in (alone, both, both):
+        M.run(plan)
+    dev.synchronize()
+    for a, b in zip((ids, w, off, rows_of, row_at), (want[0], want[1], *want[2])):
+        assert np.array_equal(a.array(), b.cpu().numpy().reshape(-1))
+    d = grad(l, want[0], torch.from_numpy(dw.array()).view(t, top).cuda(), SIGMOID, 1, 2.5)
+    assert np.array_equal(dl.array(), d.cpu().numpy().reshape(-1))
