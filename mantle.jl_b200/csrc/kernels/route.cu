@@ -26,7 +26,7 @@
 // row_at[s] its row (-1 without an expert), offsets[e] the first row of expert e.
 //
 // The gradient, with g the weights' gradient, c = scale, S the chosen and sums over S:
-//   softmax              c p_e ([e in S] g_e - sum g p)   over all experts
+//   softmax              c p_e ([e in S] g_e - sum g p)   over all experts (0 where S is empty)
 //   softmax, over sum    c u_e (g_e - sum g u)            u = p / sum p, on S
 //   sigmoid              c s_e (1 - s_e) g_e              on S
 //   sigmoid, over sum    c u_e (1 - s_e) (g_e - sum g u)  u = s / sum s, on S
@@ -755,7 +755,8 @@ __global__ void __launch_bounds__(128) route_grad_kernel(RouteGradArgs a) {
   float g = valid ? a.dweights[t * a.top + lane] : 0.0f;
   const float l = valid ? to_f32(logits[id]) : -INFINITY;
   float p[P], most = -INFINITY, total = 1.0f;
-  const bool dense = !a.sigmoid && !a.renorm;
+  // a token without experts has no gradient, whatever its logits hold
+  const bool dense = !a.sigmoid && !a.renorm && __any_sync(0xffffffffu, valid);
   if (dense) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {

@@ -386,6 +386,34 @@ def test_route_grad(dev, t, e, top, score, renorm, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("e", [5, 64, 300])
+def test_tokens_without_experts_have_no_gradient(dev, e, score, renorm, kind):
+    # padding whose logits were never set: the forward pass counts it for nothing, and so does this
+    inf, nan = float("inf"), float("nan")
+    l, g, top = 2 * normal(12, e, seed=e, kind=kind), normal(12, 3, seed=9), 3
+    ids = l.float().argsort(1, descending=True)[:, :top].to(torch.int32)
+    want = grad(l.cuda(), ids.cuda(), g.cuda(), score, renorm, 2.5)
+    bad = l.clone()
+    bad[0], bad[2, e - 1], bad[4], bad[6, 1], bad[8], bad[10] = nan, nan, inf, inf, -inf, 3.0e38
+    ids[::2], g[::4] = -1, nan
+    ids[2], ids[6] = e, -7  # outside the experts, as good as none
+    got = grad(bad.cuda(), ids.cuda(), g.cuda(), score, renorm, 2.5)
+    assert (got[::2] == 0).all() and torch.equal(got[1::2], want[1::2])
+    # what the forward pass makes of such tokens, live or not
+    live = torch.ones(12, dtype=torch.int32)
+    live[::2] = 0
+    for alive in (live, None):
+        chosen, w, _ = route(bad.cuda(), top, score, renorm, live=None if alive is None else alive.cuda())
+        none = (chosen < 0).all(1).cpu()
+        assert none[:10:2].all() if alive is not None else none[8]
+        d = grad(bad.cuda(), chosen, torch.ones(12, top, device="cuda"), score, renorm, 1.0)
+        assert (d[none.cuda()] == 0).all() and d.isfinite().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("renorm", [0, 1])
 @pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
 def test_route_grad_against_differences(dev, score, renorm):
