@@ -243,6 +243,13 @@ struct NormGradArgs {
 // The CTAs that an SM holds: the registers are dealt out for as many, about a hundred a
 // thread (at 80 the spills took 1023 x 5001 float from 20 to 22 us, 4092 rows from 48 to 61).
 constexpr int grad_residents(int most, int N) { return most == 32 ? (N == 4 ? 3 : N == 2 ? 5 : 8) : most == 128 ? 4 : most <= 320 ? 2 : 1; }
+// An SM's shared memory, less what the system keeps of each CTA's (a KiB) and its static part
+// (row_sums' slots, rounded up to 128 bytes), is the rings'.
+constexpr size_t kRing = 204 * 1024;  // of all an SM's CTAs together
+template <int MOST>
+constexpr int kSumSlots = MOST == 32 ? 2 : MOST / 16;
+template <int N, int MOST>
+constexpr bool kRingsFit = kRing + grad_residents(MOST, N) * (1024 + (2 * kSumSlots<MOST> * sizeof(float) + 127) / 128 * 128) <= 228 * 1024;
 
 // The sums of two values over the row's threads, in a fixed order. `part`: two slots a warp.
 template <bool WARP>
@@ -288,7 +295,7 @@ __global__ void __launch_bounds__(MOST == 32 ? 128 : MOST, grad_residents(MOST, 
   constexpr bool WARP = MOST == 32;  // rows of a warp each
   constexpr int K = N * 8 / kWide<T>, P = kPairs<T>;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ __align__(8) float part[2][WARP ? 2 : MOST / 16];
+  __shared__ __align__(8) float part[2][kSumSlots<MOST>];
   const int tid = threadIdx.x, B = WARP ? 32 : blockDim.x, C = a.C;
   const int64_t stride = (int64_t)gridDim.x * blockDim.y, total = a.R * C;
   int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -382,15 +389,21 @@ __global__ void __launch_bounds__(MOST == 32 ? 128 : MOST, grad_residents(MOST, 
   }
   copies_wait(0);
   if (!a.part) return;
-  if constexpr (WARP) {  // the CTA's warps' sums together
-    __shared__ float meet[4][256 * N];
+  if constexpr (WARP) {
+    // The CTA's warps' sums together, each in its warp's part of the ring (two stages or more
+    // of 1024 N bytes at least): as static memory they would take up to 16 KiB that the rings
+    // are counted on having (two CTAs an SM instead of three at 513 to 1024 columns: 8192 x
+    // 1000 bf16 20.6 us, so 16.6, 8192 x 700 float 32.6 and 21.4).
+    float* meet = reinterpret_cast<float*>(ring);
+    const int apart = RING ? a.stages * stage_bytes / 4 : 256 * N;
+    __syncwarp();  // all lanes have read their last chunks
 #pragma unroll
     for (int u = 0; u < K; ++u) {
-      if (chunk(u).on) store_each(meet[threadIdx.y], dw[u], chunk(u), C);
+      if (chunk(u).on) store_each(meet + threadIdx.y * apart, dw[u], chunk(u), C);
     }
     __syncthreads();
     for (int c = threadIdx.y * 32 + tid; c < C; c += 128)
-      a.part[(int64_t)blockIdx.x * C + c] = meet[0][c] + meet[1][c] + meet[2][c] + meet[3][c];
+      a.part[(int64_t)blockIdx.x * C + c] = meet[c] + meet[apart + c] + meet[2 * apart + c] + meet[3 * apart + c];
   } else {
 #pragma unroll
     for (int u = 0; u < K; ++u)
@@ -401,7 +414,7 @@ __global__ void __launch_bounds__(MOST == 32 ? 128 : MOST, grad_residents(MOST, 
 // dw = the CTAs' sums, in a fixed order: W columns a CTA, 1024 / W threads a column, each with
 // every 1024 / W-th sum, eight loads in flight. 32 columns where there are many; eight, a
 // sector of each sum, up to 1024 columns, whose 32 would leave most SMs idle (8192 x 200 bf16
-// 11.2 -> 9.1 us, 1500 x 777 13.7 -> 12.5; 4096 x 8192 would take 47.7 us instead of 44.9).
+// 10.7 -> 8.7 us, 1500 x 777 10.8 -> 9.7; 4096 x 8192 would take 47.7 us instead of 44.9).
 template <int W>
 __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(float* __restrict__ dw, const float* __restrict__ part, int parts, int C) {
   constexpr int kRows = 1024 / W;
@@ -430,7 +443,6 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(float* __restrict__ d
 // How a launch is laid out: CTAs of `threads` a row, `rows` rows at once a CTA, `N` eights of
 // values a thread, and the ring's stages (none: rows are loaded when their turn comes, for rows
 // too long for two stages).
-constexpr size_t kRing = 204 * 1024;  // of an SM's 227 KiB, for all its CTAs together
 struct GradShape {
   int threads, rows, N, most, per_sm, stages, device;
   int64_t ctas;
@@ -466,9 +478,10 @@ static GradShape grad_shape(int64_t R, int C, int size, bool dres, int sms) {
 template <typename T, int N, int MOST, bool PHASED, bool RING>
 static cudaError_t norm_grad_go(NormGradArgs a, const GradShape& g, cudaStream_t st) {
   a.stages = RING ? g.stages : 0;
-  const size_t smem = RING ? g.stage_bytes * g.rows * g.stages : 0;
+  const size_t smem = RING ? g.stage_bytes * g.rows * g.stages : MOST == 32 ? 4096 * N : 0;
   const auto kernel = rms_norm_grad_kernel<T, N, MOST, PHASED, RING>;
   if constexpr (RING) {
+    static_assert(kRingsFit<N, MOST>, "an SM holds fewer CTAs than grad_shape plans");
     static unsigned long long done;
     if (const cudaError_t e = allow_shared(kernel, (int)kRing, g.device, &done)) return e;
   }

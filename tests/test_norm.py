@@ -306,6 +306,56 @@ def test_norm_grad(dev, r, c, kind, wkind):
         assert none is None and torch.equal(alone, dx)
 
 
+def check_grad(dx, dw, dy, h, w, dres):
+    """The bounds at the top, in 64 bits on the device."""
+    H64, G, W64 = h.double(), dy.double(), w.double()
+    rr = 1 / torch.sqrt((H64 * H64).mean(1, keepdim=True) + 1e-6)
+    a = G * W64
+    want = rr * (a - H64 * rr * rr * (a * H64).mean(1, keepdim=True))
+    m = rr * rr * (a * H64).abs().mean(1, keepdim=True)
+    d = torch.zeros_like(want) if dres is None else dres.double()
+    tol = 128 * u * rr * (a.abs() + H64.abs() * m) + 2 * u * ((want + d).abs() + d.abs())
+    assert ((dx.double() - want - d).abs() <= tol + HALF[h.dtype] * ((want + d).abs() + tol)).all()
+    n = G * H64 * rr
+    assert ((dw.double() - n.sum(0)).abs() <= (28 + len(h)) * u * n.abs().sum(0)).all()
+
+
+# more rows than the CTAs take at once, at every count of threads a row, on 16 bytes and cut
+TURNS = [(5000, 200), (5000, 201), (3100, 500), (3100, 333), (2000, 1000), (2000, 777), (2000, 1001), (1300, 1504), (1300, 1501), (700, 3001), (700, 4099),
+         (1023, 5001), (400, 6001), (400, 7168), (300, 9001), (300, 12001), (300, 16384), (300, 20001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,wkind", [(F, F), (H, H), (H, F)])
+@pytest.mark.parametrize("r,c", TURNS)
+def test_norm_grad_over_several_turns(dev, r, c, kind, wkind):
+    # a CTA's second and later rows: the ring filled again, rows a multiple of eight apart cut alike
+    w = (1 + 0.3 * rows(1, c, F, 5)[0]).to(wkind)
+    h, dy, dres = 2 * rows(r, c, kind, 1), rows(r, c, kind, 2), rows(r, c, kind, 3)
+    for add in (None, dres):
+        ctas = M.workspace_bytes(M.kernels.rms_norm_grad, (h, w.float(), dy, h, w, add, c, int(kind == H), int(wkind == H), 1e-6), r) // (4 * c)
+        assert 0 < ctas * (4 if c <= 1024 else 1) < r
+        dx, dw = grad(dy, h, w, add)
+        check_grad(dx, dw, dy, h, w, add)
+        again = grad(dy, h, w, add)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+        alone, none = grad(dy, h, w, add, dw=False)
+        assert none is None and torch.equal(alone, dx)
+        ins = [dy.clone(), h.clone()] + ([] if add is None else [add.clone()])
+        for over in range(len(ins)):  # dx over an input
+            new = [t.clone() for t in ins]
+            got = grad(new[0], new[1], w, new[2] if add is not None else None, dx=new[over])
+            assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+    for at in (1, 3):  # every tensor as far behind 16 bytes, and only dx
+        shift = lambda t: torch.cat([torch.zeros(at, dtype=kind, device="cuda"), t.reshape(-1)])[at:].view(r, c)  # noqa: E731
+        flat = torch.full((r * c + at + 9,), 7.0, dtype=kind, device="cuda")
+        out = flat[at:at + r * c].view(r, c)
+        for ins in ((shift(dy), shift(h), shift(dres)), (dy, h, dres)):
+            got = grad(*ins[:2], w, ins[2], dx=out)
+            check_grad(got[0], got[1], dy, h, w, dres)
+            assert (flat[:at] == 7).all() and (flat[at + r * c:] == 7).all()
+
+
 @pytest.mark.gpu
 def test_norm_grad_against_differences(dev):
     # 64-bit central differences of sum(dy y) with a step of 1e-5: off by 1e-10 of third derivatives, and 1e-11 of rounding
