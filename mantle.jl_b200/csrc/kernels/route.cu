@@ -855,7 +855,7 @@ mtl_status route_experts_check(const LaunchArgs& la, const uint64_t* bytes) {
                          {"live", bytes_of({T, 4}), 4}});
 }
 
-constexpr int kRouteShared = 160 * 1024;  // more than order_shared() and the groups' values ask for
+constexpr int kRouteShared = 160 * 1024;  // more than order_shared() asks for, or 256 groups' values of every warp
 
 template <typename... K, typename... A>
 static cudaError_t cluster_launch(void (*kernel)(K...), unsigned ctas, unsigned clusters, size_t shared, bool behind, int device, unsigned long long* done, cudaStream_t st, A... args) {
@@ -876,43 +876,56 @@ static cudaError_t cluster_launch(void (*kernel)(K...), unsigned ctas, unsigned 
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// One cluster chooses and orders up to this many tokens: one launch, which costs the host less
-// and an otherwise idle GPU no more (128 tokens of 64 experts 9.4 us, 7.4 in two; of 256
-// tokens and experts 13.7 and 10.1).
-constexpr int64_t kFewTokens = 128;
+// A direct call of up to this many tokens, where a lane has P experts at most, is one launch: one
+// cluster chooses and orders, which spares the host more than the GPU loses. In microseconds a pass
+// among others, one launch and two, over softmax and sigmoid, bias and groups: 128 tokens of 64
+// experts 10.3 to 12.3 and 12.4, of 128 the same, 1 token of either 9.4 to 10.3 and 12.4; 16 tokens of
+// 256 experts 10.3 to 12.3 and 12.4, but 32 in groups 14.2 and 12.4, 64 of 512 16.4 to 18.5 and 12.4,
+// 64 of 1024 28.9 to 45 and 13.4 to 16.4 (their keys spill in a CTA of 1024 threads). The GPU alone
+// always takes longer in one (64 tokens of 32 experts 7.9 us, 6.8 in two; 128 of 64 8.4 to 11.1, 7.0
+// to 8.6), so a captured call, whose replays cost the host nothing, is two.
+template <int P>
+constexpr int64_t kFewTokens = P <= 4 ? 128 : P <= 8 ? 16 : 0;
 // Else the order is made by clusters of eight CTAs, as many as a warp has steps of 32 slots,
 // so that each places one or few (65536 slots 16.8 us by one cluster, 10.8 by eight).
 constexpr unsigned kOrderCtas = 8, kOrderClusters = 8;
 
-static bool few_tokens(const RouteArgs& a) {
-  return a.T > 0 && a.T <= kFewTokens && (a.groups == 1 || kOrderWarps * sizeof(unsigned long long) * a.groups <= kRouteShared);
+static bool captured(cudaStream_t st) {
+  cudaStreamCaptureStatus status;
+  if (cudaStreamIsCapturing(st, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
+  cudaGetLastError();  // the launch will say so itself
+  return false;
 }
 
+// `ordered`: the rows' order is made too.
 template <typename T, int P>
-static cudaError_t route_go(const RouteArgs& a, const OrderArgs* o, bool vec, int device, cudaStream_t st) {
+static cudaError_t route_go(const RouteArgs& a, const OrderArgs* o, bool vec, int device, bool* ordered, cudaStream_t st) {
   const size_t values = a.groups > 1 ? sizeof(unsigned long long) * a.groups : 0;
-  if (o && few_tokens(a)) {
-    static unsigned long long done;
-    const unsigned ctas = (unsigned)std::min<int64_t>(kOrderCtas, (a.T + kOrderWarps - 1) / kOrderWarps);
-    return cluster_launch(route_and_order_kernel<T, P>, ctas, 1, std::max(order_shared(a.E), kOrderWarps * values), false, device, &done, st, a, *o, vec);
+  if constexpr (kFewTokens<P> > 0) {
+    if (o && a.T > 0 && a.T <= kFewTokens<P> && !captured(st)) {
+      static unsigned long long done;
+      const unsigned ctas = (unsigned)std::min<int64_t>(kOrderCtas, (a.T + kOrderWarps - 1) / kOrderWarps);
+      *ordered = true;
+      return cluster_launch(route_and_order_kernel<T, P>, ctas, 1, std::max(order_shared(a.E), kOrderWarps * values), false, device, &done, st, a, *o, vec);
+    }
   }
   if (a.T) route_kernel<T, P><<<(unsigned)((a.T + 3) / 4), 128, 4 * values, st>>>(a, vec);
   return cudaSuccess;
 }
 template <typename T>
-static cudaError_t route_launch(RouteArgs a, const OrderArgs* o, bool vec, int device, cudaStream_t st) {
+static cudaError_t route_launch(RouteArgs a, const OrderArgs* o, bool vec, int device, bool* ordered, cudaStream_t st) {
   a.cut = a.groups;
   a.lanes = 1;
   while (a.lanes * 2 * a.cut <= 32) a.lanes *= 2;
   a.each = (a.E / a.cut + a.lanes - 1) / a.lanes;
   if (a.cut > 32 || a.each > 32) a.cut = 1, a.lanes = 32, a.each = (a.E + 31) / 32;
   const int most = std::max(a.each, (a.E + 31) / 32);  // of a lane, choose_long's among them
-  if (most <= 1) return route_go<T, 1>(a, o, vec, device, st);
-  if (most <= 2) return route_go<T, 2>(a, o, vec, device, st);
-  if (most <= 4) return route_go<T, 4>(a, o, vec, device, st);
-  if (most <= 8) return route_go<T, 8>(a, o, vec, device, st);
-  if (most <= 16) return route_go<T, 16>(a, o, vec, device, st);
-  return route_go<T, 32>(a, o, vec, device, st);
+  if (most <= 1) return route_go<T, 1>(a, o, vec, device, ordered, st);
+  if (most <= 2) return route_go<T, 2>(a, o, vec, device, ordered, st);
+  if (most <= 4) return route_go<T, 4>(a, o, vec, device, ordered, st);
+  if (most <= 8) return route_go<T, 8>(a, o, vec, device, ordered, st);
+  if (most <= 16) return route_go<T, 16>(a, o, vec, device, ordered, st);
+  return route_go<T, 32>(a, o, vec, device, ordered, st);
 }
 
 mtl_status route_experts_run(const LaunchArgs& la, void*, uint64_t, void* stream) {
@@ -941,8 +954,10 @@ mtl_status route_experts_run(const LaunchArgs& la, void*, uint64_t, void* stream
   o.n = a.T * a.top;
   o.E = a.E;
   o.top = a.top;
-  cudaError_t e = bf16 ? route_launch<uint16_t>(a, ordering ? &o : nullptr, vec, la.device, st) : route_launch<float>(a, ordering ? &o : nullptr, vec, la.device, st);
-  if (e == cudaSuccess && ordering && !few_tokens(a)) {
+  bool ordered = !ordering;
+  cudaError_t e = bf16 ? route_launch<uint16_t>(a, ordering ? &o : nullptr, vec, la.device, &ordered, st)
+                       : route_launch<float>(a, ordering ? &o : nullptr, vec, la.device, &ordered, st);
+  if (e == cudaSuccess && !ordered) {
     static unsigned long long done;
     const unsigned ctas = a.T ? kOrderCtas : 1, clusters = (unsigned)std::max<int64_t>(1, std::min<int64_t>(kOrderClusters, o.n / (32 * kOrderWarps * ctas)));
     e = cluster_launch(order_rows_kernel, ctas, clusters, order_shared(a.E), a.T > 0, la.device, &done, st, o);

@@ -306,6 +306,43 @@ def test_few_tokens_and_many_are_one(dev, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("t", [1, 16, 17, 96, 128, 129])
+@pytest.mark.parametrize("e,groups", [(1, 1), (32, 4), (33, 1), (60, 3), (64, 64), (65, 5), (128, 8), (129, 1), (256, 8), (256, 256), (640, 1), (1024, 8)])
+def test_a_captured_call_gives_what_a_direct_one_does(dev, t, e, groups, kind):
+    # whose launches differ: a direct call of few tokens and experts is one kernel, a captured one two
+    l, b, top = normal(t, e, seed=t, kind=kind).cuda(), (0.1 * normal(e, seed=2)).cuda(), min(6, e // groups)
+    g = dict(groups=groups, top_groups=max(1, groups // 2), best=min(2, e // groups))
+    check(l.cpu(), top, SIGMOID, 1, bias=b.cpu(), **g)
+    want = route(l, top, SIGMOID, 1, bias=b, **g)
+    out = [torch.full((n,), -7, dtype=d, device="cuda") for n, d in ((t * top, torch.int32), (t * top, F), (e + 1, torch.int32), (t * top, torch.int32), (t * top, torch.int32))]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        M.launch(M.kernels.route_experts, (*out, l, b, None, e, top, groups, g["top_groups"], g["best"], SIGMOID, 1, int(kind == H), 1.0), t, stream=stream())
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(out, (want[0], want[1], *want[2])):
+        assert torch.equal(x, y.reshape(-1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e", [(1, 8), (64, 32), (128, 64), (60, 1024), (3000, 64)])
+def test_a_replay_routes_in_two_kernels(dev, t, e):
+    # few tokens too: one cluster for both takes a GPU longer, and a replay spares the host nothing
+    L, n = M.Buffer.wrap(dev, normal(t, e).cuda(), dtype=np.float32), t * 2
+    ids, rows_of, row_at, off, w = (M.Buffer(dev, d, k) for d, k in ((np.int32, n), (np.int32, n), (np.int32, n), (np.int32, e + 1), (np.float32, n)))
+    g = M.Graph(dev)
+    R, W = (lambda p, b: M.use(p, b, read=True)), (lambda p, b: M.use(p, b, write=True))
+    M.compute(g, "route", lambda p: M.dispatch(p, M.kernels.route_experts, (
+        W(p, ids), W(p, w), W(p, off), W(p, rows_of), W(p, row_at), R(p, L), None, None, e, 2, 1, 1, 1, 0, 1, 0, 1.0), t))
+    plan = M.Plan(g)
+    M.run(plan)
+    dev.synchronize()
+    assert plan.nkernels() == 2
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t,e,top", [(0, 8, 2), (1, 1, 1), (3000, 8, 2), (2049, 16, 8), (1500, 300, 32), (9000, 1024, 2), (40000, 256, 8), (70000, 3, 1)])
 def test_rows_in_order(dev, t, e, top):
     # slots in order within an expert, experts of very different sizes, some empty, and dead tokens between
