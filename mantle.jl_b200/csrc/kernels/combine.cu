@@ -79,15 +79,17 @@ struct CombineGradArgs {
   int C, top;
 };
 
-// A CTA a token, tile by tile.
-template <typename T, typename Y, int B, bool VEC>
+// A CTA a token, tile by tile. WHOLE: the CTA has B threads, known when it is compiled (4096 x 2
+// rows of 4096 float 56.7 -> 53.6 us, 4096 x 8 of 2048 95.8 -> 91.4; bf16 rows the same either way).
+template <typename T, typename Y, int B, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(B) combine_grad_kernel(CombineGradArgs a) {
   __shared__ float part[kCombineTop][B / 32];
   const int64_t t = blockIdx.x;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = VEC ? blockDim.x >> 5 : B / 32, C = a.C;
+  const int threads = WHOLE ? B : blockDim.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = threads >> 5, C = a.C;
   const int* row_at = a.row_at + t * a.top;
   for (int tile = 0; tile * 8 * warps * 32 < C; ++tile) {
-    const int tid = VEC ? tile * blockDim.x + threadIdx.x : threadIdx.x, u = VEC ? 0 : tile;
+    const int tid = VEC ? tile * threads + threadIdx.x : threadIdx.x, u = VEC ? 0 : tile;
     float g[8];
     load_part<B, VEC>(g, static_cast<const Y*>(a.dy) + t * C, C, tid, u);
 #pragma unroll 4
@@ -134,10 +136,9 @@ static mtl_status combine_sizes(const char* kernel, const LaunchArgs& la, int64_
 
 // Threads of a CTA and tiles of a row, where tiles may have any size: 256 threads at most, the
 // tiles even and of whole warps. Against tiles of 1024 or 2048 columns: 4000 x 2 rows of 4104
-// bf16 31.2 -> 28.0 us, 8192 x 3 rows of 200 9.1 -> 6.4, their gradient 14.2 -> 10.0 (4096 x 2
-// rows of 4096 float, as even before, 53.6 -> 56). Both kernels are bound by HBM: 8192 x 8 rows
-// of 2048 bf16 with a base 58 us, 5.8 TB/s, the gradient 100 us, 5.7 TB/s. Four slots' rows loaded
-// ahead of their sums took 70 and 170.
+// bf16 31.2 -> 28.0 us, 8192 x 3 rows of 200 9.1 -> 6.4, their gradient 14.2 -> 10.0. Both kernels
+// are bound by HBM: 8192 x 8 rows of 2048 bf16 with a base 58 us, 5.8 TB/s, the gradient 100 us,
+// 5.7 TB/s. Four slots' rows loaded ahead of their sums took 70 and 170.
 constexpr int kCombineThreads = 256;
 struct Tiles {
   unsigned threads, tiles;
@@ -200,12 +201,17 @@ mtl_status combine_experts_run(const LaunchArgs& la, void*, uint64_t, void* stre
 template <typename T, typename Y>
 static void combine_grad_launch(const CombineGradArgs& a, int64_t tokens, bool vec, cudaStream_t st) {
   const unsigned grid = (unsigned)tokens;
-  if (vec)
-    combine_grad_kernel<T, Y, kCombineThreads, true><<<grid, even_tiles(a.C).threads, 0, st>>>(a);
-  else if (a.C <= 1024)
-    combine_grad_kernel<T, Y, 128, false><<<grid, 128, 0, st>>>(a);
-  else
-    combine_grad_kernel<T, Y, 256, false><<<grid, 256, 0, st>>>(a);
+  if (vec) {
+    const unsigned threads = even_tiles(a.C).threads;
+    if (threads == kCombineThreads)
+      combine_grad_kernel<T, Y, kCombineThreads, true, true><<<grid, threads, 0, st>>>(a);
+    else
+      combine_grad_kernel<T, Y, kCombineThreads, true, false><<<grid, threads, 0, st>>>(a);
+  } else if (a.C <= 1024) {
+    combine_grad_kernel<T, Y, 128, false, true><<<grid, 128, 0, st>>>(a);
+  } else {
+    combine_grad_kernel<T, Y, 256, false, true><<<grid, 256, 0, st>>>(a);
+  }
 }
 
 // Arguments: drows (B), dweights (b, f32), dy (B), rows (b), weights (b, f32), row_at (B,
