@@ -12,10 +12,12 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -63,32 +65,45 @@ def compile_one(src: Path, force: bool) -> Path:
     return obj
 
 
-LAUNCH_SRC, LAUNCH_OUT = CSRC / "python" / "launch.cpp", HERE / "mantle_cuda" / "_launch.so"
+LAUNCH_SRC = CSRC / "python" / "launch.cpp"
+LAUNCH_OUT = HERE / "mantle_cuda" / f"_launch{sysconfig.get_config_var('EXT_SUFFIX')}"  # this Python's alone
 
 
 def build_launch(force: bool = False) -> None:
-    """The Python host's short way to a launch with torch tensors (mantle_cuda/_launch.so),
-    against the torch that is installed; the library itself does without either."""
-    newest_dep = max(LAUNCH_SRC.stat().st_mtime, (ROOT / "include" / "mantle_cuda.h").stat().st_mtime)
-    if not force and LAUNCH_OUT.exists() and LAUNCH_OUT.stat().st_mtime >= newest_dep:
+    """The Python host's short way to a launch with torch tensors (mantle_cuda/_launch),
+    against the torch that is installed, and again when another is. The library does
+    without: where this cannot be built, launches take the long way."""
+    found = importlib.util.find_spec("torch")
+    if found is None:
         return
-    import sysconfig
-
+    home, stamp = Path(found.origin).parent, OBJ / "launch.stamp"
+    built_for = f"{sys.version}\n{home}\n{(home / 'version.py').read_text()}"
+    newest_dep = max(f.stat().st_mtime for f in (LAUNCH_SRC, ROOT / "include" / "mantle_cuda.h", Path(__file__)))
+    if (not force and LAUNCH_OUT.exists() and LAUNCH_OUT.stat().st_mtime >= newest_dep
+            and stamp.exists() and stamp.read_text() == built_for):
+        return
+    for old in (LAUNCH_OUT, LAUNCH_OUT.with_name("_launch.so"), stamp):  # built for something else: never loaded again
+        old.unlink(missing_ok=True)
     try:
         import torch
         from torch.utils.cpp_extension import include_paths
-    except ImportError:
+
+        if not torch.version.cuda:
+            return
+        cuda = Path(nvcc()).resolve().parent.parent / "include"
+        cmd = ["g++", "-O2", "-std=c++20", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f'-DBUILT_FOR_TORCH="{torch.__version__}"',
+               *[f"-I{d}" for d in (*include_paths(), sysconfig.get_paths()["include"], cuda)], str(LAUNCH_SRC), "-o", str(LAUNCH_OUT),
+               f"-L{home / 'lib'}", f"-Wl,-rpath,{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        why = f"{' '.join(cmd)}\n{r.stdout}\n{r.stderr}" if r.returncode else ""
+    except (ImportError, OSError) as e:  # a torch that does not load, no g++
+        why = str(e)
+    if why:
+        LAUNCH_OUT.unlink(missing_ok=True)
+        print(f"mantle_cuda/_launch was not built; launches with torch tensors cost the host more without it: {why}", file=sys.stderr)
         return
-    if not torch.version.cuda:
-        return
-    lib = Path(torch.__file__).parent / "lib"
-    cuda = Path(nvcc()).resolve().parent.parent / "include"
-    cmd = ["g++", "-O2", "-std=c++20", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{d}" for d in (*include_paths(), sysconfig.get_paths()["include"], cuda)], str(LAUNCH_SRC), "-o", str(LAUNCH_OUT),
-           f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(built_for)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

@@ -167,4 +167,14 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__launch(void) { return PyModule_Create(&module); }
+// Tensors are read by the layout of the torch that this was compiled against, so no other will do.
+PyMODINIT_FUNC PyInit__launch(void) {
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* version = torch ? PyObject_GetAttrString(torch, "__version__") : nullptr;
+  Py_XDECREF(torch);
+  if (!version) return nullptr;
+  const bool same = PyUnicode_Check(version) && PyUnicode_CompareWithASCIIString(version, BUILT_FOR_TORCH) == 0;
+  if (!same) PyErr_Format(PyExc_ImportError, "_launch was built for torch " BUILT_FOR_TORCH ", not %S", version);
+  Py_DECREF(version);
+  return same ? PyModule_Create(&module) : nullptr;
+}

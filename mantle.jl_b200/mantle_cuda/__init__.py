@@ -623,7 +623,7 @@ _KINDS = {np.dtype(t): k + "*" for k, types in {"45": (np.uint8, np.int8), "f": 
 _KIND_NAMES = {"4": "8-bit codes in e4m3", "5": "8-bit codes in e5m2", "f": "Float32", "h": "bfloat16", "i": "Int32"}
 _PTR = L.ARG_PTR
 _tensor = _current_device = None  # torch.Tensor, torch.cuda.current_device, once torch is loaded
-_short_launch = _short_plan = None  # of _launch.so, where it was built
+_short_launch = _short_plan = None  # of _launch, where it was built for this torch
 
 
 def _with_torch() -> None:
