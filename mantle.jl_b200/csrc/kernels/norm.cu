@@ -6,8 +6,10 @@
 // h, the sum of squares and y are kept in 32 bits; h and y are rounded once, to x's type,
 // where they are stored. The codes and scales are what quantize_fp8 makes of the 32-bit y
 // in 1 x 128 blocks (definitions at the top of quantize.cu), not of its rounding to
-// bfloat16. A NaN or an infinity makes its row NaN. Squares are summed in 32 bits, so a row
-// whose mean square passes 3.4e38 gives zeros.
+// bfloat16. A NaN makes its row NaN, an infinity its own value NaN and the finite ones of its
+// row zeros. Squares are summed in 32 bits: a row whose squares add up to more than 3.4e38, a
+// mean square of 3.4e38 / C, gives zeros, and its gradient is dres alone. With eps 0 squares
+// that are zeros in 32 bits (of values below 1e-23) make a row infinite, zeros a row NaN.
 //
 // With a = w dy and n = h r the gradient is
 //

@@ -256,6 +256,42 @@ def test_rows_that_are_not_numbers_stay_apart(dev, kind, c):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F, H])
+@pytest.mark.parametrize("c", [1, 200, 4096, 4099, 32768])
+def test_squares_that_pass_32_bits_together(dev, kind, c):
+    # a row on each side of the limit of its sum of squares, 3.4e38, between two others
+    top = (2 - 2.0 ** -23) * 2.0 ** 127
+    sign = torch.sign(rows(1, c, F, 1)[0] + 1e-3)
+    x, w = rows(4, c, kind, 2), (1 + 0.3 * rows(1, c, F, 5)[0])
+    x[1], x[2] = (sign * (0.8 * top / c) ** 0.5).to(kind), (sign * (1.25 * top / c) ** 0.5).to(kind)
+    square = (x.double() ** 2).sum(1)
+    assert square[1] < 0.9 * top and square[2] > 1.1 * top
+    y, _, q, s = norm(x, w, fmt=0)
+    want = exact(x, w)[1]
+    rest = [0, 1, 3]
+    check_y(y[rest], want[rest])
+    check_codes(q[rest], s[:, rest].contiguous(), want[rest], 0, 0)
+    assert (y[2] == 0).all() and (q[2].float() == 0).all()
+    dy, dres = rows(4, c, kind, 3), rows(4, c, kind, 4)
+    dx, dw = grad(dy, x, w, dres)
+    assert torch.equal(dx[2], dres[2])
+    only = dy.clone()
+    only[2] = 0  # the row gives dw nothing
+    check_grad(dx[rest], dw, dy[rest], x[rest], w, dres[rest])
+    assert torch.equal(grad(only, x, w, dres)[1], dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [64, 4099])
+def test_eps_0(dev, c):
+    x, w = rows(4, c, F, 2), torch.ones(c, device="cuda")
+    x[1], x[2] = 0, 1e-25
+    y = norm(x, w, eps=0.0)[0]
+    check_y(y[[0, 3]], exact(x, w, eps=0.0)[1][[0, 3]])
+    assert y[1].isnan().all() and (y[2] == float("inf")).all()
+
+
+@pytest.mark.gpu
 def test_norm_in_place(dev):
     # h over the residual or over x, y over x
     for c in (200, 4096, 5000):
