@@ -273,6 +273,68 @@ def test_keys_that_32_bits_do_not_tell_apart(dev):
     check(l, 8, SOFTMAX, 0, bias=(0.03 - p).float(), groups=4, top_groups=2, best=1)
 
 
+def near_pairs(score, n, seed):
+    """Two logits, and a bias of the second in 32 bits, whose keys s(x) and s(x2) + bias are (3.2 .. 32) 1e-15 of s(x) apart;
+    and which is larger, told in 80 bits. For softmax there is a third logit, the largest, which the bias excludes."""
+    r, wide = np.random.default_rng(seed), np.longdouble
+    if score == SIGMOID:
+        x = np.where(r.random(n) < 0.3, r.uniform(-1, 12, n), r.uniform(-60, 1, n)).astype(np.float32)
+        s = lambda v: 1 / (1 + np.exp(-v.astype(wide)))  # noqa: E731
+        slope = s(-x)  # of s, by s
+        m = np.zeros(n, np.float32)
+    else:
+        m = r.uniform(0, 5, n).astype(np.float32)
+        x = (m - r.uniform(0.01, 60, n)).astype(np.float32)
+    step = 3e-7 * r.uniform(0.3, 3, n)
+    if score == SIGMOID:
+        x2 = np.minimum((x - step / slope.astype(np.float64)).astype(np.float32), np.nextafter(x, np.float32(-np.inf)))
+        a, c = s(x), s(x2)
+    else:
+        x2 = np.minimum((x - step).astype(np.float32), np.nextafter(x, np.float32(-np.inf)))
+        e = [np.exp(v.astype(wide) - m.astype(wide)) for v in (m, x, x2)]
+        a, c = e[1] / sum(e), e[2] / sum(e)
+    b = (a - c).astype(np.float32)
+    apart = (a - (c + b.astype(wide))) / a
+    near = (np.abs(apart) > 3.2e-15) & (np.abs(apart) < 3.2e-14) & (b > 1e-37)
+    return x[near], x2[near], b[near], m[near], apart[near] > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
+def test_scores_hold_in_64_bits(dev, score):
+    # An exponential is off by 1e-15 of itself at most; a score has three roundings more and the sum with its bias one, of
+    # 1.1e-16 each: two keys are off by (2 * (1e-15 + 3.3e-16) + 2.2e-16) of the larger score together, below 3.2e-15.
+    x, x2, b, m, first = near_pairs(score, 60000, 1)
+    n = min(len(x), 1500)
+    assert n > 500 and 0.3 < first[:n].mean() < 0.7
+    lowest = np.float32(-np.inf) if score == SIGMOID else None
+    swap = np.arange(n) % 2 == 1  # either may have the lower index
+    l, bias = np.zeros((n, 3), np.float32), np.zeros((n, 3), np.float32)
+    l[:, 0], bias[:, 0] = (lowest if lowest is not None else m[:n]), -1.0
+    l[:, 1], l[:, 2] = np.where(swap, x2[:n], x[:n]), np.where(swap, x[:n], x2[:n])
+    bias[:, 1], bias[:, 2] = np.where(swap, b[:n], 0), np.where(swap, 0, b[:n])
+    L, B = torch.from_numpy(l).cuda(), torch.from_numpy(bias).cuda()
+    ids, w = torch.full((n,), -7, dtype=torch.int32, device="cuda"), torch.zeros(n, device="cuda")
+    for i in range(n):
+        M.launch(M.kernels.route_experts, (ids[i:i + 1], w[i:i + 1], None, None, None, L[i:i + 1], B[i], None, 3, 1, 1, 1, 1, score, 0, 0, 1.0), 1, stream=stream())
+    want = np.where(first[:n] != swap, 1, 2)
+    assert np.array_equal(ids.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_scores_that_are_denormal_in_64_bits(dev):
+    # groups' values are sums of scores: of -700 and below they are denormal, down to the smallest, and then zeros
+    a = np.array([-1, -87, -104, -650, -708, -709, -720, -730, -740, -743, -744], np.float32)
+    pairs = [(p, q) for p in a for q in a if p != q]
+    l = np.full((len(pairs), 4), -np.inf, np.float32)
+    l[:, 0], l[:, 2] = np.array(pairs).T
+    ids, _, _ = route(torch.from_numpy(l).cuda(), 1, SIGMOID, 0, groups=2, top_groups=1, best=2)
+    assert np.array_equal(ids.cpu().numpy()[:, 0], np.where(l[:, 0] > l[:, 2], 0, 2))
+    l[:, 0], l[:, 2] = -800, -750
+    ids, _, _ = route(torch.from_numpy(l).cuda(), 1, SIGMOID, 0, groups=2, top_groups=1, best=2)
+    assert (ids == 0).all()  # both zeros, and so the lower group
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("score", [SOFTMAX, SIGMOID])
 def test_biases_that_are_large_or_infinite(dev, score):
