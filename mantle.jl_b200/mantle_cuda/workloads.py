@@ -426,10 +426,6 @@ class MoeWorkload:
     plan: Plan
     tensors: dict
 
-    @property
-    def flops_step(self) -> int:
-        return 4 * self.tokens * self.top * self.width * self.hidden + 2 * self.tokens * self.width * self.experts
-
 
 def build_moe(dev, tokens: int = 4096, experts: int = 16, top: int = 2, width: int = 2048, hidden: int = 4096,
               seed: int = 13, eps: float = 1e-6, **plan_kw) -> MoeWorkload:
