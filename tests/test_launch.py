@@ -120,3 +120,41 @@ def test_buffers_take_the_long_way_to_the_same_results(dev):
         M.launch(k, (DX, DW, B(dy), DW, B(w), None, c, 0, 0, 1e-6), r, stream=dev.stream, workspace=ws)
     with pytest.raises(M.ArgumentError, match="expected Float32"):
         M.launch(k, (DX, ws, B(dy), B(h), B(w), None, c, 0, 0, 1e-6), r, stream=dev.stream, workspace=ws)
+
+
+@pytest.mark.gpu
+def test_launches_from_threads_at_once(dev):
+    # the launch runs without the interpreter's lock: each thread its own results, refusals and streams
+    import threading
+    k, errors = M.kernels, []
+    cases = [(5 + i, 64 * (i + 1)) for i in range(6)]
+    data = [(torch.randn(r, c, device="cuda"), torch.ones(c, device="cuda")) for r, c in cases]
+    want = [torch.empty_like(x) for x, _ in data]
+    for (x, w), y, (r, c) in zip(data, want, cases):
+        M.launch(k.rms_norm, norm_args(x, y, w, c=c), r, stream=stream())
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            (x, w), (r, c) = data[i], cases[i]
+            side, y = torch.cuda.Stream(), torch.empty_like(x)
+            dx, dw = torch.empty_like(x), torch.empty_like(w)
+            grad = (dx, dw, x, x, w, None, c, 0, 0, 1e-6)
+            ws = torch.empty(M.workspace_bytes(k.rms_norm_grad, grad, r), dtype=torch.uint8, device="cuda")
+            side.wait_stream(torch.cuda.current_stream())
+            for _ in range(100):
+                M.launch(k.rms_norm, norm_args(x, y, w, c=c), r, stream=side.cuda_stream)
+                M.launch(k.rms_norm_grad, grad, r, stream=side.cuda_stream, workspace=ws)
+                with pytest.raises(M.ArgumentError, match=f"y: {4 * r * c} bytes, the launch touches {4 * (r + 1) * c}"):
+                    M.launch(k.rms_norm, norm_args(x, y, w, c=c), r + 1, stream=side.cuda_stream)
+            side.synchronize()
+            assert torch.equal(y, want[i])
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
