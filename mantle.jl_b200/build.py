@@ -74,10 +74,11 @@ def build_launch(force: bool = False) -> None:
     against the torch that is installed, and again when another is. The library does
     without: where this cannot be built, launches take the long way."""
     found = importlib.util.find_spec("torch")
-    if found is None:
+    if found is None or not found.origin:  # no torch, or what is left of one
         return
     home, stamp = Path(found.origin).parent, OBJ / "launch.stamp"
-    built_for = f"{sys.version}\n{home}\n{(home / 'version.py').read_text()}"
+    version = home / "version.py"
+    built_for = f"{sys.version}\n{home}\n{version.read_text() if version.exists() else ''}"
     newest_dep = max(f.stat().st_mtime for f in (LAUNCH_SRC, ROOT / "include" / "mantle_cuda.h", Path(__file__)))
     if (not force and LAUNCH_OUT.exists() and LAUNCH_OUT.stat().st_mtime >= newest_dep
             and stamp.exists() and stamp.read_text() == built_for):

@@ -81,8 +81,9 @@ def test_a_build_without_it_goes_on_and_leaves_no_old_one(b, monkeypatch, capsys
     assert not b.LAUNCH_OUT.exists() and not old.exists() and not (b.OBJ / "launch.stamp").exists()
 
 
-def test_without_torch_there_is_nothing_to_build(b, monkeypatch):
-    monkeypatch.setattr(b.importlib.util, "find_spec", lambda name: None)
+@pytest.mark.parametrize("spec", [None, SimpleNamespace(origin=None)])
+def test_without_torch_there_is_nothing_to_build(b, monkeypatch, spec):
+    monkeypatch.setattr(b.importlib.util, "find_spec", lambda name: spec)
     b.build_launch()
     assert b.calls == []
 
